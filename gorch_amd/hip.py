@@ -104,6 +104,11 @@ SIGNATURES = {
     "gorch_hip_gqa_forward_cached": (i32, [vp, vp, vp, i32, vp, vp, i32, i32, vp, vp, C.c_size_t]),
     "gorch_hip_qwen_block_workspace_size": (C.c_size_t, [vp, i32]),
     "gorch_hip_qwen_block_forward_cached": (i32, [vp, vp, vp, i32, vp, vp, i32, i32, vp, C.c_size_t]),
+    "gorch_hip_paged_append": (i32, [vp, vp, vp, vp, vp, i64, vp, i64, vp, i64, vp]),
+    "gorch_hip_paged_read": (i32, [vp, vp, vp, vp, vp]),
+    "gorch_hip_paged_attention_workspace_size": (C.c_size_t, [vp, vp, i32]),
+    "gorch_hip_paged_attention": (i32, [vp, vp, vp, vp, i32, vp, i32, vp, C.c_size_t]),
+    "gorch_hip_process_logits": (i32, [vp, vp, vp, vp, i32, i32]),
     "gorch_hip_moe_workspace_size": (C.c_size_t, [i32, i32, i32, i32, i32]),
     "gorch_hip_moe_forward": (i32, [vp, vp, vp, i32, vp, vp, vp, vp, vp, C.c_size_t]),
     "gorch_hip_gpt_create": (vp, [vp]),
@@ -820,3 +825,219 @@ class QwenBlock:
         _ok(lib().gorch_hip_qwen_block_forward_cached(_stream(), C.byref(self.s), _p(x), S, _p(k_cache),
                                                       _p(v_cache), pos_offset, k_cache.shape[0],
                                                       self.ws.data_ptr(), self.ws.numel()))
+
+
+# ------------------------------------------------------------------ paged KV cache
+
+KV_BF16, KV_E4M3 = 0, 1
+
+
+class _PagedKVC(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("dtype", "num_pages", "page_size", "num_kv", "head_dim")] + [
+        (n, vp) for n in ("k", "v", "k_scale", "v_scale")]
+
+
+class _PagedBatchC(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("tokens", "seqs", "max_pages", "max_new", "max_kv")] + [
+        (n, vp) for n in ("cu_seqlens", "kv_lens", "page_table")]
+
+
+def _typed(t, dtype, shape, name):
+    """Device pointer of a contiguous tensor of this dtype and shape on the
+    current device (None stays None)."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.shape != shape:
+        raise ValueError(f"gorch_amd.hip: {name} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    _here(t, name)
+    return _p(t)
+
+
+def _here(t, name):
+    torch_c = _torch_c or _load_torch()
+    if t.get_device() != torch_c._cuda_getDevice():
+        raise ValueError(f"gorch_amd.hip: {name} is not on the current device")
+
+
+def _rows(t, width, tokens, name):
+    """Pointer and row stride of f32 rows [tokens, width] whose rows may lie
+    apart (a column range of a fused projection)."""
+    import torch
+
+    if t.dtype != torch.float32 or t.shape != (tokens, width) or (width > 1 and t.stride(1) != 1):
+        raise ValueError(f"gorch_amd.hip: {name} must be f32 rows [{tokens}, {width}] of unit column stride, "
+                         f"got {t.dtype} {tuple(t.shape)} of strides {tuple(t.stride())}")
+    _here(t, name)
+    stride = t.stride(0) if tokens > 1 else width
+    if stride < width:
+        raise ValueError(f"gorch_amd.hip: {name} has rows that overlap")
+    return t.data_ptr(), stride
+
+
+class PagedBatch:
+    """gorch_hip_paged_batch: `tokens` token rows of ragged sequences.
+    cu_seqlens [seqs + 1], kv_lens [seqs] and page_table [seqs, max_pages] are
+    int32 device tensors, read when the kernels run (so they can be updated in
+    place between replays of a captured step); max_new and max_kv are the
+    host's bounds on a sequence's new rows and cached length (0: none)."""
+
+    def __init__(self, cu_seqlens, kv_lens, page_table, tokens: int, max_new: int = 0, max_kv: int = 0):
+        import torch
+
+        seqs = kv_lens.shape[0]
+        if page_table.dim() != 2:
+            raise ValueError("gorch_amd.hip: page_table must be [seqs, max_pages]")
+        s = _PagedBatchC(tokens, seqs, page_table.shape[1], max_new, max_kv)
+        s.cu_seqlens = _typed(cu_seqlens, torch.int32, (seqs + 1,), "cu_seqlens")
+        s.kv_lens = _typed(kv_lens, torch.int32, (seqs,), "kv_lens")
+        s.page_table = _typed(page_table, torch.int32, (seqs, page_table.shape[1]), "page_table")
+        self.t = (cu_seqlens, kv_lens, page_table)
+        self.s = s
+        self.ref = C.byref(s)
+        self.tokens = tokens
+        self.device = kv_lens.get_device()
+
+
+class PagedKV:
+    """gorch_hip_paged_kv: one layer's K and V pools [num_pages, num_kv,
+    page_size, head_dim] (device tensors: bf16, or e4m3 codes with f32 scales
+    [num_pages, num_kv, page_size]); ``new`` allocates them. bf16 pools may
+    also be int16 storage, e4m3 ones uint8."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        import torch
+
+        if k.dim() != 4:
+            raise ValueError("gorch_amd.hip: pools must be [num_pages, num_kv, page_size, head_dim]")
+        if k.dtype in (torch.bfloat16, torch.int16):
+            dtype = KV_BF16
+        elif k.dtype in (torch.float8_e4m3fn, torch.uint8):
+            dtype = KV_E4M3
+        else:
+            raise ValueError(f"gorch_amd.hip: pools must be bf16 or e4m3, got {k.dtype}")
+        if (k_scale is None) != (dtype == KV_BF16) or (v_scale is None) != (dtype == KV_BF16):
+            raise ValueError("gorch_amd.hip: e4m3 pools need k_scale and v_scale, bf16 pools take none")
+        pages, num_kv, page, hd = k.shape
+        s = _PagedKVC(dtype, pages, page, num_kv, hd)
+        s.k = _typed(k, k.dtype, k.shape, "k")
+        s.v = _typed(v, k.dtype, k.shape, "v")
+        s.k_scale = _typed(k_scale, torch.float32, k.shape[:3], "k_scale")
+        s.v_scale = _typed(v_scale, torch.float32, k.shape[:3], "v_scale")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.num_kv, self.head_dim = num_kv, hd
+        self.s = s
+        self.ref = C.byref(s)
+        self.device = k.get_device()
+
+    @classmethod
+    def new(cls, num_pages: int, page_size: int, num_kv: int, head_dim: int, dtype: str = "bf16") -> "PagedKV":
+        """Zeroed pools of dtype "bf16" or "e4m3" on the current device."""
+        import torch
+
+        shape = (num_pages, num_kv, page_size, head_dim)
+        if dtype == "bf16":
+            return cls(*(torch.zeros(shape, dtype=torch.bfloat16, device="cuda") for _ in "kv"))
+        if dtype != "e4m3":
+            raise ValueError('gorch_amd.hip: dtype must be "bf16" or "e4m3"')
+        return cls(*(torch.zeros(shape, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in "kv"),
+                   *(torch.zeros(shape[:3], device="cuda") for _ in "kv"))
+
+    def _check(self, batch):
+        torch_c = _torch_c or _load_torch()
+        if not (self.device == batch.device == torch_c._cuda_getDevice()):
+            raise ValueError("gorch_amd.hip: the cache and the batch must be on the current device")
+
+    def append(self, batch: PagedBatch, heads: "GQA", q, k, v, q_out) -> None:
+        """gorch_hip_paged_append: the per-head norms and RoPE of ``heads``
+        (a GQA) on q and k, q to q_out, K and V into the pages. q, k, v: f32
+        rows [tokens, width], possibly column ranges of one tensor; q and
+        q_out may be None."""
+        import torch
+
+        self._check(batch)
+        T = batch.tokens
+        qp = qs = None
+        if q is not None:
+            qp, qs = _rows(q, heads.s.num_q * self.head_dim, T, "q")
+        kp, ks = _rows(k, self.num_kv * self.head_dim, T, "k")
+        vp_, vs = _rows(v, self.num_kv * self.head_dim, T, "v")
+        op = _typed(q_out, torch.float32, (T, heads.s.num_q * self.head_dim), "q_out")
+        _ok(lib().gorch_hip_paged_append(_stream(), self.ref, batch.ref, C.byref(heads.s), qp, qs or 0, kp, ks, vp_, vs,
+                                         op))
+
+    def read(self, batch: PagedBatch, k_out, v_out) -> None:
+        """gorch_hip_paged_read: the batch's tokens as f32 rows [tokens,
+        num_kv * head_dim] (either may be None)."""
+        import torch
+
+        self._check(batch)
+        shape = (batch.tokens, self.num_kv * self.head_dim)
+        _ok(lib().gorch_hip_paged_read(_stream(), self.ref, batch.ref, _typed(k_out, torch.float32, shape, "k_out"),
+                                       _typed(v_out, torch.float32, shape, "v_out")))
+
+    def workspace(self, batch: PagedBatch, num_q: int):
+        """A device workspace for attention() over this batch's bounds, or
+        None where none is needed."""
+        import torch
+
+        n = lib().gorch_hip_paged_attention_workspace_size(self.ref, batch.ref, num_q)
+        return torch.empty(n, dtype=torch.uint8, device="cuda") if n else None
+
+    def attention(self, batch: PagedBatch, q, out, causal: bool = True, ws=None) -> None:
+        """gorch_hip_paged_attention: q and out f32 [tokens, num_q *
+        head_dim]. ws from workspace() (a new one if None); calls that can
+        overlap must not share it."""
+        import torch
+
+        self._check(batch)
+        T, width = q.shape
+        if T != batch.tokens:
+            raise ValueError(f"gorch_amd.hip: q must have {batch.tokens} rows, got {T}")
+        num_q = width // self.head_dim
+        if num_q * self.head_dim != width:
+            raise ValueError("gorch_amd.hip: q's rows must be whole heads")
+        qp = _typed(q, torch.float32, (T, width), "q")
+        op = _typed(out, torch.float32, (T, width), "out")
+        if ws is None:
+            ws = self.workspace(batch, num_q)
+        elif ws.get_device() != self.device:
+            raise ValueError("gorch_amd.hip: ws is not on the current device")
+        _ok(lib().gorch_hip_paged_attention(_stream(), self.ref, batch.ref, qp, num_q, op, int(causal), _p(ws),
+                                            0 if ws is None else ws.numel() * ws.element_size()))
+
+
+class _LogitsRulesC(C.Structure):
+    _fields_ = [("history", vp), ("history_stride", C.c_int)] + [
+        (n, vp) for n in ("history_lens", "prompt_lens", "repetition", "frequency", "presence", "bias_rows", "bias_ids",
+                          "bias")] + [("biases", C.c_int), ("allowed", vp), ("allowed_stride", C.c_int)]
+
+
+def process_logits(logits, out, history=None, history_lens=None, prompt_lens=None, repetition=None, frequency=None,
+                   presence=None, bias_rows=None, bias_ids=None, bias=None, allowed=None) -> None:
+    """gorch_hip_process_logits: out (may be logits) [rows, n] = logits under
+    each row's penalties for the tokens of history int32 [rows, width], its
+    biases (CSR rows, last entry of an id counts) and its bit mask allowed
+    int32 [rows, >= ceil(n / 32)]. Every rule may be None."""
+    import torch
+
+    rows, n = logits.shape
+    f32t, i32t = torch.float32, torch.int32
+    r = _LogitsRulesC()
+    if history is not None:
+        r.history, r.history_stride = _typed(history, i32t, (rows, history.shape[-1]), "history"), history.shape[-1]
+    r.history_lens = _typed(history_lens, i32t, (rows,), "history_lens")
+    r.prompt_lens = _typed(prompt_lens, i32t, (rows,), "prompt_lens")
+    r.repetition = _typed(repetition, f32t, (rows,), "repetition")
+    r.frequency = _typed(frequency, f32t, (rows,), "frequency")
+    r.presence = _typed(presence, f32t, (rows,), "presence")
+    if bias is not None:
+        if bias_rows is None or bias_ids is None:
+            raise ValueError("gorch_amd.hip: bias needs bias_rows and bias_ids")
+        r.biases = bias.numel()
+        r.bias_rows = _typed(bias_rows, i32t, (rows + 1,), "bias_rows")
+        r.bias_ids = _typed(bias_ids, i32t, (r.biases,), "bias_ids")
+        r.bias = _typed(bias, f32t, (r.biases,), "bias")
+    if allowed is not None:
+        r.allowed, r.allowed_stride = _typed(allowed, i32t, (rows, allowed.shape[-1]), "allowed"), allowed.shape[-1]
+    _ok(lib().gorch_hip_process_logits(_stream(), C.byref(r), _typed(logits, f32t, (rows, n), "logits"),
+                                       _typed(out, f32t, (rows, n), "out"), rows, n))

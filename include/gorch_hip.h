@@ -426,6 +426,118 @@ int gorch_hip_qwen_generate_sampled(void* stream, gorch_hip_qwen* m, const int* 
                                     float* timing_ms, int flags);
 
 /* ------------------------------------------------------------------------
+ * A KV cache in pages, shared by sequences of different lengths (no
+ * counterpart in the reference, whose nn.KVCache holds one sequence,
+ * nn/kvcache.go:14-60): one serving step is the QKV Linear, then
+ * gorch_hip_paged_append, gorch_hip_paged_attention and the Wo Linear per
+ * layer, then the logits, gorch_hip_process_logits and gorch_hip_sample.
+ * ---------------------------------------------------------------------- */
+
+#define GORCH_HIP_KV_BF16 0 /* bf16 rows                                       */
+#define GORCH_HIP_KV_E4M3 1 /* OCP e4m3 codes, one f32 scale a (token, KV head) */
+
+/* One layer's pools (device): k and v [num_pages][num_kv][page_size][head_dim]
+ * of dtype, 16-byte aligned; with GORCH_HIP_KV_E4M3 also k_scale and v_scale
+ * [num_pages][num_kv][page_size], a row's value being code * scale (NULL and
+ * unused with GORCH_HIP_KV_BF16). head_dim is a multiple of 16 up to 256
+ * (else GORCH_HIP_EUNSUPPORTED); page_size is any positive number. */
+typedef struct {
+    int dtype, num_pages, page_size, num_kv, head_dim;
+    void* k; void* v;
+    float* k_scale; float* v_scale;
+} gorch_hip_paged_kv;
+
+/* A ragged batch: `tokens` token rows, those of sequence s being rows
+ * cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (device int32 [seqs + 1], not
+ * decreasing; a sequence may have none, rows of no sequence are left as they
+ * are). kv_lens (device int32 [seqs]): a sequence's cached tokens, this call's
+ * included: its row i of n stands at position kv_lens[s] - n + i. page_table
+ * (device int32 [seqs][max_pages]): position p is slot p % page_size of page
+ * page_table[s][p / page_size]. The device arrays are read when the kernels
+ * run, so a captured graph follows their contents.
+ * max_kv: no position at or past it is read or written (0: max_pages *
+ * page_size, which always holds); max_new: the most rows of a sequence (0:
+ * tokens). Both are bounds that the host knows; a kernel is chosen by them,
+ * and rows past max_new are still computed.
+ * An entry of page_table outside 0 .. num_pages - 1 is no page: nothing is
+ * written there, and its keys are not seen. Sequences may share pages that
+ * none of them writes in the same call. */
+typedef struct {
+    int tokens, seqs, max_pages, max_new, max_kv;
+    const int* cu_seqlens; const int* kv_lens; const int* page_table;
+} gorch_hip_paged_batch;
+
+/* Finishes the new tokens' q and k and writes k and v into the pages. Of w
+ * are read num_q, num_kv, head_dim, norm_eps, q_norm, k_norm, rope_cos,
+ * rope_sin, rope_max_seq and rope_neox (GQA.ForwardCached's order,
+ * nn/gqa.go:300-330): per-head RMSNorm where there is a gain (f64 sum of
+ * squares), then RoPE at the token's position where there are tables, in f32
+ * as gorch_hip_gqa_forward_cached; then K and V are rounded once: to bf16
+ * (nearest even), or to e4m3 codes of x / scale with scale = (the row's
+ * largest magnitude) / 448 (a row below 2^-100 throughout is stored as
+ * zeros; a row that holds an infinity reads back as NaN). Rows q [tokens,
+ * num_q * head_dim], k and v [tokens, num_kv * head_dim] start at multiples
+ * of their strides (in floats, multiples of 4), so the three can be column
+ * ranges of one fused projection; 16-byte aligned. q_out [tokens, num_q *
+ * head_dim] may be q if its rows are contiguous; q and q_out may both be
+ * NULL. A token whose position is negative, past max_kv or the RoPE tables, or
+ * on no page, is skipped: none of its rows is written, q_out's neither.
+ * No two tokens of a call may have the same slot. */
+int gorch_hip_paged_append(void* stream, const gorch_hip_paged_kv* kv, const gorch_hip_paged_batch* b,
+                           const gorch_hip_gqa_weights* w, const float* q, int64_t q_stride, const float* k,
+                           int64_t k_stride, const float* v, int64_t v_stride, float* q_out);
+/* The batch's tokens read back from the pages as f32 rows [tokens, num_kv *
+ * head_dim], the layout of the contiguous caches (kv_lens[s] rows for
+ * sequence s give all of it; fewer give its last ones). Either output may be
+ * NULL. Rows at positions that are negative, past max_kv or on no page are
+ * left as they are. */
+int gorch_hip_paged_read(void* stream, const gorch_hip_paged_kv* kv, const gorch_hip_paged_batch* b, float* k_out,
+                         float* v_out);
+/* Grouped-query attention of the batch's tokens over their sequences' pages
+ * (gorch_hip_gqa_attention_cached's mathematics over a cache that already
+ * holds the new rows): q and out [tokens, num_q * head_dim] f32, contiguous,
+ * 16-byte aligned; query head h reads KV head h / (num_q / num_kv); scores
+ * scaled by 1 / sqrt(head_dim). causal: a token sees the positions up to its
+ * own, else all kv_lens[s]. Products and sums keep f32 accuracy (q and the
+ * softmax weights as three bf16 terms against the cache's exact values), every
+ * sum has a fixed order. A key that a token does not see has no effect on it,
+ * whatever its page holds; a token that sees none gets zeros. The workspace
+ * (gorch_hip_paged_attention_workspace_size bytes, device, 16-byte aligned;
+ * NULL where that is 0) is the caller's: calls that can overlap must not share
+ * one. Nothing is allocated, so the call can be captured. */
+size_t gorch_hip_paged_attention_workspace_size(const gorch_hip_paged_kv* kv, const gorch_hip_paged_batch* b,
+                                                int num_q);
+int gorch_hip_paged_attention(void* stream, const gorch_hip_paged_kv* kv, const gorch_hip_paged_batch* b,
+                              const float* q, int num_q, float* out, int causal, void* workspace,
+                              size_t workspace_bytes);
+
+/* What requests ask of their logits before a token is chosen. Device
+ * pointers; NULL leaves a part out. Per row r of [rows, n]:
+ *   history [rows][history_stride] int32 token ids, of which the first
+ *   history_lens[r] count (NULL: all); the first prompt_lens[r] of those are
+ *   the prompt (NULL: none). Ids outside 0 .. n - 1 are passed over.
+ *   repetition[r]: a seen token's logit l becomes l / repetition (l > 0) or
+ *   l * repetition;
+ *   frequency[r], presence[r]: minus count * frequency, and minus presence
+ *   once, for tokens seen after the prompt;
+ *   bias: entries bias_rows[r] .. bias_rows[r + 1] - 1 (int32 [rows + 1]) of
+ *   bias_ids and bias [biases] add bias to the logit of bias_ids; of several
+ *   entries of one id the last counts;
+ *   allowed [rows][allowed_stride] uint32: token i is allowed if bit i % 32 of
+ *   word i / 32 is set; the others become -inf, whatever they were.
+ * They are applied in this order, in f32. */
+typedef struct {
+    const int* history; int history_stride; const int* history_lens; const int* prompt_lens;
+    const float* repetition; const float* frequency; const float* presence;
+    const int* bias_rows; const int* bias_ids; const float* bias; int biases;
+    const uint32_t* allowed; int allowed_stride;
+} gorch_hip_logits_rules;
+/* out [rows, n] (may be logits) = logits under the rules. A row whose mask
+ * allows nothing is -inf throughout (argmax then gives index 0). */
+int gorch_hip_process_logits(void* stream, const gorch_hip_logits_rules* r, const float* logits, float* out, int rows,
+                             int n);
+
+/* ------------------------------------------------------------------------
  * MoE FFN layer (nn.MoE.Forward, nn/moe.go:130-182).
  * ---------------------------------------------------------------------- */
 

@@ -1,0 +1,136 @@
+"""CPU-only checks of the paged cache's and the logits rules' refusals: every
+argument check comes before any device work, so fake pointers reach it."""
+import ctypes as C
+
+import pytest
+
+from gorch_amd import hip
+
+FAKE, ODD = 0x10000, 0x10004
+
+
+def cache(**over):
+    s = hip._PagedKVC(hip.KV_BF16, 8, 16, 2, 64, FAKE, FAKE, None, None)
+    for k, v in over.items():
+        setattr(s, k, v)
+    return s
+
+
+def batch(**over):
+    s = hip._PagedBatchC(4, 2, 4, 0, 0, FAKE, FAKE, FAKE)
+    for k, v in over.items():
+        setattr(s, k, v)
+    return s
+
+
+def heads(**over):
+    s = hip._GQAW()
+    s.num_q, s.num_kv, s.head_dim, s.norm_eps = 4, 2, 64, 1e-6
+    for k, v in over.items():
+        setattr(s, k, v)
+    return s
+
+
+def attend(kv, b, q=FAKE, num_q=4, out=FAKE, ws=None, n=0):
+    return hip.lib().gorch_hip_paged_attention(None, C.byref(kv), C.byref(b), q, num_q, out, 1, ws, n)
+
+
+def append(kv, b, w, q=FAKE, qs=256, k=FAKE, ks=128, v=FAKE, vs=128, out=FAKE + 64):
+    return hip.lib().gorch_hip_paged_append(None, C.byref(kv), C.byref(b), C.byref(w), q, qs, k, ks, v, vs, out)
+
+
+def read(kv, b, ko=FAKE, vo=FAKE):
+    return hip.lib().gorch_hip_paged_read(None, C.byref(kv), C.byref(b), ko, vo)
+
+
+BAD_CACHE = [(dict(dtype=7), 2), (dict(num_pages=0), 2), (dict(page_size=0), 2), (dict(num_kv=-1), 2),
+             (dict(head_dim=0), 2), (dict(head_dim=72), 1), (dict(head_dim=272), 1), (dict(k=None), 2),
+             (dict(v=None), 2), (dict(k=ODD), 1), (dict(v=ODD), 1), (dict(dtype=1), 2),
+             (dict(dtype=1, k_scale=FAKE), 2)]
+BAD_BATCH = [(dict(tokens=-1), 2), (dict(seqs=-1), 2), (dict(max_pages=-1), 2), (dict(max_new=-1), 2),
+             (dict(max_kv=-1), 2), (dict(cu_seqlens=None), 2), (dict(kv_lens=None), 2), (dict(page_table=None), 2),
+             (dict(max_pages=1 << 27), 2)]
+
+
+@pytest.mark.parametrize("over,rc", BAD_CACHE)
+def test_bad_cache_is_refused(over, rc):
+    kv, b = cache(**over), batch()
+    w = heads(head_dim=kv.head_dim, num_kv=kv.num_kv)
+    assert attend(kv, b) == rc and "paged_attention" in hip.last_error()
+    assert append(kv, b, w) == rc and "paged_append" in hip.last_error()
+    assert read(kv, b) == rc and "paged_read" in hip.last_error()
+
+
+@pytest.mark.parametrize("over,rc", BAD_BATCH)
+def test_bad_batch_is_refused(over, rc):
+    kv, b = cache(), batch(**over)
+    assert attend(kv, b) == rc
+    assert append(kv, b, heads()) == rc
+    assert read(kv, b) == rc
+    assert hip.lib().gorch_hip_paged_attention_workspace_size(C.byref(kv), C.byref(b), 4) == 0 or rc != 2
+
+
+def test_null_structs_are_refused():
+    L = hip.lib()
+    kv, b = cache(), batch()
+    assert L.gorch_hip_paged_attention(None, None, C.byref(b), FAKE, 4, FAKE, 1, None, 0) == 2
+    assert L.gorch_hip_paged_attention(None, C.byref(kv), None, FAKE, 4, FAKE, 1, None, 0) == 2
+    assert L.gorch_hip_paged_append(None, C.byref(kv), C.byref(b), None, None, 0, FAKE, 128, FAKE, 128, None) == 2
+    assert L.gorch_hip_paged_attention_workspace_size(None, C.byref(b), 4) == 0
+    assert L.gorch_hip_process_logits(None, None, FAKE, FAKE, 1, 8) == 2
+
+
+def test_attention_arguments():
+    kv, b = cache(), batch()
+    assert attend(kv, b, num_q=3) == 2 and attend(kv, b, num_q=0) == 2
+    assert attend(kv, b, q=None) == 2 and attend(kv, b, out=None) == 2
+    assert attend(kv, b, q=ODD) == 1 and attend(kv, b, out=ODD) == 1
+
+
+def test_append_arguments():
+    kv, b = cache(), batch()
+    assert append(kv, b, heads(num_kv=4)) == 2 and append(kv, b, heads(head_dim=128)) == 2
+    assert append(kv, b, heads(num_q=3)) == 2
+    assert append(kv, b, heads(), q=None) == 2 and append(kv, b, heads(), out=None) == 2
+    assert append(kv, b, heads(), k=None) == 2 and append(kv, b, heads(), v=None) == 2
+    assert append(kv, b, heads(), ks=127) == 2 and append(kv, b, heads(), qs=128) == 2
+    assert append(kv, b, heads(), ks=129) == 1 and append(kv, b, heads(), k=ODD) == 1
+    assert append(kv, b, heads(rope_cos=FAKE)) == 2
+    # q may be its own output only where its rows lie together
+    assert append(kv, b, heads(), qs=512, out=FAKE) == 2
+
+
+def test_nothing_to_do_is_no_work():
+    for b in (batch(tokens=0), batch(seqs=0), batch(tokens=0, cu_seqlens=None, kv_lens=None, page_table=None)):
+        assert attend(cache(), b) == 0 and append(cache(), b, heads()) == 0 and read(cache(), b) == 0
+    assert read(cache(), batch(), None, None) == 0
+    r = hip._LogitsRulesC()
+    assert hip.lib().gorch_hip_process_logits(None, C.byref(r), None, None, 0, 8) == 0
+    assert hip.lib().gorch_hip_process_logits(None, C.byref(r), None, None, 4, 0) == 0
+
+
+@pytest.mark.parametrize("over,rows,n,rc", [
+    ({}, -1, 8, 2), ({}, 1, -8, 2), (dict(history=FAKE, history_stride=-1), 1, 8, 2), (dict(biases=-1), 1, 8, 2),
+    (dict(biases=2, bias=FAKE, bias_ids=FAKE), 1, 8, 2), (dict(biases=2, bias=FAKE, bias_rows=FAKE), 1, 8, 2),
+    (dict(biases=2, bias_rows=FAKE, bias_ids=FAKE), 1, 8, 2), (dict(allowed=FAKE, allowed_stride=1), 1, 33, 2),
+    ({}, 65536, 8, 1)])
+def test_bad_logits_rules_are_refused(over, rows, n, rc):
+    r = hip._LogitsRulesC()
+    for k, v in over.items():
+        setattr(r, k, v)
+    assert hip.lib().gorch_hip_process_logits(None, C.byref(r), FAKE, FAKE, rows, n) == rc
+    assert hip.lib().gorch_hip_process_logits(None, C.byref(r), None, FAKE, max(rows, 1), max(n, 1)) != 0
+
+
+def test_cpu_tensors_are_refused():
+    import torch
+
+    with pytest.raises(ValueError):
+        hip._p(torch.zeros(4))
+    with pytest.raises((ValueError, RuntimeError, AssertionError)):
+        hip.PagedKV(torch.zeros((2, 2, 16, 64), dtype=torch.bfloat16), torch.zeros((2, 2, 16, 64), dtype=torch.bfloat16))
+    with pytest.raises(ValueError):
+        hip.PagedKV(torch.zeros((2, 2, 16, 64)), torch.zeros((2, 2, 16, 64)))
+    with pytest.raises(ValueError):
+        hip.PagedKV(torch.zeros((2, 2, 16, 64), dtype=torch.bfloat16), torch.zeros((2, 2, 16, 64), dtype=torch.bfloat16),
+                    torch.zeros((2, 2, 16)), torch.zeros((2, 2, 16)))
