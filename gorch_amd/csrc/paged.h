@@ -38,24 +38,38 @@ struct PagedArgs {
 // First row of sequence s, kept in range whatever the array holds.
 __device__ __forceinline__ int seq_begin(const PagedArgs& a, int s) { return min(max(a.cu[s], 0), a.tokens); }
 
-// The last s with key(s) <= x among 0 .. n - 1 (key not decreasing), -1 if
-// none; every lane of the wave calls it with the same x and gets the answer.
-// 64 candidates a step, so 64 sequences take one load and 4096 two.
+// The sequence of a batch that x belongs to: the last s with key(s, first row
+// of s) <= x (key not decreasing), its rows and its length; false if there is
+// none. Every lane of the wave calls it with the same x and gets the answer.
+// 64 candidates a step, and the last step fetches everything at once: up to
+// 64 sequences take one round trip to memory, up to 4096 two.
+struct SeqAt {
+    int s, begin, end, len;
+};
 template <typename Key>
-__device__ __forceinline__ int wave_find(int n, int x, Key key) {
+__device__ __forceinline__ bool wave_seq(const PagedArgs& a, int x, Key key, SeqAt& r) {
     const int lane = threadIdx.x & 63;
-    int lo = 0;
-    bool first = true;
-    while (n > 1 || first) {
+    int lo = 0, n = a.seqs;
+    while (n > 64) {
         const int step = (n + 63) / 64, at = lane * step;
-        const bool le = at < n && key(lo + at) <= x;
-        const int c = __popcll(__ballot(le));
-        if (c == 0) return -1;
+        const int c = __popcll(__ballot(at < n && key(lo + at, seq_begin(a, lo + at)) <= x));
+        if (c == 0) return false;
         lo += (c - 1) * step;
         n = min(step, n - (c - 1) * step);
-        first = false;
     }
-    return lo;
+    const int i = lo + min(lane, n - 1);
+    const int b = seq_begin(a, i), e = max(b, seq_begin(a, i + 1)), len = a.lens[i];
+    const int c = __popcll(__ballot(lane < n && key(i, b) <= x));
+    if (c == 0) return false;
+    r.s = lo + c - 1;
+    r.begin = __builtin_amdgcn_readlane(b, c - 1);
+    r.end = __builtin_amdgcn_readlane(e, c - 1);
+    r.len = __builtin_amdgcn_readlane(len, c - 1);
+    return true;
+}
+// The sequence that token row t belongs to.
+__device__ __forceinline__ bool token_seq(const PagedArgs& a, int t, SeqAt& r) {
+    return wave_seq(a, t, [](int, int begin) { return begin; }, r) && t < r.end;
 }
 
 // Pool row of position p of sequence s for KV head h (in rows of hd elements;

@@ -114,11 +114,9 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
     constexpr int RPB = 256 / NL;
     const int t = blockIdx.x, hd = a.p.hd, half = hd / 2, nl = hd / 4;
     const int c = threadIdx.x % NL, r = blockIdx.y * RPB + threadIdx.x / NL;
-    const int s = wave_find(a.p.seqs, t, [&](int i) { return seq_begin(a.p, i); });
-    if (s < 0) return;
-    const int end = seq_begin(a.p, s + 1);
-    if (t >= end) return;
-    const int pos = a.p.lens[s] - end + t;
+    SeqAt sq;
+    if (!token_seq(a.p, t, sq)) return;
+    const int s = sq.s, pos = sq.len - sq.end + t;
     if (pos < 0 || (a.cosT && pos >= a.rope_rows) || pool_row(a.p, s, pos, 0) < 0) return;
     const int nkv = a.p.num_kv, rows = a.hq + 2 * nkv;
     const bool live = r < rows, mine = live && c < nl;
@@ -161,11 +159,9 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
 template <bool F8>
 __global__ __launch_bounds__(256) void k_paged_read(PagedArgs p, float* ko, float* vo) {
     const int t = blockIdx.x;
-    const int s = wave_find(p.seqs, t, [&](int i) { return seq_begin(p, i); });
-    if (s < 0) return;
-    const int end = seq_begin(p, s + 1);
-    if (t >= end) return;
-    const int pos = p.lens[s] - end + t;
+    SeqAt sq;
+    if (!token_seq(p, t, sq)) return;
+    const int s = sq.s, pos = sq.len - sq.end + t;
     if (pos < 0) return;
     const int n4 = p.num_kv * p.hd / 4, hd4 = p.hd / 4;
     for (int i = threadIdx.x; i < n4; i += 256) {

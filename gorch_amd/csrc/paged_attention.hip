@@ -1,8 +1,30 @@
 // paged_attention.hip — attention of ragged new tokens over a KV cache in
 // pages (gorch_hip_gqa_attention_cached's mathematics, GQA.forwardCached
-// nn/gqa.go:308-352):
-//   o = sum_j p_j v_j / sum_j p_j, p_j = exp(q . k_j / sqrt(hd) - max_j ...)
-// over the positions j that the token sees.
+// nn/gqa.go:308-352): over the positions j that a token sees,
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(s_j - m),  s_j = log2(e) q . k_j / sqrt(hd),
+// with the running maximum m and sum of one pass over the keys.
+//
+// Accuracy: the cache's values (bf16, or e4m3 codes widened to bf16) are exact
+// matrix operands. q (scaled, f32) is split into three bf16 terms by
+// truncation, which together hold its 24 bits, and so is every p: three
+// v_mfma_f32_16x16x32_bf16 per product give f32 products summed in f32. Two
+// terms would save a third of the matrix time and leave 2^-16 of each q and p
+// (output error 3e-6 of the 2-norm against 6e-7). An e4m3 row's scale
+// multiplies the scores of its key (K) or its weight (V), never a rounded
+// operand.
+//
+// Layout: S^T = K Q^T and O^T = V^T P^T, so a lane's column is one query row
+// in both: a score's weight, and its row's maximum and rescaling, stay in the
+// lane that needs them. A key's row is fetched in 16-byte chunks, lane l of a
+// wave taking key l % 16, chunk 4 t + l / 16: that is the operand layout of K
+// (in LDS, a fragment is 1 KB in lane order, free of bank conflicts), and V's
+// fragments come out of the same layout by the LDS transpose reads, 16 columns
+// at once. The keys of a 32-key tile are numbered so that a lane's scores (4
+// keys of each 16) are its operand's 8 keys: the sum over keys has no order to
+// keep.
+#include <algorithm>
+#include <cmath>
+
 #include "paged.h"
 
 namespace gh {
@@ -11,65 +33,689 @@ struct PagedAttnArgs {
     PagedArgs p;
     const float* q;
     float* out;
+    float* part_o;   // [splits][tokens * hq][hd] unnormalised sums of a key range
+    float2* part_ml; // [splits][tokens * hq] its maximum (log2) and weight sum
     int hq, causal;
-    float scale;
+    float scale;     // log2(e) / sqrt(hd)
+    FastDiv group;   // query heads per KV head
+    int tiles;       // row tiles of this kernel's grid
+    int lo_rows, hi_rows;  // this kernel takes sequences of lo_rows <= rows <= hi_rows
+    int chunk, splits;     // keys of a split; splits == 1: no partial results
+    // the joining kernel: the other kernel's chunk and splits, for sequences
+    // of more than hi_rows rows
+    int chunk2, splits2;
 };
 
-template <bool F8>
-__device__ __forceinline__ float pool_value(const void* pool, long long i) {
-    if constexpr (F8) return e4m3_f32<0>(reinterpret_cast<const uint8_t*>(pool)[i]);
-    return bf16_lo(reinterpret_cast<const uint16_t*>(pool)[i]);
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+#define GH_LDS __attribute__((address_space(3)))
+
+// What rows and chunks that do not exist are read from.
+__device__ __align__(16) uint32_t kZeros[128];
+
+// f = t0 + t1 + t2 exactly (24 bits in 8 + 8 + 8; below 2^-110 the last ones
+// fall away): each term f's leading bits, cut off.
+__device__ __forceinline__ void split3(const float (&f)[8], bf16x8 (&t)[3]) {
+    uint32_t w[3][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t u[3][2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const float x = f[2 * i + e];
+            u[0][e] = __float_as_uint(x) & 0xffff0000u;
+            const float r = x - __uint_as_float(u[0][e]);
+            u[1][e] = __float_as_uint(r) & 0xffff0000u;
+            u[2][e] = __float_as_uint(r - __uint_as_float(u[1][e]));
+        }
+#pragma unroll
+        for (int k = 0; k < 3; k++) w[k][i] = __builtin_amdgcn_perm(u[k][1], u[k][0], 0x07060302u);
+    }
+#pragma unroll
+    for (int k = 0; k < 3; k++) t[k] = __builtin_bit_cast(bf16x8, w[k]);
 }
 
-// One wave per (query head, token): 64 keys at a time, a lane each for the
-// scores, then a lane per column (up to four) for the weighted values.
-template <bool F8>
-__global__ __launch_bounds__(64) void k_paged_attn_rows(PagedAttnArgs a) {
-    __shared__ float qs[256], ps[64];
-    __shared__ long long rows[64];
-    const int lane = threadIdx.x, h = blockIdx.x, t = blockIdx.y, hd = a.p.hd;
-    const int s = wave_find(a.p.seqs, t, [&](int i) { return seq_begin(a.p, i); });
-    if (s < 0) return;
-    const int end = seq_begin(a.p, s + 1);
-    if (t >= end) return;
-    const int len = a.p.lens[s], pos = len - end + t;
-    const int T = min(a.causal ? pos + 1 : len, a.p.limit);
-    const int kvh = h / (a.hq / a.p.num_kv);
-    for (int d = lane; d < hd; d += 64) qs[d] = a.q[((size_t)t * a.hq + h) * hd + d] * a.scale;
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int j0 = 0; j0 < T; j0 += 64) {
-        const long long row = j0 + lane < T ? pool_row(a.p, s, j0 + lane, kvh) : -1;
-        __syncthreads();
-        float sc = -INFINITY;
-        if (row >= 0) {
-            float d = 0.f;
-            for (int e = 0; e < hd; e++) d += qs[e] * pool_value<F8>(a.p.k, row * hd + e);
-            sc = F8 ? d * a.p.ks[row] : d;
-        }
-        const float mn = fmaxf(m, wave_max(sc)), use = mn == -INFINITY ? 0.f : mn;
-        const float p = row >= 0 ? expf(sc - use) : 0.f, al = expf(m - use);
-        l = l * al + wave_sum(p);
-        ps[lane] = F8 && row >= 0 ? p * a.p.vs[row] : p;
-        rows[lane] = row;
-        m = mn;
-        __syncthreads();
-        for (int i = 0; i < 4; i++) o[i] *= al;
-        for (int j = 0; j < 64; j++) {
-            if (rows[j] < 0) continue;
-            for (int i = 0; i < 4; i++)
-                if (lane + 64 * i < hd) o[i] += ps[j] * pool_value<F8>(a.p.v, rows[j] * hd + lane + 64 * i);
+// Eight e4m3 codes as bf16 (exact).
+__device__ __forceinline__ bf16x8 widen8(uint32_t a, uint32_t b) {
+    bf16x2 w[4];
+    w[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false);
+    w[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true);
+    w[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false);
+    w[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
+    return __builtin_bit_cast(bf16x8, w);
+}
+
+// Maximum and sum over the four lanes that hold one query row's scores (l, l
+// + 16, l + 32, l + 48).
+__device__ __forceinline__ float col_max(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float col_sum(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Sizes of a 32-key tile of K or V: NT 16-byte chunks of each lane for each of
+// its two 16-key groups.
+template <bool F8, int HD>
+struct Tile {
+    static constexpr int ES = F8 ? 1 : 2;
+    static constexpr int NT = HD * ES / 64;
+    static constexpr int NU = HD / 32;      // matrix steps along the head
+    static constexpr int BYTES = 32 * HD * ES;
+    static constexpr int GROUP = NT * 1024; // bytes of a 16-key group in LDS
+    // first head column of lane group g in step u (8 columns)
+    __device__ static __forceinline__ int col(int u, int g) {
+        return F8 ? 64 * (u >> 1) + 16 * g + 8 * (u & 1) : 32 * u + 8 * g;
+    }
+    // step u's operand out of a lane's chunks
+    __device__ static __forceinline__ bf16x8 frag(const u32x4 (&c)[NT], int u) {
+        if constexpr (F8) return (u & 1) ? widen8(c[u >> 1][2], c[u >> 1][3]) : widen8(c[u >> 1][0], c[u >> 1][1]);
+        else return __builtin_bit_cast(bf16x8, c[u]);
+    }
+    // V^T's operand for columns 16 dt .. 16 dt + 15 from a tile in LDS: slot
+    // 4 j + i of lane group g is key 16 j + 4 g + i
+    __device__ static __forceinline__ bf16x8 vfrag(const char* tile, int dt, int lane) {
+        const int g = lane >> 4;
+        if constexpr (F8) {
+            const int r = (lane & 15) >> 1, c = lane & 1;
+            const char* p = tile + (r >> 2) * GROUP + (dt >> 2) * 1024 + ((dt & 3) * 16 + 4 * g + (r & 3)) * 16 + 8 * c;
+            const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((GH_LDS i32x2*)p);
+            return widen8((uint32_t)w[0], (uint32_t)w[1]);
+        } else {
+            const int r = (lane & 15) >> 2, c = lane & 3, ch = 2 * dt + (c >> 1);
+            const char* p = tile + (ch >> 2) * 1024 + ((ch & 3) * 16 + 4 * g + r) * 16 + 8 * (c & 1);
+            s16x4 w[2];
+            w[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GH_LDS s16x4*)p);
+            w[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GH_LDS s16x4*)(p + GROUP));
+            return __builtin_bit_cast(bf16x8, w);
         }
     }
-    for (int i = 0; i < 4; i++)
-        if (lane + 64 * i < hd) a.out[((size_t)t * a.hq + h) * hd + lane + 64 * i] = l == 0.f ? 0.f : o[i] / l;
+};
+
+// Whether a lane's chunks hold an infinity or NaN.
+template <bool F8, int N>
+__device__ __forceinline__ bool any_nonfinite(const u32x4 (&c)[N]) {
+    if constexpr (F8) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) m |= (c[i][e] & 0x7f7f7f7fu) + 0x01010101u;
+        return (m & 0x80808080u) != 0;
+    } else {
+        u16x2 m = {0, 0};
+#pragma unroll
+        for (int i = 0; i < N; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, c[i][e] & 0x7fff7fffu));
+        return m[0] >= 0x7f80 || m[1] >= 0x7f80;
+    }
+}
+
+// A lane's fetch of one key row: its chunks, zeros where there is no row or
+// (PART: hd < HD) no column.
+template <bool F8, int HD, bool PART>
+__device__ __forceinline__ void fetch_row(const void* pool, long long row, int hd, int g, u32x4 (&c)[Tile<F8, HD>::NT]) {
+    constexpr int ES = Tile<F8, HD>::ES;
+    const char* zero = reinterpret_cast<const char*>(kZeros);
+    const char* p = row >= 0 ? static_cast<const char*>(pool) + row * (hd * ES) : zero;
+#pragma unroll
+    for (int t = 0; t < Tile<F8, HD>::NT; t++) {
+        const int o = (4 * t + g) * 16;
+        c[t] = *reinterpret_cast<const u32x4*>(PART && o >= hd * ES ? zero : p + o);
+    }
+}
+
+// One wave's query rows (NR tiles of 16) and their running state.
+template <bool F8, int HD, int NR>
+struct Rows {
+    using T = Tile<F8, HD>;
+    bf16x8 q[NR][T::NU][3];
+    floatx4 o[NR][HD / 16];
+    float m[NR], l[NR];
+    int pos[NR];   // the position of a lane's row (what it sees ends there), -1: none
+    int first, last;  // smallest and largest of the wave's rows that exist
+
+    // rows r0 + 16 i + lane % 16 of a sequence of n token rows
+    template <bool PART>
+    __device__ __forceinline__ void load(const PagedAttnArgs& a, const SeqAt& s, int r0, int kvh) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, G = a.group.d, n = s.end - s.begin;
+        int lo = 0x7fffffff, hi = -1;
+#pragma unroll
+        for (int i = 0; i < NR; i++) {
+            const int r = r0 + 16 * i + (lane & 15);
+            const int tok = (int)a.group.div((uint32_t)r), h = kvh * G + r - tok * G;
+            const bool live = r < n * G;
+            pos[i] = live ? (a.causal ? s.len - n + tok : s.len - 1) : -1;
+            if (live) lo = min(lo, pos[i]);
+            hi = max(hi, pos[i]);
+            const float* src = a.q + ((size_t)(s.begin + tok) * a.hq + h) * a.p.hd;
+#pragma unroll
+            for (int u = 0; u < T::NU; u++) {
+                const int c = T::col(u, g);
+                float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (live && (!PART || c < a.p.hd)) {
+                    const float4 x = *reinterpret_cast<const float4*>(src + c), y = *reinterpret_cast<const float4*>(src + c + 4);
+                    f[0] = x.x * a.scale;
+                    f[1] = x.y * a.scale;
+                    f[2] = x.z * a.scale;
+                    f[3] = x.w * a.scale;
+                    f[4] = y.x * a.scale;
+                    f[5] = y.y * a.scale;
+                    f[6] = y.z * a.scale;
+                    f[7] = y.w * a.scale;
+                }
+                split3(f, q[i][u]);
+            }
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+#pragma unroll
+            for (int d = 0; d < HD / 16; d++) o[i][d] = floatx4{0.f, 0.f, 0.f, 0.f};
+        }
+        for (int w = 1; w < 16; w *= 2) {
+            lo = min(lo, __shfl_xor(lo, w));
+            hi = max(hi, __shfl_xor(hi, w));
+        }
+        first = __builtin_amdgcn_readfirstlane(lo);
+        last = __builtin_amdgcn_readfirstlane(hi);
+    }
+
+    // Scores of group j's 16 keys from a lane's chunks: sc[i] of row tile i
+    // holds keys 4 g .. 4 g + 3.
+    __device__ __forceinline__ void score(const u32x4 (&c)[T::NT], floatx4 (&sc)[NR]) {
+#pragma unroll
+        for (int i = 0; i < NR; i++) sc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < T::NU; u++) {
+            const bf16x8 k = T::frag(c, u);
+#pragma unroll
+            for (int t = 2; t >= 0; t--)
+#pragma unroll
+                for (int i = 0; i < NR; i++) sc[i] = mfma16x16x32(k, q[i][u][t], sc[i]);
+        }
+    }
+
+    // A tile's 32 keys from key0 on, scores in sc[j][i], V in LDS. seen: bit k
+    // for key k there; ksc / vsc: e4m3 scales of its keys (LDS); odd: V holds
+    // an infinity or NaN.
+    __device__ __forceinline__ void take(floatx4 (&sc)[2][NR], int key0, uint32_t seen, const float* ksc, const float* vsc,
+                                         const char* vt, bool odd) {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+        floatx4 ks[2], vs[2];
+        if constexpr (F8) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                ks[j] = *reinterpret_cast<const floatx4*>(ksc + 16 * j + 4 * g);
+                vs[j] = *reinterpret_cast<const floatx4*>(vsc + 16 * j + 4 * g);
+            }
+        }
+        const bool edge = key0 + 31 > first || seen != 0xffffffffu;  // some row does not see some key
+        bf16x8 p[NR][3];
+        float al[NR];
+        bool grew = false;
+#pragma unroll
+        for (int i = 0; i < NR; i++) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float s = sc[j][i][e];
+                    if constexpr (F8) s *= ks[j][e];
+                    if (edge) {
+                        const int k = 16 * j + 4 * g + e;
+                        s = (seen >> k & 1u) && key0 + k <= pos[i] ? s : -INFINITY;
+                    }
+                    sc[j][i][e] = s;
+                    top = fmaxf(top, s);
+                }
+            const float mn = fmaxf(m[i], col_max(top)), use = mn == -INFINITY ? 0.f : mn;
+            al[i] = __builtin_amdgcn_exp2f(m[i] - use);
+            grew |= mn != m[i];
+            m[i] = mn;
+            float w[8], sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float x = __builtin_amdgcn_exp2f(sc[j][i][e] - use);
+                    sum += x;
+                    if constexpr (F8) {
+                        x *= vs[j][e];
+                        // (a scale that is not finite, of a key that is not seen)
+                        if (edge) x = sc[j][i][e] == -INFINITY ? 0.f : x;
+                    }
+                    w[4 * j + e] = x;
+                }
+            l[i] = l[i] * al[i] + sum;
+            split3(w, p[i]);
+        }
+        if (__any(grew)) {
+#pragma unroll
+            for (int i = 0; i < NR; i++)
+#pragma unroll
+                for (int d = 0; d < HD / 16; d++) o[i][d] *= al[i];
+        }
+        if (odd) return weigh_odd(p, key0, seen, vt);
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++) {
+            const bf16x8 v = T::vfrag(vt, d, lane);
+#pragma unroll
+            for (int t = 2; t >= 0; t--)
+#pragma unroll
+                for (int i = 0; i < NR; i++) o[i][d] = mfma16x16x32(v, p[i][t], o[i][d]);
+        }
+    }
+
+    // The weighted sum where V holds infinities or NaN: those values count as
+    // zeros in the products (0 x inf of a key that a row does not see would be
+    // NaN) and are added to the rows that see them, told by the products of
+    // where they are with who sees what.
+    __device__ __forceinline__ void weigh_odd(const bf16x8 (&p)[NR][3], int key0, uint32_t seen, const char* vt) {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+#pragma unroll
+        for (int i = 0; i < NR; i++) {
+            uint32_t vis[4];
+            for (int w = 0; w < 4; w++) {
+                uint32_t b = 0;
+                for (int h = 0; h < 2; h++) {
+                    const int k = 16 * (w >> 1) + 4 * g + 2 * (w & 1) + h;
+                    if ((seen >> k & 1u) && key0 + k <= pos[i]) b |= 0x3f80u << (16 * h);
+                }
+                vis[w] = b;
+            }
+            const bf16x8 see = __builtin_bit_cast(bf16x8, vis);
+#pragma unroll
+            for (int d = 0; d < HD / 16; d++) {
+                const u32x4 v = __builtin_bit_cast(u32x4, T::vfrag(vt, d, lane));
+                u32x4 fine, up, down;
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    uint32_t keep = 0, pos1 = 0, neg1 = 0;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint32_t x = v[w] >> (16 * h) & 0xffffu, a = x & 0x7fffu;
+                        if (a < 0x7f80u) keep |= 0xffffu << (16 * h);
+                        if (a > 0x7f80u || x == 0x7f80u) pos1 |= 0x3f80u << (16 * h);
+                        if (a > 0x7f80u || x == 0xff80u) neg1 |= 0x3f80u << (16 * h);
+                    }
+                    fine[w] = v[w] & keep;
+                    up[w] = pos1;
+                    down[w] = neg1;
+                }
+                const floatx4 none = {0.f, 0.f, 0.f, 0.f};
+                const floatx4 cu = mfma16x16x32(__builtin_bit_cast(bf16x8, up), see, none);
+                const floatx4 cd = mfma16x16x32(__builtin_bit_cast(bf16x8, down), see, none);
+#pragma unroll
+                for (int t = 2; t >= 0; t--) o[i][d] = mfma16x16x32(__builtin_bit_cast(bf16x8, fine), p[i][t], o[i][d]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if (cu[e] > 0.f) o[i][d][e] += INFINITY;
+                    if (cd[e] > 0.f) o[i][d][e] -= INFINITY;
+                }
+            }
+        }
+    }
+};
+
+// Where tile `tile` of 16 * rows_per_tile/16 flattened rows (token, head of the
+// group) stands: the sequence and its first row. Tiles are numbered from
+// floor(first row * G / BM) + s for sequence s, which leaves room for a part
+// tile each.
+template <int BM>
+__device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int tile, SeqAt& s, int& r0) {
+    const int G = a.group.d;
+    if (!wave_seq(a.p, tile, [&](int i, int begin) { return begin * G / BM + i; }, s)) return false;
+    r0 = (tile - (s.begin * G / BM + s.s)) * BM;
+    const int rows = (s.end - s.begin) * G;
+    return r0 < rows && rows >= a.lo_rows && rows <= a.hi_rows;
+}
+
+// Finished (or, of a split, partial) sums of four columns of a row.
+__device__ __forceinline__ void put(const PagedAttnArgs& a, int split, size_t row, int c, floatx4 o, float l) {
+    if (a.splits == 1) {
+        const float r = l == 0.f ? 0.f : 1.0f / l;  // a row that sees nothing: zeros
+        *reinterpret_cast<floatx4*>(a.out + row * a.p.hd + c) = floatx4{o[0] * r, o[1] * r, o[2] * r, o[3] * r};
+    } else {
+        *reinterpret_cast<floatx4*>(a.part_o + ((size_t)split * a.p.tokens * a.hq + row) * a.p.hd + c) = o;
+    }
+}
+
+// Few rows: a block takes 16 rows of a sequence (with their KV head) and a
+// range of its keys, its four waves 32 keys each in turn. K goes from memory
+// to the operand registers, V through a wave's own LDS; while a tile is
+// weighed, the next one's rows are on their way.
+template <bool F8, int HD, bool PART>
+__global__ __launch_bounds__(256) void k_paged_attn_few(PagedAttnArgs a) {
+    using T = Tile<F8, HD>;
+    constexpr int OROW = HD + 4;
+    constexpr int STAGE = 4 * (T::BYTES + 256), JOIN = 4 * 16 * (OROW + 2) * 4;
+    __shared__ __align__(16) char lds[STAGE > JOIN ? STAGE : JOIN];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int kvh = blockIdx.x % a.p.num_kv, rest = blockIdx.x / a.p.num_kv;
+    const int tile = rest % a.tiles, split = rest / a.tiles;
+    SeqAt s;
+    int r0;
+    if (!find_tile<16>(a, tile, s, r0)) return;
+    Rows<F8, HD, 1> rows;
+    rows.template load<PART>(a, s, r0, kvh);
+    const int T1 = min(rows.last + 1, a.p.limit);
+    const int k0 = split * a.chunk, k1 = a.splits == 1 ? T1 : min(T1, k0 + a.chunk);
+    if (k0 >= k1 && split > 0) return;
+
+    char* vt = lds + wave * (T::BYTES + 256);
+    float* sc = reinterpret_cast<float*>(vt + T::BYTES);  // K scales of the 32 keys, then V's
+    u32x4 kc[2][T::NT], vc[2][T::NT];
+    float scale = 0.f;
+    uint32_t seen = 0;
+    // the pool row of key key0 + lane % 32
+    auto lookup = [&](int key0) -> long long {
+        const int key = key0 + (lane & 31);
+        return key < k1 ? pool_row(a.p, s.s, key, kvh) : -1;
+    };
+    auto fetch = [&](long long row) {
+        const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)row, (uint32_t)row, false, false);
+        const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(row >> 32), (uint32_t)(row >> 32), false, false);
+        seen = (uint32_t)__ballot(row >= 0);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const long long r = (long long)(((uint64_t)hi[j] << 32) | lo[j]);
+            fetch_row<F8, HD, PART>(a.p.k, r, a.p.hd, g, kc[j]);
+            fetch_row<F8, HD, PART>(a.p.v, r, a.p.hd, g, vc[j]);
+        }
+        if constexpr (F8) {
+            const float* from = lane < 32 ? a.p.ks : a.p.vs;
+            scale = *(row >= 0 ? from + row : reinterpret_cast<const float*>(kZeros));
+        }
+    };
+    int key0 = k0 + 32 * wave;
+    long long next = lookup(key0);
+    if (key0 < k1) fetch(next);
+    next = lookup(key0 + 128);
+    for (; key0 < k1; key0 += 128) {
+        floatx4 scores[2][1];
+        rows.score(kc[0], scores[0]);
+        rows.score(kc[1], scores[1]);
+        const bool odd = __any(any_nonfinite<F8>(vc[0]) || any_nonfinite<F8>(vc[1]));
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int t = 0; t < T::NT; t++) *reinterpret_cast<u32x4*>(vt + j * T::GROUP + t * 1024 + lane * 16) = vc[j][t];
+        if constexpr (F8) sc[lane] = scale;
+        const uint32_t here = seen;
+        if (key0 + 128 < k1) {
+            fetch(next);
+            next = lookup(key0 + 256);
+        }
+        rows.take(scores, key0, here, sc, sc + 32, vt, odd);
+    }
+    // the waves' sums, joined in wave order
+    __syncthreads();
+    float* jo = reinterpret_cast<float*>(lds);
+    float* jm = jo + 4 * 16 * OROW;
+    float* jl = jm + 64;
+    const float l = col_sum(rows.l[0]);
+#pragma unroll
+    for (int d = 0; d < HD / 16; d++)
+        *reinterpret_cast<floatx4*>(jo + (wave * 16 + (lane & 15)) * OROW + 16 * d + 4 * g) = rows.o[0][d];
+    if (g == 0) {
+        jm[wave * 16 + lane] = rows.m[0];
+        jl[wave * 16 + lane] = l;
+    }
+    __syncthreads();
+    const int G = a.group.d, n = s.end - s.begin;
+    for (int i = threadIdx.x; i < 16 * (HD / 4); i += 256) {
+        const int r = i / (HD / 4), c = 4 * (i % (HD / 4));
+        if (r0 + r >= n * G || (PART && c >= a.p.hd)) continue;
+        float M = jm[r];
+        for (int w = 1; w < 4; w++) M = fmaxf(M, jm[w * 16 + r]);
+        const float use = M == -INFINITY ? 0.f : M;
+        floatx4 o = {0.f, 0.f, 0.f, 0.f};
+        float L = 0.f;
+        for (int w = 0; w < 4; w++) {
+            const float f = __builtin_amdgcn_exp2f(jm[w * 16 + r] - use);
+            L += f * jl[w * 16 + r];
+            const floatx4 x = *reinterpret_cast<const floatx4*>(jo + (w * 16 + r) * OROW + c);
+            for (int e = 0; e < 4; e++) o[e] += jm[w * 16 + r] == -INFINITY ? 0.f : f * x[e];
+        }
+        const int tok = (int)a.group.div((uint32_t)(r0 + r));
+        const size_t row = (size_t)(s.begin + tok) * a.hq + kvh * G + (r0 + r - tok * G);
+        put(a, split, row, c, o, L);
+        if (a.splits > 1 && c == 0) a.part_ml[(size_t)split * a.p.tokens * a.hq + row] = make_float2(M, L);
+    }
+}
+
+// Many rows: a block takes 64 NR rows of a sequence, 16 NR a wave, and its keys
+// (or a range of them) in tiles of 32 that all four waves read from LDS; two
+// tiles in LDS, the one after in registers.
+template <bool F8, int HD, bool PART, int NR>
+__global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
+    using T = Tile<F8, HD>;
+    __shared__ __align__(16) char kt[2][T::BYTES], vt[2][T::BYTES];
+    __shared__ __align__(16) float sc[2][2][32];  // scales of K and of V
+    __shared__ uint32_t seen_of[2][2], odd_of[2][2];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int kvh = blockIdx.x % a.p.num_kv, rest = blockIdx.x / a.p.num_kv;
+    // the last rows of a sequence see the most keys: they go first
+    const int tile = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
+    SeqAt s;
+    int r0;
+    if (!find_tile<64 * NR>(a, tile, s, r0)) return;
+    const int G = a.group.d, n = s.end - s.begin;
+    Rows<F8, HD, NR> rows;
+    rows.template load<PART>(a, s, r0 + 16 * NR * wave, kvh);
+    // the last position that any of the block's rows sees
+    const int end_tok = (int)a.group.div((uint32_t)(min(r0 + 64 * NR, n * G) - 1));
+    const int T1 = min((a.causal ? s.len - n + end_tok : s.len - 1) + 1, a.p.limit);
+    const int k0 = split * a.chunk, k1 = a.splits == 1 ? T1 : min(T1, k0 + a.chunk);
+    if (k0 >= k1 && split > 0) return;
+
+    // waves 0 and 1 fetch K's two groups, 2 and 3 V's
+    const int j = wave & 1;
+    const bool isv = wave >= 2;
+    u32x4 st[T::NT];
+    float scale = 0.f;
+    long long row = -1;
+    auto lookup = [&](int key0) {
+        const int key = key0 + 16 * j + (lane & 15);
+        return key < k1 ? pool_row(a.p, s.s, key, kvh) : -1ll;
+    };
+    auto fetch = [&](long long r) {
+        row = r;
+        fetch_row<F8, HD, PART>(isv ? a.p.v : a.p.k, r, a.p.hd, g, st);
+        if constexpr (F8) scale = *(r >= 0 ? (isv ? a.p.vs : a.p.ks) + r : reinterpret_cast<const float*>(kZeros));
+    };
+    auto stage = [&](int b) {
+        char* to = (isv ? vt[b] : kt[b]) + j * T::GROUP + lane * 16;
+#pragma unroll
+        for (int t = 0; t < T::NT; t++) *reinterpret_cast<u32x4*>(to + t * 1024) = st[t];
+        if constexpr (F8)
+            if (lane < 16) sc[b][isv][16 * j + lane] = scale;
+        const uint32_t here = (uint32_t)__ballot(row >= 0) & 0xffffu;
+        const bool odd = __any(any_nonfinite<F8>(st));
+        if (lane == 0) {
+            if (isv) odd_of[b][j] = odd;
+            else seen_of[b][j] = here;
+        }
+    };
+    long long next = lookup(k0);
+    if (k0 < k1) {
+        fetch(next);
+        next = lookup(k0 + 32);
+        stage(0);
+    }
+    __syncthreads();
+    for (int key0 = k0, b = 0; key0 < k1; key0 += 32, b ^= 1) {
+        const bool more = key0 + 32 < k1;
+        if (more) {
+            fetch(next);
+            next = lookup(key0 + 64);
+        }
+        if (key0 <= rows.last) {
+            floatx4 scores[2][NR];
+#pragma unroll
+            for (int jj = 0; jj < 2; jj++) {
+                u32x4 c[T::NT];
+#pragma unroll
+                for (int t = 0; t < T::NT; t++)
+                    c[t] = *reinterpret_cast<const u32x4*>(kt[b] + jj * T::GROUP + t * 1024 + lane * 16);
+                rows.score(c, scores[jj]);
+            }
+            const uint32_t seen = seen_of[b][0] | (seen_of[b][1] << 16);
+            rows.take(scores, key0, seen, sc[b][0], sc[b][1], vt[b], (odd_of[b][0] | odd_of[b][1]) != 0);
+        }
+        if (more) stage(b ^ 1);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < NR; i++) {
+        const float l = col_sum(rows.l[i]);
+        const int r = r0 + 16 * (NR * wave + i) + (lane & 15);
+        if (r >= n * G) continue;
+        const int tok = (int)a.group.div((uint32_t)r);
+        const size_t at = (size_t)(s.begin + tok) * a.hq + kvh * G + (r - tok * G);
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++)
+            if (!PART || 16 * d < a.p.hd) put(a, split, at, 16 * d + 4 * g, rows.o[i][d], l);
+        if (a.splits > 1 && g == 0) a.part_ml[(size_t)split * a.p.tokens * a.hq + at] = make_float2(rows.m[i], l);
+    }
+}
+
+// A row's splits joined in their order, each weighted by 2^(its maximum - the
+// largest); a wave per (token, query head).
+__global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttnArgs a) {
+    const int lane = threadIdx.x & 63;
+    const long long row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    const long long total = (long long)a.p.tokens * a.hq;
+    if (row >= total) return;
+    const int t = (int)(row / a.hq);
+    SeqAt s;
+    if (!token_seq(a.p, t, s)) return;
+    const int n = s.end - s.begin;
+    const bool few = n * (int)a.group.d <= a.hi_rows;
+    const int chunk = few ? a.chunk : a.chunk2, splits = few ? a.splits : a.splits2;
+    if (splits == 1) return;
+    const int T = min(a.causal ? s.len - s.end + t + 1 : s.len, a.p.limit);
+    const int nc = min(max((T + chunk - 1) / chunk, 1), splits);
+    float M = -INFINITY;
+    for (int c = 0; c < nc; c++) M = fmaxf(M, a.part_ml[c * total + row].x);
+    const float use = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    floatx4 o = {0.f, 0.f, 0.f, 0.f};
+    const int col = 4 * lane;
+    for (int c = 0; c < nc; c++) {
+        const float2 ml = a.part_ml[c * total + row];
+        if (ml.x == -INFINITY) continue;
+        const float f = __builtin_amdgcn_exp2f(ml.x - use);
+        L += f * ml.y;
+        if (col < a.p.hd) {
+            const floatx4 x = *reinterpret_cast<const floatx4*>(a.part_o + (c * total + row) * a.p.hd + col);
+            for (int e = 0; e < 4; e++) o[e] += f * x[e];
+        }
+    }
+    if (col < a.p.hd) {
+        const float r = L == 0.f ? 0.f : 1.0f / L;
+        *reinterpret_cast<floatx4*>(a.out + row * a.p.hd + col) = floatx4{o[0] * r, o[1] * r, o[2] * r, o[3] * r};
+    }
+}
+
+// ---------------------------------------------------------------- launch
+
+struct AttnPlan {
+    bool few, many;
+    int few_tiles, many_tiles;
+    int few_chunk, few_splits, many_chunk, many_splits;
+    size_t bytes;
+};
+
+// Rows (tokens x heads of a group) up to which a sequence goes to the kernel
+// for few rows.
+constexpr int kFewRows = 32;
+
+static int many_rows(int hd) { return hd <= 128 ? 128 : 64; }
+
+static AttnPlan attn_plan(const PagedArgs& p, int hq, int max_new) {
+    AttnPlan r{};
+    const long long G = hq / p.num_kv;
+    const long long most = std::min<long long>(max_new > 0 ? max_new : p.tokens, p.tokens) * G;
+    r.few = most <= kFewRows || p.seqs > 1;
+    r.many = most > kFewRows;
+    const int bm = many_rows(p.hd);
+    r.few_tiles = (int)(p.tokens * G / 16) + p.seqs;
+    r.many_tiles = (int)(p.tokens * G / bm) + p.seqs;
+    // tiles that are expected to have work, and the splits of the longest
+    // sequence that fill the chip with them
+    const auto splits = [&](long long tiles, long long want, int unit, int& chunk) {
+        const long long blocks = std::max(1ll, tiles) * p.num_kv;
+        const long long units = std::max(1ll, ((long long)p.limit + unit - 1) / unit);
+        long long n = std::min(std::max(1ll, (want + blocks - 1) / blocks), units);
+        const long long per = (units + n - 1) / n;
+        chunk = (int)std::min<long long>(per * unit, 0x7fffff00);
+        return (int)((units + per - 1) / per);
+    };
+    const long long few_real = std::min<long long>(r.few_tiles, p.seqs * ((std::min<long long>(most, kFewRows) + 15) / 16));
+    const long long many_real = std::min<long long>(r.many_tiles, p.seqs * ((most + bm - 1) / bm));
+    r.few_splits = r.few ? splits(few_real, 2048, 256, r.few_chunk) : 1;
+    r.many_splits = r.many ? splits(many_real, 512, 256, r.many_chunk) : 1;
+    const int n = std::max(r.few_splits, r.many_splits);
+    if (n > 1) r.bytes = (size_t)n * p.tokens * hq * (p.hd * 4 + 8);
+    return r;
 }
 
 static int attn_args(const gorch_hip_paged_kv* kv, const gorch_hip_paged_batch* b, int num_q, PagedAttnArgs& a) {
     GH_TRY(paged_args("gorch_hip_paged_attention", kv, b, a.p));
     GH_REQUIRE(num_q > 0 && num_q % kv->num_kv == 0, "gorch/nn: GQA NumQ must be divisible by NumKV");
+    GH_SUPPORTED((long long)b->tokens * num_q < (1ll << 28) && (long long)b->seqs < (1ll << 28) / kv->num_kv,
+                 "gorch_hip_paged_attention: tokens * num_q must be below 2^28");
     a.hq = num_q;
-    a.scale = (float)(1.0 / sqrt((double)kv->head_dim));
+    a.scale = (float)(1.4426950408889634 / std::sqrt((double)kv->head_dim));
+    a.group.set((uint32_t)(num_q / kv->num_kv));
     return GORCH_HIP_OK;
+}
+
+template <bool F8, int HD, bool PART>
+static void launch_attn(hipStream_t s, const PagedAttnArgs& base, const AttnPlan& pl) {
+    if (pl.few) {
+        PagedAttnArgs a = base;
+        a.tiles = pl.few_tiles;
+        a.lo_rows = 0;
+        a.hi_rows = pl.many ? kFewRows : 0x7fffffff;
+        a.chunk = pl.few_chunk;
+        a.splits = pl.few_splits;
+        hipLaunchKernelGGL((k_paged_attn_few<F8, HD, PART>), dim3((unsigned)a.tiles * a.p.num_kv * a.splits), dim3(256), 0,
+                           s, a);
+    }
+    if (pl.many) {
+        PagedAttnArgs a = base;
+        a.tiles = pl.many_tiles;
+        a.lo_rows = pl.few ? kFewRows + 1 : 0;
+        a.hi_rows = 0x7fffffff;
+        a.chunk = pl.many_chunk;
+        a.splits = pl.many_splits;
+        constexpr int NR = HD <= 128 ? 2 : 1;
+        hipLaunchKernelGGL((k_paged_attn_many<F8, HD, PART, NR>), dim3((unsigned)a.tiles * a.p.num_kv * a.splits), dim3(256),
+                           0, s, a);
+    }
+}
+
+template <bool F8>
+static void launch_attn_hd(hipStream_t s, const PagedAttnArgs& a, const AttnPlan& pl) {
+    const int hd = a.p.hd;
+    if (hd == 64) launch_attn<F8, 64, false>(s, a, pl);
+    else if (hd < 64) launch_attn<F8, 64, true>(s, a, pl);
+    else if (hd == 128) launch_attn<F8, 128, false>(s, a, pl);
+    else if (hd < 128) launch_attn<F8, 128, true>(s, a, pl);
+    else if (hd == 256) launch_attn<F8, 256, false>(s, a, pl);
+    else launch_attn<F8, 256, true>(s, a, pl);
 }
 
 }  // namespace gh
@@ -78,7 +724,9 @@ using namespace gh;
 
 extern "C" size_t gorch_hip_paged_attention_workspace_size(const gorch_hip_paged_kv* kv, const gorch_hip_paged_batch* b,
                                                            int num_q) {
-    return 0;
+    PagedAttnArgs a{};
+    if (attn_args(kv, b, num_q, a) != GORCH_HIP_OK || b->tokens == 0 || b->seqs == 0) return 0;
+    return attn_plan(a.p, num_q, b->max_new).bytes;
 }
 
 extern "C" int gorch_hip_paged_attention(void* stream, const gorch_hip_paged_kv* kv, const gorch_hip_paged_batch* b,
@@ -88,17 +736,33 @@ extern "C" int gorch_hip_paged_attention(void* stream, const gorch_hip_paged_kv*
     GH_TRY(attn_args(kv, b, num_q, a));
     if (b->tokens == 0 || b->seqs == 0) return GORCH_HIP_OK;
     GH_REQUIRE(q && out, "gorch_hip_paged_attention: null q or out");
-    GH_SUPPORTED(reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0,
-                 "gorch_hip_paged_attention: q and out must be 16-byte aligned");
-    GH_TRY(bf16_gate(stream_of(stream)));
+    const AttnPlan pl = attn_plan(a.p, num_q, b->max_new);
+    GH_REQUIRE(workspace_bytes >= pl.bytes && (workspace || pl.bytes == 0),
+               "gorch_hip_paged_attention: workspace too small");
+    GH_SUPPORTED(reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
+                     reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+                 "gorch_hip_paged_attention: q, out and the workspace must be 16-byte aligned");
+    hipStream_t s = stream_of(stream);
+    GH_TRY(bf16_gate(s));
     a.q = q;
     a.out = out;
     a.causal = causal != 0;
-    GH_SUPPORTED(a.p.tokens <= 65535, "gorch_hip_paged_attention: too many tokens");
-    if (kv->dtype == GORCH_HIP_KV_E4M3)
-        hipLaunchKernelGGL(k_paged_attn_rows<true>, dim3(num_q, a.p.tokens), dim3(64), 0, stream_of(stream), a);
-    else
-        hipLaunchKernelGGL(k_paged_attn_rows<false>, dim3(num_q, a.p.tokens), dim3(64), 0, stream_of(stream), a);
+    const int splits = std::max(pl.few_splits, pl.many_splits);
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)splits * a.p.tokens * num_q * a.p.hd);
+    if (kv->dtype == GORCH_HIP_KV_E4M3) launch_attn_hd<true>(s, a, pl);
+    else launch_attn_hd<false>(s, a, pl);
+    GH_TRY(check_launch("paged_attention"));
+    if (splits > 1) {
+        a.hi_rows = pl.few ? (pl.many ? kFewRows : 0x7fffffff) : -1;
+        a.chunk = pl.few_chunk;
+        a.splits = pl.few_splits;
+        a.chunk2 = pl.many_chunk;
+        a.splits2 = pl.many_splits;
+        const long long rows = (long long)a.p.tokens * num_q;
+        hipLaunchKernelGGL(k_paged_attn_join, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+        GH_TRY(check_launch("paged_attention join"));
+    }
     count(CNT_ATTENTION);
-    return finish(stream, check_launch("paged_attention"));
+    return finish(stream, GORCH_HIP_OK);
 }
