@@ -140,7 +140,11 @@ struct Tile {
     }
 };
 
-// Whether a lane's chunks hold an infinity or NaN.
+// Infinities and NaN in V. Their product with the weight 0 of a key that a row
+// does not see is NaN, so a lane that finds some in its chunks of a tile turns
+// them into zeros and notes, for every row that sees the key, +inf and -inf
+// (NaN: both) for the column: bits [0 / 1][row][column] in LDS, added to the
+// sums at the end. All that an ordinary tile pays is the test.
 template <bool F8, int N>
 __device__ __forceinline__ bool any_nonfinite(const u32x4 (&c)[N]) {
     if constexpr (F8) {
@@ -159,6 +163,51 @@ __device__ __forceinline__ bool any_nonfinite(const u32x4 (&c)[N]) {
                 m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, c[i][e] & 0x7fff7fffu));
         return m[0] >= 0x7f80 || m[1] >= 0x7f80;
     }
+}
+template <int BM, int HD>
+struct OddBits {
+    uint32_t any, bits[2][BM][HD / 32];
+};
+// A lane's chunks of key `key` in LDS (mine, 1 KB apart); the block's rows are
+// r0 .. r0 + BM - 1 of sequence s.
+template <bool F8, int BM, int HD>
+__device__ __forceinline__ void clean_odd(OddBits<BM, HD>& odd, const PagedAttnArgs& a, const SeqAt& s, int r0, int key,
+                                          int g, char* mine) {
+    constexpr int PER = F8 ? 16 : 8;
+    const int G = a.group.d, n = s.end - s.begin;
+#pragma unroll 1
+    for (int i = 0; i < Tile<F8, HD>::NT * PER; i++) {
+        const int t = i / PER, e = i % PER, col = (4 * t + g) * PER + e;
+        bool up, down;
+        if constexpr (F8) {  // no infinities, NaN is 0x7f
+            uint8_t* x = reinterpret_cast<uint8_t*>(mine + t * 1024) + e;
+            up = down = (*x & 0x7f) == 0x7f;
+            if (up) *x = 0;
+        } else {
+            uint16_t* x = reinterpret_cast<uint16_t*>(mine + t * 1024) + e;
+            const int v = *x, m = v & 0x7fff;
+            up = m > 0x7f80 || v == 0x7f80;
+            down = m > 0x7f80 || v == 0xff80;
+            if (up || down) *x = 0;
+        }
+        if (!up && !down) continue;
+        odd.any = 1;
+#pragma unroll 1
+        for (int r = 0; r < BM && r0 + r < n * G; r++) {
+            const int pos = a.causal ? s.len - n + (int)a.group.div((uint32_t)(r0 + r)) : s.len - 1;
+            if (key > pos) continue;
+            if (up) atomicOr(&odd.bits[0][r][col / 32], 1u << (col % 32));
+            if (down) atomicOr(&odd.bits[1][r][col / 32], 1u << (col % 32));
+        }
+    }
+}
+template <int BM, int HD>
+__device__ __forceinline__ floatx4 add_odd(const OddBits<BM, HD>& odd, int r, int c, floatx4 o) {
+    for (int e = 0; e < 4; e++) {
+        if (odd.bits[0][r][c / 32] >> (c % 32 + e) & 1u) o[e] += INFINITY;
+        if (odd.bits[1][r][c / 32] >> (c % 32 + e) & 1u) o[e] -= INFINITY;
+    }
+    return o;
 }
 
 // A lane's fetch of one key row: its chunks, zeros where there is no row or
@@ -245,10 +294,9 @@ struct Rows {
     }
 
     // A tile's 32 keys from key0 on, scores in sc[j][i], V in LDS. seen: bit k
-    // for key k there; ksc / vsc: e4m3 scales of its keys (LDS); odd: V holds
-    // an infinity or NaN.
+    // for key k there; ksc / vsc: e4m3 scales of its keys (LDS).
     __device__ __forceinline__ void take(floatx4 (&sc)[2][NR], int key0, uint32_t seen, const float* ksc, const float* vsc,
-                                         const char* vt, bool odd) {
+                                         const char* vt) {
         const int lane = threadIdx.x & 63, g = lane >> 4;
         floatx4 ks[2], vs[2];
         if constexpr (F8) {
@@ -305,7 +353,6 @@ struct Rows {
 #pragma unroll
                 for (int d = 0; d < HD / 16; d++) o[i][d] *= al[i];
         }
-        if (odd) return weigh_odd(p, key0, seen, vt);
 #pragma unroll
         for (int d = 0; d < HD / 16; d++) {
             const bf16x8 v = T::vfrag(vt, d, lane);
@@ -313,56 +360,6 @@ struct Rows {
             for (int t = 2; t >= 0; t--)
 #pragma unroll
                 for (int i = 0; i < NR; i++) o[i][d] = mfma16x16x32(v, p[i][t], o[i][d]);
-        }
-    }
-
-    // The weighted sum where V holds infinities or NaN: those values count as
-    // zeros in the products (0 x inf of a key that a row does not see would be
-    // NaN) and are added to the rows that see them, told by the products of
-    // where they are with who sees what.
-    __device__ __forceinline__ void weigh_odd(const bf16x8 (&p)[NR][3], int key0, uint32_t seen, const char* vt) {
-        const int lane = threadIdx.x & 63, g = lane >> 4;
-#pragma unroll
-        for (int i = 0; i < NR; i++) {
-            uint32_t vis[4];
-            for (int w = 0; w < 4; w++) {
-                uint32_t b = 0;
-                for (int h = 0; h < 2; h++) {
-                    const int k = 16 * (w >> 1) + 4 * g + 2 * (w & 1) + h;
-                    if ((seen >> k & 1u) && key0 + k <= pos[i]) b |= 0x3f80u << (16 * h);
-                }
-                vis[w] = b;
-            }
-            const bf16x8 see = __builtin_bit_cast(bf16x8, vis);
-#pragma unroll
-            for (int d = 0; d < HD / 16; d++) {
-                const u32x4 v = __builtin_bit_cast(u32x4, T::vfrag(vt, d, lane));
-                u32x4 fine, up, down;
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    uint32_t keep = 0, pos1 = 0, neg1 = 0;
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint32_t x = v[w] >> (16 * h) & 0xffffu, a = x & 0x7fffu;
-                        if (a < 0x7f80u) keep |= 0xffffu << (16 * h);
-                        if (a > 0x7f80u || x == 0x7f80u) pos1 |= 0x3f80u << (16 * h);
-                        if (a > 0x7f80u || x == 0xff80u) neg1 |= 0x3f80u << (16 * h);
-                    }
-                    fine[w] = v[w] & keep;
-                    up[w] = pos1;
-                    down[w] = neg1;
-                }
-                const floatx4 none = {0.f, 0.f, 0.f, 0.f};
-                const floatx4 cu = mfma16x16x32(__builtin_bit_cast(bf16x8, up), see, none);
-                const floatx4 cd = mfma16x16x32(__builtin_bit_cast(bf16x8, down), see, none);
-#pragma unroll
-                for (int t = 2; t >= 0; t--) o[i][d] = mfma16x16x32(__builtin_bit_cast(bf16x8, fine), p[i][t], o[i][d]);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if (cu[e] > 0.f) o[i][d][e] += INFINITY;
-                    if (cd[e] > 0.f) o[i][d][e] -= INFINITY;
-                }
-            }
         }
     }
 };
@@ -395,11 +392,12 @@ __device__ __forceinline__ void put(const PagedAttnArgs& a, int split, size_t ro
 // to the operand registers, V through a wave's own LDS; while a tile is
 // weighed, the next one's rows are on their way.
 template <bool F8, int HD, bool PART>
-__global__ __launch_bounds__(256) void k_paged_attn_few(PagedAttnArgs a) {
+__global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void k_paged_attn_few(PagedAttnArgs a) {
     using T = Tile<F8, HD>;
     constexpr int OROW = HD + 4;
     constexpr int STAGE = 4 * (T::BYTES + 256), JOIN = 4 * 16 * (OROW + 2) * 4;
     __shared__ __align__(16) char lds[STAGE > JOIN ? STAGE : JOIN];
+    __shared__ OddBits<16, HD> odd;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
     const int kvh = blockIdx.x % a.p.num_kv, rest = blockIdx.x / a.p.num_kv;
     const int tile = rest % a.tiles, split = rest / a.tiles;
@@ -437,6 +435,8 @@ __global__ __launch_bounds__(256) void k_paged_attn_few(PagedAttnArgs a) {
             scale = *(row >= 0 ? from + row : reinterpret_cast<const float*>(kZeros));
         }
     };
+    for (int i = threadIdx.x; i < (int)(sizeof(odd) / 4); i += 256) reinterpret_cast<uint32_t*>(&odd)[i] = 0;
+    __syncthreads();
     int key0 = k0 + 32 * wave;
     long long next = lookup(key0);
     if (key0 < k1) fetch(next);
@@ -445,18 +445,21 @@ __global__ __launch_bounds__(256) void k_paged_attn_few(PagedAttnArgs a) {
         floatx4 scores[2][1];
         rows.score(kc[0], scores[0]);
         rows.score(kc[1], scores[1]);
-        const bool odd = __any(any_nonfinite<F8>(vc[0]) || any_nonfinite<F8>(vc[1]));
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
             for (int t = 0; t < T::NT; t++) *reinterpret_cast<u32x4*>(vt + j * T::GROUP + t * 1024 + lane * 16) = vc[j][t];
+        if (__any(any_nonfinite<F8>(vc[0]) || any_nonfinite<F8>(vc[1])))
+#pragma unroll 1
+            for (int j = 0; j < 2; j++)
+                clean_odd<F8, 16, HD>(odd, a, s, r0, key0 + 16 * j + (lane & 15), g, vt + j * T::GROUP + lane * 16);
         if constexpr (F8) sc[lane] = scale;
         const uint32_t here = seen;
         if (key0 + 128 < k1) {
             fetch(next);
             next = lookup(key0 + 256);
         }
-        rows.take(scores, key0, here, sc, sc + 32, vt, odd);
+        rows.take(scores, key0, here, sc, sc + 32, vt);
     }
     // the waves' sums, joined in wave order
     __syncthreads();
@@ -487,6 +490,7 @@ __global__ __launch_bounds__(256) void k_paged_attn_few(PagedAttnArgs a) {
             const floatx4 x = *reinterpret_cast<const floatx4*>(jo + (w * 16 + r) * OROW + c);
             for (int e = 0; e < 4; e++) o[e] += jm[w * 16 + r] == -INFINITY ? 0.f : f * x[e];
         }
+        if (odd.any) o = add_odd(odd, r, c, o);
         const int tok = (int)a.group.div((uint32_t)(r0 + r));
         const size_t row = (size_t)(s.begin + tok) * a.hq + kvh * G + (r0 + r - tok * G);
         put(a, split, row, c, o, L);
@@ -502,7 +506,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
     using T = Tile<F8, HD>;
     __shared__ __align__(16) char kt[2][T::BYTES], vt[2][T::BYTES];
     __shared__ __align__(16) float sc[2][2][32];  // scales of K and of V
-    __shared__ uint32_t seen_of[2][2], odd_of[2][2];
+    __shared__ uint32_t seen_of[2][2];
+    __shared__ OddBits<64 * NR, HD> odd;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
     const int kvh = blockIdx.x % a.p.num_kv, rest = blockIdx.x / a.p.num_kv;
     // the last rows of a sequence see the most keys: they go first
@@ -529,8 +534,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
         const int key = key0 + 16 * j + (lane & 15);
         return key < k1 ? pool_row(a.p, s.s, key, kvh) : -1ll;
     };
-    auto fetch = [&](long long r) {
+    int at0 = 0;
+    auto fetch = [&](long long r, int key0) {
         row = r;
+        at0 = key0;
         fetch_row<F8, HD, PART>(isv ? a.p.v : a.p.k, r, a.p.hd, g, st);
         if constexpr (F8) scale = *(r >= 0 ? (isv ? a.p.vs : a.p.ks) + r : reinterpret_cast<const float*>(kZeros));
     };
@@ -538,18 +545,18 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
         char* to = (isv ? vt[b] : kt[b]) + j * T::GROUP + lane * 16;
 #pragma unroll
         for (int t = 0; t < T::NT; t++) *reinterpret_cast<u32x4*>(to + t * 1024) = st[t];
+        if (isv && __any(any_nonfinite<F8>(st)))
+            clean_odd<F8, 64 * NR, HD>(odd, a, s, r0, at0 + 16 * j + (lane & 15), g, to);
         if constexpr (F8)
             if (lane < 16) sc[b][isv][16 * j + lane] = scale;
         const uint32_t here = (uint32_t)__ballot(row >= 0) & 0xffffu;
-        const bool odd = __any(any_nonfinite<F8>(st));
-        if (lane == 0) {
-            if (isv) odd_of[b][j] = odd;
-            else seen_of[b][j] = here;
-        }
+        if (lane == 0 && !isv) seen_of[b][j] = here;
     };
+    for (int i = threadIdx.x; i < (int)(sizeof(odd) / 4); i += 256) reinterpret_cast<uint32_t*>(&odd)[i] = 0;
+    __syncthreads();
     long long next = lookup(k0);
     if (k0 < k1) {
-        fetch(next);
+        fetch(next, k0);
         next = lookup(k0 + 32);
         stage(0);
     }
@@ -557,7 +564,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
     for (int key0 = k0, b = 0; key0 < k1; key0 += 32, b ^= 1) {
         const bool more = key0 + 32 < k1;
         if (more) {
-            fetch(next);
+            fetch(next, key0 + 32);
             next = lookup(key0 + 64);
         }
         if (key0 <= rows.last) {
@@ -571,7 +578,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
                 rows.score(c, scores[jj]);
             }
             const uint32_t seen = seen_of[b][0] | (seen_of[b][1] << 16);
-            rows.take(scores, key0, seen, sc[b][0], sc[b][1], vt[b], (odd_of[b][0] | odd_of[b][1]) != 0);
+            rows.take(scores, key0, seen, sc[b][0], sc[b][1], vt[b]);
         }
         if (more) stage(b ^ 1);
         __syncthreads();
@@ -585,7 +592,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
         const size_t at = (size_t)(s.begin + tok) * a.hq + kvh * G + (r - tok * G);
 #pragma unroll
         for (int d = 0; d < HD / 16; d++)
-            if (!PART || 16 * d < a.p.hd) put(a, split, at, 16 * d + 4 * g, rows.o[i][d], l);
+            if (!PART || 16 * d < a.p.hd) {
+                const int c = 16 * d + 4 * g;
+                put(a, split, at, c, odd.any ? add_odd(odd, r - r0, c, rows.o[i][d]) : rows.o[i][d], l);
+            }
         if (a.splits > 1 && g == 0) a.part_ml[(size_t)split * a.p.tokens * a.hq + at] = make_float2(rows.m[i], l);
     }
 }
