@@ -5,8 +5,10 @@
 //
 // A block takes a slice of one row's vocabulary: it counts the row's history
 // tokens of that slice in LDS (integers, so any order gives the same counts),
-// notes the last bias entry of each, and streams the slice's logits through
-// the rules. Every block of a row reads the whole history (from L2).
+// notes the last bias entry of each, and takes the slice's logits through the
+// rules. Every block of a row reads the whole history (from L2). Bound by
+// memory: the logits and the mask go out first and arrive while the notes are
+// taken.
 #include "common.h"
 
 namespace gh {
@@ -15,54 +17,121 @@ struct LogitsArgs {
     gorch_hip_logits_rules r;
     const float* x;
     float* out;
-    int n, slice;
+    int n, wide_history;
 };
 
 constexpr uint32_t kInPrompt = 0x80000000u;  // beside the count of tokens after the prompt
 
-// note: per token of the slice, kInPrompt | count after the prompt; last: the
-// last bias entry + 1
+// A thread takes U groups of four tokens. Slices start where x is 16-byte
+// aligned, up to three tokens before a multiple of their size, so rows of any
+// length move in 16-byte pieces; SAME: out is aligned as x is (else it is
+// stored token by token).
+template <int U, bool SAME>
 __global__ __launch_bounds__(256) void k_process_logits(LogitsArgs a) {
-    extern __shared__ uint32_t note[];
-    const int row = blockIdx.y, lo = blockIdx.x * a.slice, n = min(a.slice, a.n - lo);
+    constexpr int SLICE = 1024 * U;
+    extern __shared__ __align__(16) uint32_t note[];  // per token: kInPrompt | count after the prompt
     const gorch_hip_logits_rules& r = a.r;
-    uint32_t* last = note + (r.history ? a.slice : 0);
-    if (r.history)
-        for (int i = threadIdx.x; i < n; i += 256) note[i] = 0;
-    if (r.bias)
-        for (int i = threadIdx.x; i < n; i += 256) last[i] = 0;
-    __syncthreads();
-    if (r.history) {
-        const int len = r.history_lens ? min(max(r.history_lens[row], 0), r.history_stride) : r.history_stride;
-        const int prompt = r.prompt_lens ? r.prompt_lens[row] : 0;
-        const int* h = r.history + (size_t)row * r.history_stride;
-        for (int i = threadIdx.x; i < len; i += 256) {
-            const int id = h[i] - lo;
-            if ((unsigned)id >= (unsigned)n) continue;
-            if (i < prompt) atomicOr(&note[id], kInPrompt);
-            else atomicAdd(&note[id], 1u);
+    uint32_t* last = note + (r.history ? SLICE : 0);  // per token: last bias entry + 1
+    const int row = blockIdx.y, tid = threadIdx.x;
+    const float* x = a.x + (size_t)row * a.n;
+    float* out = a.out + (size_t)row * a.n;
+    const int lo = (int)blockIdx.x * SLICE - (int)(reinterpret_cast<uintptr_t>(x) / 4 % 4);
+    float4 v[U];
+    uint32_t ok[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int t = lo + 4 * (u * 256 + tid);
+        if (t >= 0 && t + 4 <= a.n) {
+            v[u] = *reinterpret_cast<const float4*>(x + t);
+        } else {
+            v[u].x = t >= 0 && t < a.n ? x[t] : 0.f;
+            v[u].y = t + 1 >= 0 && t + 1 < a.n ? x[t + 1] : 0.f;
+            v[u].z = t + 2 >= 0 && t + 2 < a.n ? x[t + 2] : 0.f;
+            v[u].w = t + 3 >= 0 && t + 3 < a.n ? x[t + 3] : 0.f;
+        }
+        ok[u] = 15u;
+        if (r.allowed) {
+            // bits of tokens t .. t + 3 (those before the row or past it are never stored)
+            const uint32_t* m = r.allowed + (size_t)row * r.allowed_stride;
+            const int w0 = min(max(t, 0), a.n - 1) / 32, w1 = min(max(t + 3, 0), a.n - 1) / 32;
+            const uint64_t bits = m[w0] | ((uint64_t)m[w1] << 32);
+            ok[u] = t >= 0 ? (uint32_t)(bits >> (t % 32)) : (uint32_t)(bits << -t);
         }
     }
-    if (r.bias) {
-        const int b0 = min(max(r.bias_rows[row], 0), r.biases), b1 = min(max(r.bias_rows[row + 1], b0), r.biases);
-        for (int i = b0 + threadIdx.x; i < b1; i += 256) {
-            const int id = r.bias_ids[i] - lo;
-            if ((unsigned)id < (unsigned)n) atomicMax(&last[id], (uint32_t)i + 1);
+    if (r.history || r.bias) {
+        const uint4 none = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (r.history) reinterpret_cast<uint4*>(note)[u * 256 + tid] = none;
+            if (r.bias) reinterpret_cast<uint4*>(last)[u * 256 + tid] = none;
         }
+        __syncthreads();
+        if (r.history) {
+            const int len = r.history_lens ? min(max(r.history_lens[row], 0), r.history_stride) : r.history_stride;
+            const int prompt = r.prompt_lens ? r.prompt_lens[row] : 0;
+            const int* h = r.history + (size_t)row * r.history_stride;
+            auto take = [&](int i, int id) {
+                const unsigned at = (unsigned)(id - lo);
+                if (i >= len || at >= (unsigned)SLICE || (unsigned)id >= (unsigned)a.n) return;
+                if (i < prompt) atomicOr(&note[at], kInPrompt);
+                else atomicAdd(&note[at], 1u);
+            };
+            if (a.wide_history) {
+                for (int i = 4 * tid; i < len; i += 1024) {
+                    const int4 id = *reinterpret_cast<const int4*>(h + i);
+                    take(i, id.x);
+                    take(i + 1, id.y);
+                    take(i + 2, id.z);
+                    take(i + 3, id.w);
+                }
+            } else {
+                for (int i = tid; i < len; i += 256) take(i, h[i]);
+            }
+        }
+        if (r.bias) {
+            const int b0 = min(max(r.bias_rows[row], 0), r.biases), b1 = min(max(r.bias_rows[row + 1], b0), r.biases);
+            for (int i = b0 + tid; i < b1; i += 256) {
+                const int id = r.bias_ids[i];
+                const unsigned at = (unsigned)(id - lo);
+                if (at < (unsigned)SLICE && (unsigned)id < (unsigned)a.n) atomicMax(&last[at], (uint32_t)i + 1);
+            }
+        }
+        __syncthreads();
     }
-    __syncthreads();
     const float rep = r.repetition ? r.repetition[row] : 1.f, fr = r.frequency ? r.frequency[row] : 0.f,
                 pr = r.presence ? r.presence[row] : 0.f;
-    for (int i = threadIdx.x; i < n; i += 256) {
-        float x = a.x[(size_t)row * a.n + lo + i];
-        if (r.history && note[i]) {
-            const uint32_t c = note[i] & ~kInPrompt;
-            if (r.repetition) x = x > 0.f ? x / rep : x * rep;
-            if (c) x = x - fr * (float)c - pr;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int t = lo + 4 * (u * 256 + tid);
+        float e[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+        if (r.history) {
+            const uint4 w = reinterpret_cast<const uint4*>(note)[u * 256 + tid];
+            const uint32_t c[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (c[i] == 0) continue;
+                const uint32_t k = c[i] & ~kInPrompt;
+                if (r.repetition) e[i] = e[i] > 0.f ? e[i] / rep : e[i] * rep;
+                if (k) e[i] = e[i] - fr * (float)k - pr;
+            }
         }
-        if (r.bias && last[i]) x += r.bias[last[i] - 1];
-        if (r.allowed && !(r.allowed[(size_t)row * r.allowed_stride + (lo + i) / 32] >> ((lo + i) % 32) & 1u)) x = -INFINITY;
-        a.out[(size_t)row * a.n + lo + i] = x;
+        if (r.bias) {
+            const uint4 w = reinterpret_cast<const uint4*>(last)[u * 256 + tid];
+            const uint32_t c[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (c[i]) e[i] += r.bias[c[i] - 1];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (!(ok[u] >> i & 1u)) e[i] = -INFINITY;
+        if (SAME && t >= 0 && t + 4 <= a.n) {
+            *reinterpret_cast<float4*>(out + t) = make_float4(e[0], e[1], e[2], e[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (t + i >= 0 && t + i < a.n) out[t + i] = e[i];
+        }
     }
 }
 
@@ -81,10 +150,26 @@ extern "C" int gorch_hip_process_logits(void* stream, const gorch_hip_logits_rul
     GH_SUPPORTED(rows <= 65535, "gorch_hip_process_logits: more than 65535 rows");
     if (rows == 0 || n == 0) return GORCH_HIP_OK;
     GH_REQUIRE(logits && out, "gorch_hip_process_logits: null logits or out");
-    LogitsArgs a{*r, logits, out, n, 4096};
+    GH_SUPPORTED(reinterpret_cast<uintptr_t>(logits) % 4 == 0 && n < 0x7fff0000,
+                 "gorch_hip_process_logits: logits must be 4-byte aligned, n below 2^31 - 2^16");
+    LogitsArgs a{*r, logits, out, n, 0};
     if (r->biases == 0) a.r.bias = nullptr;
-    const size_t lds = (size_t)((a.r.history ? 1 : 0) + (a.r.bias ? 1 : 0)) * a.slice * 4;
-    hipLaunchKernelGGL(k_process_logits, dim3((n + a.slice - 1) / a.slice, rows), dim3(256), lds, stream_of(stream), a);
+    a.wide_history = reinterpret_cast<uintptr_t>(r->history) % 16 == 0 && r->history_stride % 4 == 0;
+    const bool same = (reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(out)) % 16 == 0;
+    const int words = (a.r.history ? 1 : 0) + (a.r.bias ? 1 : 0);
+    const auto go = [&](auto kernel, int slice) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(((long long)n + 3 + slice - 1) / slice), rows), dim3(256),
+                           (size_t)words * slice * 4, stream_of(stream), a);
+    };
+    // few rows: slices of 1024 tokens, so that more CUs share the latency;
+    // many: of 4096, so that fewer blocks read a row's history
+    if ((long long)rows * n < 512 * 4096ll) {
+        if (same) go(k_process_logits<1, true>, 1024);
+        else go(k_process_logits<1, false>, 1024);
+    } else {
+        if (same) go(k_process_logits<4, true>, 4096);
+        else go(k_process_logits<4, false>, 4096);
+    }
     count(CNT_ELEMENTWISE);
     return finish(stream, check_launch("process_logits"));
 }

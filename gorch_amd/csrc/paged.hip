@@ -48,17 +48,50 @@ int paged_args(const char* who, const gorch_hip_paged_kv* kv, const gorch_hip_pa
     return GORCH_HIP_OK;
 }
 
-// Sums and maxima over the NL lanes of a row (NL a power of two).
+// v of the lane M lanes away within a row's lanes (lane ^ M; M = 8, 16, 32),
+// on the vector unit's lane network.
+template <int M>
+__device__ __forceinline__ float across(float v) {
+    if constexpr (M == 8) {
+        return dpp_f<0x128>(v);  // 16 lanes rotated by 8
+    } else {
+        const uint32_t u = __float_as_uint(v);
+        const bool odd = (threadIdx.x & M) != 0;
+        if constexpr (M == 16) {
+            const auto w = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+            return __uint_as_float(odd ? w[0] : w[1]);
+        } else {
+            const auto w = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+            return __uint_as_float(odd ? w[0] : w[1]);
+        }
+    }
+}
+template <int M>
+__device__ __forceinline__ double across_d(double v) {
+    const unsigned long long b = (unsigned long long)__double_as_longlong(v);
+    const uint32_t lo = __float_as_uint(across<M>(__uint_as_float((uint32_t)b))),
+                   hi = __float_as_uint(across<M>(__uint_as_float((uint32_t)(b >> 32))));
+    return __longlong_as_double((long long)(((unsigned long long)hi << 32) | lo));
+}
+// Sums and maxima over the NL lanes of a row (NL = 16, 32 or 64).
 template <int NL>
 __device__ __forceinline__ double row_sum_d(double v) {
-#pragma unroll
-    for (int m = 1; m < NL; m *= 2) v += __shfl_xor(v, m);
+    v += dpp_d<kDppQuadSwap1>(v);
+    v += dpp_d<kDppQuadSwap2>(v);
+    v += dpp_d<kDppRowHalfMirror>(v);
+    v += dpp_d<kDppRowMirror>(v);
+    if constexpr (NL >= 32) v += across_d<16>(v);
+    if constexpr (NL >= 64) v += across_d<32>(v);
     return v;
 }
 template <int NL>
 __device__ __forceinline__ float row_max_f(float v) {
-#pragma unroll
-    for (int m = 1; m < NL; m *= 2) v = fmaxf(v, __shfl_xor(v, m));
+    v = fmaxf(v, dpp_f<kDppQuadSwap1>(v));
+    v = fmaxf(v, dpp_f<kDppQuadSwap2>(v));
+    v = fmaxf(v, dpp_f<kDppRowHalfMirror>(v));
+    v = fmaxf(v, dpp_f<kDppRowMirror>(v));
+    if constexpr (NL >= 32) v = fmaxf(v, across<16>(v));
+    if constexpr (NL >= 64) v = fmaxf(v, across<32>(v));
     return v;
 }
 
@@ -104,98 +137,169 @@ struct AppendArgs {
 };
 
 // One token's rows: q heads, then k heads, then v heads, NL lanes a row of hd
-// floats (lane c < hd / 4 holds elements 4c .. 4c + 3), a wave one row of
-// lanes at a time. Same operations per row, in the same order, as
+// floats (lane c < hd / 4 holds elements 4c .. 4c + 3; FULL: hd = 4 NL), P
+// rows per group of lanes. Same operations per row, in the same order, as
 // k_norm_rope_rows: x * inv * gain with inv from the f64 sum of squares, then
 // the pair rotated with every product and sum rounded on its own.
-template <bool F8, int NL>
+// Bound by memory: the rows go out before anything else, and the chain
+// sequence -> page -> store runs beside them.
+template <bool F8, int NL, bool FULL, int P>
 __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
 #pragma clang fp contract(off)
     constexpr int RPB = 256 / NL;
-    const int t = blockIdx.x, hd = a.p.hd, half = hd / 2, nl = hd / 4;
-    const int c = threadIdx.x % NL, r = blockIdx.y * RPB + threadIdx.x / NL;
+    const int t = blockIdx.x, hd = FULL ? 4 * NL : a.p.hd, half = hd / 2, nl = hd / 4;
+    const int c = threadIdx.x % NL, r0 = blockIdx.y * RPB * P + threadIdx.x / NL;
+    const int nkv = a.p.num_kv, rows = a.hq + 2 * nkv;
+    const bool lane_in = FULL || c < nl;
+    float4 x[P], g[P];
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+        const int r = min(r0 + i * RPB, rows - 1);
+        const bool isq = r < a.hq, isk = !isq && r < a.hq + nkv;
+        const int h = isq ? r : (isk ? r - a.hq : r - a.hq - nkv);
+        const float* src = isq ? a.q + t * a.qs : (isk ? a.k + t * a.ks : a.v + t * a.vs);
+        x[i] = lane_in ? *reinterpret_cast<const float4*>(src + (size_t)h * hd + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
     SeqAt sq;
     if (!token_seq(a.p, t, sq)) return;
     const int s = sq.s, pos = sq.len - sq.end + t;
-    if (pos < 0 || (a.cosT && pos >= a.rope_rows) || pool_row(a.p, s, pos, 0) < 0) return;
-    const int nkv = a.p.num_kv, rows = a.hq + 2 * nkv;
-    const bool live = r < rows, mine = live && c < nl;
-    const bool isq = r < a.hq, isk = !isq && r < a.hq + nkv;
-    const int h = isq ? r : (isk ? r - a.hq : r - a.hq - nkv);
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), g = make_float4(1.f, 1.f, 1.f, 1.f);
-    const float* src = isq ? a.q + t * a.qs : (isk ? a.k + t * a.ks : a.v + t * a.vs);
-    if (mine) x = *reinterpret_cast<const float4*>(src + (size_t)h * hd + 4 * c);
-    const float* gain = isq ? a.gq : (isk ? a.gk : nullptr);
-    const double ss = row_sum_d<NL>(((double)x.x * (double)x.x + (double)x.y * (double)x.y) +
-                                    ((double)x.z * (double)x.z + (double)x.w * (double)x.w));
-    if (gain && mine) {
-        g = make_float4(gain[4 * c], gain[4 * c + 1], gain[4 * c + 2], gain[4 * c + 3]);
-        const float inv = (float)rsqrt_f64(div_rcp(ss, (double)hd, 1.0 / hd) + (double)a.eps);
-        x = make_float4(x.x * inv * g.x, x.y * inv * g.y, x.z * inv * g.z, x.w * inv * g.w);
-    }
+    if (pos < 0 || (a.cosT && pos >= a.rope_rows)) return;
+    const long long row0 = pool_row(a.p, s, pos, 0);
+    if (row0 < 0) return;
+    float co[4], sn[4];
+    const bool lo = c < nl / 2;
     if (a.cosT) {
-        const bool lo = c < nl / 2;
-        const int lane = threadIdx.x & 63, other = lo ? lane + nl / 2 : lane - nl / 2;
-        const float e[4] = {x.x, x.y, x.z, x.w};
-        float o[4];
-        for (int i = 0; i < 4; i++) {
-            const float p = __shfl(e[a.neox ? i ^ 1 : i], a.neox ? lane : other);
-            const int at = a.neox ? 2 * c + i / 2 : (lo ? 4 * c + i : 4 * c + i - half);
-            const bool first = a.neox ? (i & 1) == 0 : lo;
-            float co = 1.f, si = 0.f;
-            if (mine) {
-                co = a.cosT[(size_t)pos * half + at];
-                si = a.sinT[(size_t)pos * half + at];
-            }
-            o[i] = first ? e[i] * co - p * si : p * si + e[i] * co;
+        // elements 4c .. 4c + 3 turn by angles 4c mod half .. (neox: 2c, 2c, 2c + 1, 2c + 1)
+        const size_t at = (size_t)pos * half + (a.neox ? 2 * c : (lo ? 4 * c : 4 * c - half));
+        if (!lane_in) {
+            for (int i = 0; i < 4; i++) co[i] = sn[i] = 0.f;
+        } else if (a.neox) {
+            const float2 cc = *reinterpret_cast<const float2*>(a.cosT + at), ss = *reinterpret_cast<const float2*>(a.sinT + at);
+            co[0] = co[1] = cc.x;
+            co[2] = co[3] = cc.y;
+            sn[0] = sn[1] = ss.x;
+            sn[2] = sn[3] = ss.y;
+        } else {
+            const float4 cc = *reinterpret_cast<const float4*>(a.cosT + at), ss = *reinterpret_cast<const float4*>(a.sinT + at);
+            co[0] = cc.x, co[1] = cc.y, co[2] = cc.z, co[3] = cc.w;
+            sn[0] = ss.x, sn[1] = ss.y, sn[2] = ss.z, sn[3] = ss.w;
         }
-        if (isq || isk) x = make_float4(o[0], o[1], o[2], o[3]);
     }
-    if (isq && mine) *reinterpret_cast<float4*>(a.q_out + ((size_t)t * a.hq + h) * hd + 4 * c) = x;
-    const long long row = live && !isq ? pool_row(a.p, s, pos, h) : -1;
-    store_kv<F8, NL>(isk ? a.p.k : a.p.v, isk ? a.p.ks : a.p.vs, row, hd, c, mine, x);
+    if (a.gq || a.gk) {
+#pragma unroll
+        for (int i = 0; i < P; i++) {
+            const int r = r0 + i * RPB;
+            const float* gain = r < a.hq ? a.gq : (r < a.hq + nkv ? a.gk : nullptr);
+            if (gain && lane_in) g[i] = make_float4(gain[4 * c], gain[4 * c + 1], gain[4 * c + 2], gain[4 * c + 3]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+        const int r = r0 + i * RPB;
+        const bool mine = r < rows && lane_in, isq = r < a.hq, isk = !isq && r < a.hq + nkv;
+        const int h = isq ? r : (isk ? r - a.hq : r - a.hq - nkv);
+        float4 y = x[i];
+        if (a.gq || a.gk) {
+            const double ss = row_sum_d<NL>(((double)y.x * (double)y.x + (double)y.y * (double)y.y) +
+                                            ((double)y.z * (double)y.z + (double)y.w * (double)y.w));
+            if (isq ? a.gq != nullptr : (isk && a.gk != nullptr)) {
+                const float inv = (float)rsqrt_f64(div_rcp(ss, (double)hd, 1.0 / hd) + (double)a.eps);
+                y = make_float4(y.x * inv * g[i].x, y.y * inv * g[i].y, y.z * inv * g[i].z, y.w * inv * g[i].w);
+            }
+        }
+        if (a.cosT) {
+            const float e[4] = {y.x, y.y, y.z, y.w};
+            float o[4];
+            if (a.neox) {
+#pragma unroll
+                for (int q = 0; q < 4; q += 2) {
+                    o[q] = e[q] * co[q] - e[q + 1] * sn[q];
+                    o[q + 1] = e[q] * sn[q] + e[q + 1] * co[q];
+                }
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    float p;
+                    if constexpr (FULL) p = across<NL / 2>(e[q]);
+                    else p = __shfl(e[q], (int)(threadIdx.x & 63) + (lo ? nl / 2 : -(nl / 2)));
+                    o[q] = lo ? e[q] * co[q] - p * sn[q] : p * sn[q] + e[q] * co[q];
+                }
+            }
+            if (isq || isk) y = make_float4(o[0], o[1], o[2], o[3]);
+        }
+        if (isq && mine) *reinterpret_cast<float4*>(a.q_out + ((size_t)t * a.hq + h) * hd + 4 * c) = y;
+        // the pool rows of a position's heads lie a page's slots apart
+        const long long row = mine && !isq ? row0 + (long long)h * a.p.page.d : -1;
+        store_kv<F8, NL>(isk ? a.p.k : a.p.v, isk ? a.p.ks : a.p.vs, row, hd, c, mine, y);
+    }
 }
 
+// kReadTok tokens a block: their places first, then every load of K and V (a
+// thread keeps its four columns), then the stores.
+constexpr int kReadTok = 4;
 template <bool F8>
 __global__ __launch_bounds__(256) void k_paged_read(PagedArgs p, float* ko, float* vo) {
-    const int t = blockIdx.x;
-    SeqAt sq;
-    if (!token_seq(p, t, sq)) return;
-    const int s = sq.s, pos = sq.len - sq.end + t;
-    if (pos < 0) return;
-    const int n4 = p.num_kv * p.hd / 4, hd4 = p.hd / 4;
-    for (int i = threadIdx.x; i < n4; i += 256) {
-        const int h = i / hd4, c = i - h * hd4;
-        const long long row = pool_row(p, s, pos, h);
-        if (row < 0) return;
-        for (int w = 0; w < 2; w++) {
+    const int t0 = blockIdx.x * kReadTok, hd4 = p.hd / 4, n4 = p.num_kv * hd4;
+    const int i0 = blockIdx.y * 256 + threadIdx.x, i = min(i0, n4 - 1), h = i / hd4, c = i - h * hd4;
+    long long row[kReadTok];
+#pragma unroll
+    for (int j = 0; j < kReadTok; j++) {
+        SeqAt sq;
+        row[j] = -1;
+        if (t0 + j < p.tokens && token_seq(p, t0 + j, sq)) row[j] = pool_row(p, sq.s, sq.len - sq.end + t0 + j, h);
+    }
+    if (i0 >= n4) return;
+    using Raw = typename std::conditional<F8, uint32_t, uint2>::type;
+    Raw u[2][kReadTok];
+    float sc[2][kReadTok];
+#pragma unroll
+    for (int w = 0; w < 2; w++)
+#pragma unroll
+        for (int j = 0; j < kReadTok; j++) {
+            if (row[j] < 0 || !(w ? vo : ko)) continue;
+            u[w][j] = reinterpret_cast<const Raw*>(w ? p.v : p.k)[row[j] * hd4 + c];
+            if constexpr (F8) sc[w][j] = (w ? p.vs : p.ks)[row[j]];
+        }
+#pragma unroll
+    for (int w = 0; w < 2; w++)
+#pragma unroll
+        for (int j = 0; j < kReadTok; j++) {
             float* o = w ? vo : ko;
-            if (!o) continue;
-            const void* pool = w ? p.v : p.k;
+            if (row[j] < 0 || !o) continue;
             float4 x;
             if constexpr (F8) {
-                const uint32_t u = reinterpret_cast<const uint32_t*>(pool)[row * hd4 + c];
-                const float sc = (w ? p.vs : p.ks)[row];
-                x = make_float4(e4m3_f32<0>(u) * sc, e4m3_f32<1>(u) * sc, e4m3_f32<2>(u) * sc, e4m3_f32<3>(u) * sc);
+                const uint32_t v = u[w][j];
+                const float f = sc[w][j];
+                x = make_float4(e4m3_f32<0>(v) * f, e4m3_f32<1>(v) * f, e4m3_f32<2>(v) * f, e4m3_f32<3>(v) * f);
             } else {
-                const uint2 u = reinterpret_cast<const uint2*>(pool)[row * hd4 + c];
-                x = make_float4(bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y));
+                x = make_float4(bf16_lo(u[w][j].x), bf16_hi(u[w][j].x), bf16_lo(u[w][j].y), bf16_hi(u[w][j].y));
             }
-            *reinterpret_cast<float4*>(o + (size_t)t * p.num_kv * p.hd + 4 * i) = x;
+            *reinterpret_cast<float4*>(o + ((size_t)(t0 + j) * n4 + i) * 4) = x;
         }
-    }
 }
 
+// Rows per lane group: one while the call's blocks leave CUs idle (a step's
+// latency), else as many as spare a token a second block, up to 4.
+template <bool F8, int NL, bool FULL>
+static void launch_append_nl(hipStream_t s, const AppendArgs& a) {
+    constexpr int RPB = 256 / NL;
+    const int rows = a.hq + 2 * a.p.num_kv, groups = (rows + RPB - 1) / RPB;
+    const auto go = [&](auto kernel, int per) {
+        hipLaunchKernelGGL(kernel, dim3(a.p.tokens, (groups + per - 1) / per), dim3(256), 0, s, a);
+    };
+    if (groups == 1 || (long long)a.p.tokens * groups <= 1024) go(k_paged_append<F8, NL, FULL, 1>, 1);
+    else if (groups == 2) go(k_paged_append<F8, NL, FULL, 2>, 2);
+    else go(k_paged_append<F8, NL, FULL, 4>, 4);
+}
 template <bool F8>
 static void launch_append(hipStream_t s, const AppendArgs& a) {
-    const int rows = a.hq + 2 * a.p.num_kv, nl = a.p.hd / 4;
-    const auto go = [&](auto kernel, int lanes) {
-        const int rpb = 256 / lanes;
-        hipLaunchKernelGGL(kernel, dim3(a.p.tokens, (rows + rpb - 1) / rpb), dim3(256), 0, s, a);
-    };
-    if (nl <= 16) go(k_paged_append<F8, 16>, 16);
-    else if (nl <= 32) go(k_paged_append<F8, 32>, 32);
-    else go(k_paged_append<F8, 64>, 64);
+    const int hd = a.p.hd;
+    if (hd == 64) launch_append_nl<F8, 16, true>(s, a);
+    else if (hd < 64) launch_append_nl<F8, 16, false>(s, a);
+    else if (hd == 128) launch_append_nl<F8, 32, true>(s, a);
+    else if (hd < 128) launch_append_nl<F8, 32, false>(s, a);
+    else if (hd == 256) launch_append_nl<F8, 64, true>(s, a);
+    else launch_append_nl<F8, 64, false>(s, a);
 }
 
 }  // namespace gh
@@ -221,8 +325,8 @@ extern "C" int gorch_hip_paged_append(void* stream, const gorch_hip_paged_kv* kv
     GH_REQUIRE(q_out != q || !q || q_stride == qd || b->tokens == 1,
                "gorch_hip_paged_append: q_out may only be q where q's rows are contiguous");
     GH_SUPPORTED(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(q_out, 16) && (!q || q_stride % 4 == 0) &&
-                     k_stride % 4 == 0 && v_stride % 4 == 0,
-                 "gorch_hip_paged_append: rows must be 16-byte aligned");
+                     k_stride % 4 == 0 && v_stride % 4 == 0 && aligned(w->rope_cos, 16) && aligned(w->rope_sin, 16),
+                 "gorch_hip_paged_append: rows and RoPE tables must be 16-byte aligned");
     a.q = q;
     a.k = k;
     a.v = v;
@@ -250,10 +354,11 @@ extern "C" int gorch_hip_paged_read(void* stream, const gorch_hip_paged_kv* kv, 
     GH_TRY(paged_args("gorch_hip_paged_read", kv, b, p));
     GH_SUPPORTED(aligned(k_out, 16) && aligned(v_out, 16), "gorch_hip_paged_read: outputs must be 16-byte aligned");
     if (b->tokens == 0 || b->seqs == 0 || (!k_out && !v_out)) return GORCH_HIP_OK;
+    const dim3 grid((p.tokens + kReadTok - 1) / kReadTok, (p.num_kv * p.hd / 4 + 255) / 256);
     if (kv->dtype == GORCH_HIP_KV_E4M3)
-        hipLaunchKernelGGL(k_paged_read<true>, dim3(p.tokens), dim3(256), 0, stream_of(stream), p, k_out, v_out);
+        hipLaunchKernelGGL(k_paged_read<true>, grid, dim3(256), 0, stream_of(stream), p, k_out, v_out);
     else
-        hipLaunchKernelGGL(k_paged_read<false>, dim3(p.tokens), dim3(256), 0, stream_of(stream), p, k_out, v_out);
+        hipLaunchKernelGGL(k_paged_read<false>, grid, dim3(256), 0, stream_of(stream), p, k_out, v_out);
     count(CNT_CODEC);
     return finish(stream, check_launch("paged_read"));
 }

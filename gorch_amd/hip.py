@@ -842,36 +842,40 @@ class _PagedBatchC(C.Structure):
         (n, vp) for n in ("cu_seqlens", "kv_lens", "page_table")]
 
 
-def _typed(t, dtype, shape, name):
-    """Device pointer of a contiguous tensor of this dtype and shape on the
-    current device (None stays None)."""
+_f32_t = _i32_t = None  # torch.float32 and torch.int32, once torch is loaded
+
+
+def _device():
+    """The current device's index."""
+    global _f32_t, _i32_t
+    torch_c = _torch_c or _load_torch()
+    if _f32_t is None:
+        import torch
+
+        _f32_t, _i32_t = torch.float32, torch.int32
+    return torch_c._cuda_getDevice()
+
+
+def _typed(t, dtype, shape, name, device):
+    """Device pointer of a contiguous tensor of this dtype and shape on this
+    device (None stays None)."""
     if t is None:
         return None
-    if t.dtype != dtype or t.shape != shape:
-        raise ValueError(f"gorch_amd.hip: {name} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    _here(t, name)
-    return _p(t)
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != device:
+        raise ValueError(f"gorch_amd.hip: {name} must be contiguous {dtype} {tuple(shape)} on the current device, got "
+                         f"{t.dtype} {tuple(t.shape)} of strides {tuple(t.stride())} on {t.device}")
+    return t.data_ptr()
 
 
-def _here(t, name):
-    torch_c = _torch_c or _load_torch()
-    if t.get_device() != torch_c._cuda_getDevice():
-        raise ValueError(f"gorch_amd.hip: {name} is not on the current device")
-
-
-def _rows(t, width, tokens, name):
+def _rows(t, width, tokens, name, device):
     """Pointer and row stride of f32 rows [tokens, width] whose rows may lie
     apart (a column range of a fused projection)."""
-    import torch
-
-    if t.dtype != torch.float32 or t.shape != (tokens, width) or (width > 1 and t.stride(1) != 1):
-        raise ValueError(f"gorch_amd.hip: {name} must be f32 rows [{tokens}, {width}] of unit column stride, "
-                         f"got {t.dtype} {tuple(t.shape)} of strides {tuple(t.stride())}")
-    _here(t, name)
-    stride = t.stride(0) if tokens > 1 else width
-    if stride < width:
-        raise ValueError(f"gorch_amd.hip: {name} has rows that overlap")
-    return t.data_ptr(), stride
+    stride, col = t.stride() if t.dim() == 2 else (0, 0)
+    if t.dtype is not _f32_t or t.shape != (tokens, width) or (col != 1 and width > 1) or (
+            stride < width and tokens > 1) or t.get_device() != device:
+        raise ValueError(f"gorch_amd.hip: {name} must be f32 rows [{tokens}, {width}] of unit column stride on the "
+                         f"current device, got {t.dtype} {tuple(t.shape)} of strides {tuple(t.stride())} on {t.device}")
+    return t.data_ptr(), stride if tokens > 1 else width
 
 
 class PagedBatch:
@@ -882,20 +886,19 @@ class PagedBatch:
     host's bounds on a sequence's new rows and cached length (0: none)."""
 
     def __init__(self, cu_seqlens, kv_lens, page_table, tokens: int, max_new: int = 0, max_kv: int = 0):
-        import torch
-
+        dev = _device()
         seqs = kv_lens.shape[0]
         if page_table.dim() != 2:
             raise ValueError("gorch_amd.hip: page_table must be [seqs, max_pages]")
         s = _PagedBatchC(tokens, seqs, page_table.shape[1], max_new, max_kv)
-        s.cu_seqlens = _typed(cu_seqlens, torch.int32, (seqs + 1,), "cu_seqlens")
-        s.kv_lens = _typed(kv_lens, torch.int32, (seqs,), "kv_lens")
-        s.page_table = _typed(page_table, torch.int32, (seqs, page_table.shape[1]), "page_table")
+        s.cu_seqlens = _typed(cu_seqlens, _i32_t, (seqs + 1,), "cu_seqlens", dev)
+        s.kv_lens = _typed(kv_lens, _i32_t, (seqs,), "kv_lens", dev)
+        s.page_table = _typed(page_table, _i32_t, (seqs, page_table.shape[1]), "page_table", dev)
         self.t = (cu_seqlens, kv_lens, page_table)
         self.s = s
         self.ref = C.byref(s)
         self.tokens = tokens
-        self.device = kv_lens.get_device()
+        self.device = dev
 
 
 class PagedKV:
@@ -917,17 +920,18 @@ class PagedKV:
             raise ValueError(f"gorch_amd.hip: pools must be bf16 or e4m3, got {k.dtype}")
         if (k_scale is None) != (dtype == KV_BF16) or (v_scale is None) != (dtype == KV_BF16):
             raise ValueError("gorch_amd.hip: e4m3 pools need k_scale and v_scale, bf16 pools take none")
+        dev = _device()
         pages, num_kv, page, hd = k.shape
         s = _PagedKVC(dtype, pages, page, num_kv, hd)
-        s.k = _typed(k, k.dtype, k.shape, "k")
-        s.v = _typed(v, k.dtype, k.shape, "v")
-        s.k_scale = _typed(k_scale, torch.float32, k.shape[:3], "k_scale")
-        s.v_scale = _typed(v_scale, torch.float32, k.shape[:3], "v_scale")
+        s.k = _typed(k, k.dtype, k.shape, "k", dev)
+        s.v = _typed(v, k.dtype, k.shape, "v", dev)
+        s.k_scale = _typed(k_scale, torch.float32, k.shape[:3], "k_scale", dev)
+        s.v_scale = _typed(v_scale, torch.float32, k.shape[:3], "v_scale", dev)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_kv, self.head_dim = num_kv, hd
         self.s = s
         self.ref = C.byref(s)
-        self.device = k.get_device()
+        self.device = dev
 
     @classmethod
     def new(cls, num_pages: int, page_size: int, num_kv: int, head_dim: int, dtype: str = "bf16") -> "PagedKV":
@@ -943,37 +947,30 @@ class PagedKV:
                    *(torch.zeros(shape[:3], device="cuda") for _ in "kv"))
 
     def _check(self, batch):
-        torch_c = _torch_c or _load_torch()
-        if not (self.device == batch.device == torch_c._cuda_getDevice()):
+        dev = _device()
+        if self.device != dev or batch.device != dev:
             raise ValueError("gorch_amd.hip: the cache and the batch must be on the current device")
+        return dev
 
     def append(self, batch: PagedBatch, heads: "GQA", q, k, v, q_out) -> None:
         """gorch_hip_paged_append: the per-head norms and RoPE of ``heads``
         (a GQA) on q and k, q to q_out, K and V into the pages. q, k, v: f32
         rows [tokens, width], possibly column ranges of one tensor; q and
         q_out may be None."""
-        import torch
-
-        self._check(batch)
-        T = batch.tokens
-        qp = qs = None
-        if q is not None:
-            qp, qs = _rows(q, heads.s.num_q * self.head_dim, T, "q")
-        kp, ks = _rows(k, self.num_kv * self.head_dim, T, "k")
-        vp_, vs = _rows(v, self.num_kv * self.head_dim, T, "v")
-        op = _typed(q_out, torch.float32, (T, heads.s.num_q * self.head_dim), "q_out")
-        _ok(lib().gorch_hip_paged_append(_stream(), self.ref, batch.ref, C.byref(heads.s), qp, qs or 0, kp, ks, vp_, vs,
-                                         op))
+        dev, T, w = self._check(batch), batch.tokens, heads.s
+        qd, kvd = w.num_q * self.head_dim, self.num_kv * self.head_dim
+        qp, qs = (None, 0) if q is None else _rows(q, qd, T, "q", dev)
+        kp, ks = _rows(k, kvd, T, "k", dev)
+        vp_, vs = _rows(v, kvd, T, "v", dev)
+        _ok(lib().gorch_hip_paged_append(_stream(), self.ref, batch.ref, C.byref(w), qp, qs, kp, ks, vp_, vs,
+                                         _typed(q_out, _f32_t, (T, qd), "q_out", dev)))
 
     def read(self, batch: PagedBatch, k_out, v_out) -> None:
         """gorch_hip_paged_read: the batch's tokens as f32 rows [tokens,
         num_kv * head_dim] (either may be None)."""
-        import torch
-
-        self._check(batch)
-        shape = (batch.tokens, self.num_kv * self.head_dim)
-        _ok(lib().gorch_hip_paged_read(_stream(), self.ref, batch.ref, _typed(k_out, torch.float32, shape, "k_out"),
-                                       _typed(v_out, torch.float32, shape, "v_out")))
+        dev, shape = self._check(batch), (batch.tokens, self.num_kv * self.head_dim)
+        _ok(lib().gorch_hip_paged_read(_stream(), self.ref, batch.ref, _typed(k_out, _f32_t, shape, "k_out", dev),
+                                       _typed(v_out, _f32_t, shape, "v_out", dev)))
 
     def workspace(self, batch: PagedBatch, num_q: int):
         """A device workspace for attention() over this batch's bounds, or
@@ -987,22 +984,16 @@ class PagedKV:
         """gorch_hip_paged_attention: q and out f32 [tokens, num_q *
         head_dim]. ws from workspace() (a new one if None); calls that can
         overlap must not share it."""
-        import torch
-
-        self._check(batch)
-        T, width = q.shape
-        if T != batch.tokens:
-            raise ValueError(f"gorch_amd.hip: q must have {batch.tokens} rows, got {T}")
-        num_q = width // self.head_dim
-        if num_q * self.head_dim != width:
-            raise ValueError("gorch_amd.hip: q's rows must be whole heads")
-        qp = _typed(q, torch.float32, (T, width), "q")
-        op = _typed(out, torch.float32, (T, width), "out")
+        dev, shape = self._check(batch), q.shape
+        num_q = shape[-1] // self.head_dim
+        if len(shape) != 2 or shape[0] != batch.tokens or num_q * self.head_dim != shape[1]:
+            raise ValueError(f"gorch_amd.hip: q must be [{batch.tokens}, whole heads of {self.head_dim}], got {tuple(shape)}")
         if ws is None:
             ws = self.workspace(batch, num_q)
-        elif ws.get_device() != self.device:
+        elif ws.get_device() != dev:
             raise ValueError("gorch_amd.hip: ws is not on the current device")
-        _ok(lib().gorch_hip_paged_attention(_stream(), self.ref, batch.ref, qp, num_q, op, int(causal), _p(ws),
+        _ok(lib().gorch_hip_paged_attention(_stream(), self.ref, batch.ref, _typed(q, _f32_t, shape, "q", dev), num_q,
+                                            _typed(out, _f32_t, shape, "out", dev), int(causal), _p(ws),
                                             0 if ws is None else ws.numel() * ws.element_size()))
 
 
@@ -1018,26 +1009,32 @@ def process_logits(logits, out, history=None, history_lens=None, prompt_lens=Non
     each row's penalties for the tokens of history int32 [rows, width], its
     biases (CSR rows, last entry of an id counts) and its bit mask allowed
     int32 [rows, >= ceil(n / 32)]. Every rule may be None."""
-    import torch
-
-    rows, n = logits.shape
-    f32t, i32t = torch.float32, torch.int32
+    dev = _device()
+    rows, n = shape = logits.shape
+    each = (rows,)
     r = _LogitsRulesC()
     if history is not None:
-        r.history, r.history_stride = _typed(history, i32t, (rows, history.shape[-1]), "history"), history.shape[-1]
-    r.history_lens = _typed(history_lens, i32t, (rows,), "history_lens")
-    r.prompt_lens = _typed(prompt_lens, i32t, (rows,), "prompt_lens")
-    r.repetition = _typed(repetition, f32t, (rows,), "repetition")
-    r.frequency = _typed(frequency, f32t, (rows,), "frequency")
-    r.presence = _typed(presence, f32t, (rows,), "presence")
+        r.history_stride = width = history.shape[-1]
+        r.history = _typed(history, _i32_t, (rows, width), "history", dev)
+        if history_lens is not None:
+            r.history_lens = _typed(history_lens, _i32_t, each, "history_lens", dev)
+        if prompt_lens is not None:
+            r.prompt_lens = _typed(prompt_lens, _i32_t, each, "prompt_lens", dev)
+    if repetition is not None:
+        r.repetition = _typed(repetition, _f32_t, each, "repetition", dev)
+    if frequency is not None:
+        r.frequency = _typed(frequency, _f32_t, each, "frequency", dev)
+    if presence is not None:
+        r.presence = _typed(presence, _f32_t, each, "presence", dev)
     if bias is not None:
         if bias_rows is None or bias_ids is None:
             raise ValueError("gorch_amd.hip: bias needs bias_rows and bias_ids")
-        r.biases = bias.numel()
-        r.bias_rows = _typed(bias_rows, i32t, (rows + 1,), "bias_rows")
-        r.bias_ids = _typed(bias_ids, i32t, (r.biases,), "bias_ids")
-        r.bias = _typed(bias, f32t, (r.biases,), "bias")
+        r.biases = count = bias.numel()
+        r.bias_rows = _typed(bias_rows, _i32_t, (rows + 1,), "bias_rows", dev)
+        r.bias_ids = _typed(bias_ids, _i32_t, (count,), "bias_ids", dev)
+        r.bias = _typed(bias, _f32_t, (count,), "bias", dev)
     if allowed is not None:
-        r.allowed, r.allowed_stride = _typed(allowed, i32t, (rows, allowed.shape[-1]), "allowed"), allowed.shape[-1]
-    _ok(lib().gorch_hip_process_logits(_stream(), C.byref(r), _typed(logits, f32t, (rows, n), "logits"),
-                                       _typed(out, f32t, (rows, n), "out"), rows, n))
+        r.allowed_stride = words = allowed.shape[-1]
+        r.allowed = _typed(allowed, _i32_t, (rows, words), "allowed", dev)
+    _ok(lib().gorch_hip_process_logits(_stream(), C.byref(r), _typed(logits, _f32_t, shape, "logits", dev),
+                                       _typed(out, _f32_t, shape, "out", dev), rows, n))

@@ -478,7 +478,8 @@ typedef struct {
  * zeros; a row that holds an infinity reads back as NaN). Rows q [tokens,
  * num_q * head_dim], k and v [tokens, num_kv * head_dim] start at multiples
  * of their strides (in floats, multiples of 4), so the three can be column
- * ranges of one fused projection; 16-byte aligned. q_out [tokens, num_q *
+ * ranges of one fused projection; rows and RoPE tables are 16-byte aligned
+ * (else GORCH_HIP_EUNSUPPORTED). q_out [tokens, num_q *
  * head_dim] may be q if its rows are contiguous; q and q_out may both be
  * NULL. A token whose position is negative, past max_kv or the RoPE tables, or
  * on no page, is skipped: none of its rows is written, q_out's neither.

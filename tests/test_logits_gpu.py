@@ -167,3 +167,21 @@ def test_wrong_tensors_are_refused(gpu):
         gpu.process_logits(x, x[:1])
     with pytest.raises(gpu.HipError):
         gpu.process_logits(x, x, allowed=i[:, :1].contiguous())
+
+
+@pytest.mark.parametrize("first,out_first", [(0, 1), (1, 1), (1, 2), (2, 0), (3, 2)])
+@pytest.mark.parametrize("n", [5, 1023, 4099])
+def test_rows_at_any_address(gpu, first, out_first, n):
+    # rows of a larger tensor start at any multiple of 4 bytes, in and out each their own
+    rng = np.random.default_rng(n + first)
+    x = (rng.standard_normal((3, n)) * 4).astype(np.float32)
+    r = rules(rng, 3, n, 37, 6)
+    want, tol = definition(x, r)
+    space = torch.zeros(3 * n + 8, device="cuda")
+    xd = space[first:first + 3 * n].view(3, n)
+    xd.copy_(dev(x))
+    room = torch.full((3 * n + 8,), 55.0, device="cuda")
+    gpu.process_logits(xd, room[out_first:out_first + 3 * n].view(3, n), **{k: dev(v) for k, v in r.items()})
+    got = host(room)
+    check(got[out_first:out_first + 3 * n].reshape(3, n), want, tol)
+    assert (got[:out_first] == 55).all() and (got[out_first + 3 * n:] == 55).all()

@@ -96,6 +96,7 @@ def test_append_arguments():
     assert append(kv, b, heads(), ks=127) == 2 and append(kv, b, heads(), qs=128) == 2
     assert append(kv, b, heads(), ks=129) == 1 and append(kv, b, heads(), k=ODD) == 1
     assert append(kv, b, heads(rope_cos=FAKE)) == 2
+    assert append(kv, b, heads(rope_cos=FAKE, rope_sin=ODD)) == 1
     # q may be its own output only where its rows lie together
     assert append(kv, b, heads(), qs=512, out=FAKE) == 2
 
