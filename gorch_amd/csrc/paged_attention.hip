@@ -234,35 +234,39 @@ struct Rows {
     int pos[NR];   // the position of a lane's row (what it sees ends there), -1: none
     int first, last;  // smallest and largest of the wave's rows that exist
 
-    // rows r0 + 16 i + lane % 16 of a sequence of n token rows
+    // Rows r0 + 16 i + lane % 16 of a sequence: where they stand, and their q on
+    // the way.
     template <bool PART>
-    __device__ __forceinline__ void load(const PagedAttnArgs& a, const SeqAt& s, int r0, int kvh) {
+    __device__ __forceinline__ void fetch(const PagedAttnArgs& a, const SeqAt& s, int r0, int kvh, float4 (&x)[NR][T::NU][2]) {
         const int lane = threadIdx.x & 63, g = lane >> 4, G = a.group.d, n = s.end - s.begin;
-        int lo = 0x7fffffff, hi = -1;
 #pragma unroll
         for (int i = 0; i < NR; i++) {
             const int r = r0 + 16 * i + (lane & 15);
             const int tok = (int)a.group.div((uint32_t)r), h = kvh * G + r - tok * G;
             const bool live = r < n * G;
             pos[i] = live ? (a.causal ? s.len - n + tok : s.len - 1) : -1;
-            if (live) lo = min(lo, pos[i]);
-            hi = max(hi, pos[i]);
-            const float* src = a.q + ((size_t)(s.begin + tok) * a.hq + h) * a.p.hd;
+            const float* src = live ? a.q + ((size_t)(s.begin + tok) * a.hq + h) * a.p.hd : reinterpret_cast<const float*>(kZeros);
 #pragma unroll
             for (int u = 0; u < T::NU; u++) {
                 const int c = T::col(u, g);
-                float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (live && (!PART || c < a.p.hd)) {
-                    const float4 x = *reinterpret_cast<const float4*>(src + c), y = *reinterpret_cast<const float4*>(src + c + 4);
-                    f[0] = x.x * a.scale;
-                    f[1] = x.y * a.scale;
-                    f[2] = x.z * a.scale;
-                    f[3] = x.w * a.scale;
-                    f[4] = y.x * a.scale;
-                    f[5] = y.y * a.scale;
-                    f[6] = y.z * a.scale;
-                    f[7] = y.w * a.scale;
-                }
+                const float* p = live && (!PART || c < a.p.hd) ? src + c : reinterpret_cast<const float*>(kZeros);
+                x[i][u][0] = *reinterpret_cast<const float4*>(p);
+                x[i][u][1] = *reinterpret_cast<const float4*>(p + 4);
+            }
+        }
+        const int at = r0 < n * G ? (int)a.group.div((uint32_t)r0) : 0;
+        const int to = (int)a.group.div((uint32_t)(min(r0 + 16 * NR, n * G) - 1));
+        first = r0 < n * G ? (a.causal ? s.len - n + at : s.len - 1) : 0x7fffffff;
+        last = r0 < n * G ? (a.causal ? s.len - n + to : s.len - 1) : -1;
+    }
+    __device__ __forceinline__ void begin(const PagedAttnArgs& a, const float4 (&x)[NR][T::NU][2]) {
+#pragma unroll
+        for (int i = 0; i < NR; i++) {
+#pragma unroll
+            for (int u = 0; u < T::NU; u++) {
+                const float4 y = x[i][u][0], z = x[i][u][1];
+                const float f[8] = {y.x * a.scale, y.y * a.scale, y.z * a.scale, y.w * a.scale,
+                                    z.x * a.scale, z.y * a.scale, z.z * a.scale, z.w * a.scale};
                 split3(f, q[i][u]);
             }
             m[i] = -INFINITY;
@@ -270,12 +274,6 @@ struct Rows {
 #pragma unroll
             for (int d = 0; d < HD / 16; d++) o[i][d] = floatx4{0.f, 0.f, 0.f, 0.f};
         }
-        for (int w = 1; w < 16; w *= 2) {
-            lo = min(lo, __shfl_xor(lo, w));
-            hi = max(hi, __shfl_xor(hi, w));
-        }
-        first = __builtin_amdgcn_readfirstlane(lo);
-        last = __builtin_amdgcn_readfirstlane(hi);
     }
 
     // Scores of group j's 16 keys from a lane's chunks: sc[i] of row tile i
@@ -387,15 +385,27 @@ __device__ __forceinline__ void put(const PagedAttnArgs& a, int split, size_t ro
     }
 }
 
+// The pool row of key `key` of a sequence, -1 if it is not below k1 or on no
+// page; no branch around the load (0 < k1 <= limit).
+__device__ __forceinline__ long long key_row(const PagedArgs& a, int s, int key, int k1, int kvh) {
+    const int p = min(key, k1 - 1);
+    const uint32_t i = a.page.div((uint32_t)p);
+    const int page = a.table[(size_t)s * a.max_pages + i];
+    const long long row = ((long long)page * a.num_kv + kvh) * a.page.d + (p - (int)(i * a.page.d));
+    return key < k1 && (unsigned)page < (unsigned)a.num_pages ? row : -1;
+}
+
 // Few rows: a block takes 16 rows of a sequence (with their KV head) and a
-// range of its keys, its four waves 32 keys each in turn. K goes from memory
-// to the operand registers, V through a wave's own LDS; while a tile is
-// weighed, the next one's rows are on their way.
+// range of its keys, its NW waves 32 keys each in turn. K goes from memory to
+// the operand registers, V through a wave's own LDS; NB tiles of rows are on
+// their way while one is weighed (a fetch is unconditional: a branch around
+// loads would make the next use wait for all of them).
 template <bool F8, int HD, bool PART>
 __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void k_paged_attn_few(PagedAttnArgs a) {
     using T = Tile<F8, HD>;
+    constexpr int NW = 4, STEP = 32 * NW, NB = T::NT <= 2 ? 2 : 1;
     constexpr int OROW = HD + 4;
-    constexpr int STAGE = 4 * (T::BYTES + 256), JOIN = 4 * 16 * (OROW + 2) * 4;
+    constexpr int STAGE = NW * (T::BYTES + 256), JOIN = NW * 16 * (OROW + 2) * 4;
     __shared__ __align__(16) char lds[STAGE > JOIN ? STAGE : JOIN];
     __shared__ OddBits<16, HD> odd;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
@@ -404,68 +414,87 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void k_paged_attn_few(PagedA
     SeqAt s;
     int r0;
     if (!find_tile<16>(a, tile, s, r0)) return;
-    Rows<F8, HD, 1> rows;
-    rows.template load<PART>(a, s, r0, kvh);
-    const int T1 = min(rows.last + 1, a.p.limit);
+    const int G = a.group.d, n = s.end - s.begin;
+    const int end_tok = (int)a.group.div((uint32_t)(min(r0 + 16, n * G) - 1));
+    const int T1 = min((a.causal ? s.len - n + end_tok : s.len - 1) + 1, a.p.limit);
     const int k0 = split * a.chunk, k1 = a.splits == 1 ? T1 : min(T1, k0 + a.chunk);
     if (k0 >= k1 && split > 0) return;
 
     char* vt = lds + wave * (T::BYTES + 256);
     float* sc = reinterpret_cast<float*>(vt + T::BYTES);  // K scales of the 32 keys, then V's
-    u32x4 kc[2][T::NT], vc[2][T::NT];
-    float scale = 0.f;
-    uint32_t seen = 0;
-    // the pool row of key key0 + lane % 32
-    auto lookup = [&](int key0) -> long long {
-        const int key = key0 + (lane & 31);
-        return key < k1 ? pool_row(a.p, s.s, key, kvh) : -1;
-    };
-    auto fetch = [&](long long row) {
+    struct Buf {
+        u32x4 k[2][T::NT], v[2][T::NT];
+        float scale;
+        uint32_t seen;
+    } buf[NB];
+    // row: the pool row of key lane % 32 of the tile
+    auto fetch = [&](long long row, Buf& b) {
         const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)row, (uint32_t)row, false, false);
         const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(row >> 32), (uint32_t)(row >> 32), false, false);
-        seen = (uint32_t)__ballot(row >= 0);
+        b.seen = (uint32_t)__ballot(row >= 0);
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const long long r = (long long)(((uint64_t)hi[j] << 32) | lo[j]);
-            fetch_row<F8, HD, PART>(a.p.k, r, a.p.hd, g, kc[j]);
-            fetch_row<F8, HD, PART>(a.p.v, r, a.p.hd, g, vc[j]);
-        }
+        for (int j = 0; j < 2; j++)
+            fetch_row<F8, HD, PART>(a.p.k, (long long)(((uint64_t)hi[j] << 32) | lo[j]), a.p.hd, g, b.k[j]);
         if constexpr (F8) {
             const float* from = lane < 32 ? a.p.ks : a.p.vs;
-            scale = *(row >= 0 ? from + row : reinterpret_cast<const float*>(kZeros));
+            b.scale = *(row >= 0 ? from + row : reinterpret_cast<const float*>(kZeros));
         }
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+            fetch_row<F8, HD, PART>(a.p.v, (long long)(((uint64_t)hi[j] << 32) | lo[j]), a.p.hd, g, b.v[j]);
     };
-    for (int i = threadIdx.x; i < (int)(sizeof(odd) / 4); i += 256) reinterpret_cast<uint32_t*>(&odd)[i] = 0;
-    __syncthreads();
+    Rows<F8, HD, 1> rows;
     int key0 = k0 + 32 * wave;
-    long long next = lookup(key0);
-    if (key0 < k1) fetch(next);
-    next = lookup(key0 + 128);
-    for (; key0 < k1; key0 += 128) {
+    long long next = -1;
+    if (k0 < k1) {
+        long long r[NB];
+#pragma unroll
+        for (int i = 0; i < NB; i++) r[i] = key_row(a.p, s.s, key0 + i * STEP + (lane & 31), k1, kvh);
+        next = key_row(a.p, s.s, key0 + NB * STEP + (lane & 31), k1, kvh);
+        float4 x[1][T::NU][2];
+        rows.template fetch<PART>(a, s, r0, kvh, x);
+#pragma unroll
+        for (int i = 0; i < NB; i++) fetch(r[i], buf[i]);
+        for (int i = threadIdx.x; i < (int)(sizeof(odd) / 4); i += 64 * NW) reinterpret_cast<uint32_t*>(&odd)[i] = 0;
+        rows.begin(a, x);
+    } else {
+        // no key is seen: zeros
+        rows.m[0] = -INFINITY;
+        rows.l[0] = 0.f;
+        for (int d = 0; d < HD / 16; d++) rows.o[0][d] = floatx4{0.f, 0.f, 0.f, 0.f};
+        if (threadIdx.x == 0) odd.any = 0;
+    }
+    __syncthreads();
+    auto step = [&](Buf& b, int key) {
         floatx4 scores[2][1];
-        rows.score(kc[0], scores[0]);
-        rows.score(kc[1], scores[1]);
+        rows.score(b.k[0], scores[0]);
+        rows.score(b.k[1], scores[1]);
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int t = 0; t < T::NT; t++) *reinterpret_cast<u32x4*>(vt + j * T::GROUP + t * 1024 + lane * 16) = vc[j][t];
-        if (__any(any_nonfinite<F8>(vc[0]) || any_nonfinite<F8>(vc[1])))
+            for (int t = 0; t < T::NT; t++) *reinterpret_cast<u32x4*>(vt + j * T::GROUP + t * 1024 + lane * 16) = b.v[j][t];
+        if (__any(any_nonfinite<F8>(b.v[0]) || any_nonfinite<F8>(b.v[1])))
 #pragma unroll 1
             for (int j = 0; j < 2; j++)
-                clean_odd<F8, 16, HD>(odd, a, s, r0, key0 + 16 * j + (lane & 15), g, vt + j * T::GROUP + lane * 16);
-        if constexpr (F8) sc[lane] = scale;
-        const uint32_t here = seen;
-        if (key0 + 128 < k1) {
-            fetch(next);
-            next = lookup(key0 + 256);
+                clean_odd<F8, 16, HD>(odd, a, s, r0, key + 16 * j + (lane & 15), g, vt + j * T::GROUP + lane * 16);
+        if constexpr (F8) sc[lane] = b.scale;
+        const uint32_t here = b.seen;
+        fetch(next, b);
+        next = key_row(a.p, s.s, key + (NB + 1) * STEP + (lane & 31), k1, kvh);
+        rows.take(scores, key, here, sc, sc + 32, vt);
+    };
+    while (key0 < k1) {
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            if (i == 0 || key0 < k1) step(buf[i], key0);
+            key0 += STEP;
         }
-        rows.take(scores, key0, here, sc, sc + 32, vt);
     }
     // the waves' sums, joined in wave order
     __syncthreads();
     float* jo = reinterpret_cast<float*>(lds);
-    float* jm = jo + 4 * 16 * OROW;
-    float* jl = jm + 64;
+    float* jm = jo + NW * 16 * OROW;
+    float* jl = jm + NW * 16;
     const float l = col_sum(rows.l[0]);
 #pragma unroll
     for (int d = 0; d < HD / 16; d++)
@@ -475,20 +504,21 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void k_paged_attn_few(PagedA
         jl[wave * 16 + lane] = l;
     }
     __syncthreads();
-    const int G = a.group.d, n = s.end - s.begin;
-    for (int i = threadIdx.x; i < 16 * (HD / 4); i += 256) {
+    for (int i = threadIdx.x; i < 16 * (HD / 4); i += 64 * NW) {
         const int r = i / (HD / 4), c = 4 * (i % (HD / 4));
         if (r0 + r >= n * G || (PART && c >= a.p.hd)) continue;
         float M = jm[r];
-        for (int w = 1; w < 4; w++) M = fmaxf(M, jm[w * 16 + r]);
+#pragma unroll
+        for (int w = 1; w < NW; w++) M = fmaxf(M, jm[w * 16 + r]);
         const float use = M == -INFINITY ? 0.f : M;
         floatx4 o = {0.f, 0.f, 0.f, 0.f};
         float L = 0.f;
-        for (int w = 0; w < 4; w++) {
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
             const float f = __builtin_amdgcn_exp2f(jm[w * 16 + r] - use);
             L += f * jl[w * 16 + r];
             const floatx4 x = *reinterpret_cast<const floatx4*>(jo + (w * 16 + r) * OROW + c);
-            for (int e = 0; e < 4; e++) o[e] += jm[w * 16 + r] == -INFINITY ? 0.f : f * x[e];
+            for (int e = 0; e < 4; e++) o[e] += f * x[e];
         }
         if (odd.any) o = add_odd(odd, r, c, o);
         const int tok = (int)a.group.div((uint32_t)(r0 + r));
@@ -517,7 +547,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
     if (!find_tile<64 * NR>(a, tile, s, r0)) return;
     const int G = a.group.d, n = s.end - s.begin;
     Rows<F8, HD, NR> rows;
-    rows.template load<PART>(a, s, r0 + 16 * NR * wave, kvh);
+    float4 qx[NR][T::NU][2];
+    rows.template fetch<PART>(a, s, r0 + 16 * NR * wave, kvh, qx);
     // the last position that any of the block's rows sees
     const int end_tok = (int)a.group.div((uint32_t)(min(r0 + 64 * NR, n * G) - 1));
     const int T1 = min((a.causal ? s.len - n + end_tok : s.len - 1) + 1, a.p.limit);
@@ -530,10 +561,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
     u32x4 st[T::NT];
     float scale = 0.f;
     long long row = -1;
-    auto lookup = [&](int key0) {
-        const int key = key0 + 16 * j + (lane & 15);
-        return key < k1 ? pool_row(a.p, s.s, key, kvh) : -1ll;
-    };
+    auto lookup = [&](int key0) { return key_row(a.p, s.s, key0 + 16 * j + (lane & 15), k1, kvh); };
     int at0 = 0;
     auto fetch = [&](long long r, int key0) {
         row = r;
@@ -554,11 +582,15 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
     };
     for (int i = threadIdx.x; i < (int)(sizeof(odd) / 4); i += 256) reinterpret_cast<uint32_t*>(&odd)[i] = 0;
     __syncthreads();
-    long long next = lookup(k0);
+    long long next = -1;
     if (k0 < k1) {
+        next = lookup(k0);
         fetch(next, k0);
         next = lookup(k0 + 32);
+        rows.begin(a, qx);
         stage(0);
+    } else {
+        rows.begin(a, qx);
     }
     __syncthreads();
     for (int key0 = k0, b = 0; key0 < k1; key0 += 32, b ^= 1) {
@@ -600,42 +632,64 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
     }
 }
 
-// A row's splits joined in their order, each weighted by 2^(its maximum - the
-// largest); a wave per (token, query head).
+// A row's splits joined, each weighted by 2^(its maximum - the largest): WPR
+// waves per (token, query head), 16 bytes of a split's columns a lane, the
+// splits dealt to SLOTS groups of lanes (sums in a fixed order: a slot's
+// splits, then the slots). The first loads go out before the sequence is
+// known; splits past the row's last are then left out.
+constexpr int kMaxSplits = 128;
+template <int NL, int WPR>
 __global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttnArgs a) {
-    const int lane = threadIdx.x & 63;
-    const long long row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    constexpr int SLOTS = WPR * 64 / NL, RPB = 4 / WPR;
+    __shared__ floatx4 so[RPB][SLOTS][NL];
+    const int lane = threadIdx.x & 63, sub = threadIdx.x / (64 * WPR), tid = threadIdx.x % (64 * WPR);
     const long long total = (long long)a.p.tokens * a.hq;
-    if (row >= total) return;
+    const long long row = min(__builtin_amdgcn_readfirstlane(blockIdx.x * RPB + sub), (int)total - 1);
+    const bool mine = (long long)blockIdx.x * RPB + sub < total;
+    const int c = tid % NL, slot = tid / NL, col = min(4 * c, a.p.hd - 4), most = max(a.splits, a.splits2);
+    float2 ml[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) ml[i] = a.part_ml[min(lane + 64 * i, most - 1) * total + row];
+    auto part = [&](int j) {
+        return *reinterpret_cast<const floatx4*>(a.part_o + (min(j, most - 1) * total + row) * a.p.hd + col);
+    };
+    floatx4 x = part(slot);
     const int t = (int)(row / a.hq);
     SeqAt s;
-    if (!token_seq(a.p, t, s)) return;
-    const int n = s.end - s.begin;
-    const bool few = n * (int)a.group.d <= a.hi_rows;
-    const int chunk = few ? a.chunk : a.chunk2, splits = few ? a.splits : a.splits2;
-    if (splits == 1) return;
-    const int T = min(a.causal ? s.len - s.end + t + 1 : s.len, a.p.limit);
-    const int nc = min(max((T + chunk - 1) / chunk, 1), splits);
-    float M = -INFINITY;
-    for (int c = 0; c < nc; c++) M = fmaxf(M, a.part_ml[c * total + row].x);
-    const float use = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
+    int nc = 0;
+    if (token_seq(a.p, t, s)) {
+        const bool few = (s.end - s.begin) * (int)a.group.d <= a.hi_rows;
+        const int chunk = few ? a.chunk : a.chunk2, splits = few ? a.splits : a.splits2;
+        const int T = min(a.causal ? s.len - s.end + t + 1 : s.len, a.p.limit);
+        nc = splits == 1 ? 0 : min(max((T + chunk - 1) / chunk, 1), splits);  // (one split: out is written)
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        if (lane + 64 * i >= nc) ml[i] = make_float2(-INFINITY, 0.f);
+        top = fmaxf(top, ml[i].x);
+    }
+    const float M = wave_max(top), use = M == -INFINITY ? 0.f : M;
+    const float w0 = __builtin_amdgcn_exp2f(ml[0].x - use), w1 = __builtin_amdgcn_exp2f(ml[1].x - use);
+    const float L = wave_sum(w0 * ml[0].y + w1 * ml[1].y);
     floatx4 o = {0.f, 0.f, 0.f, 0.f};
-    const int col = 4 * lane;
-    for (int c = 0; c < nc; c++) {
-        const float2 ml = a.part_ml[c * total + row];
-        if (ml.x == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(ml.x - use);
-        L += f * ml.y;
-        if (col < a.p.hd) {
-            const floatx4 x = *reinterpret_cast<const floatx4*>(a.part_o + (c * total + row) * a.p.hd + col);
+    for (int j = slot; j - slot < nc; j += SLOTS) {
+        const floatx4 y = part(j + SLOTS);
+        const float f = __shfl(j < 64 ? w0 : w1, j & 63);
+        if (j < nc)
+#pragma unroll
             for (int e = 0; e < 4; e++) o[e] += f * x[e];
-        }
+        x = y;
     }
-    if (col < a.p.hd) {
-        const float r = L == 0.f ? 0.f : 1.0f / L;
-        *reinterpret_cast<floatx4*>(a.out + row * a.p.hd + col) = floatx4{o[0] * r, o[1] * r, o[2] * r, o[3] * r};
-    }
+    so[sub][slot][c] = o;
+    __syncthreads();
+    if (tid >= NL || nc == 0 || !mine || 4 * c >= a.p.hd) return;
+#pragma unroll
+    for (int j = 1; j < SLOTS; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] += so[sub][j][c][e];
+    const float r = L == 0.f ? 0.f : 1.0f / L;
+    *reinterpret_cast<floatx4*>(a.out + row * a.p.hd + col) = floatx4{o[0] * r, o[1] * r, o[2] * r, o[3] * r};
 }
 
 // ---------------------------------------------------------------- launch
@@ -667,7 +721,7 @@ static AttnPlan attn_plan(const PagedArgs& p, int hq, int max_new) {
     const auto splits = [&](long long tiles, long long want, int unit, int& chunk) {
         const long long blocks = std::max(1ll, tiles) * p.num_kv;
         const long long units = std::max(1ll, ((long long)p.limit + unit - 1) / unit);
-        long long n = std::min(std::max(1ll, (want + blocks - 1) / blocks), units);
+        long long n = std::min({std::max(1ll, (want + blocks - 1) / blocks), units, (long long)kMaxSplits});
         const long long per = (units + n - 1) / n;
         chunk = (int)std::min<long long>(per * unit, 0x7fffff00);
         return (int)((units + per - 1) / per);
@@ -728,6 +782,18 @@ static void launch_attn_hd(hipStream_t s, const PagedAttnArgs& a, const AttnPlan
     else launch_attn<F8, 256, true>(s, a, pl);
 }
 
+// A wave per row, or a block for many splits.
+static void launch_join(hipStream_t s, const PagedAttnArgs& a, int splits) {
+    const long long rows = (long long)a.p.tokens * a.hq;
+    const auto go = [&](auto kernel, int per) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, a);
+    };
+    const bool wide = splits > 8;
+    if (a.p.hd <= 64) wide ? go(k_paged_attn_join<16, 4>, 1) : go(k_paged_attn_join<16, 1>, 4);
+    else if (a.p.hd <= 128) wide ? go(k_paged_attn_join<32, 4>, 1) : go(k_paged_attn_join<32, 1>, 4);
+    else wide ? go(k_paged_attn_join<64, 4>, 1) : go(k_paged_attn_join<64, 1>, 4);
+}
+
 }  // namespace gh
 
 using namespace gh;
@@ -769,8 +835,7 @@ extern "C" int gorch_hip_paged_attention(void* stream, const gorch_hip_paged_kv*
         a.splits = pl.few_splits;
         a.chunk2 = pl.many_chunk;
         a.splits2 = pl.many_splits;
-        const long long rows = (long long)a.p.tokens * num_q;
-        hipLaunchKernelGGL(k_paged_attn_join, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+        launch_join(s, a, splits);
         GH_TRY(check_launch("paged_attention join"));
     }
     count(CNT_ATTENTION);
