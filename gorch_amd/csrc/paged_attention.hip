@@ -392,33 +392,209 @@ __device__ __forceinline__ long long key_row(const PagedArgs& a, int s, int key,
     const uint32_t i = a.page.div((uint32_t)p);
     const int page = a.table[(size_t)s * a.max_pages + i];
     const long long row = ((long long)page * a.num_kv + kvh) * a.page.d + (p - (int)(i * a.page.d));
-    return key < k1 && (unsigned)page < (unsigned)a.num_pages ? row : -1;
+    return (key < k1) & ((unsigned)page < (unsigned)a.num_pages) ? row : -1;
 }
 
-// Few rows: a block takes 16 rows of a sequence (with their KV head) and a
-// range of its keys, its NW waves 32 keys each in turn. K goes from memory to
-// the operand registers, V through a wave's own LDS; NB tiles of rows are on
-// their way while one is weighed (a fetch is unconditional: a branch around
-// loads would make the next use wait for all of them).
-template <bool F8, int HD, bool PART>
-__global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void k_paged_attn_few(PagedAttnArgs a) {
+// A block's rows of which none sees a key: zeros (or an empty partial result).
+// (A path of its own: joined with the others before the loop over keys, it
+// makes the compiler wait there for every load in flight.)
+template <int BM>
+__device__ __forceinline__ void put_nothing(const PagedAttnArgs& a, int split, const SeqAt& s, int r0, int kvh) {
+    const int G = a.group.d, rows = min(BM, (s.end - s.begin) * G - r0), hd4 = a.p.hd / 4;
+    for (int i = threadIdx.x; i < rows * hd4; i += 256) {
+        const int r = r0 + i / hd4, c = 4 * (i % hd4), tok = (int)a.group.div((uint32_t)r);
+        const size_t row = (size_t)(s.begin + tok) * a.hq + kvh * G + (r - tok * G);
+        put(a, split, row, c, floatx4{0.f, 0.f, 0.f, 0.f}, 0.f);
+        if (a.splits > 1 && c == 0) a.part_ml[(size_t)split * a.p.tokens * a.hq + row] = make_float2(-INFINITY, 0.f);
+    }
+}
+
+// The rows of a wave that has few: CW (4, 8 or 16) query rows of one sequence,
+// a row in 16 / CW columns of the operand, each with terms of its own: with up
+// to 4 rows one matrix instruction makes all three terms' products, with up to
+// 8 two do (NP). A score is the sum of its row's columns, and a lane's weights
+// are the terms of its own columns; the columns of O are added at the end.
+// (One term a column against three instructions: 64 decoding conversations of
+// 2 rows per KV head, 200k tokens in e4m3, 101 -> FEWUS us.)
+template <bool F8, int HD, int CW>
+struct FewRows {
     using T = Tile<F8, HD>;
+    static constexpr int TP = 16 / CW;          // terms side by side
+    static constexpr int NP = (3 + TP - 1) / TP;
+    bf16x8 q[T::NU][NP];
+    floatx4 o[HD / 16];
+    float m, l;
+    int pos, first;
+
+    __device__ __forceinline__ static bf16x8 pick(const bf16x8 (&t)[3], int p) {
+        if constexpr (CW == 16) return t[p];
+        const int k = p * TP + (int)(threadIdx.x & 15) / CW;
+        const uint32_t is[3] = {k == 0 ? ~0u : 0u, k == 1 ? ~0u : 0u, k == 2 ? ~0u : 0u};
+        u32x4 r = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 3; i++) r |= __builtin_bit_cast(u32x4, t[i]) & is[i];
+        return __builtin_bit_cast(bf16x8, r);
+    }
+    template <bool PART>
+    __device__ __forceinline__ void fetch(const PagedAttnArgs& a, const SeqAt& s, int r0, int kvh, float4 (&x)[T::NU][2]) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, G = a.group.d, n = s.end - s.begin;
+        const int r = r0 + (lane & (CW - 1));
+        const int tok = (int)a.group.div((uint32_t)r), h = kvh * G + r - tok * G;
+        const bool live = r < n * G;
+        pos = live ? (a.causal ? s.len - n + tok : s.len - 1) : -1;
+        const float* zero = reinterpret_cast<const float*>(kZeros);
+        const float* src = a.q + ((size_t)(s.begin + tok) * a.hq + h) * a.p.hd;
+#pragma unroll
+        for (int u = 0; u < T::NU; u++) {
+            const int c = T::col(u, g);
+            const float* p = live && (!PART || c < a.p.hd) ? src + c : zero;
+            x[u][0] = *reinterpret_cast<const float4*>(p);
+            x[u][1] = *reinterpret_cast<const float4*>(p + 4);
+        }
+        first = a.causal ? s.len - n + (int)a.group.div((uint32_t)r0) : s.len - 1;
+    }
+    __device__ __forceinline__ void begin(const PagedAttnArgs& a, const float4 (&x)[T::NU][2]) {
+#pragma unroll
+        for (int u = 0; u < T::NU; u++) {
+            const float4 y = x[u][0], z = x[u][1];
+            const float f[8] = {y.x * a.scale, y.y * a.scale, y.z * a.scale, y.w * a.scale,
+                                z.x * a.scale, z.y * a.scale, z.z * a.scale, z.w * a.scale};
+            bf16x8 t[3];
+            split3(f, t);
+#pragma unroll
+            for (int p = 0; p < NP; p++) q[u][p] = pick(t, p);
+        }
+        clear();
+    }
+    __device__ __forceinline__ void clear() {
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++) o[d] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+    // scores of a group's 16 keys: lane group g holds keys 4 g .. 4 g + 3
+    __device__ __forceinline__ floatx4 score(const u32x4 (&c)[T::NT]) {
+        floatx4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < T::NU; u++) {
+            const bf16x8 k = T::frag(c, u);
+#pragma unroll
+            for (int p = NP - 1; p >= 0; p--) s = mfma16x16x32(k, q[u][p], s);
+        }
+        if constexpr (CW <= 8)
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[e] += dpp_f<0x128>(s[e]);  // 16 lanes rotated by 8
+        if constexpr (CW <= 4)
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[e] += dpp_f<0x124>(s[e]);  // and by 4
+        return s;
+    }
+    // a tile's 32 keys from key0 on (as Rows::take)
+    __device__ __forceinline__ void take(floatx4 (&sc)[2], int key0, uint32_t seen, const float* ksc, const float* vsc,
+                                         const char* vt) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, k = (lane & 15) / CW;
+        floatx4 vs[2];
+        if constexpr (F8) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const floatx4 ks = *reinterpret_cast<const floatx4*>(ksc + 16 * j + 4 * g);
+                vs[j] = *reinterpret_cast<const floatx4*>(vsc + 16 * j + 4 * g);
+#pragma unroll
+                for (int e = 0; e < 4; e++) sc[j][e] *= ks[e];
+            }
+        }
+        const bool edge = key0 + 31 > first || seen != 0xffffffffu;
+        if (edge) {
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int at = 16 * j + 4 * g + e;
+                    sc[j][e] = (seen >> at & 1u) && key0 + at <= pos ? sc[j][e] : -INFINITY;
+                }
+        }
+        float top = sc[0][0];
+#pragma unroll
+        for (int e = 1; e < 8; e++) top = fmaxf(top, sc[e >> 2][e & 3]);
+        const float mn = fmaxf(m, col_max(top)), use = mn == -INFINITY ? 0.f : mn;
+        const float al = __builtin_amdgcn_exp2f(m - use);
+        const bool grew = mn != m;
+        m = mn;
+        float w[8], sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            float x = __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] - use);
+            sum += x;
+            if constexpr (F8) {
+                x *= vs[e >> 2][e & 3];
+                if (edge) x = sc[e >> 2][e & 3] == -INFINITY ? 0.f : x;
+            }
+            w[e] = x;
+        }
+        l = l * al + sum;
+        bf16x8 p[NP];
+        if constexpr (CW == 4) {
+            // a term's leading bits are cut off by the packing: term k of x is
+            // x, what its first term leaves, or what both leave (the fourth
+            // column's sum is never looked at)
+            uint32_t u[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float r1 = w[e] - __uint_as_float(__float_as_uint(w[e]) & 0xffff0000u);
+                const float r2 = r1 - __uint_as_float(__float_as_uint(r1) & 0xffff0000u);
+                u[e] = __float_as_uint(k == 0 ? w[e] : (k == 1 ? r1 : r2));
+            }
+            uint32_t x[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = __builtin_amdgcn_perm(u[2 * e + 1], u[2 * e], 0x07060302u);
+            p[0] = __builtin_bit_cast(bf16x8, x);
+        } else {
+            bf16x8 t[3];
+            split3(w, t);
+#pragma unroll
+            for (int i = 0; i < NP; i++) p[i] = pick(t, i);
+        }
+        if (__any(grew)) {
+#pragma unroll
+            for (int d = 0; d < HD / 16; d++) o[d] *= al;
+        }
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++) {
+            const bf16x8 v = T::vfrag(vt, d, lane);
+#pragma unroll
+            for (int i = NP - 1; i >= 0; i--) o[d] = mfma16x16x32(v, p[i], o[d]);
+        }
+    }
+};
+
+// Few rows: a block takes CW rows of a sequence (with their KV head) and a
+// range of its keys, its four waves 32 keys each in turn. K goes from memory
+// to the operand registers, V through a wave's own LDS; NB tiles of rows are
+// on their way while one is weighed (a fetch is unconditional: a branch around
+// loads would make the next use wait for all of them).
+template <bool F8, int HD, bool PART, int CW>
+__global__ __launch_bounds__(256, HD > 128 ? 1 : (HD == 64 && CW < 16 ? 3 : 2)) void k_paged_attn_few(PagedAttnArgs a) {
+    using T = Tile<F8, HD>;
+    using R = FewRows<F8, HD, CW>;
     constexpr int NW = 4, STEP = 32 * NW, NB = T::NT <= 2 ? 2 : 1;
     constexpr int OROW = HD + 4;
     constexpr int STAGE = NW * (T::BYTES + 256), JOIN = NW * 16 * (OROW + 2) * 4;
     __shared__ __align__(16) char lds[STAGE > JOIN ? STAGE : JOIN];
-    __shared__ OddBits<16, HD> odd;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    __shared__ OddBits<CW, HD> odd;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     const int kvh = blockIdx.x % a.p.num_kv, rest = blockIdx.x / a.p.num_kv;
     const int tile = rest % a.tiles, split = rest / a.tiles;
     SeqAt s;
     int r0;
-    if (!find_tile<16>(a, tile, s, r0)) return;
+    if (!find_tile<CW>(a, tile, s, r0)) return;
     const int G = a.group.d, n = s.end - s.begin;
-    const int end_tok = (int)a.group.div((uint32_t)(min(r0 + 16, n * G) - 1));
+    const int end_tok = (int)a.group.div((uint32_t)(min(r0 + CW, n * G) - 1));
     const int T1 = min((a.causal ? s.len - n + end_tok : s.len - 1) + 1, a.p.limit);
     const int k0 = split * a.chunk, k1 = a.splits == 1 ? T1 : min(T1, k0 + a.chunk);
-    if (k0 >= k1 && split > 0) return;
+    if (k0 >= k1) {
+        if (split == 0) put_nothing<CW>(a, split, s, r0, kvh);
+        return;
+    }
 
     char* vt = lds + wave * (T::BYTES + 256);
     float* sc = reinterpret_cast<float*>(vt + T::BYTES);  // K scales of the 32 keys, then V's
@@ -443,68 +619,69 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void k_paged_attn_few(PagedA
         for (int j = 0; j < 2; j++)
             fetch_row<F8, HD, PART>(a.p.v, (long long)(((uint64_t)hi[j] << 32) | lo[j]), a.p.hd, g, b.v[j]);
     };
-    Rows<F8, HD, 1> rows;
+    R rows;
     int key0 = k0 + 32 * wave;
-    long long next = -1;
-    if (k0 < k1) {
+    long long next;
+    {
         long long r[NB];
 #pragma unroll
         for (int i = 0; i < NB; i++) r[i] = key_row(a.p, s.s, key0 + i * STEP + (lane & 31), k1, kvh);
         next = key_row(a.p, s.s, key0 + NB * STEP + (lane & 31), k1, kvh);
-        float4 x[1][T::NU][2];
+        float4 x[T::NU][2];
         rows.template fetch<PART>(a, s, r0, kvh, x);
 #pragma unroll
         for (int i = 0; i < NB; i++) fetch(r[i], buf[i]);
         for (int i = threadIdx.x; i < (int)(sizeof(odd) / 4); i += 64 * NW) reinterpret_cast<uint32_t*>(&odd)[i] = 0;
         rows.begin(a, x);
-    } else {
-        // no key is seen: zeros
-        rows.m[0] = -INFINITY;
-        rows.l[0] = 0.f;
-        for (int d = 0; d < HD / 16; d++) rows.o[0][d] = floatx4{0.f, 0.f, 0.f, 0.f};
-        if (threadIdx.x == 0) odd.any = 0;
     }
     __syncthreads();
+    // (what is fetched does not depend on whether a tile is past the end, so
+    // the loads in flight are the same on every way to the next tile)
     auto step = [&](Buf& b, int key) {
-        floatx4 scores[2][1];
-        rows.score(b.k[0], scores[0]);
-        rows.score(b.k[1], scores[1]);
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-#pragma unroll
-            for (int t = 0; t < T::NT; t++) *reinterpret_cast<u32x4*>(vt + j * T::GROUP + t * 1024 + lane * 16) = b.v[j][t];
-        if (__any(any_nonfinite<F8>(b.v[0]) || any_nonfinite<F8>(b.v[1])))
-#pragma unroll 1
-            for (int j = 0; j < 2; j++)
-                clean_odd<F8, 16, HD>(odd, a, s, r0, key + 16 * j + (lane & 15), g, vt + j * T::GROUP + lane * 16);
-        if constexpr (F8) sc[lane] = b.scale;
+        const bool on = key < k1;
         const uint32_t here = b.seen;
-        fetch(next, b);
-        next = key_row(a.p, s.s, key + (NB + 1) * STEP + (lane & 31), k1, kvh);
-        rows.take(scores, key, here, sc, sc + 32, vt);
-    };
-    while (key0 < k1) {
+        floatx4 scores[2];
+        if (on) {
+            scores[0] = rows.score(b.k[0]);
+            scores[1] = rows.score(b.k[1]);
 #pragma unroll
-        for (int i = 0; i < NB; i++) {
-            if (i == 0 || key0 < k1) step(buf[i], key0);
-            key0 += STEP;
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int t = 0; t < T::NT; t++)
+                    *reinterpret_cast<u32x4*>(vt + j * T::GROUP + t * 1024 + lane * 16) = b.v[j][t];
+            if (__any(any_nonfinite<F8>(b.v[0]) | any_nonfinite<F8>(b.v[1])))
+#pragma unroll 1
+                for (int j = 0; j < 2; j++)
+                    clean_odd<F8, CW, HD>(odd, a, s, r0, key + 16 * j + (lane & 15), g, vt + j * T::GROUP + lane * 16);
+            if constexpr (F8) sc[lane] = b.scale;
         }
+        // (the page of the tile after goes out first: loads are waited for in
+        // order, and the next fetch waits for it)
+        const long long after = key_row(a.p, s.s, key + (NB + 1) * STEP + (lane & 31), k1, kvh);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(next, b);
+        next = after;
+        if (on) rows.take(scores, key, here, sc, sc + 32, vt);
+    };
+    for (; key0 < k1; key0 += NB * STEP) {
+        step(buf[0], key0);
+        if constexpr (NB == 2) step(buf[1], key0 + STEP);
     }
     // the waves' sums, joined in wave order
     __syncthreads();
     float* jo = reinterpret_cast<float*>(lds);
     float* jm = jo + NW * 16 * OROW;
     float* jl = jm + NW * 16;
-    const float l = col_sum(rows.l[0]);
+    const float l = col_sum(rows.l);
 #pragma unroll
     for (int d = 0; d < HD / 16; d++)
-        *reinterpret_cast<floatx4*>(jo + (wave * 16 + (lane & 15)) * OROW + 16 * d + 4 * g) = rows.o[0][d];
+        *reinterpret_cast<floatx4*>(jo + (wave * 16 + (lane & 15)) * OROW + 16 * d + 4 * g) = rows.o[d];
     if (g == 0) {
-        jm[wave * 16 + lane] = rows.m[0];
+        jm[wave * 16 + lane] = rows.m;
         jl[wave * 16 + lane] = l;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * (HD / 4); i += 64 * NW) {
+    for (int i = threadIdx.x; i < CW * (HD / 4); i += 64 * NW) {
         const int r = i / (HD / 4), c = 4 * (i % (HD / 4));
         if (r0 + r >= n * G || (PART && c >= a.p.hd)) continue;
         float M = jm[r];
@@ -517,8 +694,12 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void k_paged_attn_few(PagedA
         for (int w = 0; w < NW; w++) {
             const float f = __builtin_amdgcn_exp2f(jm[w * 16 + r] - use);
             L += f * jl[w * 16 + r];
-            const floatx4 x = *reinterpret_cast<const floatx4*>(jo + (w * 16 + r) * OROW + c);
-            for (int e = 0; e < 4; e++) o[e] += f * x[e];
+#pragma unroll
+            for (int t = 0; t < 3 && t < R::TP; t++) {
+                const floatx4 x = *reinterpret_cast<const floatx4*>(jo + (w * 16 + t * CW + r) * OROW + c);
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[e] += f * x[e];
+            }
         }
         if (odd.any) o = add_odd(odd, r, c, o);
         const int tok = (int)a.group.div((uint32_t)(r0 + r));
@@ -538,7 +719,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
     __shared__ __align__(16) float sc[2][2][32];  // scales of K and of V
     __shared__ uint32_t seen_of[2][2];
     __shared__ OddBits<64 * NR, HD> odd;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     const int kvh = blockIdx.x % a.p.num_kv, rest = blockIdx.x / a.p.num_kv;
     // the last rows of a sequence see the most keys: they go first
     const int tile = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
@@ -553,7 +734,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
     const int end_tok = (int)a.group.div((uint32_t)(min(r0 + 64 * NR, n * G) - 1));
     const int T1 = min((a.causal ? s.len - n + end_tok : s.len - 1) + 1, a.p.limit);
     const int k0 = split * a.chunk, k1 = a.splits == 1 ? T1 : min(T1, k0 + a.chunk);
-    if (k0 >= k1 && split > 0) return;
+    if (k0 >= k1) {
+        if (split == 0) put_nothing<64 * NR>(a, split, s, r0, kvh);
+        return;
+    }
 
     // waves 0 and 1 fetch K's two groups, 2 and 3 V's
     const int j = wave & 1;
@@ -582,16 +766,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
     };
     for (int i = threadIdx.x; i < (int)(sizeof(odd) / 4); i += 256) reinterpret_cast<uint32_t*>(&odd)[i] = 0;
     __syncthreads();
-    long long next = -1;
-    if (k0 < k1) {
-        next = lookup(k0);
-        fetch(next, k0);
-        next = lookup(k0 + 32);
-        rows.begin(a, qx);
-        stage(0);
-    } else {
-        rows.begin(a, qx);
-    }
+    long long next = lookup(k0);
+    fetch(next, k0);
+    next = lookup(k0 + 32);
+    rows.begin(a, qx);
+    stage(0);
     __syncthreads();
     for (int key0 = k0, b = 0; key0 < k1; key0 += 32, b ^= 1) {
         const bool more = key0 + 32 < k1;
@@ -696,13 +875,15 @@ __global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttnArgs a) {
 
 struct AttnPlan {
     bool few, many;
+    int few_width;  // rows of a tile of the kernel for few rows: 4, 8 or 16
+    int few_rows;   // sequences of up to so many rows go to it
     int few_tiles, many_tiles;
     int few_chunk, few_splits, many_chunk, many_splits;
     size_t bytes;
 };
 
-// Rows (tokens x heads of a group) up to which a sequence goes to the kernel
-// for few rows.
+// Rows (tokens x heads of a group) up to which a batch whose sequences have no
+// more goes to the kernel for few rows alone.
 constexpr int kFewRows = 32;
 
 static int many_rows(int hd) { return hd <= 128 ? 128 : 64; }
@@ -711,10 +892,14 @@ static AttnPlan attn_plan(const PagedArgs& p, int hq, int max_new) {
     AttnPlan r{};
     const long long G = hq / p.num_kv;
     const long long most = std::min<long long>(max_new > 0 ? max_new : p.tokens, p.tokens) * G;
-    r.few = most <= kFewRows || p.seqs > 1;
     r.many = most > kFewRows;
+    // beside prompts, the kernel for few rows takes the single tokens
+    const long long rows = r.many ? G : most;
+    r.few_width = rows <= 4 ? 4 : (rows <= 8 ? 8 : 16);
+    r.few_rows = !r.many ? 0x7fffffff : (r.few_width < 16 ? r.few_width : kFewRows);
+    r.few = !r.many || p.seqs > 1;
     const int bm = many_rows(p.hd);
-    r.few_tiles = (int)(p.tokens * G / 16) + p.seqs;
+    r.few_tiles = (int)(p.tokens * G / r.few_width) + p.seqs;
     r.many_tiles = (int)(p.tokens * G / bm) + p.seqs;
     // tiles that are expected to have work, and the splits of the longest
     // sequence that fill the chip with them
@@ -726,7 +911,7 @@ static AttnPlan attn_plan(const PagedArgs& p, int hq, int max_new) {
         chunk = (int)std::min<long long>(per * unit, 0x7fffff00);
         return (int)((units + per - 1) / per);
     };
-    const long long few_real = std::min<long long>(r.few_tiles, p.seqs * ((std::min<long long>(most, kFewRows) + 15) / 16));
+    const long long few_real = std::min<long long>(r.few_tiles, p.seqs * ((rows + r.few_width - 1) / r.few_width));
     const long long many_real = std::min<long long>(r.many_tiles, p.seqs * ((most + bm - 1) / bm));
     r.few_splits = r.few ? splits(few_real, 2048, 256, r.few_chunk) : 1;
     r.many_splits = r.many ? splits(many_real, 512, 256, r.many_chunk) : 1;
@@ -752,16 +937,18 @@ static void launch_attn(hipStream_t s, const PagedAttnArgs& base, const AttnPlan
         PagedAttnArgs a = base;
         a.tiles = pl.few_tiles;
         a.lo_rows = 0;
-        a.hi_rows = pl.many ? kFewRows : 0x7fffffff;
+        a.hi_rows = pl.few_rows;
         a.chunk = pl.few_chunk;
         a.splits = pl.few_splits;
-        hipLaunchKernelGGL((k_paged_attn_few<F8, HD, PART>), dim3((unsigned)a.tiles * a.p.num_kv * a.splits), dim3(256), 0,
-                           s, a);
+        const dim3 grid((unsigned)a.tiles * a.p.num_kv * a.splits);
+        if (pl.few_width == 4) hipLaunchKernelGGL((k_paged_attn_few<F8, HD, PART, 4>), grid, dim3(256), 0, s, a);
+        else if (pl.few_width == 8) hipLaunchKernelGGL((k_paged_attn_few<F8, HD, PART, 8>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((k_paged_attn_few<F8, HD, PART, 16>), grid, dim3(256), 0, s, a);
     }
     if (pl.many) {
         PagedAttnArgs a = base;
         a.tiles = pl.many_tiles;
-        a.lo_rows = pl.few ? kFewRows + 1 : 0;
+        a.lo_rows = pl.few ? pl.few_rows + 1 : 0;
         a.hi_rows = 0x7fffffff;
         a.chunk = pl.many_chunk;
         a.splits = pl.many_splits;
@@ -830,7 +1017,7 @@ extern "C" int gorch_hip_paged_attention(void* stream, const gorch_hip_paged_kv*
     else launch_attn_hd<false>(s, a, pl);
     GH_TRY(check_launch("paged_attention"));
     if (splits > 1) {
-        a.hi_rows = pl.few ? (pl.many ? kFewRows : 0x7fffffff) : -1;
+        a.hi_rows = pl.few ? pl.few_rows : -1;
         a.chunk = pl.few_chunk;
         a.splits = pl.few_splits;
         a.chunk2 = pl.many_chunk;
