@@ -41,6 +41,7 @@ struct PagedAttnArgs {
     int tiles;       // row tiles of this kernel's grid
     int lo_rows, hi_rows;  // this kernel takes sequences of lo_rows <= rows <= hi_rows
     int chunk, splits;     // keys of a split; splits == 1: no partial results
+    int last_first;        // the blocks of the last splits go first
     // the joining kernel: the other kernel's chunk and splits, for sequences
     // of more than hi_rows rows
     int chunk2, splits2;
@@ -146,7 +147,7 @@ struct Tile {
 // (NaN: both) for the column: bits [0 / 1][row][column] in LDS, added to the
 // sums at the end. All that an ordinary tile pays is the test.
 template <bool F8, int N>
-__device__ __forceinline__ bool any_nonfinite(const u32x4 (&c)[N]) {
+__device__ __forceinline__ int any_nonfinite(const u32x4 (&c)[N]) {
     if constexpr (F8) {
         uint32_t m = 0;
 #pragma unroll
@@ -168,23 +169,22 @@ template <int BM, int HD>
 struct OddBits {
     uint32_t any, bits[2][BM][HD / 32];
 };
-// A lane's chunks of key `key` in LDS (mine, 1 KB apart); the block's rows are
-// r0 .. r0 + BM - 1 of sequence s.
+// One chunk of key `key` in LDS, columns col0 on; the block's rows are r0 .. r0
+// + BM - 1 of sequence s.
 template <bool F8, int BM, int HD>
 __device__ __forceinline__ void clean_odd(OddBits<BM, HD>& odd, const PagedAttnArgs& a, const SeqAt& s, int r0, int key,
-                                          int g, char* mine) {
-    constexpr int PER = F8 ? 16 : 8;
+                                          int col0, char* chunk) {
     const int G = a.group.d, n = s.end - s.begin;
 #pragma unroll 1
-    for (int i = 0; i < Tile<F8, HD>::NT * PER; i++) {
-        const int t = i / PER, e = i % PER, col = (4 * t + g) * PER + e;
+    for (int e = 0; e < (F8 ? 16 : 8); e++) {
+        const int col = col0 + e;
         bool up, down;
         if constexpr (F8) {  // no infinities, NaN is 0x7f
-            uint8_t* x = reinterpret_cast<uint8_t*>(mine + t * 1024) + e;
+            uint8_t* x = reinterpret_cast<uint8_t*>(chunk) + e;
             up = down = (*x & 0x7f) == 0x7f;
             if (up) *x = 0;
         } else {
-            uint16_t* x = reinterpret_cast<uint16_t*>(mine + t * 1024) + e;
+            uint16_t* x = reinterpret_cast<uint16_t*>(chunk) + e;
             const int v = *x, m = v & 0x7fff;
             up = m > 0x7f80 || v == 0x7f80;
             down = m > 0x7f80 || v == 0xff80;
@@ -300,8 +300,8 @@ struct Rows {
         if constexpr (F8) {
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                ks[j] = *reinterpret_cast<const floatx4*>(ksc + 16 * j + 4 * g);
-                vs[j] = *reinterpret_cast<const floatx4*>(vsc + 16 * j + 4 * g);
+                ks[j] = *reinterpret_cast<const floatx4*>(ksc + 64 * j + 4 * g);
+                vs[j] = *reinterpret_cast<const floatx4*>(vsc + 64 * j + 4 * g);
             }
         }
         const bool edge = key0 + 31 > first || seen != 0xffffffffu;  // some row does not see some key
@@ -351,13 +351,17 @@ struct Rows {
 #pragma unroll
                 for (int d = 0; d < HD / 16; d++) o[i][d] *= al[i];
         }
+        // the next columns' operands are read while these are multiplied
+        bf16x8 v = T::vfrag(vt, 0, lane);
 #pragma unroll
         for (int d = 0; d < HD / 16; d++) {
-            const bf16x8 v = T::vfrag(vt, d, lane);
+            const bf16x8 ahead = d + 1 < HD / 16 ? T::vfrag(vt, d + 1, lane) : v;
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int t = 2; t >= 0; t--)
 #pragma unroll
                 for (int i = 0; i < NR; i++) o[i][d] = mfma16x16x32(v, p[i][t], o[i][d]);
+            v = ahead;
         }
     }
 };
@@ -385,14 +389,17 @@ __device__ __forceinline__ void put(const PagedAttnArgs& a, int split, size_t ro
     }
 }
 
-// The pool row of key `key` of a sequence, -1 if it is not below k1 or on no
-// page; no branch around the load (0 < k1 <= limit).
-__device__ __forceinline__ long long key_row(const PagedArgs& a, int s, int key, int k1, int kvh) {
+// The page that holds key `key` of a sequence (of key k1 - 1 for those past it;
+// 0 < k1 <= limit), no branch around the load; and the pool row of the key
+// there, -1 if it is not below k1 or on no page.
+__device__ __forceinline__ int key_page(const PagedArgs& a, int s, int key, int k1) {
+    return a.table[(size_t)s * a.max_pages + a.page.div((uint32_t)min(key, k1 - 1))];
+}
+__device__ __forceinline__ long long key_row(const PagedArgs& a, int page, int key, int k1, int kvh) {
     const int p = min(key, k1 - 1);
-    const uint32_t i = a.page.div((uint32_t)p);
-    const int page = a.table[(size_t)s * a.max_pages + i];
-    const long long row = ((long long)page * a.num_kv + kvh) * a.page.d + (p - (int)(i * a.page.d));
-    return (key < k1) & ((unsigned)page < (unsigned)a.num_pages) ? row : -1;
+    const long long row = ((long long)page * a.num_kv + kvh) * a.page.d + (p - (int)(a.page.div((uint32_t)p) * a.page.d));
+    const int there = (key < k1 ? 1 : 0) & ((unsigned)page < (unsigned)a.num_pages ? 1 : 0);
+    return there ? row : -1;
 }
 
 // A block's rows of which none sees a key: zeros (or an empty partial result).
@@ -401,7 +408,7 @@ __device__ __forceinline__ long long key_row(const PagedArgs& a, int s, int key,
 template <int BM>
 __device__ __forceinline__ void put_nothing(const PagedAttnArgs& a, int split, const SeqAt& s, int r0, int kvh) {
     const int G = a.group.d, rows = min(BM, (s.end - s.begin) * G - r0), hd4 = a.p.hd / 4;
-    for (int i = threadIdx.x; i < rows * hd4; i += 256) {
+    for (int i = threadIdx.x; i < rows * hd4; i += blockDim.x) {
         const int r = r0 + i / hd4, c = 4 * (i % hd4), tok = (int)a.group.div((uint32_t)r);
         const size_t row = (size_t)(s.begin + tok) * a.hq + kvh * G + (r - tok * G);
         put(a, split, row, c, floatx4{0.f, 0.f, 0.f, 0.f}, 0.f);
@@ -583,7 +590,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : (HD == 64 && CW < 16 ? 3 : 2)) 
     __shared__ OddBits<CW, HD> odd;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     const int kvh = blockIdx.x % a.p.num_kv, rest = blockIdx.x / a.p.num_kv;
-    const int tile = rest % a.tiles, split = rest / a.tiles;
+    const int tile = rest % a.tiles, split = a.last_first ? a.splits - 1 - rest / a.tiles : rest / a.tiles;
     SeqAt s;
     int r0;
     if (!find_tile<CW>(a, tile, s, r0)) return;
@@ -621,16 +628,16 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : (HD == 64 && CW < 16 ? 3 : 2)) 
     };
     R rows;
     int key0 = k0 + 32 * wave;
-    long long next;
+    int next;  // the page of the next tile to fetch
     {
-        long long r[NB];
+        int page[NB];
 #pragma unroll
-        for (int i = 0; i < NB; i++) r[i] = key_row(a.p, s.s, key0 + i * STEP + (lane & 31), k1, kvh);
-        next = key_row(a.p, s.s, key0 + NB * STEP + (lane & 31), k1, kvh);
+        for (int i = 0; i < NB; i++) page[i] = key_page(a.p, s.s, key0 + i * STEP + (lane & 31), k1);
+        next = key_page(a.p, s.s, key0 + NB * STEP + (lane & 31), k1);
         float4 x[T::NU][2];
         rows.template fetch<PART>(a, s, r0, kvh, x);
 #pragma unroll
-        for (int i = 0; i < NB; i++) fetch(r[i], buf[i]);
+        for (int i = 0; i < NB; i++) fetch(key_row(a.p, page[i], key0 + i * STEP + (lane & 31), k1, kvh), buf[i]);
         for (int i = threadIdx.x; i < (int)(sizeof(odd) / 4); i += 64 * NW) reinterpret_cast<uint32_t*>(&odd)[i] = 0;
         rows.begin(a, x);
     }
@@ -651,15 +658,18 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : (HD == 64 && CW < 16 ? 3 : 2)) 
                     *reinterpret_cast<u32x4*>(vt + j * T::GROUP + t * 1024 + lane * 16) = b.v[j][t];
             if (__any(any_nonfinite<F8>(b.v[0]) | any_nonfinite<F8>(b.v[1])))
 #pragma unroll 1
-                for (int j = 0; j < 2; j++)
-                    clean_odd<F8, CW, HD>(odd, a, s, r0, key + 16 * j + (lane & 15), g, vt + j * T::GROUP + lane * 16);
+                for (int i = 0; i < 2 * T::NT; i++) {
+                    const int j = i & 1, t = i >> 1;
+                    clean_odd<F8, CW, HD>(odd, a, s, r0, key + 16 * j + (lane & 15), (4 * t + g) * (16 / T::ES),
+                                          vt + j * T::GROUP + t * 1024 + lane * 16);
+                }
             if constexpr (F8) sc[lane] = b.scale;
         }
         // (the page of the tile after goes out first: loads are waited for in
         // order, and the next fetch waits for it)
-        const long long after = key_row(a.p, s.s, key + (NB + 1) * STEP + (lane & 31), k1, kvh);
+        const int after = key_page(a.p, s.s, key + (NB + 1) * STEP + (lane & 31), k1);
         __builtin_amdgcn_sched_barrier(0);
-        fetch(next, b);
+        fetch(key_row(a.p, next, key + NB * STEP + (lane & 31), k1, kvh), b);
         next = after;
         if (on) rows.take(scores, key, here, sc, sc + 32, vt);
     };
@@ -709,75 +719,96 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : (HD == 64 && CW < 16 ? 3 : 2)) 
     }
 }
 
-// Many rows: a block takes 64 NR rows of a sequence, 16 NR a wave, and its keys
-// (or a range of them) in tiles of 32 that all four waves read from LDS; two
-// tiles in LDS, the one after in registers.
+// Many rows: a block takes 128 rows of a sequence, 16 NR a wave, and its keys
+// (or a range of them) in tiles of 32 that all NW waves read from LDS. Loads
+// go straight to LDS, two tiles ahead of the one that is weighed: one on its
+// way, one landed, in which the waves look for infinities in V.
+constexpr int kManyRows = 128;
 template <bool F8, int HD, bool PART, int NR>
-__global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
+__global__ __launch_bounds__(kManyRows / NR * 4, 2) void k_paged_attn_many(PagedAttnArgs a) {
     using T = Tile<F8, HD>;
-    __shared__ __align__(16) char kt[2][T::BYTES], vt[2][T::BYTES];
-    __shared__ __align__(16) float sc[2][2][32];  // scales of K and of V
-    __shared__ uint32_t seen_of[2][2];
-    __shared__ OddBits<64 * NR, HD> odd;
+    constexpr int BM = kManyRows, NW = BM / (16 * NR);
+    __shared__ __align__(16) char kt[3][T::BYTES], vt[3][T::BYTES];
+    __shared__ __align__(16) float sc[3][4][64];  // e4m3 scales: K's two groups, V's two (16 each)
+    __shared__ uint32_t seen_of[3][2];
+    __shared__ OddBits<BM, HD> odd;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     const int kvh = blockIdx.x % a.p.num_kv, rest = blockIdx.x / a.p.num_kv;
     // the last rows of a sequence see the most keys: they go first
     const int tile = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
     SeqAt s;
     int r0;
-    if (!find_tile<64 * NR>(a, tile, s, r0)) return;
+    if (!find_tile<BM>(a, tile, s, r0)) return;
     const int G = a.group.d, n = s.end - s.begin;
-    Rows<F8, HD, NR> rows;
-    float4 qx[NR][T::NU][2];
-    rows.template fetch<PART>(a, s, r0 + 16 * NR * wave, kvh, qx);
     // the last position that any of the block's rows sees
-    const int end_tok = (int)a.group.div((uint32_t)(min(r0 + 64 * NR, n * G) - 1));
+    const int end_tok = (int)a.group.div((uint32_t)(min(r0 + BM, n * G) - 1));
     const int T1 = min((a.causal ? s.len - n + end_tok : s.len - 1) + 1, a.p.limit);
     const int k0 = split * a.chunk, k1 = a.splits == 1 ? T1 : min(T1, k0 + a.chunk);
     if (k0 >= k1) {
-        if (split == 0) put_nothing<64 * NR>(a, split, s, r0, kvh);
+        if (split == 0) put_nothing<BM>(a, split, s, r0, kvh);
         return;
     }
 
-    // waves 0 and 1 fetch K's two groups, 2 and 3 V's
+    // of four waves, 0 and 1 fetch K's two groups of a tile, 2 and 3 V's
     const int j = wave & 1;
-    const bool isv = wave >= 2;
-    u32x4 st[T::NT];
-    float scale = 0.f;
-    long long row = -1;
-    auto lookup = [&](int key0) { return key_row(a.p, s.s, key0 + 16 * j + (lane & 15), k1, kvh); };
-    int at0 = 0;
-    auto fetch = [&](long long r, int key0) {
-        row = r;
-        at0 = key0;
-        fetch_row<F8, HD, PART>(isv ? a.p.v : a.p.k, r, a.p.hd, g, st);
-        if constexpr (F8) scale = *(r >= 0 ? (isv ? a.p.vs : a.p.ks) + r : reinterpret_cast<const float*>(kZeros));
-    };
-    auto stage = [&](int b) {
-        char* to = (isv ? vt[b] : kt[b]) + j * T::GROUP + lane * 16;
+    const bool isv = (wave & 2) != 0;
+    auto page_of = [&](int key0) { return key_page(a.p, s.s, key0 + 16 * j + (lane & 15), k1); };
+    auto fetch = [&](int page, int key0, int b) {
+        const long long row = key_row(a.p, page, key0 + 16 * j + (lane & 15), k1, kvh);
+        typedef __attribute__((address_space(1))) const uint32_t* global_ptr;
+        typedef GH_LDS uint32_t* lds_ptr;
+        const char* zero = reinterpret_cast<const char*>(kZeros);
+        const char* p = row >= 0 ? static_cast<const char*>(isv ? a.p.v : a.p.k) + row * (a.p.hd * T::ES) : zero;
+        char* to = (isv ? vt[b] : kt[b]) + j * T::GROUP;
 #pragma unroll
-        for (int t = 0; t < T::NT; t++) *reinterpret_cast<u32x4*>(to + t * 1024) = st[t];
-        if (isv && __any(any_nonfinite<F8>(st)))
-            clean_odd<F8, 64 * NR, HD>(odd, a, s, r0, at0 + 16 * j + (lane & 15), g, to);
-        if constexpr (F8)
-            if (lane < 16) sc[b][isv][16 * j + lane] = scale;
-        const uint32_t here = (uint32_t)__ballot(row >= 0) & 0xffffu;
-        if (lane == 0 && !isv) seen_of[b][j] = here;
-    };
-    for (int i = threadIdx.x; i < (int)(sizeof(odd) / 4); i += 256) reinterpret_cast<uint32_t*>(&odd)[i] = 0;
-    __syncthreads();
-    long long next = lookup(k0);
-    fetch(next, k0);
-    next = lookup(k0 + 32);
-    rows.begin(a, qx);
-    stage(0);
-    __syncthreads();
-    for (int key0 = k0, b = 0; key0 < k1; key0 += 32, b ^= 1) {
-        const bool more = key0 + 32 < k1;
-        if (more) {
-            fetch(next, key0 + 32);
-            next = lookup(key0 + 64);
+        for (int t0 = 0; t0 < T::NT; t0 += NW / 4) {
+            const int t = t0 + (wave >> 2), o = (4 * t + g) * 16;
+            __builtin_amdgcn_global_load_lds((global_ptr)(PART && o >= a.p.hd * T::ES ? zero : p + o),
+                                             (lds_ptr)(to + t * 1024), 16, 0, 0);
         }
+        if (F8 && wave < 4) {
+            const float* f = row >= 0 ? (isv ? a.p.vs : a.p.ks) + row : reinterpret_cast<const float*>(kZeros);
+            __builtin_amdgcn_global_load_lds((global_ptr)f, (lds_ptr)sc[b][wave], 4, 0, 0);
+        }
+        const uint32_t here = (uint32_t)__ballot(row >= 0) & 0xffffu;
+        if (lane == 0 && wave < 2) seen_of[b][j] = here;
+    };
+    // a wave's share of a landed tile's V
+    auto check = [&](int key0, int b) {
+        int any = 0;
+#pragma unroll
+        for (int i0 = 0; i0 < 2 * T::NT; i0 += NW) {
+            const int i = i0 + wave;
+            if (2 * T::NT % NW != 0 && i >= 2 * T::NT) break;
+            u32x4 c[1] = {*reinterpret_cast<const u32x4*>(vt[b] + (i & 1) * T::GROUP + (i >> 1) * 1024 + lane * 16)};
+            any |= any_nonfinite<F8>(c);
+        }
+        if (__any(any))
+#pragma unroll 1
+            for (int i = wave; i < 2 * T::NT; i += NW)
+                clean_odd<F8, BM, HD>(odd, a, s, r0, key0 + 16 * (i & 1) + (lane & 15),
+                                           (4 * (i >> 1) + g) * (16 / T::ES),
+                                           vt[b] + (i & 1) * T::GROUP + (i >> 1) * 1024 + lane * 16);
+    };
+    Rows<F8, HD, NR> rows;
+    int next = page_of(k0 + 32);
+    fetch(page_of(k0), k0, 0);
+    {
+        float4 x[NR][T::NU][2];
+        rows.template fetch<PART>(a, s, r0 + 16 * NR * wave, kvh, x);
+        fetch(next, k0 + 32, 1);
+        next = page_of(k0 + 64);
+        for (int i = threadIdx.x; i < (int)(sizeof(odd) / 4); i += 64 * NW) reinterpret_cast<uint32_t*>(&odd)[i] = 0;
+        rows.begin(a, x);
+    }
+    block_sync_dma();
+    check(k0, 0);
+    block_sync_dma();
+    for (int key0 = k0, b = 0; key0 < k1; key0 += 32) {
+        const int b1 = b == 2 ? 0 : b + 1, b2 = b1 == 2 ? 0 : b1 + 1;
+        const int after = page_of(key0 + 96);
+        fetch(next, key0 + 64, b2);
+        next = after;
         if (key0 <= rows.last) {
             floatx4 scores[2][NR];
 #pragma unroll
@@ -788,11 +819,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
                     c[t] = *reinterpret_cast<const u32x4*>(kt[b] + jj * T::GROUP + t * 1024 + lane * 16);
                 rows.score(c, scores[jj]);
             }
-            const uint32_t seen = seen_of[b][0] | (seen_of[b][1] << 16);
-            rows.take(scores, key0, seen, sc[b][0], sc[b][1], vt[b]);
+            rows.take(scores, key0, seen_of[b][0] | (seen_of[b][1] << 16), sc[b][0], sc[b][2], vt[b]);
         }
-        if (more) stage(b ^ 1);
-        __syncthreads();
+        check(key0 + 32, b1);
+        block_sync_dma();
+        b = b1;
     }
 #pragma unroll
     for (int i = 0; i < NR; i++) {
@@ -816,7 +847,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
 // splits dealt to SLOTS groups of lanes (sums in a fixed order: a slot's
 // splits, then the slots). The first loads go out before the sequence is
 // known; splits past the row's last are then left out.
-constexpr int kMaxSplits = 128;
+constexpr int kMaxSplits = 64;
 template <int NL, int WPR>
 __global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttnArgs a) {
     constexpr int SLOTS = WPR * 64 / NL, RPB = 4 / WPR;
@@ -826,9 +857,7 @@ __global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttnArgs a) {
     const long long row = min(__builtin_amdgcn_readfirstlane(blockIdx.x * RPB + sub), (int)total - 1);
     const bool mine = (long long)blockIdx.x * RPB + sub < total;
     const int c = tid % NL, slot = tid / NL, col = min(4 * c, a.p.hd - 4), most = max(a.splits, a.splits2);
-    float2 ml[2];
-#pragma unroll
-    for (int i = 0; i < 2; i++) ml[i] = a.part_ml[min(lane + 64 * i, most - 1) * total + row];
+    float2 ml = a.part_ml[min(lane, most - 1) * total + row];
     auto part = [&](int j) {
         return *reinterpret_cast<const floatx4*>(a.part_o + (min(j, most - 1) * total + row) * a.p.hd + col);
     };
@@ -842,19 +871,14 @@ __global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttnArgs a) {
         const int T = min(a.causal ? s.len - s.end + t + 1 : s.len, a.p.limit);
         nc = splits == 1 ? 0 : min(max((T + chunk - 1) / chunk, 1), splits);  // (one split: out is written)
     }
-    float top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        if (lane + 64 * i >= nc) ml[i] = make_float2(-INFINITY, 0.f);
-        top = fmaxf(top, ml[i].x);
-    }
-    const float M = wave_max(top), use = M == -INFINITY ? 0.f : M;
-    const float w0 = __builtin_amdgcn_exp2f(ml[0].x - use), w1 = __builtin_amdgcn_exp2f(ml[1].x - use);
-    const float L = wave_sum(w0 * ml[0].y + w1 * ml[1].y);
+    if (lane >= nc) ml = make_float2(-INFINITY, 0.f);
+    const float M = wave_max(ml.x), use = M == -INFINITY ? 0.f : M;
+    const float w = __builtin_amdgcn_exp2f(ml.x - use);
+    const float L = wave_sum(w * ml.y);
     floatx4 o = {0.f, 0.f, 0.f, 0.f};
     for (int j = slot; j - slot < nc; j += SLOTS) {
         const floatx4 y = part(j + SLOTS);
-        const float f = __shfl(j < 64 ? w0 : w1, j & 63);
+        const float f = __shfl(w, j & 63);
         if (j < nc)
 #pragma unroll
             for (int e = 0; e < 4; e++) o[e] += f * x[e];
@@ -879,14 +903,13 @@ struct AttnPlan {
     int few_rows;   // sequences of up to so many rows go to it
     int few_tiles, many_tiles;
     int few_chunk, few_splits, many_chunk, many_splits;
+    bool few_last_first;
     size_t bytes;
 };
 
 // Rows (tokens x heads of a group) up to which a batch whose sequences have no
 // more goes to the kernel for few rows alone.
 constexpr int kFewRows = 32;
-
-static int many_rows(int hd) { return hd <= 128 ? 128 : 64; }
 
 static AttnPlan attn_plan(const PagedArgs& p, int hq, int max_new) {
     AttnPlan r{};
@@ -898,23 +921,35 @@ static AttnPlan attn_plan(const PagedArgs& p, int hq, int max_new) {
     r.few_width = rows <= 4 ? 4 : (rows <= 8 ? 8 : 16);
     r.few_rows = !r.many ? 0x7fffffff : (r.few_width < 16 ? r.few_width : kFewRows);
     r.few = !r.many || p.seqs > 1;
-    const int bm = many_rows(p.hd);
+    const int bm = kManyRows;
     r.few_tiles = (int)(p.tokens * G / r.few_width) + p.seqs;
     r.many_tiles = (int)(p.tokens * G / bm) + p.seqs;
-    // tiles that are expected to have work, and the splits of the longest
-    // sequence that fill the chip with them
-    const auto splits = [&](long long tiles, long long want, int unit, int& chunk) {
-        const long long blocks = std::max(1ll, tiles) * p.num_kv;
+    // how `keys` keys are split into at most n ranges of whole units
+    const auto split = [&](long long n, int unit, int& chunk) {
         const long long units = std::max(1ll, ((long long)p.limit + unit - 1) / unit);
-        long long n = std::min({std::max(1ll, (want + blocks - 1) / blocks), units, (long long)kMaxSplits});
+        n = std::max(1ll, std::min({n, units, (long long)kMaxSplits}));
         const long long per = (units + n - 1) / n;
         chunk = (int)std::min<long long>(per * unit, 0x7fffff00);
         return (int)((units + per - 1) / per);
     };
-    const long long few_real = std::min<long long>(r.few_tiles, p.seqs * ((rows + r.few_width - 1) / r.few_width));
-    const long long many_real = std::min<long long>(r.many_tiles, p.seqs * ((most + bm - 1) / bm));
-    r.few_splits = r.few ? splits(few_real, 2048, 256, r.few_chunk) : 1;
-    r.many_splits = r.many ? splits(many_real, 512, 256, r.many_chunk) : 1;
+    const auto over = [](long long a, long long b) { return (a + b - 1) / b; };
+    // blocks that are expected to have work, unsplit
+    const long long few = std::max(1ll, std::min<long long>(r.few_tiles, p.seqs * over(rows, r.few_width))) * p.num_kv;
+    const long long many = std::min<long long>(p.tokens * G / bm + over(p.tokens * G, most), p.seqs * over(most, bm)) * p.num_kv;
+    r.few_splits = r.many_splits = 1;
+    if (r.few) {
+        // 1024 blocks, four a CU; ranges of at most 2048 keys, so that the
+        // longest sequence's end is not waited for alone
+        const long long n = std::max(over(1024, few), few < 2048 ? over(p.limit, 2048) : 1);
+        const int unit = few * over(p.limit, 256) < 128 ? 128 : 256;
+        r.few_splits = split(n, unit, r.few_chunk);
+        // more blocks than run at once: the last splits first, which are the
+        // long sequences' (64 conversations in e4m3 97.5 -> 93.8 us; where all
+        // run at once it costs: 3 x 32,749 keys 17.4 -> 21 us)
+        r.few_last_first = few * r.few_splits > 768;
+    }
+    // (two blocks a CU, three with up to 64 columns, all at once)
+    if (r.many) r.many_splits = split(over(p.hd <= 64 ? 768 : 512, many), 256, r.many_chunk);
     const int n = std::max(r.few_splits, r.many_splits);
     if (n > 1) r.bytes = (size_t)n * p.tokens * hq * (p.hd * 4 + 8);
     return r;
@@ -940,6 +975,7 @@ static void launch_attn(hipStream_t s, const PagedAttnArgs& base, const AttnPlan
         a.hi_rows = pl.few_rows;
         a.chunk = pl.few_chunk;
         a.splits = pl.few_splits;
+        a.last_first = pl.few_last_first;
         const dim3 grid((unsigned)a.tiles * a.p.num_kv * a.splits);
         if (pl.few_width == 4) hipLaunchKernelGGL((k_paged_attn_few<F8, HD, PART, 4>), grid, dim3(256), 0, s, a);
         else if (pl.few_width == 8) hipLaunchKernelGGL((k_paged_attn_few<F8, HD, PART, 8>), grid, dim3(256), 0, s, a);
@@ -953,8 +989,8 @@ static void launch_attn(hipStream_t s, const PagedAttnArgs& base, const AttnPlan
         a.chunk = pl.many_chunk;
         a.splits = pl.many_splits;
         constexpr int NR = HD <= 128 ? 2 : 1;
-        hipLaunchKernelGGL((k_paged_attn_many<F8, HD, PART, NR>), dim3((unsigned)a.tiles * a.p.num_kv * a.splits), dim3(256),
-                           0, s, a);
+        hipLaunchKernelGGL((k_paged_attn_many<F8, HD, PART, NR>), dim3((unsigned)a.tiles * a.p.num_kv * a.splits),
+                           dim3(kManyRows / NR * 4), 0, s, a);
     }
 }
 
