@@ -39,6 +39,7 @@ struct PagedAttnArgs {
     float scale;     // log2(e) / sqrt(hd)
     FastDiv group;   // query heads per KV head
     int tiles;       // row tiles of this kernel's grid
+    int per;         // of them, of each sequence (the kernel for few rows)
     int lo_rows, hi_rows;  // this kernel takes sequences of lo_rows <= rows <= hi_rows
     int chunk, splits;     // keys of a split; splits == 1: no partial results
     int last_first;        // the blocks of the last splits go first
@@ -276,18 +277,30 @@ struct Rows {
         }
     }
 
-    // Scores of group j's 16 keys from a lane's chunks: sc[i] of row tile i
-    // holds keys 4 g .. 4 g + 3.
-    __device__ __forceinline__ void score(const u32x4 (&c)[T::NT], floatx4 (&sc)[NR]) {
+    // Scores of a tile's two 16-key groups, K in LDS: sc[j][i] of row tile i holds
+    // keys 16 j + 4 g .. + 3. A chunk is read while the one before is multiplied.
+    __device__ __forceinline__ void score(const char* kt, floatx4 (&sc)[2][NR]) {
+        const char* mine = kt + (threadIdx.x & 63) * 16;
+        constexpr int PER = F8 ? 2 : 1;  // matrix steps of a chunk
+        u32x4 c[1] = {*reinterpret_cast<const u32x4*>(mine)};
 #pragma unroll
-        for (int i = 0; i < NR; i++) sc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < 2 * T::NT; n++) {
+            u32x4 ahead = c[0];
+            if (n + 1 < 2 * T::NT) ahead = *reinterpret_cast<const u32x4*>(mine + (n + 1) * 1024);
+            __builtin_amdgcn_sched_barrier(0);
+            const int j = n / T::NT;
+            if (n % T::NT == 0)
 #pragma unroll
-        for (int u = 0; u < T::NU; u++) {
-            const bf16x8 k = T::frag(c, u);
+                for (int i = 0; i < NR; i++) sc[j][i] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int t = 2; t >= 0; t--)
+            for (int h = 0; h < PER; h++) {
+                const bf16x8 k = F8 ? widen8(c[0][2 * h], c[0][2 * h + 1]) : __builtin_bit_cast(bf16x8, c[0]);
 #pragma unroll
-                for (int i = 0; i < NR; i++) sc[i] = mfma16x16x32(k, q[i][u][t], sc[i]);
+                for (int t = 2; t >= 0; t--)
+#pragma unroll
+                    for (int i = 0; i < NR; i++) sc[j][i] = mfma16x16x32(k, q[i][n % T::NT * PER + h][t], sc[j][i]);
+            }
+            c[0] = ahead;
         }
     }
 
@@ -580,20 +593,22 @@ struct FewRows {
 // on their way while one is weighed (a fetch is unconditional: a branch around
 // loads would make the next use wait for all of them).
 template <bool F8, int HD, bool PART, int CW>
-__global__ __launch_bounds__(256, HD > 128 ? 1 : (HD == 64 && CW < 16 ? 3 : 2)) void k_paged_attn_few(PagedAttnArgs a) {
+struct FewBlock {
+    static constexpr int NW = 4, OROW = HD + 4;
+    static constexpr int STAGE = NW * (Tile<F8, HD>::BYTES + 256), JOIN = NW * 16 * (OROW + 2) * 4;
+    char lds[STAGE > JOIN ? STAGE : JOIN];
+    OddBits<CW, HD> odd;
+};
+template <bool F8, int HD, bool PART, int CW>
+__device__ __forceinline__ void few_tile(const PagedAttnArgs& a, const SeqAt& s, int r0, int kvh, int split,
+                                         FewBlock<F8, HD, PART, CW>& sh) {
     using T = Tile<F8, HD>;
     using R = FewRows<F8, HD, CW>;
-    constexpr int NW = 4, STEP = 32 * NW, NB = T::NT <= 2 ? 2 : 1;
-    constexpr int OROW = HD + 4;
-    constexpr int STAGE = NW * (T::BYTES + 256), JOIN = NW * 16 * (OROW + 2) * 4;
-    __shared__ __align__(16) char lds[STAGE > JOIN ? STAGE : JOIN];
-    __shared__ OddBits<CW, HD> odd;
+    using Sh = FewBlock<F8, HD, PART, CW>;
+    constexpr int NW = Sh::NW, STEP = 32 * NW, NB = T::NT <= 2 ? 2 : 1, OROW = Sh::OROW;
+    char* const lds = sh.lds;
+    auto& odd = sh.odd;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
-    const int kvh = blockIdx.x % a.p.num_kv, rest = blockIdx.x / a.p.num_kv;
-    const int tile = rest % a.tiles, split = a.last_first ? a.splits - 1 - rest / a.tiles : rest / a.tiles;
-    SeqAt s;
-    int r0;
-    if (!find_tile<CW>(a, tile, s, r0)) return;
     const int G = a.group.d, n = s.end - s.begin;
     const int end_tok = (int)a.group.div((uint32_t)(min(r0 + CW, n * G) - 1));
     const int T1 = min((a.causal ? s.len - n + end_tok : s.len - 1) + 1, a.p.limit);
@@ -718,6 +733,23 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : (HD == 64 && CW < 16 ? 3 : 2)) 
         if (a.splits > 1 && c == 0) a.part_ml[(size_t)split * a.p.tokens * a.hq + row] = make_float2(M, L);
     }
 }
+// The grid has `per` tiles for every sequence (enough for max_new).
+template <bool F8, int HD, bool PART, int CW>
+__global__ __launch_bounds__(256, HD > 128 ? 1 : (HD == 64 && CW < 16 ? 3 : 2)) void k_paged_attn_few(PagedAttnArgs a) {
+    __shared__ __align__(16) FewBlock<F8, HD, PART, CW> sh;
+    const int kvh = blockIdx.x % a.p.num_kv, rest = blockIdx.x / a.p.num_kv;
+    const int tile = rest % a.tiles, split = a.last_first ? a.splits - 1 - rest / a.tiles : rest / a.tiles;
+    SeqAt s;
+    s.s = tile / a.per;
+    const int b = seq_begin(a.p, s.s), e = seq_begin(a.p, s.s + 1), len = a.p.lens[s.s];
+    s.begin = __builtin_amdgcn_readfirstlane(b);
+    s.end = __builtin_amdgcn_readfirstlane(max(b, e));
+    s.len = __builtin_amdgcn_readfirstlane(len);
+    const int rows = (s.end - s.begin) * (int)a.group.d;
+    if (rows < a.lo_rows || rows > a.hi_rows) return;
+    const int r0 = (tile - s.s * a.per) * CW;
+    if (r0 < rows) few_tile<F8, HD, PART, CW>(a, s, r0, kvh, split, sh);
+}
 
 // Many rows: a block takes 128 rows of a sequence, 16 NR a wave, and its keys
 // (or a range of them) in tiles of 32 that all NW waves read from LDS. Loads
@@ -725,7 +757,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : (HD == 64 && CW < 16 ? 3 : 2)) 
 // way, one landed, in which the waves look for infinities in V.
 constexpr int kManyRows = 128;
 template <bool F8, int HD, bool PART, int NR>
-__global__ __launch_bounds__(kManyRows / NR * 4, 2) void k_paged_attn_many(PagedAttnArgs a) {
+__global__ __launch_bounds__(kManyRows / NR * 4, HD == 64 ? 3 : 2) void k_paged_attn_many(PagedAttnArgs a) {
     using T = Tile<F8, HD>;
     constexpr int BM = kManyRows, NW = BM / (16 * NR);
     __shared__ __align__(16) char kt[3][T::BYTES], vt[3][T::BYTES];
@@ -811,14 +843,7 @@ __global__ __launch_bounds__(kManyRows / NR * 4, 2) void k_paged_attn_many(Paged
         next = after;
         if (key0 <= rows.last) {
             floatx4 scores[2][NR];
-#pragma unroll
-            for (int jj = 0; jj < 2; jj++) {
-                u32x4 c[T::NT];
-#pragma unroll
-                for (int t = 0; t < T::NT; t++)
-                    c[t] = *reinterpret_cast<const u32x4*>(kt[b] + jj * T::GROUP + t * 1024 + lane * 16);
-                rows.score(c, scores[jj]);
-            }
+            rows.score(kt[b], scores);
             rows.take(scores, key0, seen_of[b][0] | (seen_of[b][1] << 16), sc[b][0], sc[b][2], vt[b]);
         }
         check(key0 + 32, b1);
@@ -901,7 +926,7 @@ struct AttnPlan {
     bool few, many;
     int few_width;  // rows of a tile of the kernel for few rows: 4, 8 or 16
     int few_rows;   // sequences of up to so many rows go to it
-    int few_tiles, many_tiles;
+    int few_per, few_tiles, many_tiles;
     int few_chunk, few_splits, many_chunk, many_splits;
     bool few_last_first;
     size_t bytes;
@@ -921,8 +946,10 @@ static AttnPlan attn_plan(const PagedArgs& p, int hq, int max_new) {
     r.few_width = rows <= 4 ? 4 : (rows <= 8 ? 8 : 16);
     r.few_rows = !r.many ? 0x7fffffff : (r.few_width < 16 ? r.few_width : kFewRows);
     r.few = !r.many || p.seqs > 1;
+    const auto over = [](long long a, long long b) { return (a + b - 1) / b; };
     const int bm = kManyRows;
-    r.few_tiles = (int)(p.tokens * G / r.few_width) + p.seqs;
+    r.few_per = (int)over(r.many ? std::min<long long>(r.few_rows, most) : most, r.few_width);
+    r.few_tiles = r.few_per * p.seqs;
     r.many_tiles = (int)(p.tokens * G / bm) + p.seqs;
     // how `keys` keys are split into at most n ranges of whole units
     const auto split = [&](long long n, int unit, int& chunk) {
@@ -932,9 +959,8 @@ static AttnPlan attn_plan(const PagedArgs& p, int hq, int max_new) {
         chunk = (int)std::min<long long>(per * unit, 0x7fffff00);
         return (int)((units + per - 1) / per);
     };
-    const auto over = [](long long a, long long b) { return (a + b - 1) / b; };
     // blocks that are expected to have work, unsplit
-    const long long few = std::max(1ll, std::min<long long>(r.few_tiles, p.seqs * over(rows, r.few_width))) * p.num_kv;
+    const long long few = std::max(1ll, p.seqs * over(rows, r.few_width)) * p.num_kv;
     const long long many = std::min<long long>(p.tokens * G / bm + over(p.tokens * G, most), p.seqs * over(most, bm)) * p.num_kv;
     r.few_splits = r.many_splits = 1;
     if (r.few) {
@@ -971,6 +997,7 @@ static void launch_attn(hipStream_t s, const PagedAttnArgs& base, const AttnPlan
     if (pl.few) {
         PagedAttnArgs a = base;
         a.tiles = pl.few_tiles;
+        a.per = pl.few_per;
         a.lo_rows = 0;
         a.hi_rows = pl.few_rows;
         a.chunk = pl.few_chunk;

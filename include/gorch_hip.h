@@ -456,9 +456,9 @@ typedef struct {
  * page_table[s][p / page_size]. The device arrays are read when the kernels
  * run, so a captured graph follows their contents.
  * max_kv: no position at or past it is read or written (0: max_pages *
- * page_size, which always holds); max_new: the most rows of a sequence (0:
- * tokens). Both are bounds that the host knows; a kernel is chosen by them,
- * and rows past max_new are still computed.
+ * page_size, which always holds); max_new: no sequence has more rows (0: any
+ * number; gorch_hip_paged_attention may leave rows past it uncomputed). Both
+ * are bounds that the host knows, and kernels are chosen by them.
  * An entry of page_table outside 0 .. num_pages - 1 is no page: nothing is
  * written there, and its keys are not seen. Sequences may share pages that
  * none of them writes in the same call. */
