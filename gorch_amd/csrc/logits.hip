@@ -28,7 +28,7 @@ constexpr uint32_t kInPrompt = 0x80000000u;  // beside the count of tokens after
 // stored token by token).
 template <int U, bool SAME>
 __global__ __launch_bounds__(256) void k_process_logits(LogitsArgs a) {
-    constexpr int SLICE = 1024 * U;
+    constexpr int SLICE = 1024 * U, HISTORY = 4;
     extern __shared__ __align__(16) uint32_t note[];  // per token: kInPrompt | count after the prompt
     const gorch_hip_logits_rules& r = a.r;
     uint32_t* last = note + (r.history ? SLICE : 0);  // per token: last bias entry + 1
@@ -36,8 +36,26 @@ __global__ __launch_bounds__(256) void k_process_logits(LogitsArgs a) {
     const float* x = a.x + (size_t)row * a.n;
     float* out = a.out + (size_t)row * a.n;
     const int lo = (int)blockIdx.x * SLICE - (int)(reinterpret_cast<uintptr_t>(x) / 4 % 4);
+    // everything that the block is sure to read goes out at once
+    int len = 0, prompt = 0, b0 = 0, b1 = 0;
+    const int* h = r.history + (size_t)row * r.history_stride;
+    int4 id[HISTORY];
+    if (r.history) {
+        len = r.history_lens ? min(max(r.history_lens[row], 0), r.history_stride) : r.history_stride;
+        prompt = r.prompt_lens ? r.prompt_lens[row] : 0;
+        if (a.wide_history)
+#pragma unroll
+            for (int u = 0; u < HISTORY; u++) {
+                const int i = 4 * (u * 256 + tid);
+                if (i < r.history_stride) id[u] = *reinterpret_cast<const int4*>(h + i);
+            }
+    }
+    if (r.bias) {
+        b0 = min(max(r.bias_rows[row], 0), r.biases);
+        b1 = min(max(r.bias_rows[row + 1], b0), r.biases);
+    }
     float4 v[U];
-    uint32_t ok[U];
+    uint32_t w0[U], w1[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int t = lo + 4 * (u * 256 + tid);
@@ -49,13 +67,11 @@ __global__ __launch_bounds__(256) void k_process_logits(LogitsArgs a) {
             v[u].z = t + 2 >= 0 && t + 2 < a.n ? x[t + 2] : 0.f;
             v[u].w = t + 3 >= 0 && t + 3 < a.n ? x[t + 3] : 0.f;
         }
-        ok[u] = 15u;
+        w0[u] = w1[u] = ~0u;
         if (r.allowed) {
-            // bits of tokens t .. t + 3 (those before the row or past it are never stored)
             const uint32_t* m = r.allowed + (size_t)row * r.allowed_stride;
-            const int w0 = min(max(t, 0), a.n - 1) / 32, w1 = min(max(t + 3, 0), a.n - 1) / 32;
-            const uint64_t bits = m[w0] | ((uint64_t)m[w1] << 32);
-            ok[u] = t >= 0 ? (uint32_t)(bits >> (t % 32)) : (uint32_t)(bits << -t);
+            w0[u] = m[min(max(t, 0), a.n - 1) / 32];
+            w1[u] = m[min(max(t + 3, 0), a.n - 1) / 32];
         }
     }
     if (r.history || r.bias) {
@@ -67,35 +83,33 @@ __global__ __launch_bounds__(256) void k_process_logits(LogitsArgs a) {
         }
         __syncthreads();
         if (r.history) {
-            const int len = r.history_lens ? min(max(r.history_lens[row], 0), r.history_stride) : r.history_stride;
-            const int prompt = r.prompt_lens ? r.prompt_lens[row] : 0;
-            const int* h = r.history + (size_t)row * r.history_stride;
-            auto take = [&](int i, int id) {
-                const unsigned at = (unsigned)(id - lo);
-                if (i >= len || at >= (unsigned)SLICE || (unsigned)id >= (unsigned)a.n) return;
+            auto take = [&](int i, int token) {
+                const unsigned at = (unsigned)(token - lo);
+                if (i >= len || at >= (unsigned)SLICE || (unsigned)token >= (unsigned)a.n) return;
                 if (i < prompt) atomicOr(&note[at], kInPrompt);
                 else atomicAdd(&note[at], 1u);
             };
+            auto take4 = [&](int i, const int4& t) {
+                take(i, t.x);
+                take(i + 1, t.y);
+                take(i + 2, t.z);
+                take(i + 3, t.w);
+            };
             if (a.wide_history) {
-                for (int i = 4 * tid; i < len; i += 1024) {
-                    const int4 id = *reinterpret_cast<const int4*>(h + i);
-                    take(i, id.x);
-                    take(i + 1, id.y);
-                    take(i + 2, id.z);
-                    take(i + 3, id.w);
-                }
+#pragma unroll
+                for (int u = 0; u < HISTORY; u++)
+                    if (4 * (u * 256 + tid) < len) take4(4 * (u * 256 + tid), id[u]);
+                for (int i = 4 * (HISTORY * 256 + tid); i < len; i += 1024) take4(i, *reinterpret_cast<const int4*>(h + i));
             } else {
                 for (int i = tid; i < len; i += 256) take(i, h[i]);
             }
         }
-        if (r.bias) {
-            const int b0 = min(max(r.bias_rows[row], 0), r.biases), b1 = min(max(r.bias_rows[row + 1], b0), r.biases);
+        if (r.bias)
             for (int i = b0 + tid; i < b1; i += 256) {
-                const int id = r.bias_ids[i];
-                const unsigned at = (unsigned)(id - lo);
-                if (at < (unsigned)SLICE && (unsigned)id < (unsigned)a.n) atomicMax(&last[at], (uint32_t)i + 1);
+                const int token = r.bias_ids[i];
+                const unsigned at = (unsigned)(token - lo);
+                if (at < (unsigned)SLICE && (unsigned)token < (unsigned)a.n) atomicMax(&last[at], (uint32_t)i + 1);
             }
-        }
         __syncthreads();
     }
     const float rep = r.repetition ? r.repetition[row] : 1.f, fr = r.frequency ? r.frequency[row] : 0.f,
@@ -104,6 +118,9 @@ __global__ __launch_bounds__(256) void k_process_logits(LogitsArgs a) {
     for (int u = 0; u < U; u++) {
         const int t = lo + 4 * (u * 256 + tid);
         float e[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+        // bits of tokens t .. t + 3 (those before the row or past it are never stored)
+        const uint64_t bits = w0[u] | ((uint64_t)w1[u] << 32);
+        const uint32_t ok = t >= 0 ? (uint32_t)(bits >> (t % 32)) : (uint32_t)(bits << -t);
         if (r.history) {
             const uint4 w = reinterpret_cast<const uint4*>(note)[u * 256 + tid];
             const uint32_t c[4] = {w.x, w.y, w.z, w.w};
@@ -124,7 +141,7 @@ __global__ __launch_bounds__(256) void k_process_logits(LogitsArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            if (!(ok[u] >> i & 1u)) e[i] = -INFINITY;
+            if (!(ok >> i & 1u)) e[i] = -INFINITY;
         if (SAME && t >= 0 && t + 4 <= a.n) {
             *reinterpret_cast<float4*>(out + t) = make_float4(e[0], e[1], e[2], e[3]);
         } else {
