@@ -234,28 +234,29 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
     }
 }
 
-// kReadTok tokens a block: their places first, then every load of K and V (a
-// thread keeps its four columns), then the stores.
-constexpr int kReadTok = 4;
-template <bool F8>
+// TOK tokens a block: their places first, then every load of K and V (a thread
+// keeps its four columns), then the stores. Bound by memory: 60,000 tokens of
+// 8 x 128 in e4m3 116 us with four tokens a block (5.1 TB/s), 172 with one;
+// few tokens have one a block (1,000 in bf16 4.3 us against 5.0).
+template <bool F8, int TOK>
 __global__ __launch_bounds__(256) void k_paged_read(PagedArgs p, float* ko, float* vo) {
-    const int t0 = blockIdx.x * kReadTok, hd4 = p.hd / 4, n4 = p.num_kv * hd4;
+    const int t0 = blockIdx.x * TOK, hd4 = p.hd / 4, n4 = p.num_kv * hd4;
     const int i0 = blockIdx.y * 256 + threadIdx.x, i = min(i0, n4 - 1), h = i / hd4, c = i - h * hd4;
-    long long row[kReadTok];
+    long long row[TOK];
 #pragma unroll
-    for (int j = 0; j < kReadTok; j++) {
+    for (int j = 0; j < TOK; j++) {
         SeqAt sq;
         row[j] = -1;
         if (t0 + j < p.tokens && token_seq(p, t0 + j, sq)) row[j] = pool_row(p, sq.s, sq.len - sq.end + t0 + j, h);
     }
     if (i0 >= n4) return;
     using Raw = typename std::conditional<F8, uint32_t, uint2>::type;
-    Raw u[2][kReadTok];
-    float sc[2][kReadTok];
+    Raw u[2][TOK];
+    float sc[2][TOK];
 #pragma unroll
     for (int w = 0; w < 2; w++)
 #pragma unroll
-        for (int j = 0; j < kReadTok; j++) {
+        for (int j = 0; j < TOK; j++) {
             if (row[j] < 0 || !(w ? vo : ko)) continue;
             u[w][j] = reinterpret_cast<const Raw*>(w ? p.v : p.k)[row[j] * hd4 + c];
             if constexpr (F8) sc[w][j] = (w ? p.vs : p.ks)[row[j]];
@@ -263,7 +264,7 @@ __global__ __launch_bounds__(256) void k_paged_read(PagedArgs p, float* ko, floa
 #pragma unroll
     for (int w = 0; w < 2; w++)
 #pragma unroll
-        for (int j = 0; j < kReadTok; j++) {
+        for (int j = 0; j < TOK; j++) {
             float* o = w ? vo : ko;
             if (row[j] < 0 || !o) continue;
             float4 x;
@@ -354,11 +355,13 @@ extern "C" int gorch_hip_paged_read(void* stream, const gorch_hip_paged_kv* kv, 
     GH_TRY(paged_args("gorch_hip_paged_read", kv, b, p));
     GH_SUPPORTED(aligned(k_out, 16) && aligned(v_out, 16), "gorch_hip_paged_read: outputs must be 16-byte aligned");
     if (b->tokens == 0 || b->seqs == 0 || (!k_out && !v_out)) return GORCH_HIP_OK;
-    const dim3 grid((p.tokens + kReadTok - 1) / kReadTok, (p.num_kv * p.hd / 4 + 255) / 256);
-    if (kv->dtype == GORCH_HIP_KV_E4M3)
-        hipLaunchKernelGGL(k_paged_read<true>, grid, dim3(256), 0, stream_of(stream), p, k_out, v_out);
-    else
-        hipLaunchKernelGGL(k_paged_read<false>, grid, dim3(256), 0, stream_of(stream), p, k_out, v_out);
+    const auto go = [&](auto kernel, int tok) {
+        hipLaunchKernelGGL(kernel, dim3((p.tokens + tok - 1) / tok, (p.num_kv * p.hd / 4 + 255) / 256), dim3(256), 0,
+                           stream_of(stream), p, k_out, v_out);
+    };
+    const bool f8 = kv->dtype == GORCH_HIP_KV_E4M3;
+    if (p.tokens < 4096) f8 ? go(k_paged_read<true, 1>, 1) : go(k_paged_read<false, 1>, 1);
+    else f8 ? go(k_paged_read<true, 4>, 4) : go(k_paged_read<false, 4>, 4);
     count(CNT_CODEC);
     return finish(stream, check_launch("paged_read"));
 }

@@ -88,7 +88,9 @@ GROUPS = [("history", "repetition"), ("history", "history_lens", "prompt_lens", 
 
 @pytest.mark.parametrize("rows,n,width,biases", [(1, 1, 1, 1), (3, 31, 5, 9), (2, 33, 300, 3), (5, 1000, 40, 20),
                                                  (2, 50257, 300, 40), (3, 8193, 9000, 300), (2, 4096, 0, 1),
-                                                 (1, 151936, 4001, 300), (70, 4099, 7, 2)])
+                                                 (1, 151936, 4001, 300), (70, 4099, 7, 2),
+                                                 # more than 2^21 logits: the larger blocks
+                                                 (520, 4099, 30, 4), (16, 131075, 5001, 40)])
 @pytest.mark.parametrize("group", range(len(GROUPS)))
 def test_matches_definition(gpu, rows, n, width, biases, group):
     rng = np.random.default_rng(n + group)
@@ -170,7 +172,7 @@ def test_wrong_tensors_are_refused(gpu):
 
 
 @pytest.mark.parametrize("first,out_first", [(0, 1), (1, 1), (1, 2), (2, 0), (3, 2)])
-@pytest.mark.parametrize("n", [5, 1023, 4099])
+@pytest.mark.parametrize("n", [5, 1023, 4099, 700001])
 def test_rows_at_any_address(gpu, first, out_first, n):
     # rows of a larger tensor start at any multiple of 4 bytes, in and out each their own
     rng = np.random.default_rng(n + first)

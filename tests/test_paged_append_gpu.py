@@ -211,6 +211,20 @@ def test_read_is_the_cache(gpu, dtype, hkv, hd, page):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+def test_read_of_many_tokens(gpu, dtype):
+    # more tokens than the small blocks take, none of some sequences, an end inside a block
+    c = Case(dtype, 1, 32, 16, [(3001, 3001), (0, 0), (1500, 1210), (2, 1)], seed=9)
+    kv, b = c.cache(gpu), c.batch(gpu, 1)
+    outs = [torch.full((c.tokens + 1, 32), SENTINEL, device="cuda") for _ in "kv"]
+    kv.read(b, *outs)
+    for out, name in zip(outs, "kv"):
+        got = host(out)
+        want = np.concatenate([c.rows(name, s)[0][length - n:] for s, (length, n) in enumerate(c.seqs) if n])
+        assert np.array_equal(got[:c.tokens], want.reshape(c.tokens, 32).astype(np.float32))
+        assert (got[c.tokens:] == SENTINEL).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
 def test_serving_step(gpu, dtype):
     """One layer of a serving step from the framework's own pieces: a fused QKV Linear, append, attention, the Wo
     Linear, logits under their rules and a token drawn, for a prompt's chunks and then single tokens; the attention
