@@ -318,25 +318,29 @@ struct Rows {
             }
         }
         const bool edge = key0 + 31 > first || seen != 0xffffffffu;  // some row does not see some key
+        if constexpr (F8)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < NR; i++) sc[j][i] *= ks[j];
+        if (edge) {
+#pragma unroll
+            for (int i = 0; i < NR; i++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int k = 16 * (e >> 2) + 4 * g + (e & 3);
+                    const int sees = (int)(seen >> k & 1u) & (key0 + k <= pos[i] ? 1 : 0);
+                    sc[e >> 2][i][e & 3] = sees ? sc[e >> 2][i][e & 3] : -INFINITY;
+                }
+        }
         bf16x8 p[NR][3];
         float al[NR];
         bool grew = false;
 #pragma unroll
         for (int i = 0; i < NR; i++) {
-            float top = -INFINITY;
+            float top = sc[0][i][0];
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    float s = sc[j][i][e];
-                    if constexpr (F8) s *= ks[j][e];
-                    if (edge) {
-                        const int k = 16 * j + 4 * g + e;
-                        s = (seen >> k & 1u) && key0 + k <= pos[i] ? s : -INFINITY;
-                    }
-                    sc[j][i][e] = s;
-                    top = fmaxf(top, s);
-                }
+            for (int e = 1; e < 8; e++) top = fmaxf(top, sc[e >> 2][i][e & 3]);
             const float mn = fmaxf(m[i], col_max(top)), use = mn == -INFINITY ? 0.f : mn;
             al[i] = __builtin_amdgcn_exp2f(m[i] - use);
             grew |= mn != m[i];
@@ -402,14 +406,15 @@ __device__ __forceinline__ void put(const PagedAttnArgs& a, int split, size_t ro
     }
 }
 
-// The page that holds key `key` of a sequence (of key k1 - 1 for those past it;
-// 0 < k1 <= limit), no branch around the load; and the pool row of the key
-// there, -1 if it is not below k1 or on no page.
-__device__ __forceinline__ int key_page(const PagedArgs& a, int s, int key, int k1) {
-    return a.table[(size_t)s * a.max_pages + a.page.div((uint32_t)min(key, k1 - 1))];
+// The page that holds key `key` of a sequence (of the last position for those
+// past it), read without knowing the sequence's length and with no branch
+// around the load; and the pool row of the key there, -1 if it is not below k1
+// or on no page.
+__device__ __forceinline__ int key_page(const PagedArgs& a, int s, int key) {
+    return a.table[(size_t)s * a.max_pages + a.page.div((uint32_t)min(key, max(a.limit, 1) - 1))];
 }
 __device__ __forceinline__ long long key_row(const PagedArgs& a, int page, int key, int k1, int kvh) {
-    const int p = min(key, k1 - 1);
+    const int p = min(key, max(a.limit, 1) - 1);
     const long long row = ((long long)page * a.num_kv + kvh) * a.page.d + (p - (int)(a.page.div((uint32_t)p) * a.page.d));
     const int there = (key < k1 ? 1 : 0) & ((unsigned)page < (unsigned)a.num_pages ? 1 : 0);
     return there ? row : -1;
@@ -530,7 +535,8 @@ struct FewRows {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const int at = 16 * j + 4 * g + e;
-                    sc[j][e] = (seen >> at & 1u) && key0 + at <= pos ? sc[j][e] : -INFINITY;
+                    const int sees = (int)(seen >> at & 1u) & (key0 + at <= pos ? 1 : 0);
+                    sc[j][e] = sees ? sc[j][e] : -INFINITY;
                 }
         }
         float top = sc[0][0];
@@ -594,18 +600,19 @@ struct FewRows {
 // loads would make the next use wait for all of them).
 template <bool F8, int HD, bool PART, int CW>
 struct FewBlock {
-    static constexpr int NW = 4, OROW = HD + 4;
+    static constexpr int NW = 4, NB = Tile<F8, HD>::NT <= 2 ? 2 : 1, OROW = HD + 4;
     static constexpr int STAGE = NW * (Tile<F8, HD>::BYTES + 256), JOIN = NW * 16 * (OROW + 2) * 4;
     char lds[STAGE > JOIN ? STAGE : JOIN];
     OddBits<CW, HD> odd;
 };
 template <bool F8, int HD, bool PART, int CW>
 __device__ __forceinline__ void few_tile(const PagedAttnArgs& a, const SeqAt& s, int r0, int kvh, int split,
+                                         const int (&page)[FewBlock<F8, HD, PART, CW>::NB + 1],
                                          FewBlock<F8, HD, PART, CW>& sh) {
     using T = Tile<F8, HD>;
     using R = FewRows<F8, HD, CW>;
     using Sh = FewBlock<F8, HD, PART, CW>;
-    constexpr int NW = Sh::NW, STEP = 32 * NW, NB = T::NT <= 2 ? 2 : 1, OROW = Sh::OROW;
+    constexpr int NW = Sh::NW, STEP = 32 * NW, NB = Sh::NB, OROW = Sh::OROW;
     char* const lds = sh.lds;
     auto& odd = sh.odd;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
@@ -645,10 +652,7 @@ __device__ __forceinline__ void few_tile(const PagedAttnArgs& a, const SeqAt& s,
     int key0 = k0 + 32 * wave;
     int next;  // the page of the next tile to fetch
     {
-        int page[NB];
-#pragma unroll
-        for (int i = 0; i < NB; i++) page[i] = key_page(a.p, s.s, key0 + i * STEP + (lane & 31), k1);
-        next = key_page(a.p, s.s, key0 + NB * STEP + (lane & 31), k1);
+        next = page[NB];
         float4 x[T::NU][2];
         rows.template fetch<PART>(a, s, r0, kvh, x);
 #pragma unroll
@@ -682,7 +686,7 @@ __device__ __forceinline__ void few_tile(const PagedAttnArgs& a, const SeqAt& s,
         }
         // (the page of the tile after goes out first: loads are waited for in
         // order, and the next fetch waits for it)
-        const int after = key_page(a.p, s.s, key + (NB + 1) * STEP + (lane & 31), k1);
+        const int after = key_page(a.p, s.s, key + (NB + 1) * STEP + (lane & 31));
         __builtin_amdgcn_sched_barrier(0);
         fetch(key_row(a.p, next, key + NB * STEP + (lane & 31), k1, kvh), b);
         next = after;
@@ -741,6 +745,13 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : (HD == 64 && CW < 16 ? 3 : 2)) 
     const int tile = rest % a.tiles, split = a.last_first ? a.splits - 1 - rest / a.tiles : rest / a.tiles;
     SeqAt s;
     s.s = tile / a.per;
+    // the first tiles' pages, beside the sequence's place (the range's start is
+    // known without it)
+    using Sh = FewBlock<F8, HD, PART, CW>;
+    int page[Sh::NB + 1];
+#pragma unroll
+    for (int i = 0; i <= Sh::NB; i++)
+        page[i] = key_page(a.p, s.s, split * a.chunk + 32 * (int)(threadIdx.x >> 6) + i * 32 * Sh::NW + (int)(threadIdx.x & 31));
     const int b = seq_begin(a.p, s.s), e = seq_begin(a.p, s.s + 1), len = a.p.lens[s.s];
     s.begin = __builtin_amdgcn_readfirstlane(b);
     s.end = __builtin_amdgcn_readfirstlane(max(b, e));
@@ -748,7 +759,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : (HD == 64 && CW < 16 ? 3 : 2)) 
     const int rows = (s.end - s.begin) * (int)a.group.d;
     if (rows < a.lo_rows || rows > a.hi_rows) return;
     const int r0 = (tile - s.s * a.per) * CW;
-    if (r0 < rows) few_tile<F8, HD, PART, CW>(a, s, r0, kvh, split, sh);
+    if (r0 < rows) few_tile<F8, HD, PART, CW>(a, s, r0, kvh, split, page, sh);
 }
 
 // Many rows: a block takes 128 rows of a sequence, 16 NR a wave, and its keys
@@ -784,7 +795,7 @@ __global__ __launch_bounds__(kManyRows / NR * 4, HD == 64 ? 3 : 2) void k_paged_
     // of four waves, 0 and 1 fetch K's two groups of a tile, 2 and 3 V's
     const int j = wave & 1;
     const bool isv = (wave & 2) != 0;
-    auto page_of = [&](int key0) { return key_page(a.p, s.s, key0 + 16 * j + (lane & 15), k1); };
+    auto page_of = [&](int key0) { return key_page(a.p, s.s, key0 + 16 * j + (lane & 15)); };
     auto fetch = [&](int page, int key0, int b) {
         const long long row = key_row(a.p, page, key0 + 16 * j + (lane & 15), k1, kvh);
         typedef __attribute__((address_space(1))) const uint32_t* global_ptr;
@@ -961,7 +972,8 @@ static AttnPlan attn_plan(const PagedArgs& p, int hq, int max_new) {
     };
     // blocks that are expected to have work, unsplit
     const long long few = std::max(1ll, p.seqs * over(rows, r.few_width)) * p.num_kv;
-    const long long many = std::min<long long>(p.tokens * G / bm + over(p.tokens * G, most), p.seqs * over(most, bm)) * p.num_kv;
+    const long long many = std::min<long long>(over(p.tokens * G, bm) + (over(p.tokens * G, most) - 1) / 2,
+                                                   p.seqs * over(most, bm)) * p.num_kv;
     r.few_splits = r.many_splits = 1;
     if (r.few) {
         // 1024 blocks, four a CU; ranges of at most 2048 keys, so that the
@@ -975,7 +987,7 @@ static AttnPlan attn_plan(const PagedArgs& p, int hq, int max_new) {
         r.few_last_first = few * r.few_splits > 768;
     }
     // (two blocks a CU, three with up to 64 columns, all at once)
-    if (r.many) r.many_splits = split(over(p.hd <= 64 ? 768 : 512, many), 256, r.many_chunk);
+    if (r.many) r.many_splits = split(over(p.hd <= 64 ? 768 : 512, many), 128, r.many_chunk);
     const int n = std::max(r.few_splits, r.many_splits);
     if (n > 1) r.bytes = (size_t)n * p.tokens * hq * (p.hd * 4 + 8);
     return r;
@@ -986,6 +998,11 @@ static int attn_args(const gorch_hip_paged_kv* kv, const gorch_hip_paged_batch* 
     GH_REQUIRE(num_q > 0 && num_q % kv->num_kv == 0, "gorch/nn: GQA NumQ must be divisible by NumKV");
     GH_SUPPORTED((long long)b->tokens * num_q < (1ll << 28) && (long long)b->seqs < (1ll << 28) / kv->num_kv,
                  "gorch_hip_paged_attention: tokens * num_q must be below 2^28");
+    // (no position at all: the kernels' reads of a page go elsewhere)
+    if (a.p.limit == 0) {
+        a.p.table = a.p.cu;
+        a.p.max_pages = 0;
+    }
     a.hq = num_q;
     a.scale = (float)(1.4426950408889634 / std::sqrt((double)kv->head_dim));
     a.group.set((uint32_t)(num_q / kv->num_kv));
