@@ -22,7 +22,9 @@ int paged_args(const char* who, const gorch_hip_paged_kv* kv, const gorch_hip_pa
     if (kv->head_dim % 16 != 0 || kv->head_dim > 256)
         return fail(GORCH_HIP_EUNSUPPORTED, "head_dim must be a multiple of 16 up to 256");
     const long long room = (long long)b->max_pages * kv->page_size;
-    if (room > 0x7fffffffll) return fail(GORCH_HIP_EINVAL, "max_pages * page_size must be below 2^31");
+    // (2^16 below 2^31: the kernels look a few tiles past the last position)
+    if (room > 0x7fff0000ll) return fail(GORCH_HIP_EINVAL, "max_pages * page_size must be below 2^31 - 2^16");
+    if (b->tokens >= 1 << 24 || kv->num_kv > 0xffff) return fail(GORCH_HIP_EUNSUPPORTED, "tokens must be below 2^24, num_kv below 2^16");
     if (b->tokens > 0 && b->seqs > 0) {
         if (!kv->k || !kv->v || !b->cu_seqlens || !b->kv_lens || (b->max_pages > 0 && !b->page_table))
             return fail(GORCH_HIP_EINVAL, "null pool or batch array");
@@ -324,6 +326,7 @@ extern "C" int gorch_hip_paged_append(void* stream, const gorch_hip_paged_kv* kv
                "gorch_hip_paged_append: the heads and the cache differ in num_kv or head_dim");
     GH_REQUIRE(!q == !q_out, "gorch_hip_paged_append: need both q and q_out or neither");
     GH_REQUIRE(!q || (w->num_q > 0 && w->num_q % w->num_kv == 0), "gorch/nn: GQA NumQ must be divisible by NumKV");
+    GH_SUPPORTED(!q || w->num_q <= 0xffff, "gorch_hip_paged_append: num_q must be below 2^16");
     GH_REQUIRE(!w->rope_cos == !w->rope_sin, "gorch_hip_paged_append: need both RoPE tables");
     if (b->tokens == 0 || b->seqs == 0) return GORCH_HIP_OK;
     GH_REQUIRE(k && v, "gorch_hip_paged_append: null k or v");

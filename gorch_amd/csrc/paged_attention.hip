@@ -8,8 +8,8 @@
 // matrix operands. q (scaled, f32) is split into three bf16 terms by
 // truncation, which together hold its 24 bits, and so is every p: three
 // v_mfma_f32_16x16x32_bf16 per product give f32 products summed in f32. Two
-// terms would save a third of the matrix time and leave 2^-16 of each q and p
-// (output error 3e-6 of the 2-norm against 6e-7). An e4m3 row's scale
+// terms would save a third of the matrix time and leave errors of 2^-16 of each
+// q and p, 30 times those of f32 sums. An e4m3 row's scale
 // multiplies the scores of its key (K) or its weight (V), never a rounded
 // operand.
 //
@@ -393,7 +393,7 @@ __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int tile, SeqA
     if (!wave_seq(a.p, tile, [&](int i, int begin) { return begin * G / BM + i; }, s)) return false;
     r0 = (tile - (s.begin * G / BM + s.s)) * BM;
     const int rows = (s.end - s.begin) * G;
-    return r0 < rows && rows >= a.lo_rows && rows <= a.hi_rows;
+    return r0 >= 0 && r0 < rows && rows >= a.lo_rows && rows <= a.hi_rows;
 }
 
 // Finished (or, of a split, partial) sums of four columns of a row.
@@ -993,6 +993,21 @@ static AttnPlan attn_plan(const PagedArgs& p, int hq, int max_new) {
     return r;
 }
 
+const char* paged_attn_choice_name(int tokens, int seqs, int hq, int hkv, int hd, int max_new, int positions) {
+    PagedArgs p{};
+    p.tokens = tokens;
+    p.seqs = seqs;
+    p.num_kv = hkv;
+    p.hd = hd;
+    p.limit = positions;
+    const AttnPlan pl = attn_plan(p, hq, max_new);
+    static const char* const few[3][2] = {{"few4", "few4 split"}, {"few8", "few8 split"}, {"few16", "few16 split"}};
+    static const char* const both[3][2] = {{"few4+many", "few4+many split"}, {"few8+many", "few8+many split"}, {"few16+many", "few16+many split"}};
+    const int w = pl.few_width == 4 ? 0 : (pl.few_width == 8 ? 1 : 2), split = pl.bytes > 0;
+    if (!pl.few) return split ? "many split" : "many";
+    return pl.many ? both[w][split] : few[w][split];
+}
+
 static int attn_args(const gorch_hip_paged_kv* kv, const gorch_hip_paged_batch* b, int num_q, PagedAttnArgs& a) {
     GH_TRY(paged_args("gorch_hip_paged_attention", kv, b, a.p));
     GH_REQUIRE(num_q > 0 && num_q % kv->num_kv == 0, "gorch/nn: GQA NumQ must be divisible by NumKV");
@@ -1080,6 +1095,10 @@ extern "C" int gorch_hip_paged_attention(void* stream, const gorch_hip_paged_kv*
     if (b->tokens == 0 || b->seqs == 0) return GORCH_HIP_OK;
     GH_REQUIRE(q && out, "gorch_hip_paged_attention: null q or out");
     const AttnPlan pl = attn_plan(a.p, num_q, b->max_new);
+    // (a launch has less than 2^32 threads)
+    GH_SUPPORTED((!pl.few || (long long)pl.few_tiles * kv->num_kv * pl.few_splits < 1 << 24) &&
+                     (!pl.many || (long long)pl.many_tiles * kv->num_kv * pl.many_splits < 1 << 23),
+                 "gorch_hip_paged_attention: too many sequences or tokens for one call");
     GH_REQUIRE(workspace_bytes >= pl.bytes && (workspace || pl.bytes == 0),
                "gorch_hip_paged_attention: workspace too small");
     GH_SUPPORTED(reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&

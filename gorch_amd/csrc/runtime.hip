@@ -496,6 +496,9 @@ const char* gorch_hip_kernel_choice(const char* op, const int* d, int n) {
         return moe_choice_name(d[0], d[1], d[2], d[3], d[4], !moe_up);
     if (is("attention", 7) && d[0] > 0 && d[1] > 0 && d[3] > 0 && d[5] > 0 && (!d[4] || d[3] % d[4] == 0))
         return attn_choice_name(d[0], d[1], d[2], d[3], d[4], d[5], d[6]);
+    if (is("paged_attention", 7) && d[0] > 0 && d[0] < 1 << 24 && d[1] > 0 && d[3] > 0 && d[2] > 0 && d[2] % d[3] == 0 &&
+        (long long)d[0] * d[2] < 1 << 28 && (long long)d[1] * d[3] < 1 << 28 && d[4] > 0 && d[4] <= 256 && d[4] % 16 == 0)
+        return paged_attn_choice_name(d[0], d[1], d[2], d[3], d[4], d[5], d[6]);
     return nullptr;
 }
 

@@ -151,7 +151,10 @@ void gorch_hip_reset_dispatch_counts(void);
  *     gorch_hip_moe_forward's expert GEMMs;
  *   "attention" {batch, new rows, cached rows, heads, KV heads (0: one per
  *     head), head_dim, max_seq}: a causal attention_cached call over 16-byte
- *     aligned buffers.
+ *     aligned buffers;
+ *   "paged_attention" {tokens, sequences, heads, KV heads, head_dim, max_new,
+ *     positions (max_kv or what the page table holds)}: fewN (tiles of N rows
+ *     for sequences of few), many, both; "split": key ranges and a join.
  * The names are not an interface: they change with the kernels. */
 const char* gorch_hip_kernel_choice(const char* op, const int* dims, int n);
 
@@ -439,8 +442,9 @@ int gorch_hip_qwen_generate_sampled(void* stream, gorch_hip_qwen* m, const int* 
 /* One layer's pools (device): k and v [num_pages][num_kv][page_size][head_dim]
  * of dtype, 16-byte aligned; with GORCH_HIP_KV_E4M3 also k_scale and v_scale
  * [num_pages][num_kv][page_size], a row's value being code * scale (NULL and
- * unused with GORCH_HIP_KV_BF16). head_dim is a multiple of 16 up to 256
- * (else GORCH_HIP_EUNSUPPORTED); page_size is any positive number. */
+ * unused with GORCH_HIP_KV_BF16). head_dim is a multiple of 16 up to 256,
+ * num_kv below 2^16 (else GORCH_HIP_EUNSUPPORTED); page_size is any positive
+ * number. */
 typedef struct {
     int dtype, num_pages, page_size, num_kv, head_dim;
     void* k; void* v;
@@ -461,7 +465,8 @@ typedef struct {
  * are bounds that the host knows, and kernels are chosen by them.
  * An entry of page_table outside 0 .. num_pages - 1 is no page: nothing is
  * written there, and its keys are not seen. Sequences may share pages that
- * none of them writes in the same call. */
+ * none of them writes in the same call. tokens is below 2^24, max_pages *
+ * page_size below 2^31 - 2^16. */
 typedef struct {
     int tokens, seqs, max_pages, max_new, max_kv;
     const int* cu_seqlens; const int* kv_lens; const int* page_table;
@@ -502,7 +507,10 @@ int gorch_hip_paged_read(void* stream, const gorch_hip_paged_kv* kv, const gorch
  * own, else all kv_lens[s]. Products and sums keep f32 accuracy (q and the
  * softmax weights as three bf16 terms against the cache's exact values), every
  * sum has a fixed order. A key that a token does not see has no effect on it,
- * whatever its page holds; a token that sees none gets zeros. The workspace
+ * whatever its page holds; a token that sees none gets zeros; one that sees
+ * an infinite key, or has an infinite q, may get NaN. Weighted values are
+ * summed before they are divided, so values past f32's largest / keys may
+ * overflow. tokens * num_q is below 2^28. The workspace
  * (gorch_hip_paged_attention_workspace_size bytes, device, 16-byte aligned;
  * NULL where that is 0) is the caller's: calls that can overlap must not share
  * one. Nothing is allocated, so the call can be captured. */

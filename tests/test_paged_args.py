@@ -46,10 +46,11 @@ def read(kv, b, ko=FAKE, vo=FAKE):
 BAD_CACHE = [(dict(dtype=7), 2), (dict(num_pages=0), 2), (dict(page_size=0), 2), (dict(num_kv=-1), 2),
              (dict(head_dim=0), 2), (dict(head_dim=72), 1), (dict(head_dim=272), 1), (dict(k=None), 2),
              (dict(v=None), 2), (dict(k=ODD), 1), (dict(v=ODD), 1), (dict(dtype=1), 2),
-             (dict(dtype=1, k_scale=FAKE), 2)]
+             (dict(dtype=1, k_scale=FAKE), 2), (dict(num_kv=1 << 16), 1)]
 BAD_BATCH = [(dict(tokens=-1), 2), (dict(seqs=-1), 2), (dict(max_pages=-1), 2), (dict(max_new=-1), 2),
              (dict(max_kv=-1), 2), (dict(cu_seqlens=None), 2), (dict(kv_lens=None), 2), (dict(page_table=None), 2),
-             (dict(max_pages=1 << 27), 2)]
+             (dict(max_pages=1 << 27), 2), (dict(max_pages=0x7fff001), 2),
+             (dict(tokens=1 << 24), 1)]
 
 
 @pytest.mark.parametrize("over,rc", BAD_CACHE)
@@ -135,3 +136,37 @@ def test_cpu_tensors_are_refused():
     with pytest.raises(ValueError):
         hip.PagedKV(torch.zeros((2, 2, 16, 64), dtype=torch.bfloat16), torch.zeros((2, 2, 16, 64), dtype=torch.bfloat16),
                     torch.zeros((2, 2, 16)), torch.zeros((2, 2, 16)))
+
+
+def test_too_many_heads_are_refused():
+    w = heads(num_q=1 << 16)
+    assert append(cache(), batch(), w, qs=1 << 23) == 1 and "num_q" in hip.last_error()
+    assert append(cache(), batch(tokens=0), w) == 1
+
+
+def test_too_large_a_launch_is_refused():
+    # 2^24 sequences of a token or less, 1 KV head: one launch has fewer blocks
+    kv, b = cache(num_kv=1), batch(tokens=16, seqs=1 << 25, max_new=1)
+    assert attend(kv, b, num_q=4, ws=FAKE, n=1 << 60) == 1 and "too many" in hip.last_error()
+    assert attend(cache(num_kv=8), batch(tokens=1 << 20), num_q=512) == 1
+
+
+@pytest.mark.parametrize("dims,name", [
+    # 2 heads per KV head: a conversation's step short and long, many of them, prompts, a chunk, a mixed batch
+    # (4 prompts may all be short ones: 32 tiles of few rows, split)
+    ((1, 1, 16, 8, 128, 1, 60), "few4"), ((1, 1, 16, 8, 128, 1, 777), "few4 split"),
+    ((64, 64, 16, 8, 128, 1, 8192), "few4 split"), ((4096, 4096, 16, 8, 128, 1, 4096), "few4"),
+    ((8192, 4, 16, 8, 128, 2048, 2048), "few4+many split"), ((2048, 1, 16, 8, 128, 2048, 16384), "many split"),
+    ((600, 27, 16, 8, 128, 500, 4000), "few4+many split"),
+    # 7 heads per KV head, 16 draft rows, one KV head for all
+    ((3, 3, 14, 2, 64, 1, 32749), "few8 split"), ((64, 16, 16, 8, 128, 4, 2000), "few8 split"),
+    ((80, 16, 16, 8, 128, 5, 2000), "few16 split"), ((4, 4, 32, 1, 128, 1, 200), "few16 split"),
+    ((2, 1, 16, 8, 128, 0, 100), "few4"), ((100, 1, 16, 8, 128, 0, 100), "many")])
+def test_kernel_choice(dims, name):
+    assert hip.kernel_choice("paged_attention", *dims) == name
+
+
+def test_kernel_choice_of_nothing():
+    for dims in ((0, 1, 16, 8, 128, 1, 60), (1, 0, 16, 8, 128, 1, 60), (1, 1, 15, 8, 128, 1, 60),
+                 (1, 1, 16, 8, 72, 1, 60), (1, 1, 16, 0, 128, 1, 60), (1 << 24, 1, 16, 8, 128, 1, 60)):
+        assert hip.kernel_choice("paged_attention", *dims) is None

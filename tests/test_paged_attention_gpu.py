@@ -209,6 +209,106 @@ def test_captured_step_follows_the_batch(gpu):
             check(host(out).reshape(3, 4, 64), want, tol)
 
 
+def test_captured_mixed_step_follows_the_batch(gpu):
+    # prompts beside single tokens: both kernels, split, and their join in one graph
+    c = Case("bf16", 2, 128, 16, [(900, 1), (1200, 150), (640, 1), (333, 60)], seed=16)
+    hq = 4
+    q = queries(c, hq)
+    kv, b = c.cache(gpu), c.batch(gpu, max_new=150, max_kv=1200)
+    assert gpu.kernel_choice("paged_attention", c.tokens, 4, hq, 2, 128, 150, 1200).endswith("+many split")
+    qd, out = dev(q.reshape(c.tokens, -1)), torch.empty((c.tokens, hq * 128), device="cuda")
+    ws = kv.workspace(b, hq)
+    kv.attention(b, qd, out, ws=ws)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        kv.attention(b, qd, out, ws=ws)
+    for seqs in ([(900, 1), (1200, 150), (640, 1), (333, 60)], [(700, 60), (40, 1), (1, 1), (150, 150)],
+                 [(0, 0), (1199, 3), (639, 130), (1, 1)]):
+        c.seqs, c.lens[:], c.cu[1:] = seqs, [n for n, _ in seqs], np.cumsum([n for _, n in seqs])
+        live = c.cu[-1]
+        b.t[0].copy_(dev(c.cu))
+        b.t[1].copy_(dev(c.lens))
+        torch.cuda.synchronize()
+        want, tol = c.attention(q, hq)
+        for _ in range(2):
+            out.fill_(SENTINEL)
+            ws.fill_(0xff)  # nothing is taken from an earlier call's sums
+            g.replay()
+            got = host(out).reshape(-1, hq, 128)
+            check(got[:live], want[:live], tol[:live])
+            assert (got[live:] == SENTINEL).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("hq,hkv,hd,seqs", [
+    # key ranges of the kernel for many rows, each width of its heads, whole and in part
+    (2, 1, 256, [(700, 90)]), (2, 1, 208, [(700, 90), (300, 1)]), (3, 1, 112, [(900, 70)]), (2, 2, 32, [(900, 70)]),
+    # tiles of 4, 8 and 16 rows, split
+    (4, 2, 192, [(1500, 1), (1100, 2)]), (7, 1, 96, [(1500, 1)]), (16, 1, 256, [(1500, 1), (3, 1)]),
+    (5, 1, 32, [(1500, 3)]), (1, 1, 16, [(1500, 9)])])
+def test_splits(gpu, dtype, hq, hkv, hd, seqs):
+    c = Case(dtype, hkv, hd, 24, seqs, seed=hd + hq)
+    bounds = dict(max_new=max(n for _, n in seqs), max_kv=max(n for n, _ in seqs))
+    assert "split" in gpu.kernel_choice("paged_attention", c.tokens, len(seqs), hq, hkv, hd, *bounds.values())
+    q = queries(c, hq)
+    want, tol = c.attention(q, hq)
+    check(attend(gpu, c, q, hq, **bounds), want, tol)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("count,bounds", [(70, {}), (70, dict(max_new=1, max_kv=500)), (1100, dict(max_new=1)), (4200, {})])
+def test_many_sequences(gpu, dtype, count, bounds):
+    # a search of one, two and three steps for a token's sequence; more blocks than run at once
+    rng = np.random.default_rng(count)
+    single = "max_new" in bounds
+    seqs = [(int(rng.integers(0, 40)), 1 if single else int(rng.integers(0, 3))) for _ in range(count)]
+    seqs[3], seqs[-2] = (500, 1), ((40, 1) if single else (90, 60))
+    c = Case(dtype, 1, 32, 16, seqs, seed=count)
+    q = queries(c, 2)
+    want, tol = c.attention(q, 2)
+    check(attend(gpu, c, q, 2, extra=1, **bounds), want, tol)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+def test_a_shared_prefix(gpu, dtype):
+    # the same pages in several sequences, and valid pages named past a sequence's last position
+    c = Case(dtype, 2, 64, 16, [(200, 1), (170, 4), (230, 70), (40, 1)], seed=17)
+    c.table[1, :5], c.table[2, :7] = c.table[0, :5], c.table[0, :7]
+    c.table[c.table >= c.pages] = c.table[0, 0]
+    q = queries(c, 4)
+    want, tol = c.attention(q, 4)
+    for bounds in ({}, dict(max_new=70, max_kv=230), dict(max_kv=4000)):
+        check(attend(gpu, c, q, 4, **bounds), want, tol)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_no_pages_at_all(gpu, n):
+    c = Case("bf16", 1, 64, 16, [(n, n), (0, 0)], seed=18)
+    kv, b = c.cache(gpu), gpu.PagedBatch(dev(c.cu), dev(c.lens), torch.empty((2, 0), dtype=torch.int32, device="cuda"), n)
+    out, rows = torch.full((n, 128), SENTINEL, device="cuda"), torch.full((n, 64), SENTINEL, device="cuda")
+    kv.attention(b, dev(queries(c, 2).reshape(n, -1)), out)
+    kv.read(b, rows, None)
+    assert (host(out) == 0).all() and (host(rows) == SENTINEL).all()
+
+
+@pytest.mark.parametrize("length,n", [(70, 1), (900, 2), (60, 50), (900, 50)])
+def test_infinite_values_of_both_signs(gpu, length, n):
+    # column 2: +inf, 3: -inf, 4: both, 5: NaN, in keys that all see
+    c = Case("bf16", 1, 64, 16, [(length, n)], seed=19)
+    for p, col, code in ((3, 2, 0x7f80), (4, 3, 0xff80), (5, 4, 0x7f80), (9, 4, 0xff80), (2, 5, 0xffc1)):
+        c.v[c.slot(0, p)][:, col] = code
+    q = queries(c, 2, 0.1)
+    with np.errstate(invalid="ignore"):
+        want, tol = c.attention(q, 2)
+    got = attend(gpu, c, q, 2)
+    assert (got[-1, :, 2] == np.inf).all() and (got[-1, :, 3] == -np.inf).all() and np.isnan(got[-1, :, 4:6]).all()
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+    fine = np.isfinite(want)
+    np.testing.assert_array_equal(got[np.isinf(want)], want[np.isinf(want)])
+    check(got[fine], want[fine], tol[fine])
+
+
 def test_small_workspace_is_refused(gpu):
     c = Case("bf16", 1, 128, 16, [(5000, 1)], seed=14)
     kv, b = c.cache(gpu), c.batch(gpu, max_new=1, max_kv=5000)
