@@ -737,11 +737,11 @@ __device__ __forceinline__ void few_tile(const PagedAttnArgs& a, const SeqAt& s,
         if (a.splits > 1 && c == 0) a.part_ml[(size_t)split * a.p.tokens * a.hq + row] = make_float2(M, L);
     }
 }
-// The grid has `per` tiles for every sequence (enough for max_new).
+// Block `block` of a grid that has `per` tiles for every sequence (enough for
+// max_new).
 template <bool F8, int HD, bool PART, int CW>
-__global__ __launch_bounds__(256, HD > 128 ? 1 : (HD == 64 && CW < 16 ? 3 : 2)) void k_paged_attn_few(PagedAttnArgs a) {
-    __shared__ __align__(16) FewBlock<F8, HD, PART, CW> sh;
-    const int kvh = blockIdx.x % a.p.num_kv, rest = blockIdx.x / a.p.num_kv;
+__device__ __forceinline__ void few_block(const PagedAttnArgs& a, int block, FewBlock<F8, HD, PART, CW>& sh) {
+    const int kvh = block % a.p.num_kv, rest = block / a.p.num_kv;
     const int tile = rest % a.tiles, split = a.last_first ? a.splits - 1 - rest / a.tiles : rest / a.tiles;
     SeqAt s;
     s.s = tile / a.per;
@@ -761,22 +761,35 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : (HD == 64 && CW < 16 ? 3 : 2)) 
     const int r0 = (tile - s.s * a.per) * CW;
     if (r0 < rows) few_tile<F8, HD, PART, CW>(a, s, r0, kvh, split, page, sh);
 }
+template <bool F8, int HD, bool PART, int CW>
+__global__ __launch_bounds__(256, HD > 128 ? 1 : (HD == 64 && CW < 16 ? 3 : 2)) void k_paged_attn_few(PagedAttnArgs a) {
+    __shared__ __align__(16) FewBlock<F8, HD, PART, CW> sh;
+    few_block<F8, HD, PART, CW>(a, (int)blockIdx.x, sh);
+}
 
 // Many rows: a block takes 128 rows of a sequence, 16 NR a wave, and its keys
 // (or a range of them) in tiles of 32 that all NW waves read from LDS. Loads
 // go straight to LDS, two tiles ahead of the one that is weighed: one on its
 // way, one landed, in which the waves look for infinities in V.
 constexpr int kManyRows = 128;
+template <bool F8, int HD>
+struct ManyBlock {
+    alignas(16) char kt[3][Tile<F8, HD>::BYTES], vt[3][Tile<F8, HD>::BYTES];
+    alignas(16) float sc[3][4][F8 ? 64 : 1];  // e4m3 scales: K's two groups, V's two (16 each)
+    uint32_t seen_of[3][2];
+    OddBits<kManyRows, HD> odd;
+};
 template <bool F8, int HD, bool PART, int NR>
-__global__ __launch_bounds__(kManyRows / NR * 4, HD == 64 ? 3 : 2) void k_paged_attn_many(PagedAttnArgs a) {
+__device__ __forceinline__ void many_block(const PagedAttnArgs& a, int block, ManyBlock<F8, HD>& sh) {
     using T = Tile<F8, HD>;
     constexpr int BM = kManyRows, NW = BM / (16 * NR);
-    __shared__ __align__(16) char kt[3][T::BYTES], vt[3][T::BYTES];
-    __shared__ __align__(16) float sc[3][4][64];  // e4m3 scales: K's two groups, V's two (16 each)
-    __shared__ uint32_t seen_of[3][2];
-    __shared__ OddBits<BM, HD> odd;
+    auto& kt = sh.kt;
+    auto& vt = sh.vt;
+    auto& sc = sh.sc;
+    auto& seen_of = sh.seen_of;
+    auto& odd = sh.odd;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
-    const int kvh = blockIdx.x % a.p.num_kv, rest = blockIdx.x / a.p.num_kv;
+    const int kvh = block % a.p.num_kv, rest = block / a.p.num_kv;
     // the last rows of a sequence see the most keys: they go first
     const int tile = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
     SeqAt s;
@@ -876,6 +889,24 @@ __global__ __launch_bounds__(kManyRows / NR * 4, HD == 64 ? 3 : 2) void k_paged_
             }
         if (a.splits > 1 && g == 0) a.part_ml[(size_t)split * a.p.tokens * a.hq + at] = make_float2(rows.m[i], l);
     }
+}
+template <bool F8, int HD, bool PART, int NR>
+__global__ __launch_bounds__(kManyRows / NR * 4, HD == 64 ? 3 : 2) void k_paged_attn_many(PagedAttnArgs a) {
+    __shared__ __align__(16) ManyBlock<F8, HD> sh;
+    many_block<F8, HD, PART, NR>(a, (int)blockIdx.x, sh);
+}
+// Both in one launch, for up to 128 columns, where their blocks are of one
+// size: the blocks of few rows, which wait for memory, run beside those of
+// many, which keep the matrix cores busy.
+template <bool F8, int HD, bool PART, int CW>
+__global__ __launch_bounds__(256, HD == 64 && CW < 16 ? 3 : 2) void k_paged_attn_both(PagedAttnArgs many, PagedAttnArgs few,
+                                                                                     int many_blocks) {
+    __shared__ __align__(16) union {
+        ManyBlock<F8, HD> many;
+        FewBlock<F8, HD, PART, CW> few;
+    } sh;
+    if ((int)blockIdx.x < many_blocks) many_block<F8, HD, PART, 2>(many, (int)blockIdx.x, sh.many);
+    else few_block<F8, HD, PART, CW>(few, (int)blockIdx.x - many_blocks, sh.few);
 }
 
 // A row's splits joined, each weighted by 2^(its maximum - the largest): WPR
@@ -1026,31 +1057,39 @@ static int attn_args(const gorch_hip_paged_kv* kv, const gorch_hip_paged_batch* 
 
 template <bool F8, int HD, bool PART>
 static void launch_attn(hipStream_t s, const PagedAttnArgs& base, const AttnPlan& pl) {
-    if (pl.few) {
-        PagedAttnArgs a = base;
-        a.tiles = pl.few_tiles;
-        a.per = pl.few_per;
-        a.lo_rows = 0;
-        a.hi_rows = pl.few_rows;
-        a.chunk = pl.few_chunk;
-        a.splits = pl.few_splits;
-        a.last_first = pl.few_last_first;
-        const dim3 grid((unsigned)a.tiles * a.p.num_kv * a.splits);
-        if (pl.few_width == 4) hipLaunchKernelGGL((k_paged_attn_few<F8, HD, PART, 4>), grid, dim3(256), 0, s, a);
-        else if (pl.few_width == 8) hipLaunchKernelGGL((k_paged_attn_few<F8, HD, PART, 8>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((k_paged_attn_few<F8, HD, PART, 16>), grid, dim3(256), 0, s, a);
-    }
-    if (pl.many) {
-        PagedAttnArgs a = base;
-        a.tiles = pl.many_tiles;
-        a.lo_rows = pl.few ? pl.few_rows + 1 : 0;
-        a.hi_rows = 0x7fffffff;
-        a.chunk = pl.many_chunk;
-        a.splits = pl.many_splits;
-        constexpr int NR = HD <= 128 ? 2 : 1;
-        hipLaunchKernelGGL((k_paged_attn_many<F8, HD, PART, NR>), dim3((unsigned)a.tiles * a.p.num_kv * a.splits),
-                           dim3(kManyRows / NR * 4), 0, s, a);
-    }
+    constexpr int NR = HD <= 128 ? 2 : 1, NT = kManyRows / NR * 4;
+    PagedAttnArgs few = base, many = base;
+    few.tiles = pl.few_tiles;
+    few.per = pl.few_per;
+    few.lo_rows = 0;
+    few.hi_rows = pl.few_rows;
+    few.chunk = pl.few_chunk;
+    few.splits = pl.few_splits;
+    few.last_first = pl.few_last_first;
+    many.tiles = pl.many_tiles;
+    many.lo_rows = pl.few ? pl.few_rows + 1 : 0;
+    many.hi_rows = 0x7fffffff;
+    many.chunk = pl.many_chunk;
+    many.splits = pl.many_splits;
+    const int few_blocks = few.tiles * few.p.num_kv * few.splits, many_blocks = many.tiles * many.p.num_kv * many.splits;
+    const auto width = [&](auto go) {
+        if (pl.few_width == 4) go(std::integral_constant<int, 4>{});
+        else if (pl.few_width == 8) go(std::integral_constant<int, 8>{});
+        else go(std::integral_constant<int, 16>{});
+    };
+    if constexpr (HD <= 128)
+        if (pl.few && pl.many) {
+            width([&](auto w) {
+                hipLaunchKernelGGL((k_paged_attn_both<F8, HD, PART, decltype(w)::value>), dim3((unsigned)(many_blocks + few_blocks)),
+                                   dim3(256), 0, s, many, few, many_blocks);
+            });
+            return;
+        }
+    if (pl.few)
+        width([&](auto w) {
+            hipLaunchKernelGGL((k_paged_attn_few<F8, HD, PART, decltype(w)::value>), dim3((unsigned)few_blocks), dim3(256), 0, s, few);
+        });
+    if (pl.many) hipLaunchKernelGGL((k_paged_attn_many<F8, HD, PART, NR>), dim3((unsigned)many_blocks), dim3(NT), 0, s, many);
 }
 
 template <bool F8>
