@@ -434,26 +434,28 @@ __device__ __forceinline__ void put_nothing(const PagedAttnArgs& a, int split, c
     }
 }
 
-// The rows of a wave that has few: CW (4, 8 or 16) query rows of one sequence,
-// a row in 16 / CW columns of the operand, each with terms of its own: with up
-// to 4 rows one matrix instruction makes all three terms' products, with up to
-// 8 two do (NP). A score is the sum of its row's columns, and a lane's weights
-// are the terms of its own columns; the columns of O are added at the end.
-// (One term a column against three instructions: 64 decoding conversations of
-// 2 rows per KV head, 200k tokens in e4m3, 101 -> FEWUS us.)
+// The rows of a wave that has few: CW query rows of one sequence. CW = 16: a
+// row a column of the operand and an instruction a term, as for many rows.
+// CW = 4: a row in four columns, which hold its terms, so that one matrix
+// instruction makes all three terms' products; a score is the sum of its row's
+// columns, a lane's weights are the terms of its own columns, and the columns
+// of O are added at the end. (24 single tokens of 12 heads beside 3 prompts
+// 49 us with 16, 42 with 4; 64 of 2 rows per KV head 95.8 and 95.)
 template <bool F8, int HD, int CW>
 struct FewRows {
     using T = Tile<F8, HD>;
-    static constexpr int TP = 16 / CW;          // terms side by side
-    static constexpr int NP = (3 + TP - 1) / TP;
+    static_assert(CW == 4 || CW == 16);
+    static constexpr int TP = 16 / CW;  // columns of a row
+    static constexpr int NP = CW == 4 ? 1 : 3;
     bf16x8 q[T::NU][NP];
     floatx4 o[HD / 16];
     float m, l;
     int pos, first;
 
+    // a lane's operand p of the terms t
     __device__ __forceinline__ static bf16x8 pick(const bf16x8 (&t)[3], int p) {
         if constexpr (CW == 16) return t[p];
-        const int k = p * TP + (int)(threadIdx.x & 15) / CW;
+        const int k = (int)(threadIdx.x & 15) / CW;
         const uint32_t is[3] = {k == 0 ? ~0u : 0u, k == 1 ? ~0u : 0u, k == 2 ? ~0u : 0u};
         u32x4 r = {0, 0, 0, 0};
 #pragma unroll
@@ -506,12 +508,12 @@ struct FewRows {
 #pragma unroll
             for (int p = NP - 1; p >= 0; p--) s = mfma16x16x32(k, q[u][p], s);
         }
-        if constexpr (CW <= 8)
+        if constexpr (CW == 4)
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[e] += dpp_f<0x128>(s[e]);  // 16 lanes rotated by 8
-        if constexpr (CW <= 4)
-#pragma unroll
-            for (int e = 0; e < 4; e++) s[e] += dpp_f<0x124>(s[e]);  // and by 4
+            for (int e = 0; e < 4; e++) {
+                s[e] += dpp_f<0x128>(s[e]);  // 16 lanes rotated by 8
+                s[e] += dpp_f<0x124>(s[e]);  // and by 4
+            }
         return s;
     }
     // a tile's 32 keys from key0 on (as Rows::take)
@@ -578,7 +580,7 @@ struct FewRows {
             bf16x8 t[3];
             split3(w, t);
 #pragma unroll
-            for (int i = 0; i < NP; i++) p[i] = pick(t, i);
+            for (int i = 0; i < NP; i++) p[i] = t[i];
         }
         if (__any(grew)) {
 #pragma unroll
@@ -762,7 +764,7 @@ __device__ __forceinline__ void few_block(const PagedAttnArgs& a, int block, Few
     if (r0 < rows) few_tile<F8, HD, PART, CW>(a, s, r0, kvh, split, page, sh);
 }
 template <bool F8, int HD, bool PART, int CW>
-__global__ __launch_bounds__(256, HD > 128 ? 1 : (HD == 64 && CW < 16 ? 3 : 2)) void k_paged_attn_few(PagedAttnArgs a) {
+__global__ __launch_bounds__(256, HD > 128 ? 1 : (HD == 64 && CW == 4 ? 3 : 2)) void k_paged_attn_few(PagedAttnArgs a) {
     __shared__ __align__(16) FewBlock<F8, HD, PART, CW> sh;
     few_block<F8, HD, PART, CW>(a, (int)blockIdx.x, sh);
 }
@@ -899,7 +901,7 @@ __global__ __launch_bounds__(kManyRows / NR * 4, HD == 64 ? 3 : 2) void k_paged_
 // size: the blocks of few rows, which wait for memory, run beside those of
 // many, which keep the matrix cores busy.
 template <bool F8, int HD, bool PART, int CW>
-__global__ __launch_bounds__(256, HD == 64 && CW < 16 ? 3 : 2) void k_paged_attn_both(PagedAttnArgs many, PagedAttnArgs few,
+__global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn_both(PagedAttnArgs many, PagedAttnArgs few,
                                                                                      int many_blocks) {
     __shared__ __align__(16) union {
         ManyBlock<F8, HD> many;
@@ -966,7 +968,7 @@ __global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttnArgs a) {
 
 struct AttnPlan {
     bool few, many;
-    int few_width;  // rows of a tile of the kernel for few rows: 4, 8 or 16
+    int few_width;  // rows of a tile of the kernel for few rows: 4 or 16
     int few_rows;   // sequences of up to so many rows go to it
     int few_per, few_tiles, many_tiles;
     int few_chunk, few_splits, many_chunk, many_splits;
@@ -980,15 +982,15 @@ constexpr int kFewRows = 32;
 
 static AttnPlan attn_plan(const PagedArgs& p, int hq, int max_new) {
     AttnPlan r{};
+    const auto over = [](long long a, long long b) { return (a + b - 1) / b; };
     const long long G = hq / p.num_kv;
     const long long most = std::min<long long>(max_new > 0 ? max_new : p.tokens, p.tokens) * G;
     r.many = most > kFewRows;
     // beside prompts, the kernel for few rows takes the single tokens
     const long long rows = r.many ? G : most;
-    r.few_width = rows <= 4 ? 4 : (rows <= 8 ? 8 : 16);
-    r.few_rows = !r.many ? 0x7fffffff : (r.few_width < 16 ? r.few_width : kFewRows);
-    r.few = !r.many || p.seqs > 1;
-    const auto over = [](long long a, long long b) { return (a + b - 1) / b; };
+    r.few_width = rows <= 4 ? 4 : 16;
+    r.few_rows = !r.many ? 0x7fffffff : (int)over(rows, r.few_width) * r.few_width;
+    r.few = !r.many || (p.seqs > 1 && rows <= kFewRows);
     const int bm = kManyRows;
     r.few_per = (int)over(r.many ? std::min<long long>(r.few_rows, most) : most, r.few_width);
     r.few_tiles = r.few_per * p.seqs;
@@ -1032,9 +1034,9 @@ const char* paged_attn_choice_name(int tokens, int seqs, int hq, int hkv, int hd
     p.hd = hd;
     p.limit = positions;
     const AttnPlan pl = attn_plan(p, hq, max_new);
-    static const char* const few[3][2] = {{"few4", "few4 split"}, {"few8", "few8 split"}, {"few16", "few16 split"}};
-    static const char* const both[3][2] = {{"few4+many", "few4+many split"}, {"few8+many", "few8+many split"}, {"few16+many", "few16+many split"}};
-    const int w = pl.few_width == 4 ? 0 : (pl.few_width == 8 ? 1 : 2), split = pl.bytes > 0;
+    static const char* const few[2][2] = {{"few4", "few4 split"}, {"few16", "few16 split"}};
+    static const char* const both[2][2] = {{"few4+many", "few4+many split"}, {"few16+many", "few16+many split"}};
+    const int w = pl.few_width == 4 ? 0 : 1, split = pl.bytes > 0;
     if (!pl.few) return split ? "many split" : "many";
     return pl.many ? both[w][split] : few[w][split];
 }
@@ -1074,7 +1076,6 @@ static void launch_attn(hipStream_t s, const PagedAttnArgs& base, const AttnPlan
     const int few_blocks = few.tiles * few.p.num_kv * few.splits, many_blocks = many.tiles * many.p.num_kv * many.splits;
     const auto width = [&](auto go) {
         if (pl.few_width == 4) go(std::integral_constant<int, 4>{});
-        else if (pl.few_width == 8) go(std::integral_constant<int, 8>{});
         else go(std::integral_constant<int, 16>{});
     };
     if constexpr (HD <= 128)
@@ -1103,13 +1104,15 @@ static void launch_attn_hd(hipStream_t s, const PagedAttnArgs& a, const AttnPlan
     else launch_attn<F8, 256, true>(s, a, pl);
 }
 
-// A wave per row, or a block for many splits.
+// A wave per row; a block for many splits where rows are few (single tokens
+// beside prompts: 30 sequences of 14 heads, 4 chunks of up to 400 rows over
+// 2,500 keys 57 -> 47 us; 3 tokens over 32,749 keys 17 us against 20).
 static void launch_join(hipStream_t s, const PagedAttnArgs& a, int splits) {
     const long long rows = (long long)a.p.tokens * a.hq;
     const auto go = [&](auto kernel, int per) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, a);
     };
-    const bool wide = splits > 8;
+    const bool wide = splits > 8 && rows <= 2048;
     if (a.p.hd <= 64) wide ? go(k_paged_attn_join<16, 4>, 1) : go(k_paged_attn_join<16, 1>, 4);
     else if (a.p.hd <= 128) wide ? go(k_paged_attn_join<32, 4>, 1) : go(k_paged_attn_join<32, 1>, 4);
     else wide ? go(k_paged_attn_join<64, 4>, 1) : go(k_paged_attn_join<64, 1>, 4);

@@ -159,9 +159,9 @@ def test_too_large_a_launch_is_refused():
     ((8192, 4, 16, 8, 128, 2048, 2048), "few4+many split"), ((2048, 1, 16, 8, 128, 2048, 16384), "many split"),
     ((600, 27, 16, 8, 128, 500, 4000), "few4+many split"),
     # 7 heads per KV head, 16 draft rows, one KV head for all
-    ((3, 3, 14, 2, 64, 1, 32749), "few8 split"), ((64, 16, 16, 8, 128, 4, 2000), "few8 split"),
+    ((3, 3, 14, 2, 64, 1, 32749), "few16 split"), ((64, 16, 16, 8, 128, 4, 2000), "few16 split"),
     ((80, 16, 16, 8, 128, 5, 2000), "few16 split"), ((4, 4, 32, 1, 128, 1, 200), "few16 split"),
-    ((2, 1, 16, 8, 128, 0, 100), "few4"), ((100, 1, 16, 8, 128, 0, 100), "many")])
+    ((2, 1, 16, 8, 128, 0, 100), "few4"), ((60, 9, 40, 1, 64, 20, 90), "many"), ((100, 1, 16, 8, 128, 0, 100), "many")])
 def test_kernel_choice(dims, name):
     assert hip.kernel_choice("paged_attention", *dims) == name
 

@@ -244,7 +244,7 @@ def test_captured_mixed_step_follows_the_batch(gpu):
 @pytest.mark.parametrize("hq,hkv,hd,seqs", [
     # key ranges of the kernel for many rows, each width of its heads, whole and in part
     (2, 1, 256, [(700, 90)]), (2, 1, 208, [(700, 90), (300, 1)]), (3, 1, 112, [(900, 70)]), (2, 2, 32, [(900, 70)]),
-    # tiles of 4, 8 and 16 rows, split
+    # tiles of 4 and 16 rows, split
     (4, 2, 192, [(1500, 1), (1100, 2)]), (7, 1, 96, [(1500, 1)]), (16, 1, 256, [(1500, 1), (3, 1)]),
     (5, 1, 32, [(1500, 3)]), (1, 1, 16, [(1500, 9)])])
 def test_splits(gpu, dtype, hq, hkv, hd, seqs):
