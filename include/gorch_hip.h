@@ -461,7 +461,7 @@ typedef struct {
  * run, so a captured graph follows their contents.
  * max_kv: no position at or past it is read or written (0: max_pages *
  * page_size, which always holds); max_new: no sequence has more rows (0: any
- * number; gorch_hip_paged_attention may leave rows past it uncomputed). Both
+ * number; what gorch_hip_paged_attention gives for rows past it is undefined). Both
  * are bounds that the host knows, and kernels are chosen by them.
  * An entry of page_table outside 0 .. num_pages - 1 is no page: nothing is
  * written there, and its keys are not seen. Sequences may share pages that
