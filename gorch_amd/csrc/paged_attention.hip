@@ -778,9 +778,9 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : (HD == 64 && CW == 4 ? 3 : 2)) 
 // go straight to LDS, two tiles ahead of the one that is weighed: one on its
 // way, one landed, in which the waves look for infinities in V. Bound by the
 // matrix cores: 2,048 rows of 16 heads of 128 over 16,384 keys (257 GFLOP, 771
-// in three terms) 642 us, 1.2 PFLOP/s of matrix instructions, as a large bf16
-// product reaches here. (Waves of 32 rows: 16 a wave read K and V from LDS
-// twice as often; a ring of four or five tiles was no faster.)
+// in three terms) 642-662 us, 1.2 PFLOP/s of matrix instructions, the rate of a
+// large bf16 product here. (No faster: a ring of four or five tiles, operands
+// read two or three steps ahead, priorities by wave.)
 constexpr int kManyRows = 128;
 template <bool F8, int HD>
 struct ManyBlock {
