@@ -33,8 +33,10 @@ struct PagedAttnArgs {
     PagedArgs p;
     const float* q;
     float* out;
-    float* part_o;   // [splits][tokens * hq][hd] unnormalised sums of a key range
-    float2* part_ml; // [splits][tokens * hq] its maximum (log2) and weight sum
+    float* part_o;   // [splits][part_rows][hd] unnormalised sums of a key range
+    float2* part_ml; // [splits][part_rows] its maximum (log2) and weight sum
+    long long part_rows;  // tokens * hq, row (token, head); or, of a few_cap > 0,
+    int few_cap;          // seqs * few_cap * num_kv, row (sequence, row there, KV head)
     int hq, causal;
     float scale;     // log2(e) / sqrt(hd)
     FastDiv group;   // query heads per KV head
@@ -43,9 +45,12 @@ struct PagedAttnArgs {
     int lo_rows, hi_rows;  // this kernel takes sequences of lo_rows <= rows <= hi_rows
     int chunk, splits;     // keys of a split; splits == 1: no partial results
     int last_first;        // the blocks of the last splits go first
-    // the joining kernel: the other kernel's chunk and splits, for sequences
-    // of more than hi_rows rows
+    // the joining kernel: chunk and splits of sequences of more than hi_rows
+    // rows, and with few_cap the partial sums of the others
     int chunk2, splits2;
+    float* few_o;
+    float2* few_ml;
+    long long few_rows;
 };
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
@@ -396,13 +401,26 @@ __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int tile, SeqA
     return r0 >= 0 && r0 < rows && rows >= a.lo_rows && rows <= a.hi_rows;
 }
 
+// Row r of sequence s for KV head kvh among (token, head) rows, and among those
+// of partial sums.
+struct RowAt {
+    size_t row, part;
+};
+__device__ __forceinline__ RowAt row_at(const PagedAttnArgs& a, const SeqAt& s, int r, int kvh) {
+    const int G = a.group.d, tok = (int)a.group.div((uint32_t)r);
+    RowAt at;
+    at.row = (size_t)(s.begin + tok) * a.hq + kvh * G + (r - tok * G);
+    at.part = a.few_cap ? ((size_t)s.s * a.few_cap + r) * a.p.num_kv + kvh : at.row;
+    return at;
+}
+
 // Finished (or, of a split, partial) sums of four columns of a row.
-__device__ __forceinline__ void put(const PagedAttnArgs& a, int split, size_t row, int c, floatx4 o, float l) {
+__device__ __forceinline__ void put(const PagedAttnArgs& a, int split, const RowAt& at, int c, floatx4 o, float l) {
     if (a.splits == 1) {
         const float r = l == 0.f ? 0.f : 1.0f / l;  // a row that sees nothing: zeros
-        *reinterpret_cast<floatx4*>(a.out + row * a.p.hd + c) = floatx4{o[0] * r, o[1] * r, o[2] * r, o[3] * r};
+        *reinterpret_cast<floatx4*>(a.out + at.row * a.p.hd + c) = floatx4{o[0] * r, o[1] * r, o[2] * r, o[3] * r};
     } else {
-        *reinterpret_cast<floatx4*>(a.part_o + ((size_t)split * a.p.tokens * a.hq + row) * a.p.hd + c) = o;
+        *reinterpret_cast<floatx4*>(a.part_o + ((size_t)split * a.part_rows + at.part) * a.p.hd + c) = o;
     }
 }
 
@@ -427,10 +445,10 @@ template <int BM>
 __device__ __forceinline__ void put_nothing(const PagedAttnArgs& a, int split, const SeqAt& s, int r0, int kvh) {
     const int G = a.group.d, rows = min(BM, (s.end - s.begin) * G - r0), hd4 = a.p.hd / 4;
     for (int i = threadIdx.x; i < rows * hd4; i += blockDim.x) {
-        const int r = r0 + i / hd4, c = 4 * (i % hd4), tok = (int)a.group.div((uint32_t)r);
-        const size_t row = (size_t)(s.begin + tok) * a.hq + kvh * G + (r - tok * G);
-        put(a, split, row, c, floatx4{0.f, 0.f, 0.f, 0.f}, 0.f);
-        if (a.splits > 1 && c == 0) a.part_ml[(size_t)split * a.p.tokens * a.hq + row] = make_float2(-INFINITY, 0.f);
+        const int r = r0 + i / hd4, c = 4 * (i % hd4);
+        const RowAt at = row_at(a, s, r, kvh);
+        put(a, split, at, c, floatx4{0.f, 0.f, 0.f, 0.f}, 0.f);
+        if (a.splits > 1 && c == 0) a.part_ml[(size_t)split * a.part_rows + at.part] = make_float2(-INFINITY, 0.f);
     }
 }
 
@@ -737,10 +755,9 @@ __device__ __forceinline__ void few_tile(const PagedAttnArgs& a, const SeqAt& s,
             }
         }
         if (odd.any) o = add_odd(odd, r, c, o);
-        const int tok = (int)a.group.div((uint32_t)(r0 + r));
-        const size_t row = (size_t)(s.begin + tok) * a.hq + kvh * G + (r0 + r - tok * G);
-        put(a, split, row, c, o, L);
-        if (a.splits > 1 && c == 0) a.part_ml[(size_t)split * a.p.tokens * a.hq + row] = make_float2(M, L);
+        const RowAt at = row_at(a, s, r0 + r, kvh);
+        put(a, split, at, c, o, L);
+        if (a.splits > 1 && c == 0) a.part_ml[(size_t)split * a.part_rows + at.part] = make_float2(M, L);
     }
 }
 // Block `block` of a grid that has `per` tiles for every sequence (enough for
@@ -889,15 +906,14 @@ __device__ __forceinline__ void many_block(const PagedAttnArgs& a, int block, Ma
         const float l = col_sum(rows.l[i]);
         const int r = r0 + 16 * (NR * wave + i) + (lane & 15);
         if (r >= n * G) continue;
-        const int tok = (int)a.group.div((uint32_t)r);
-        const size_t at = (size_t)(s.begin + tok) * a.hq + kvh * G + (r - tok * G);
+        const RowAt at = row_at(a, s, r, kvh);
 #pragma unroll
         for (int d = 0; d < HD / 16; d++)
             if (!PART || 16 * d < a.p.hd) {
                 const int c = 16 * d + 4 * g;
                 put(a, split, at, c, odd.any ? add_odd(odd, r - r0, c, rows.o[i][d]) : rows.o[i][d], l);
             }
-        if (a.splits > 1 && g == 0) a.part_ml[(size_t)split * a.p.tokens * a.hq + at] = make_float2(rows.m[i], l);
+        if (a.splits > 1 && g == 0) a.part_ml[(size_t)split * a.part_rows + at.part] = make_float2(rows.m[i], l);
     }
 }
 template <bool F8, int HD, bool PART, int NR>
@@ -923,7 +939,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn_both(Paged
 // waves per (token, query head), 16 bytes of a split's columns a lane, the
 // splits dealt to SLOTS groups of lanes (sums in a fixed order: a slot's
 // splits, then the slots). The first loads go out before the sequence is
-// known; splits past the row's last are then left out.
+// known, as if it were no exception (few_cap); splits past the row's last are
+// then left out.
 constexpr int kMaxSplits = 64;
 template <int NL, int WPR>
 __global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttnArgs a) {
@@ -933,10 +950,13 @@ __global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttnArgs a) {
     const long long total = (long long)a.p.tokens * a.hq;
     const long long row = min(__builtin_amdgcn_readfirstlane(blockIdx.x * RPB + sub), (int)total - 1);
     const bool mine = (long long)blockIdx.x * RPB + sub < total;
-    const int c = tid % NL, slot = tid / NL, col = min(4 * c, a.p.hd - 4), most = max(a.splits, a.splits2);
-    float2 ml = a.part_ml[min(lane, most - 1) * total + row];
+    const int c = tid % NL, slot = tid / NL, col = min(4 * c, a.p.hd - 4);
+    const float* po = a.part_o;
+    long long stride = a.part_rows, at = min(row, a.part_rows - 1);
+    int last = (a.few_cap && a.splits2 > 1 ? a.splits2 : max(a.splits, a.splits2)) - 1;
+    float2 ml = a.part_ml[min(lane, last) * stride + at];
     auto part = [&](int j) {
-        return *reinterpret_cast<const floatx4*>(a.part_o + (min(j, most - 1) * total + row) * a.p.hd + col);
+        return *reinterpret_cast<const floatx4*>(po + (min(j, last) * stride + at) * a.p.hd + col);
     };
     floatx4 x = part(slot);
     const int t = (int)(row / a.hq);
@@ -947,6 +967,15 @@ __global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttnArgs a) {
         const int chunk = few ? a.chunk : a.chunk2, splits = few ? a.splits : a.splits2;
         const int T = min(a.causal ? s.len - s.end + t + 1 : s.len, a.p.limit);
         nc = splits == 1 ? 0 : min(max((T + chunk - 1) / chunk, 1), splits);  // (one split: out is written)
+        if (few && a.few_cap && nc > 0) {
+            const int G = a.group.d, h = (int)(row - (long long)t * a.hq), kvh = h / G;
+            po = a.few_o;
+            stride = a.few_rows;
+            at = ((long long)s.s * a.few_cap + (t - s.begin) * G + (h - kvh * G)) * a.p.num_kv + kvh;
+            last = splits - 1;
+            ml = a.few_ml[min(lane, last) * stride + at];
+            x = part(slot);
+        }
     }
     if (lane >= nc) ml = make_float2(-INFINITY, 0.f);
     const float M = wave_max(ml.x), use = M == -INFINITY ? 0.f : M;
@@ -981,6 +1010,8 @@ struct AttnPlan {
     int few_per, few_tiles, many_tiles;
     int few_chunk, few_splits, many_chunk, many_splits;
     bool few_last_first;
+    int few_cap;
+    long long few_part, many_part;  // rows of partial sums
     size_t bytes;
 };
 
@@ -1021,7 +1052,8 @@ static AttnPlan attn_plan(const PagedArgs& p, int hq, int max_new) {
         // longest sequence's end is not waited for alone
         const long long n = std::max(over(1024, few), few < 2048 ? over(p.limit, 2048) : 1);
         const int unit = few * over(p.limit, 256) < 128 ? 128 : 256;
-        r.few_splits = split(n, unit, r.few_chunk);
+        // (past 2^25 rows a join would leave a launch's range)
+        r.few_splits = split((long long)p.tokens * hq < 1 << 25 ? n : 1, unit, r.few_chunk);
         // more blocks than run at once: the last splits first, which are the
         // long sequences' (64 conversations in e4m3 97.5 -> 93.8 us; where all
         // run at once it costs: 3 x 32,749 keys 17.4 -> 21 us)
@@ -1029,8 +1061,12 @@ static AttnPlan attn_plan(const PagedArgs& p, int hq, int max_new) {
     }
     // (two blocks a CU, three with up to 64 columns, all at once)
     if (r.many) r.many_splits = split(over(p.hd <= 64 ? 768 : 512, many), 128, r.many_chunk);
-    const int n = std::max(r.few_splits, r.many_splits);
-    if (n > 1) r.bytes = (size_t)n * p.tokens * hq * (p.hd * 4 + 8);
+    // (single tokens beside prompts have rows of their own: as part of the
+    // prompts' they would take hundreds of times the memory)
+    r.few_cap = r.few && r.many ? r.few_per * r.few_width : 0;
+    r.many_part = r.many_splits > 1 ? p.tokens * (long long)hq : 0;
+    r.few_part = r.few_splits == 1 ? 0 : (r.few_cap ? (long long)p.seqs * r.few_cap * p.num_kv : p.tokens * (long long)hq);
+    r.bytes = (size_t)(r.few_splits * r.few_part + r.many_splits * r.many_part) * (p.hd * 4 + 8);
     return r;
 }
 
@@ -1069,6 +1105,11 @@ template <bool F8, int HD, bool PART>
 static void launch_attn(hipStream_t s, const PagedAttnArgs& base, const AttnPlan& pl) {
     constexpr int NR = HD <= 128 ? 2 : 1, NT = kManyRows / NR * 4;
     PagedAttnArgs few = base, many = base;
+    few.part_o = base.few_o;
+    few.part_ml = base.few_ml;
+    few.part_rows = pl.few_part;
+    few.few_cap = pl.few_cap;
+    many.part_rows = pl.many_part;
     few.tiles = pl.few_tiles;
     few.per = pl.few_per;
     few.lo_rows = 0;
@@ -1146,7 +1187,7 @@ extern "C" int gorch_hip_paged_attention(void* stream, const gorch_hip_paged_kv*
     GH_REQUIRE(q && out, "gorch_hip_paged_attention: null q or out");
     const AttnPlan pl = attn_plan(a.p, num_q, b->max_new);
     // (a launch has less than 2^32 threads)
-    GH_SUPPORTED((!pl.few || (long long)pl.few_tiles * kv->num_kv * pl.few_splits < 1 << 24) &&
+    GH_SUPPORTED((!pl.few || (long long)pl.few_tiles * kv->num_kv * pl.few_splits < 1 << 23) &&
                      (!pl.many || (long long)pl.many_tiles * kv->num_kv * pl.many_splits < 1 << 23),
                  "gorch_hip_paged_attention: too many sequences or tokens for one call");
     GH_REQUIRE(workspace_bytes >= pl.bytes && (workspace || pl.bytes == 0),
@@ -1160,8 +1201,11 @@ extern "C" int gorch_hip_paged_attention(void* stream, const gorch_hip_paged_kv*
     a.out = out;
     a.causal = causal != 0;
     const int splits = std::max(pl.few_splits, pl.many_splits);
-    a.part_o = static_cast<float*>(workspace);
-    a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)splits * a.p.tokens * num_q * a.p.hd);
+    const size_t few_part = (size_t)pl.few_splits * pl.few_part, many_part = (size_t)pl.many_splits * pl.many_part;
+    a.few_o = static_cast<float*>(workspace);
+    a.part_o = a.few_o + few_part * a.p.hd;
+    a.few_ml = reinterpret_cast<float2*>(a.part_o + many_part * a.p.hd);
+    a.part_ml = a.few_ml + few_part;
     if (kv->dtype == GORCH_HIP_KV_E4M3) launch_attn_hd<true>(s, a, pl);
     else launch_attn_hd<false>(s, a, pl);
     GH_TRY(check_launch("paged_attention"));
@@ -1171,6 +1215,14 @@ extern "C" int gorch_hip_paged_attention(void* stream, const gorch_hip_paged_kv*
         a.splits = pl.few_splits;
         a.chunk2 = pl.many_chunk;
         a.splits2 = pl.many_splits;
+        a.few_cap = pl.few_cap;
+        a.few_rows = pl.few_part;
+        a.part_rows = pl.many_part;
+        if (pl.many_part == 0) {  // (of few rows alone, or read for nothing)
+            a.part_o = a.few_o;
+            a.part_ml = a.few_ml;
+            a.part_rows = pl.few_part;
+        }
         launch_join(s, a, splits);
         GH_TRY(check_launch("paged_attention join"));
     }

@@ -144,6 +144,13 @@ def test_too_many_heads_are_refused():
     assert append(cache(), batch(tokens=0), w) == 1
 
 
+def test_workspace_of_a_long_prompt_beside_single_tokens_stays_small():
+    # 64 key ranges for the 7 single tokens' rows alone
+    n = hip.lib().gorch_hip_paged_attention_workspace_size(
+        C.byref(cache(num_kv=8, head_dim=128)), C.byref(batch(tokens=8199, seqs=8, max_pages=8192)), 32)
+    assert 64 * 7 * 32 * 130 * 4 <= n < 32 << 20
+
+
 def test_too_large_a_launch_is_refused():
     # 2^24 sequences of a token or less, 1 KV head: one launch has fewer blocks
     kv, b = cache(num_kv=1), batch(tokens=16, seqs=1 << 25, max_new=1)

@@ -246,7 +246,10 @@ def test_captured_mixed_step_follows_the_batch(gpu):
     (2, 1, 256, [(700, 90)]), (2, 1, 208, [(700, 90), (300, 1)]), (3, 1, 112, [(900, 70)]), (2, 2, 32, [(900, 70)]),
     # tiles of 4 and 16 rows, split
     (4, 2, 192, [(1500, 1), (1100, 2)]), (7, 1, 96, [(1500, 1)]), (16, 1, 256, [(1500, 1), (3, 1)]),
-    (5, 1, 32, [(1500, 3)]), (1, 1, 16, [(1500, 9)])])
+    (5, 1, 32, [(1500, 3)]), (1, 1, 16, [(1500, 9)]),
+    # both kinds of rows: one split, the other, both; two tiles of single rows; heads that fill more than two
+    (4, 4, 64, [(100, 1)] * 3 + [(700, 400)]), (2, 1, 128, [(4000, 2), (90, 90)]), (20, 1, 80, [(1500, 1), (900, 70)]),
+    (40, 1, 64, [(300, 1), (70, 1), (900, 2)])])
 def test_splits(gpu, dtype, hq, hkv, hd, seqs):
     c = Case(dtype, hkv, hd, 24, seqs, seed=hd + hq)
     bounds = dict(max_new=max(n for _, n in seqs), max_kv=max(n for n, _ in seqs))
