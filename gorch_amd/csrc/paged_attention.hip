@@ -388,7 +388,7 @@ struct Rows {
     }
 };
 
-// Where tile `tile` of 16 * rows_per_tile/16 flattened rows (token, head of the
+// Where tile `tile` of BM flattened rows (token, head of the
 // group) stands: the sequence and its first row. Tiles are numbered from
 // floor(first row * G / BM) + s for sequence s, which leaves room for a part
 // tile each.
@@ -1048,9 +1048,14 @@ static AttnPlan attn_plan(const PagedArgs& p, int hq, int max_new) {
                                                    p.seqs * over(most, bm)) * p.num_kv;
     r.few_splits = r.many_splits = 1;
     if (r.few) {
-        // 1024 blocks, four a CU; ranges of at most 2048 keys, so that the
-        // longest sequence's end is not waited for alone
-        const long long n = std::max(over(1024, few), few < 2048 ? over(p.limit, 2048) : 1);
+        // 1024 blocks, four a CU, whose ends even out over ragged lengths; of up
+        // to 32 tiles, or where a CU holds one block (more than 128 columns), one
+        // a CU: 3 tokens over up to 32,749 keys 16.5 -> 13.8 us, 4 of 32/8 x 128
+        // over 10,000 32 -> 26, 64 of 8/1 x 256 over 8,192 91 -> 70; but 64 of
+        // 14/2 x 64 over 4,096 15.8 -> 21. Ranges of at most 2048 keys, so that
+        // the longest sequence's end is not waited for alone
+        const long long blocks = few <= 32 || p.hd > 128 ? 256 : 1024;
+        const long long n = std::max(over(blocks, few), few < 2048 ? over(p.limit, 2048) : 1);
         const int unit = few * over(p.limit, 256) < 128 ? 128 : 256;
         // (past 2^25 rows a join would leave a launch's range)
         r.few_splits = split((long long)p.tokens * hq < 1 << 25 ? n : 1, unit, r.few_chunk);
