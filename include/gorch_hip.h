@@ -478,8 +478,8 @@ typedef struct {
  * nn/gqa.go:300-330): per-head RMSNorm where there is a gain (f64 sum of
  * squares), then RoPE at the token's position where there are tables, in f32
  * as gorch_hip_gqa_forward_cached; then K and V are rounded once: to bf16
- * (nearest even), or to e4m3 codes of x / scale with scale = (the row's
- * largest magnitude) / 448 (a row below 2^-100 throughout is stored as
+ * (nearest even), or to e4m3 codes of x * (448 / m) with scale = m / 448, m the
+ * row's largest magnitude (a row below 2^-100 throughout is stored as
  * zeros; a row that holds an infinity reads back as NaN). Rows q [tokens,
  * num_q * head_dim], k and v [tokens, num_kv * head_dim] start at multiples
  * of their strides (in floats, multiples of 4), so the three can be column
