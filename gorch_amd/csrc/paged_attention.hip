@@ -985,9 +985,10 @@ __global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttnArgs a) {
     for (int j = slot; j - slot < nc; j += SLOTS) {
         const floatx4 y = part(j + SLOTS);
         const float f = __shfl(w, j & 63);
+        // (an infinity is a value's, noted: it stays where its range's weight, f, is 0)
         if (j < nc)
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[e] += f * x[e];
+            for (int e = 0; e < 4; e++) o[e] += __builtin_isinf(x[e]) ? x[e] : f * x[e];
         x = y;
     }
     so[sub][slot][c] = o;
