@@ -1048,6 +1048,8 @@ static AttnPlan attn_plan(const PagedArgs& p, int hq, int max_new) {
     const long long many = std::min<long long>(over(p.tokens * G, bm) + (over(p.tokens * G, most) - 1) / 2,
                                                    p.seqs * over(most, bm)) * p.num_kv;
     r.few_splits = r.many_splits = 1;
+    // (past 2^25 rows a join would leave a launch's range)
+    const bool joins = (long long)p.tokens * hq < 1 << 25;
     if (r.few) {
         // 1024 blocks, four a CU, whose ends even out over ragged lengths; of up
         // to 32 tiles, or where a CU holds one block (more than 128 columns), one
@@ -1058,15 +1060,14 @@ static AttnPlan attn_plan(const PagedArgs& p, int hq, int max_new) {
         const long long blocks = few <= 32 || p.hd > 128 ? 256 : 1024;
         const long long n = std::max(over(blocks, few), few < 2048 ? over(p.limit, 2048) : 1);
         const int unit = few * over(p.limit, 256) < 128 ? 128 : 256;
-        // (past 2^25 rows a join would leave a launch's range)
-        r.few_splits = split((long long)p.tokens * hq < 1 << 25 ? n : 1, unit, r.few_chunk);
+        r.few_splits = split(joins ? n : 1, unit, r.few_chunk);
         // more blocks than run at once: the last splits first, which are the
         // long sequences' (64 conversations in e4m3 97.5 -> 93.8 us; where all
         // run at once it costs: 3 x 32,749 keys 17.4 -> 21 us)
         r.few_last_first = few * r.few_splits > 768;
     }
     // (two blocks a CU, three with up to 64 columns, all at once)
-    if (r.many) r.many_splits = split(over(p.hd <= 64 ? 768 : 512, many), 128, r.many_chunk);
+    if (r.many) r.many_splits = split(joins ? over(p.hd <= 64 ? 768 : 512, many) : 1, 128, r.many_chunk);
     // (single tokens beside prompts have rows of their own: as part of the
     // prompts' they would take hundreds of times the memory)
     r.few_cap = r.few && r.many ? r.few_per * r.few_width : 0;
