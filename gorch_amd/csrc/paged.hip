@@ -146,7 +146,7 @@ struct AppendArgs {
 // the pair rotated with every product and sum rounded on its own.
 // Bound by memory: the rows go out before anything else, and the chain
 // sequence -> page -> store runs beside them. Large calls (P > 1) read them
-// past the caches: 12,288 tokens of 14 + 2 + 2 heads of 64 into e4m3 38.7 ->
+// past the caches: 15,518 tokens of 14 + 2 + 2 heads of 64 into e4m3 38.7 ->
 // 35.5 us (3.8 TB/s; two or four tokens a block: 39.4, 46). One token 3.6 us
 // on the GPU.
 template <bool F8, int NL, bool FULL, int P>
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
 }
 
 // TOK tokens a block: their places first, then every load of K and V (a thread
-// keeps its four columns), then the stores. Bound by memory: 60,000 tokens of
+// keeps its four columns), then the stores. Bound by memory: 57,512 tokens of
 // 8 x 128 in e4m3 116 us with four tokens a block (5.1 TB/s), 172 with one;
 // few tokens have one a block (1,000 in bf16 4.3 us against 5.0).
 template <bool F8, int TOK>

@@ -617,11 +617,14 @@ struct FewRows {
 // range of its keys, its four waves 32 keys each in turn. K goes from memory
 // to the operand registers, V through a wave's own LDS; NB tiles of rows are
 // on their way while one is weighed (a fetch is unconditional: a branch around
-// loads would make the next use wait for all of them). Bound by memory: 64
-// conversations of up to 8,192 tokens, 8 x 128 in e4m3 (395 MB), 95 us with
-// the join, 4.2 TB/s of the 4.9 that a copy reaches, the rest being a block's
-// first loads and the last ranges to end; one token over 777 keys 6.7 us and 3.4
-// for the join, three dependent round trips (page, key, key of the next step).
+// loads would make the next use wait for all of them; one tile where two would
+// leave the registers, bf16 of 128 columns and either type of 256). Bound by
+// the loads that a CU keeps in flight: 64 conversations of up to 8,192 tokens,
+// 8 x 128 in e4m3 (397 MB), 96 us with the join, 4.1 TB/s (in bf16 170 us, 4.5),
+// where plain reads reach 7.1; waves wait a quarter of their cycles, the matrix
+// cores are busy 5%, and a block's first loads and the last ranges' ends are
+// not covered by others. One token over 777 keys 6.7 us and 3.4 for the join,
+// three dependent round trips (page, key, key of the next step).
 template <bool F8, int HD, bool PART, int CW>
 struct FewBlock {
     static constexpr int NW = 4, NB = Tile<F8, HD>::NT <= 2 ? 2 : 1, OROW = HD + 4;
@@ -793,11 +796,14 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : (HD == 64 && CW == 4 ? 3 : 2)) 
 // Many rows: a block takes 128 rows of a sequence, 16 NR a wave, and its keys
 // (or a range of them) in tiles of 32 that all NW waves read from LDS. Loads
 // go straight to LDS, two tiles ahead of the one that is weighed: one on its
-// way, one landed, in which the waves look for infinities in V. Bound by the
-// matrix cores: 2,048 rows of 16 heads of 128 over 16,384 keys (257 GFLOP, 771
-// in three terms) 642-662 us, 1.2 PFLOP/s of matrix instructions, the rate of a
-// large bf16 product here. (No faster: a ring of four or five tiles, operands
-// read two or three steps ahead, priorities by wave.)
+// way, one landed, in which the waves look for infinities in V. 2,048 rows of 16
+// heads of 128 over 16,384 keys (257 GFLOP, 771 in three terms) 641-662 us (e4m3,
+// which every wave widens for itself, 728): 1.2 PFLOP/s of matrix instructions,
+// the rate of a large bf16 product here, of the 2.05 that a plain loop of them
+// reaches. The matrix cores are busy 53%; a wave's exponentials, splits and LDS
+// reads stand between its products, and the block meets every 32 keys with all
+// its loads landed. (No faster: a ring of four or five tiles, operands read two
+// or three steps ahead, priorities by wave.)
 constexpr int kManyRows = 128;
 template <bool F8, int HD>
 struct ManyBlock {
@@ -1051,22 +1057,27 @@ static AttnPlan attn_plan(const PagedArgs& p, int hq, int max_new) {
     // (past 2^25 rows a join would leave a launch's range)
     const bool joins = (long long)p.tokens * hq < 1 << 25;
     if (r.few) {
-        // 1024 blocks, four a CU, whose ends even out over ragged lengths; of up
-        // to 32 tiles, or where a CU holds one block (more than 128 columns), one
-        // a CU: 3 tokens over up to 32,749 keys 16.5 -> 13.8 us, 4 of 32/8 x 128
-        // over 10,000 32 -> 26, 64 of 8/1 x 256 over 8,192 91 -> 70; but 64 of
-        // 14/2 x 64 over 4,096 15.8 -> 21. Ranges of at most 2048 keys, so that
-        // the longest sequence's end is not waited for alone
+        // 1024 blocks, four for each CU (which holds two to four at once), whose
+        // ends even out over ragged lengths; of up to 32 tiles, or where a CU
+        // holds one block (more than 128 columns), one a CU: 3 tokens over up to
+        // 32,749 keys 16.5 -> 13.8 us, 4 of 32/8 x 128 over 10,000 32 -> 26, 64 of
+        // 8/1 x 256 over 8,192 91 -> 70; but 64 of 14/2 x 64 over 4,096 15.8 -> 21.
+        // Ranges of at most 2048 keys, so that the longest sequence's end is not
+        // waited for alone; not from 2048 tiles on, where it costs a batch of one
+        // long sequence: one of 32,768 keys (16/8 x 128, bf16) and others of 500,
+        // 154 us for 255 sequences, 500 for 256
         const long long blocks = few <= 32 || p.hd > 128 ? 256 : 1024;
         const long long n = std::max(over(blocks, few), few < 2048 ? over(p.limit, 2048) : 1);
         const int unit = few * over(p.limit, 256) < 128 ? 128 : 256;
         r.few_splits = split(joins ? n : 1, unit, r.few_chunk);
-        // more blocks than run at once: the last splits first, which are the
-        // long sequences' (64 conversations in e4m3 97.5 -> 93.8 us; where all
-        // run at once it costs: 3 x 32,749 keys 17.4 -> 21 us)
+        // more blocks than most kernels run at once (256 to 1024 by type, columns
+        // and tile): the last splits first, which are the long sequences' (64
+        // conversations in e4m3 97.5 -> 93.8 us; where all run at once it costs: 3
+        // x 32,749 keys 17.4 -> 21 us)
         r.few_last_first = few * r.few_splits > 768;
     }
-    // (two blocks a CU, three with up to 64 columns, all at once)
+    // (two blocks a CU, three with up to 64 columns, all at once; with more than
+    // 128, whose 512 threads have a CU alone, two rounds)
     if (r.many) r.many_splits = split(joins ? over(p.hd <= 64 ? 768 : 512, many) : 1, 128, r.many_chunk);
     // (single tokens beside prompts have rows of their own: as part of the
     // prompts' they would take hundreds of times the memory)
