@@ -1,0 +1,144 @@
+// mx.h — MXFP4 and the matrix instructions that take it.
+//
+// A value is an e2m1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives)
+// times 2^(s - 127), s the e8m0 scale byte of its group of 32 along a row
+// (255: NaN). v_mfma_scale_f32_16x16x128_f8f6f4 multiplies such groups as they
+// lie in memory: lane l holds row l % 16, columns 32 (l / 16) .. + 31 of an
+// operand (a group and its scale byte) of either side, and lane (g, c) of the
+// result rows 4 g .. 4 g + 3 of column c.
+//
+// The other operand is f32: x in a group of 32 is the sum of five terms
+//   x = sum_t d_t 2^(e - 5 t),   d_t a multiple of 1/8 with |d_t| <= 2,
+// e the exponent of the group's largest magnitude: |x| / 2^e < 2, what rounding
+// to eighths leaves is at most 1/16 = 2 / 32, and so on. An e2m3 (6-bit) code
+// holds every such d exactly, and five of them leave at most 2^-24 of the
+// largest, which itself is kept whole: f32's own rounding of the group's
+// largest value. The five products run at four times the bf16 rate each, with
+// no code widened, where three bf16 terms would need it; four terms (2^-19)
+// would leave errors ten times those of f32 sums. Products and their sums are
+// exact to 2^-24 of the sum of their magnitudes (measured).
+#pragma once
+#include "common.h"
+
+namespace gh {
+
+constexpr int kMxGroup = 32;
+constexpr int kMxTerms = 5;
+constexpr uint32_t kMxNaN = 255;           // a scale byte
+constexpr uint32_t kMxTiny = 27u << 23;    // 2^-100: groups below it throughout are stored as zeros
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x6 __attribute__((ext_vector_type(6)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx32 __attribute__((ext_vector_type(32)));
+typedef __bf16 mx_bf16x2 __attribute__((ext_vector_type(2)));
+
+// The scale byte of a group whose largest magnitude has these bits: the
+// smallest power of two that it exceeds at most 7 times (codes end at 6, and 7
+// is half a step above), 255 for infinities and NaN, 0 for next to nothing.
+__host__ __device__ __forceinline__ uint32_t mx_scale(uint32_t top) {
+    if (top >= 0x7f800000u) return kMxNaN;
+    return top < kMxTiny ? 0 : ((top + 0x1fffffu) >> 23) - 2;
+}
+
+// Eight values of a group with this scale byte as codes (nearest even,
+// clipped at 6), the first in the low nibble.
+__device__ __forceinline__ uint32_t mx_encode8(const float (&x)[8], uint32_t scale) {
+    const float s = __uint_as_float(scale << 23);
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], s, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
+    return scale == 0 || scale == kMxNaN ? 0 : w;
+}
+
+// Four of them.
+__device__ __forceinline__ uint32_t mx_encode4(float a, float b, float c, float d, uint32_t scale) {
+    const float s = __uint_as_float(scale << 23);
+    uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, a, b, s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, c, d, s, 1);
+    return scale == 0 || scale == kMxNaN ? 0 : w;
+}
+
+// Two codes of byte B of w as bf16 times 2^0 (exact).
+template <int B>
+__device__ __forceinline__ uint32_t mx_pair(uint32_t w, float s) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, B));
+}
+// Eight codes as bf16 times s, a power of two of a normal f32 (exact).
+__device__ __forceinline__ u32x4 mx_widen8(uint32_t w, float s) {
+    return u32x4{mx_pair<0>(w, s), mx_pair<1>(w, s), mx_pair<2>(w, s), mx_pair<3>(w, s)};
+}
+
+// 2^(s - 127) as f32 (NaN for 255).
+__device__ __forceinline__ float mx_power(uint32_t s) {
+    return __uint_as_float(s == 0 ? 0x00400000u : (s == kMxNaN ? 0x7fc00000u : s << 23));
+}
+
+// The five terms of a group of 32 (see above): 24-byte operands in order of
+// the values, and their scale bytes, those of terms 0 .. 3 in `scale`, that of
+// term 4 in `last`. An infinity or NaN in the group makes them NaN.
+// (The conversions of 32 values write their result in several passes, and the
+// compiler may give it a register that a later pass still reads, the scale's:
+// the empty asm keeps all they read alive past them.)
+__device__ __forceinline__ u32x6 mx_to6(floatx32 x, float s) {
+    floatx16 a, b;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        a[i] = x[2 * i];
+        b[i] = x[2 * i + 1];
+    }
+    const u32x6 r = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, s);
+    asm volatile("" ::"v"(a), "v"(b), "v"(s), "v"(r));
+    return r;
+}
+__device__ __forceinline__ floatx32 mx_from6(u32x6 t, float s) {
+    const floatx32 r = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(t, s);
+    asm volatile("" ::"v"(t), "v"(s), "v"(r));
+    return r;
+}
+struct MxTerms {
+    u32x6 t[kMxTerms];
+    uint32_t scale, last;
+};
+__device__ __forceinline__ void mx_split(floatx32 x, MxTerms& r) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 32; i++) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    const bool odd = top >= 0x7f800000u;
+    // (the last term's scale is a normal number)
+    const uint32_t e = max(top >> 23, 5u * (kMxTerms - 1) + 1);
+#pragma unroll
+    for (int t = 0; t < kMxTerms; t++) {
+        const float s = __uint_as_float((odd ? 127u : e - 5 * t) << 23);
+        r.t[t] = mx_to6(x, s);
+        if (t + 1 < kMxTerms) x -= mx_from6(r.t[t], s);
+    }
+    r.scale = odd ? ~0u : e * 0x01010101u - 0x0f0a0500u;
+    r.last = odd ? kMxNaN : e - 20;
+}
+
+__device__ __forceinline__ i32x8 mx_op6(u32x4 lo, u32x2 hi) {
+    return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], 0, 0};
+}
+__device__ __forceinline__ i32x8 mx_op6(u32x6 t) {
+    return i32x8{(int)t[0], (int)t[1], (int)t[2], (int)t[3], (int)t[4], (int)t[5], 0, 0};
+}
+__device__ __forceinline__ i32x8 mx_op4(u32x4 c) {
+    return i32x8{(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
+}
+// c + six . four^T: rows are the 6-bit operand's, columns the codes'. SB6, SB4:
+// the byte of each scale word.
+template <int SB6, int SB4>
+__device__ __forceinline__ floatx4 mx_mfma(i32x8 six, uint32_t s6, i32x8 four, uint32_t s4, floatx4 c) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(six, four, c, 2, 4, SB6, (int)s6, SB4, (int)s4);
+}
+// c + four . six^T: rows are the codes'.
+template <int SB4, int SB6>
+__device__ __forceinline__ floatx4 mx_mfma_t(i32x8 four, uint32_t s4, i32x8 six, uint32_t s6, floatx4 c) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(four, six, c, 4, 2, SB4, (int)s4, SB6, (int)s6);
+}
+
+}  // namespace gh

@@ -1,7 +1,8 @@
 // paged.hip — a KV cache in pages: new tokens' q and k finished (per-head
 // RMSNorm, RoPE; GQA.ForwardCached's order, nn/gqa.go:300-330) and K and V
-// written in bf16 or quantised to e4m3 (gorch_hip_paged_append), and rows
-// read back as f32 (gorch_hip_paged_read).
+// written in bf16 or quantised to e4m3 or MXFP4 (gorch_hip_paged_append), and
+// rows read back as f32 (gorch_hip_paged_read).
+#include "mx.h"
 #include "paged.h"
 
 namespace gh {
@@ -14,7 +15,8 @@ int paged_args(const char* who, const gorch_hip_paged_kv* kv, const gorch_hip_pa
         return rc;
     };
     if (!kv || !b) return fail(GORCH_HIP_EINVAL, "null cache or batch");
-    if (kv->dtype != GORCH_HIP_KV_BF16 && kv->dtype != GORCH_HIP_KV_E4M3) return fail(GORCH_HIP_EINVAL, "unknown cache dtype");
+    if (kv->dtype != GORCH_HIP_KV_BF16 && kv->dtype != GORCH_HIP_KV_E4M3 && kv->dtype != GORCH_HIP_KV_MXFP4)
+        return fail(GORCH_HIP_EINVAL, "unknown cache dtype");
     if (kv->num_pages <= 0 || kv->page_size <= 0 || kv->num_kv <= 0 || kv->head_dim <= 0)
         return fail(GORCH_HIP_EINVAL, "cache sizes must be positive");
     if (b->tokens < 0 || b->seqs < 0 || b->max_pages < 0 || b->max_new < 0 || b->max_kv < 0)
@@ -29,8 +31,8 @@ int paged_args(const char* who, const gorch_hip_paged_kv* kv, const gorch_hip_pa
     if (b->tokens > 0 && b->seqs > 0) {
         if (!kv->k || !kv->v || !b->cu_seqlens || !b->kv_lens || (b->max_pages > 0 && !b->page_table))
             return fail(GORCH_HIP_EINVAL, "null pool or batch array");
-        if (kv->dtype == GORCH_HIP_KV_E4M3 && (!kv->k_scale || !kv->v_scale))
-            return fail(GORCH_HIP_EINVAL, "e4m3 pools need k_scale and v_scale");
+        if (kv->dtype != GORCH_HIP_KV_BF16 && (!kv->k_scale || !kv->v_scale))
+            return fail(GORCH_HIP_EINVAL, "e4m3 and MXFP4 pools need k_scale and v_scale");
         if (!aligned(kv->k, 16) || !aligned(kv->v, 16)) return fail(GORCH_HIP_EUNSUPPORTED, "pools must be 16-byte aligned");
     }
     a.k = kv->k;
@@ -103,10 +105,24 @@ __device__ __forceinline__ float row_max_f(float v) {
 constexpr float kTinyRow = 0x1p-100f;
 
 // Four values of a row to its pool row: bf16, or codes of x / scale, scale =
-// amax / 448 the row's (NL lanes; every lane of the wave calls it).
-template <bool F8, int NL>
+// amax / 448 the row's (NL lanes; every lane of the wave calls it), or MXFP4
+// (eight lanes a group). KV: the pools' dtype.
+template <int KV, int NL>
 __device__ __forceinline__ void store_kv(void* pool, float* scales, long long row, int hd, int c, bool mine, float4 x) {
-    if constexpr (F8) {
+    if constexpr (KV == GORCH_HIP_KV_MXFP4) {
+        if (!mine) x = make_float4(0.f, 0.f, 0.f, 0.f);
+        const auto bits = [](float v) { return __float_as_uint(v) & 0x7fffffffu; };
+        uint32_t top = max(max(bits(x.x), bits(x.y)), max(bits(x.z), bits(x.w)));
+        top = max(top, __float_as_uint(dpp_f<kDppQuadSwap1>(__uint_as_float(top))));
+        top = max(top, __float_as_uint(dpp_f<kDppQuadSwap2>(__uint_as_float(top))));
+        top = max(top, __float_as_uint(dpp_f<kDppRowHalfMirror>(__uint_as_float(top))));
+        const uint32_t s = mx_scale(top);
+        const uint32_t w = mx_encode4(x.x, x.y, x.z, x.w, s);
+        if (mine && row >= 0) {
+            reinterpret_cast<uint16_t*>(pool)[(row * hd) / 4 + c] = (uint16_t)w;
+            if (c % 8 == 0) reinterpret_cast<uint8_t*>(scales)[row * ((hd + 31) / 32) + c / 8] = (uint8_t)s;
+        }
+    } else if constexpr (KV == GORCH_HIP_KV_E4M3) {
         const float m = row_max_f<NL>(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
         const float inv = m >= kTinyRow ? 448.0f / m : 0.0f;
         int w = __builtin_amdgcn_cvt_pk_fp8_f32(x.x * inv, x.y * inv, 0, false);
@@ -149,7 +165,7 @@ struct AppendArgs {
 // past the caches: 15,518 tokens of 14 + 2 + 2 heads of 64 into e4m3 38.7 ->
 // 35.5 us (3.8 TB/s; two or four tokens a block: 39.4, 46). One token 3.6 us
 // on the GPU.
-template <bool F8, int NL, bool FULL, int P>
+template <int KV, int NL, bool FULL, int P>
 __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
 #pragma clang fp contract(off)
     constexpr int RPB = 256 / NL;
@@ -241,7 +257,7 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
         if (isq && mine) *reinterpret_cast<float4*>(a.q_out + ((size_t)t * a.hq + h) * hd + 4 * c) = y;
         // the pool rows of a position's heads lie a page's slots apart
         const long long row = mine && !isq ? row0 + (long long)h * a.p.page.d : -1;
-        store_kv<F8, NL>(isk ? a.p.k : a.p.v, isk ? a.p.ks : a.p.vs, row, hd, c, mine, y);
+        store_kv<KV, NL>(isk ? a.p.k : a.p.v, isk ? a.p.ks : a.p.vs, row, hd, c, mine, y);
     }
 }
 
@@ -249,7 +265,7 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
 // keeps its four columns), then the stores. Bound by memory: 57,512 tokens of
 // 8 x 128 in e4m3 116 us with four tokens a block (5.1 TB/s), 172 with one;
 // few tokens have one a block (1,000 in bf16 4.3 us against 5.0).
-template <bool F8, int TOK>
+template <int KV, int TOK>
 __global__ __launch_bounds__(256) void k_paged_read(PagedArgs p, float* ko, float* vo) {
     const int t0 = blockIdx.x * TOK, hd4 = p.hd / 4, n4 = p.num_kv * hd4;
     const int i0 = blockIdx.y * 256 + threadIdx.x, i = min(i0, n4 - 1), h = i / hd4, c = i - h * hd4;
@@ -261,7 +277,8 @@ __global__ __launch_bounds__(256) void k_paged_read(PagedArgs p, float* ko, floa
         if (t0 + j < p.tokens && token_seq(p, t0 + j, sq)) row[j] = pool_row(p, sq.s, sq.len - sq.end + t0 + j, h);
     }
     if (i0 >= n4) return;
-    using Raw = typename std::conditional<F8, uint32_t, uint2>::type;
+    constexpr bool F8 = KV == GORCH_HIP_KV_E4M3, F4 = KV == GORCH_HIP_KV_MXFP4;
+    using Raw = typename std::conditional<F4, uint16_t, typename std::conditional<F8, uint32_t, uint2>::type>::type;
     Raw u[2][TOK];
     float sc[2][TOK];
 #pragma unroll
@@ -271,6 +288,8 @@ __global__ __launch_bounds__(256) void k_paged_read(PagedArgs p, float* ko, floa
             if (row[j] < 0 || !(w ? vo : ko)) continue;
             u[w][j] = reinterpret_cast<const Raw*>(w ? p.v : p.k)[row[j] * hd4 + c];
             if constexpr (F8) sc[w][j] = (w ? p.vs : p.ks)[row[j]];
+            if constexpr (F4)
+                sc[w][j] = mx_power(reinterpret_cast<const uint8_t*>(w ? p.vs : p.ks)[row[j] * ((p.hd + 31) / 32) + c / 8]);
         }
 #pragma unroll
     for (int w = 0; w < 2; w++)
@@ -283,6 +302,10 @@ __global__ __launch_bounds__(256) void k_paged_read(PagedArgs p, float* ko, floa
                 const uint32_t v = u[w][j];
                 const float f = sc[w][j];
                 x = make_float4(e4m3_f32<0>(v) * f, e4m3_f32<1>(v) * f, e4m3_f32<2>(v) * f, e4m3_f32<3>(v) * f);
+            } else if constexpr (F4) {
+                const uint32_t lo = mx_pair<0>(u[w][j], 1.0f), hi = mx_pair<1>(u[w][j], 1.0f);
+                const float f = sc[w][j];
+                x = make_float4(bf16_lo(lo) * f, bf16_hi(lo) * f, bf16_lo(hi) * f, bf16_hi(hi) * f);
             } else {
                 x = make_float4(bf16_lo(u[w][j].x), bf16_hi(u[w][j].x), bf16_lo(u[w][j].y), bf16_hi(u[w][j].y));
             }
@@ -292,26 +315,26 @@ __global__ __launch_bounds__(256) void k_paged_read(PagedArgs p, float* ko, floa
 
 // Rows per lane group: one while the call's blocks leave CUs idle (a step's
 // latency), else as many as spare a token a second block, up to 4.
-template <bool F8, int NL, bool FULL>
+template <int KV, int NL, bool FULL>
 static void launch_append_nl(hipStream_t s, const AppendArgs& a) {
     constexpr int RPB = 256 / NL;
     const int rows = a.hq + 2 * a.p.num_kv, groups = (rows + RPB - 1) / RPB;
     const auto go = [&](auto kernel, int per) {
         hipLaunchKernelGGL(kernel, dim3(a.p.tokens, (groups + per - 1) / per), dim3(256), 0, s, a);
     };
-    if (groups == 1 || (long long)a.p.tokens * groups <= 1024) go(k_paged_append<F8, NL, FULL, 1>, 1);
-    else if (groups == 2) go(k_paged_append<F8, NL, FULL, 2>, 2);
-    else go(k_paged_append<F8, NL, FULL, 4>, 4);
+    if (groups == 1 || (long long)a.p.tokens * groups <= 1024) go(k_paged_append<KV, NL, FULL, 1>, 1);
+    else if (groups == 2) go(k_paged_append<KV, NL, FULL, 2>, 2);
+    else go(k_paged_append<KV, NL, FULL, 4>, 4);
 }
-template <bool F8>
+template <int KV>
 static void launch_append(hipStream_t s, const AppendArgs& a) {
     const int hd = a.p.hd;
-    if (hd == 64) launch_append_nl<F8, 16, true>(s, a);
-    else if (hd < 64) launch_append_nl<F8, 16, false>(s, a);
-    else if (hd == 128) launch_append_nl<F8, 32, true>(s, a);
-    else if (hd < 128) launch_append_nl<F8, 32, false>(s, a);
-    else if (hd == 256) launch_append_nl<F8, 64, true>(s, a);
-    else launch_append_nl<F8, 64, false>(s, a);
+    if (hd == 64) launch_append_nl<KV, 16, true>(s, a);
+    else if (hd < 64) launch_append_nl<KV, 16, false>(s, a);
+    else if (hd == 128) launch_append_nl<KV, 32, true>(s, a);
+    else if (hd < 128) launch_append_nl<KV, 32, false>(s, a);
+    else if (hd == 256) launch_append_nl<KV, 64, true>(s, a);
+    else launch_append_nl<KV, 64, false>(s, a);
 }
 
 }  // namespace gh
@@ -355,8 +378,9 @@ extern "C" int gorch_hip_paged_append(void* stream, const gorch_hip_paged_kv* kv
     a.sinT = w->rope_sin;
     a.rope_rows = w->rope_max_seq;
     a.neox = w->rope_neox;
-    if (kv->dtype == GORCH_HIP_KV_E4M3) launch_append<true>(stream_of(stream), a);
-    else launch_append<false>(stream_of(stream), a);
+    if (kv->dtype == GORCH_HIP_KV_MXFP4) launch_append<GORCH_HIP_KV_MXFP4>(stream_of(stream), a);
+    else if (kv->dtype == GORCH_HIP_KV_E4M3) launch_append<GORCH_HIP_KV_E4M3>(stream_of(stream), a);
+    else launch_append<GORCH_HIP_KV_BF16>(stream_of(stream), a);
     count(CNT_ELEMENTWISE);
     return finish(stream, check_launch("paged_append"));
 }
@@ -371,9 +395,13 @@ extern "C" int gorch_hip_paged_read(void* stream, const gorch_hip_paged_kv* kv, 
         hipLaunchKernelGGL(kernel, dim3((p.tokens + tok - 1) / tok, (p.num_kv * p.hd / 4 + 255) / 256), dim3(256), 0,
                            stream_of(stream), p, k_out, v_out);
     };
-    const bool f8 = kv->dtype == GORCH_HIP_KV_E4M3;
-    if (p.tokens < 4096) f8 ? go(k_paged_read<true, 1>, 1) : go(k_paged_read<false, 1>, 1);
-    else f8 ? go(k_paged_read<true, 4>, 4) : go(k_paged_read<false, 4>, 4);
+    const auto of = [&](auto kind) {
+        constexpr int KV = decltype(kind)::value;
+        p.tokens < 4096 ? go(k_paged_read<KV, 1>, 1) : go(k_paged_read<KV, 4>, 4);
+    };
+    if (kv->dtype == GORCH_HIP_KV_MXFP4) of(std::integral_constant<int, GORCH_HIP_KV_MXFP4>{});
+    else if (kv->dtype == GORCH_HIP_KV_E4M3) of(std::integral_constant<int, GORCH_HIP_KV_E4M3>{});
+    else of(std::integral_constant<int, GORCH_HIP_KV_BF16>{});
     count(CNT_CODEC);
     return finish(stream, check_launch("paged_read"));
 }

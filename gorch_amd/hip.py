@@ -72,6 +72,12 @@ SIGNATURES = {
     "gorch_hip_kernel_choice": (C.c_char_p, [C.c_char_p, C.POINTER(i32), i32]),
     "gorch_hip_bf16_to_f32": (i32, [vp, vp, vp, i64]),
     "gorch_hip_f32_to_bf16": (i32, [vp, vp, vp, i64]),
+    "gorch_hip_mxfp4_encode": (i32, [vp, vp, i32, i64, vp, vp, i64, i64]),
+    "gorch_hip_mxfp4_decode": (i32, [vp, vp, vp, vp, i32, i64, i64, i64]),
+    "gorch_hip_packed_mxfp4_bytes": (C.c_size_t, [i32, i32]),
+    "gorch_hip_pack_mxfp4": (i32, [vp, vp, vp, vp, i32, i32]),
+    "gorch_hip_linear_mxfp4_workspace_size": (C.c_size_t, [i32, i32, i32]),
+    "gorch_hip_linear_mxfp4": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, C.c_size_t]),
     "gorch_hip_matmul_dt": (i32, [vp, vp, vp, vp, u32, u32, u32, i32, i32, i32, i32]),
     "gorch_hip_batched_matmul_dt": (i32, [vp, vp, vp, vp, u32, u32, u32, u32, i32, i32, i32, i32]),
     "gorch_hip_linear_bf16": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32]),
@@ -294,6 +300,43 @@ def f32_to_bf16(inp, out) -> None:
     _ok(lib().gorch_hip_f32_to_bf16(_stream(), _p(inp), _p(out), inp.numel()))
 
 
+def _mx_values(t, device):
+    """Pointer, bf16 flag and row stride of the values [rows, cols] of an MXFP4 codec call."""
+    import torch
+
+    if t.dim() != 2 or t.dtype not in (torch.float32, torch.bfloat16) or (t.stride(1) != 1 and t.shape[1] > 1) or (
+            t.stride(0) < t.shape[1] and t.shape[0] > 1) or t.get_device() != device:
+        raise ValueError(f"gorch_amd.hip: values must be f32 or bf16 rows of unit column stride on the current device, got "
+                         f"{t.dtype} {tuple(t.shape)} of strides {tuple(t.stride())} on {t.device}")
+    return t.data_ptr(), int(t.dtype is torch.bfloat16), t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _mx_held(codes, scales, rows, cols, device):
+    import torch
+
+    return (_typed(codes, torch.uint8, (rows, cols // 2), "codes", device),
+            _typed(scales, torch.uint8, (rows, -(-cols // 32)), "scales", device))
+
+
+def mxfp4_encode(x, codes, scales) -> None:
+    """gorch_hip_mxfp4_encode: x [rows, cols] (f32 or bf16, rows possibly
+    apart) to codes uint8 [rows, cols / 2] and scales uint8 [rows, ceil(cols /
+    32)]."""
+    dev, (rows, cols) = _device(), x.shape
+    p, bf16, stride = _mx_values(x, dev)
+    c, s = _mx_held(codes, scales, rows, cols, dev)
+    _ok(lib().gorch_hip_mxfp4_encode(_stream(), p, bf16, stride, c, s, rows, cols))
+
+
+def mxfp4_decode(codes, scales, out) -> None:
+    """gorch_hip_mxfp4_decode: the values of codes and scales to out [rows,
+    cols] (f32 or bf16, rows possibly apart)."""
+    dev, (rows, cols) = _device(), out.shape
+    p, bf16, stride = _mx_values(out, dev)
+    c, s = _mx_held(codes, scales, rows, cols, dev)
+    _ok(lib().gorch_hip_mxfp4_decode(_stream(), c, s, p, bf16, stride, rows, cols))
+
+
 # ------------------------------------------------------------------ matmul
 
 def matmul_dt(A, B, C_, M, N, K, transA=False, transB=False, aBF16=False, bBF16=False) -> None:
@@ -435,6 +478,49 @@ def linear_bf16_packed(x, Wp, N, bias, y, residual=None, epilogue=EPI_NONE) -> N
     M, K = x.shape
     _ok(lib().gorch_hip_linear_bf16_packed(_stream(), _p(x), _p(Wp), _p(bias), _p(residual), _p(y), M, N, K,
                                            epilogue))
+
+
+def pack_mxfp4(codes, scales):
+    """The MXFP4 weight [N, K] of mxfp4_encode's codes and scales in
+    linear_mxfp4's resident layout (a flat uint8 tensor)."""
+    import torch
+
+    dev, N, K = _device(), codes.shape[0], 2 * codes.shape[-1]
+    c, s = _mx_held(codes, scales, N, K, dev)
+    Wp = torch.empty(lib().gorch_hip_packed_mxfp4_bytes(N, K), dtype=torch.uint8, device=codes.device)
+    _ok(lib().gorch_hip_pack_mxfp4(_stream(), c, s, _p(Wp), N, K))
+    return Wp
+
+
+def linear_mxfp4_workspace(M, N, K):
+    """A device workspace for linear_mxfp4 of M rows, or None where none is
+    needed."""
+    import torch
+
+    n = lib().gorch_hip_linear_mxfp4_workspace_size(M, N, K)
+    return torch.empty(n, dtype=torch.uint8, device="cuda") if n else None
+
+
+def linear_mxfp4(x, Wp, N, bias, y, residual=None, epilogue=EPI_NONE, ws=None) -> None:
+    """gorch_hip_linear_mxfp4: y = residual + epi(x @ W^T + bias) over a
+    pack_mxfp4 weight of N rows; x [M, K] and y [M, N] f32. ws from
+    linear_mxfp4_workspace (a new one if None); calls that can overlap must not
+    share it."""
+    dev = _device()
+    if x.dim() != 2:
+        raise ValueError("gorch_amd.hip: x must be [M, K]")
+    M, K = x.shape
+    if ws is None:
+        ws = linear_mxfp4_workspace(M, N, K)
+    elif ws.get_device() != dev:
+        raise ValueError("gorch_amd.hip: ws is not on the current device")
+    if Wp.get_device() != dev or Wp.numel() * Wp.element_size() != lib().gorch_hip_packed_mxfp4_bytes(N, K):
+        raise ValueError(f"gorch_amd.hip: Wp must be a packed weight [{N}, {K}] on the current device")
+    _ok(lib().gorch_hip_linear_mxfp4(_stream(), _typed(x, _f32_t, (M, K), "x", dev), _p(Wp),
+                                     _typed(bias, _f32_t, (N,), "bias", dev),
+                                     _typed(residual, _f32_t, (M, N), "residual", dev),
+                                     _typed(y, _f32_t, (M, N), "y", dev), M, N, K, epilogue, _p(ws),
+                                     0 if ws is None else ws.numel() * ws.element_size()))
 
 
 # ------------------------------------------------------------------ GPT engine
@@ -829,7 +915,7 @@ class QwenBlock:
 
 # ------------------------------------------------------------------ paged KV cache
 
-KV_BF16, KV_E4M3 = 0, 1
+KV_BF16, KV_E4M3, KV_MXFP4 = 0, 1, 2
 
 
 class _PagedKVC(C.Structure):
@@ -905,7 +991,8 @@ class PagedKV:
     """gorch_hip_paged_kv: one layer's K and V pools [num_pages, num_kv,
     page_size, head_dim] (device tensors: bf16, or e4m3 codes with f32 scales
     [num_pages, num_kv, page_size]); ``new`` allocates them. bf16 pools may
-    also be int16 storage, e4m3 ones uint8."""
+    also be int16 storage, e4m3 ones uint8. MXFP4 pools are uint8 [..., head_dim
+    / 2] with uint8 scales [..., ceil(head_dim / 32)]: the scales' type tells."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         import torch
@@ -914,6 +1001,8 @@ class PagedKV:
             raise ValueError("gorch_amd.hip: pools must be [num_pages, num_kv, page_size, head_dim]")
         if k.dtype in (torch.bfloat16, torch.int16):
             dtype = KV_BF16
+        elif k.dtype is torch.uint8 and k_scale is not None and k_scale.dtype is torch.uint8:
+            dtype = KV_MXFP4
         elif k.dtype in (torch.float8_e4m3fn, torch.uint8):
             dtype = KV_E4M3
         else:
@@ -922,11 +1011,15 @@ class PagedKV:
             raise ValueError("gorch_amd.hip: e4m3 pools need k_scale and v_scale, bf16 pools take none")
         dev = _device()
         pages, num_kv, page, hd = k.shape
+        scales, kind = k.shape[:3], torch.float32
+        if dtype == KV_MXFP4:
+            hd *= 2
+            scales, kind = scales + (-(-hd // 32),), torch.uint8
         s = _PagedKVC(dtype, pages, page, num_kv, hd)
         s.k = _typed(k, k.dtype, k.shape, "k", dev)
         s.v = _typed(v, k.dtype, k.shape, "v", dev)
-        s.k_scale = _typed(k_scale, torch.float32, k.shape[:3], "k_scale", dev)
-        s.v_scale = _typed(v_scale, torch.float32, k.shape[:3], "v_scale", dev)
+        s.k_scale = _typed(k_scale, kind, scales, "k_scale", dev)
+        s.v_scale = _typed(v_scale, kind, scales, "v_scale", dev)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_kv, self.head_dim = num_kv, hd
         self.s = s
@@ -935,14 +1028,18 @@ class PagedKV:
 
     @classmethod
     def new(cls, num_pages: int, page_size: int, num_kv: int, head_dim: int, dtype: str = "bf16") -> "PagedKV":
-        """Zeroed pools of dtype "bf16" or "e4m3" on the current device."""
+        """Zeroed pools of dtype "bf16", "e4m3" or "mxfp4" on the current device."""
         import torch
 
         shape = (num_pages, num_kv, page_size, head_dim)
         if dtype == "bf16":
             return cls(*(torch.zeros(shape, dtype=torch.bfloat16, device="cuda") for _ in "kv"))
+        if dtype == "mxfp4":
+            widths = (head_dim // 2, -(-head_dim // 32)) * 2
+            k, ks, v, vs = (torch.zeros(shape[:3] + (w,), dtype=torch.uint8, device="cuda") for w in widths)
+            return cls(k, v, ks, vs)
         if dtype != "e4m3":
-            raise ValueError('gorch_amd.hip: dtype must be "bf16" or "e4m3"')
+            raise ValueError('gorch_amd.hip: dtype must be "bf16", "e4m3" or "mxfp4"')
         return cls(*(torch.zeros(shape, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in "kv"),
                    *(torch.zeros(shape[:3], device="cuda") for _ in "kv"))
 

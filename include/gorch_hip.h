@@ -164,6 +164,24 @@ const char* gorch_hip_kernel_choice(const char* op, const int* dims, int n);
 int gorch_hip_bf16_to_f32(void* stream, const uint16_t* in, float* out, int64_t n);
 int gorch_hip_f32_to_bf16(void* stream, const float* in, uint16_t* out, int64_t n);
 
+/* MXFP4 (OCP microscaling; no counterpart in the reference): rows of cols
+ * values as 4-bit e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6; bit 3 the sign), two
+ * a byte with the first in the low nibble, [rows][cols / 2], and one e8m0 scale
+ * byte s per group of 32 of a row (the last may be shorter), [rows][ceil(cols /
+ * 32)]: a value is code * 2^(s - 127), NaN where s is 255. cols is a multiple
+ * of 8, rows * cols at most 2^40 (else GORCH_HIP_EUNSUPPORTED).
+ * Encoding takes the smallest scale that the group's largest magnitude exceeds
+ * at most 7 times and rounds to the nearest code, ties to even: half a step at
+ * most, everywhere. A group below 2^-100 throughout becomes zeros (s = 0), one
+ * that holds an infinity or NaN becomes NaN (s = 255). Decoding is exact in f32
+ * and in bf16. The values are f32, or with the flag bf16, in rows that begin at
+ * multiples of the stride (in elements); rows are 16-byte and codes 4-byte
+ * aligned. */
+int gorch_hip_mxfp4_encode(void* stream, const void* in, int in_bf16, int64_t in_stride, uint8_t* codes,
+                           uint8_t* scales, int64_t rows, int64_t cols);
+int gorch_hip_mxfp4_decode(void* stream, const uint8_t* codes, const uint8_t* scales, void* out, int out_bf16,
+                           int64_t out_stride, int64_t rows, int64_t cols);
+
 /* ------------------------------------------------------------------------
  * Matmul family.
  * ---------------------------------------------------------------------- */
@@ -231,6 +249,28 @@ int gorch_hip_linear_bf16_packed(void* stream, const float* x, const uint16_t* W
  * the array's address and runs the bf16 probe, which allocates). */
 int gorch_hip_linear_bf16_noalloc(void* stream, const float* x, const uint16_t* W, const float* bias,
                                   const float* residual, float* y, int M, int N, int K, int epilogue);
+
+/* A Linear's weight in MXFP4 as gorch_hip_linear_mxfp4 reads it: the codes of
+ * 16 rows and 128 columns as one contiguous KB in matrix-operand order, then
+ * the scales, padded with zeros to whole tiles. From gorch_hip_mxfp4_encode's
+ * arrays of [N, K] (K % 8 == 0, N up to 2^20 - 16; Wp 16-byte aligned) into
+ * gorch_hip_packed_mxfp4_bytes of device memory, once at load. */
+size_t gorch_hip_packed_mxfp4_bytes(int N, int K);
+int gorch_hip_pack_mxfp4(void* stream, const uint8_t* codes, const uint8_t* scales, void* Wp, int N, int K);
+/* gorch_hip_linear_bf16 (nn/module.go:61-88) over a weight in MXFP4, for any
+ * number of rows: y[m,n] = residual[m,n] + epi(sum_k x[m,k] W[n,k] + bias[n])
+ * with the weight's values exact and x held to 2^-24 of the largest magnitude
+ * among each 32 of a row's columns (k / 32), products and sums in f32: f32
+ * accuracy, in a fixed order of sums. An infinity or NaN in x makes its row of
+ * y NaN, a NaN group of W its column. bias and residual may be NULL; residual
+ * may alias y, x must not. K % 8 == 0, M up to 2^20, K up to 2^24, x, Wp and
+ * the workspace 16-byte aligned (else GORCH_HIP_EUNSUPPORTED). The workspace
+ * (gorch_hip_linear_mxfp4_workspace_size bytes of device memory; NULL where
+ * that is 0) is the caller's: calls that can overlap must not share one.
+ * Nothing is allocated, so the call can be captured. */
+size_t gorch_hip_linear_mxfp4_workspace_size(int M, int N, int K);
+int gorch_hip_linear_mxfp4(void* stream, const float* x, const void* Wp, const float* bias, const float* residual,
+                           float* y, int M, int N, int K, int epilogue, void* workspace, size_t workspace_bytes);
 
 /* ------------------------------------------------------------------------
  * Decode-step ops (the forward halves of gorch's op layer on this path).
@@ -438,11 +478,15 @@ int gorch_hip_qwen_generate_sampled(void* stream, gorch_hip_qwen* m, const int* 
 
 #define GORCH_HIP_KV_BF16 0 /* bf16 rows                                       */
 #define GORCH_HIP_KV_E4M3 1 /* OCP e4m3 codes, one f32 scale a (token, KV head) */
+#define GORCH_HIP_KV_MXFP4 2 /* MXFP4: 4-bit codes, one e8m0 byte per 32 columns */
 
 /* One layer's pools (device): k and v [num_pages][num_kv][page_size][head_dim]
  * of dtype, 16-byte aligned; with GORCH_HIP_KV_E4M3 also k_scale and v_scale
  * [num_pages][num_kv][page_size], a row's value being code * scale (NULL and
- * unused with GORCH_HIP_KV_BF16). head_dim is a multiple of 16 up to 256,
+ * unused with GORCH_HIP_KV_BF16). With GORCH_HIP_KV_MXFP4 k and v are
+ * [num_pages][num_kv][page_size][head_dim / 2] bytes of codes as
+ * gorch_hip_mxfp4_encode writes rows of head_dim, and k_scale and v_scale point
+ * at bytes, [num_pages][num_kv][page_size][ceil(head_dim / 32)]. head_dim is a multiple of 16 up to 256,
  * num_kv below 2^16 (else GORCH_HIP_EUNSUPPORTED); page_size is any positive
  * number. */
 typedef struct {
@@ -483,7 +527,8 @@ typedef struct {
  * as gorch_hip_gqa_forward_cached; then K and V are rounded once: to bf16
  * (nearest even), or to e4m3 codes of x * (448 / m) with scale = m / 448, m the
  * row's largest magnitude (a row below 2^-100 throughout is stored as
- * zeros; a row that holds an infinity reads back as NaN). Rows q [tokens,
+ * zeros; a row that holds an infinity reads back as NaN), or to MXFP4 as
+ * gorch_hip_mxfp4_encode rounds. Rows q [tokens,
  * num_q * head_dim], k and v [tokens, num_kv * head_dim] start at multiples
  * of their strides (in floats, multiples of 4), so the three can be column
  * ranges of one fused projection; rows and RoPE tables are 16-byte aligned

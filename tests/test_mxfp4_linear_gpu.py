@@ -1,0 +1,205 @@
+"""gorch_hip_linear_mxfp4 against its definition in 64 bits: rows from one to
+thousands, odd sizes of every kind, epilogues, magnitudes that differ within a
+row, infinities and NaN, streams, graphs and shared workspaces."""
+import numpy as np
+import pytest
+import torch
+
+from tests.mx_case import GROUP, groups, values
+from tests.paged_case import dev, host
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+def weight(rng, N, K):
+    codes = rng.integers(0, 256, (N, K // 2)).astype(np.uint8)
+    scales = rng.integers(115, 124, (N, -(-K // GROUP))).astype(np.uint8)
+    return codes, scales
+
+
+def gelu(x):
+    return x / (1 + np.exp(-2 * 0.7978845608 * (x + 0.044715 * x ** 3)))
+
+
+def expected(x, codes, scales, bias=None, residual=None, act=False):
+    """y in 64 bits and the bound of the f32 result. x is held to U of the largest magnitude of its group; each of the
+    5 ceil(K / 128) matrix instructions of a sum adds its products to 2 U of the sum of their magnitudes, joining up to
+    eight waves' and five terms' sums takes 13 more additions; bias, GELU (slope at most 1.13; its own arithmetic, the
+    hardware exponential's and reciprocal's last places on values up to |v|, within 16 U) and residual round once each."""
+    W = values(codes, scales)
+    K = W.shape[1]
+    x64 = x.astype(np.float64)
+    top = np.repeat(np.abs(groups(x64)).max(-1), GROUP, -1)[:, :K]
+    v = x64 @ W.T
+    size = np.abs(x64) @ np.abs(W).T
+    tol = U * ((10 * -(-K // 128) + 13) * size + top @ np.abs(W).T)
+    if bias is not None:
+        v = v + bias
+        tol = tol + U * np.abs(v)
+    if act:
+        tol = 1.13 * tol + 16 * U * np.abs(v)
+        v = gelu(v)
+    if residual is not None:
+        v = v + residual
+        tol = tol + U * np.abs(v)
+    return v, tol * 1.001 + 2.0 ** -126
+
+
+def call(gpu, x, codes, scales, bias=None, residual=None, act=False, ws=None, alias=False):
+    M, N = x.shape[0], codes.shape[0]
+    r = None if residual is None else dev(residual)
+    y = r if alias else torch.full((M, N), 55.0, device="cuda")
+    gpu.linear_mxfp4(dev(x), gpu.pack_mxfp4(dev(codes), dev(scales)), N, None if bias is None else dev(bias), y,
+                     residual=r, epilogue=gpu.EPI_GELU if act else gpu.EPI_NONE, ws=ws)
+    return host(y)
+
+
+def check(got, want, tol):
+    assert np.isfinite(got).all()
+    off = np.abs(got - want) - tol
+    assert (off <= 0).all(), f"{(off > 0).sum()} values off, the worst {off.max()} beyond its bound"
+
+
+def inputs(seed, M, N, K):
+    rng = np.random.default_rng(seed)
+    x = (rng.standard_normal((M, K)) * np.exp(rng.standard_normal(K))).astype(np.float32)
+    return rng, x, *weight(rng, N, K)
+
+
+SIZES = [(64, 128), (16, 8), (1, 512), (50, 1600), (300, 520), (1000, 136), (33, 4864), (2304, 768), (17, 24)]
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 7, 15, 16, 17, 33, 64, 65, 130])
+@pytest.mark.parametrize("N,K", SIZES)
+def test_matches_definition(gpu, M, N, K):
+    rng, x, codes, scales = inputs(M + N, M, N, K)
+    b = rng.standard_normal(N).astype(np.float32) if M % 2 else None
+    r = rng.standard_normal((M, N)).astype(np.float32) if N % 2 == 0 else None
+    check(call(gpu, x, codes, scales, b, r), *expected(x, codes, scales, b, r))
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 4096, 1024), (1, 20011, 256), (2, 9000, 4096), (16, 6400, 1600), (12, 896, 9728),
+                                   (3, 512, 20000), (5, 30000, 136), (257, 1024, 2048), (1000, 777, 1032), (2000, 130, 264)])
+@pytest.mark.parametrize("act", [False, True])
+def test_larger(gpu, M, N, K, act):
+    rng, x, codes, scales = inputs(K, M, N, K)
+    b = rng.standard_normal(N).astype(np.float32)
+    check(call(gpu, x, codes, scales, b, None, act), *expected(x, codes, scales, b, None, act))
+
+
+@pytest.mark.parametrize("M", [1, 9, 40])
+def test_residual_may_be_the_output(gpu, M):
+    rng, x, codes, scales = inputs(M, M, 100, 264)
+    r = rng.standard_normal((M, 100)).astype(np.float32)
+    check(call(gpu, x, codes, scales, None, r, act=True, alias=True), *expected(x, codes, scales, None, r, True))
+
+
+@pytest.mark.parametrize("M", [1, 3, 4, 16, 50])
+def test_magnitudes(gpu, M):
+    # each group's largest value decides what its others are held to; powers of two far apart from group to group
+    rng, x, codes, scales = inputs(M, M, 70, 512)
+    x *= np.exp2(rng.integers(-60, 60, (M, 16)).astype(np.float32)).repeat(32, 1)
+    x[:, 5] *= 1000
+    x[0, 64:96] = 0
+    x[0, 96:128] = np.float32(1e-42)  # below the normal range
+    check(call(gpu, x, codes, scales), *expected(x, codes, scales))
+
+
+@pytest.mark.parametrize("M", [1, 2, 16, 70])
+def test_every_value_alone(gpu, M):
+    # one nonzero value a group: its product is exact to f32
+    rng = np.random.default_rng(3)
+    N, K = 64, 256
+    codes, scales = weight(rng, N, K)
+    x = np.zeros((M, K), np.float32)
+    x[:, rng.integers(0, 32)] = rng.standard_normal(M).astype(np.float32)
+    got = call(gpu, x, codes, scales)
+    want = x.astype(np.float64) @ values(codes, scales).T
+    assert (np.abs(got - want) <= 2 * U * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("M", [1, 3, 5, 16, 20, 100])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_nonfinite_rows_and_columns_stay_apart(gpu, M, bad):
+    rng, x, codes, scales = inputs(M, M, 90, 264)
+    want, tol = expected(x, codes, scales)
+    x[M // 2, 200] = bad
+    scales[33, 2] = 255
+    got = call(gpu, x, codes, scales)
+    assert np.isnan(got[M // 2]).all() and np.isnan(got[:, 33]).all()
+    rows, cols = np.arange(M) != M // 2, np.arange(90) != 33
+    if M > 1:
+        check(got[rows][:, cols], want[rows][:, cols], tol[rows][:, cols])
+
+
+@pytest.mark.parametrize("M", [1, 6, 16, 90])
+def test_same_bits_every_time_whatever_the_workspace_held(gpu, M):
+    rng, x, codes, scales = inputs(M, M, 200, 1160)
+    first = call(gpu, x, codes, scales)
+    for fill in (0, 0xff):
+        ws = gpu.linear_mxfp4_workspace(M, 200, 1160)
+        if ws is not None:
+            ws.fill_(fill)
+        np.testing.assert_array_equal(call(gpu, x, codes, scales, ws=ws), first)
+
+
+def test_rows_do_not_depend_on_their_batch(gpu):
+    rng, x, codes, scales = inputs(4, 80, 160, 1024)
+    whole = call(gpu, x, codes, scales)
+    np.testing.assert_array_equal(call(gpu, x[:40], codes, scales), whole[:40])
+
+
+@pytest.mark.parametrize("M", [1, 4, 100])
+def test_captured_and_replayed(gpu, M):
+    rng, x, codes, scales = inputs(M, M, 300, 520)
+    Wp = gpu.pack_mxfp4(dev(codes), dev(scales))
+    xd, b, y = dev(x), dev(rng.standard_normal(300).astype(np.float32)), torch.zeros((M, 300), device="cuda")
+    ws = gpu.linear_mxfp4_workspace(M, 300, 520)
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=side):
+        gpu.linear_mxfp4(xd, Wp, 300, b, y, ws=ws)
+    for turn in range(3):
+        x = rng.standard_normal((M, 520)).astype(np.float32)
+        xd.copy_(dev(x))
+        y.fill_(7)
+        graph.replay()
+        check(host(y), *expected(x, codes, scales, host(b)))
+        again = torch.empty_like(y)
+        gpu.linear_mxfp4(xd, Wp, 300, b, again)
+        assert torch.equal(again, y)
+
+
+def test_on_another_stream(gpu):
+    rng, x, codes, scales = inputs(8, 30, 512, 1024)
+    Wp, xd, y = gpu.pack_mxfp4(dev(codes), dev(scales)), dev(x), torch.zeros((30, 512), device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        gpu.linear_mxfp4(xd, Wp, 512, None, y)
+    side.synchronize()
+    check(host(y), *expected(x, codes, scales))
+
+
+def test_reaches_past_32_bit_offsets(gpu):
+    # codes past 2^32 bytes, and y past 2^31 elements (a launch's smaller dimensions stay small)
+    N, K, M = 1 << 19, 16640, 4200
+    rng = np.random.default_rng(2)
+    codes = torch.zeros((N, K // 2), dtype=torch.uint8, device="cuda")
+    scales = torch.full((N, K // 32), 120, dtype=torch.uint8, device="cuda")
+    some = [0, 70000, N - 17, N - 1]
+    c, s = weight(rng, len(some), K)
+    codes[some], scales[some] = dev(c), dev(s)
+    Wp = gpu.pack_mxfp4(codes, scales)
+    del codes, scales
+    x = rng.standard_normal((M, K)).astype(np.float32)
+    want, tol = expected(x[[0, M - 1]], c, s)
+    for rows in (1, M):
+        y = torch.full((rows, N), 3.0, device="cuda")
+        gpu.linear_mxfp4(dev(x[M - rows:]), Wp, N, None, y)
+        got = host(y[[0, rows - 1]][:, some])
+        check(got[1], want[1], tol[1])
+        check(got[0], want[0 if rows == M else 1], tol[0 if rows == M else 1])
+        assert int(y[rows - 1].count_nonzero()) <= len(some)
