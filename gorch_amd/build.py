@@ -22,7 +22,7 @@ FLAGS = [
     "--offload-arch=gfx950",
     "-O3",
     "-fPIC",
-    "-std=c++17",
+    "-std=c++20",
     # Packed-f32 VALU forms are kept out of every kernel.
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall",

@@ -99,17 +99,22 @@ __device__ __forceinline__ floatx32 mx_from6(u32x6 t, float s) {
     asm volatile("" ::"v"(t), "v"(s), "v"(r));
     return r;
 }
+// The largest magnitude's bits, and the byte of the first term's scale (the
+// last term's, 20 less, is one of a normal number).
+__device__ __forceinline__ uint32_t mx_top(const floatx32& x) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 32; i++) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    return top;
+}
+__device__ __forceinline__ uint32_t mx_exponent(uint32_t top) { return max(top >> 23, 5u * (kMxTerms - 1) + 1); }
 struct MxTerms {
     u32x6 t[kMxTerms];
     uint32_t scale, last;
 };
 __device__ __forceinline__ void mx_split(floatx32 x, MxTerms& r) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 32; i++) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    const uint32_t top = mx_top(x), e = mx_exponent(top);
     const bool odd = top >= 0x7f800000u;
-    // (the last term's scale is a normal number)
-    const uint32_t e = max(top >> 23, 5u * (kMxTerms - 1) + 1);
 #pragma unroll
     for (int t = 0; t < kMxTerms; t++) {
         const float s = __uint_as_float((odd ? 127u : e - 5 * t) << 23);
@@ -118,6 +123,24 @@ __device__ __forceinline__ void mx_split(floatx32 x, MxTerms& r) {
     }
     r.scale = odd ? ~0u : e * 0x01010101u - 0x0f0a0500u;
     r.last = odd ? kMxNaN : e - 20;
+}
+// Term t alone, the same bits: the terms before it add up to x rounded to
+// multiples of 2^(e + 2 - 5 t), which adding and taking off 1.5 * 2^23 of those
+// leaves (of 2^(e + 40) for t = 0: nothing).
+__device__ __forceinline__ u32x6 mx_term(floatx32 x, int t, uint32_t& scale) {
+    const uint32_t top = mx_top(x);
+    uint32_t e = mx_exponent(top);
+    const bool odd = top >= 0x7f800000u;
+    scale = odd ? kMxNaN : e - 5 * t;
+    if (__any(e > 200)) {  // (that constant would leave f32)
+        const bool far = e > 200;
+        x *= far ? 0x1p-64f : 1.0f;
+        e -= far ? 64 : 0;
+    }
+    const float c = __uint_as_float(t == 0 ? (e + 40) << 23 : ((e + 25 - 5 * t) << 23) | 0x400000u);
+#pragma unroll
+    for (int i = 0; i < 32; i++) x[i] -= (x[i] + c) - c;
+    return mx_to6(x, __uint_as_float((e - 5 * t) << 23));
 }
 
 __device__ __forceinline__ i32x8 mx_op6(u32x4 lo, u32x2 hi) {

@@ -3,6 +3,7 @@
 // codes go to the matrix cores as they are; x goes there as the five 6-bit
 // terms of mx.h, which keep f32's accuracy.
 #include <algorithm>
+#include <iterator>
 
 #include "mx.h"
 #include "stage_lds.h"
@@ -18,8 +19,13 @@ struct MxLinearArgs {
     float* y;
     int M, N, K, epi;
     int nt, nk, nq;  // 16-row tiles of W, 128-column tiles, words of four of those
-    int chunk;       // column tiles whose terms a block holds at once
     char* terms;     // of more than 16 rows: x's operands (k_mx_terms)
+    // of up to 16 rows: K in `slices` ranges of `chunks` * T column tiles, W's
+    // row tiles `per` to a block; of several slices, partial sums [row
+    // tile][slice][lane][4] and a counter for each block of row tiles
+    int slices, chunks, per, blocks;
+    float* part;
+    unsigned* done;
 };
 
 // Barrier for LDS alone: loads into registers stay in flight.
@@ -30,16 +36,18 @@ __device__ __forceinline__ void lds_sync() {
     asm volatile("" ::: "memory");
 }
 
-// The 32 values of row m, columns k .. k + 31 (zeros past K or without a row).
+// The 32 values of row m, columns k .. k + 31 (zeros past K or without a row;
+// no load stands under a branch, where each would be waited for by itself).
 __device__ __forceinline__ floatx32 load_group(const float* x, int m, int M, int k, int K) {
+    const float* row = x + (size_t)min(m, M - 1) * K;
+    floatx4 f[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) f[i] = *reinterpret_cast<const floatx4*>(row + min(k + 4 * i, K - 4));
     floatx32 v;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        floatx4 f = {0.f, 0.f, 0.f, 0.f};
-        if (m < M && k + 4 * i < K) f = *reinterpret_cast<const floatx4*>(x + (size_t)m * K + k + 4 * i);
+    for (int i = 0; i < 8; i++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[4 * i + e] = f[e];
-    }
+        for (int e = 0; e < 4; e++) v[4 * i + e] = m < M && k + 4 * i < K ? f[i][e] : 0.f;
     return v;
 }
 
@@ -51,143 +59,41 @@ __device__ __forceinline__ void mx_store(const MxLinearArgs& a, int m, int n, fl
     a.y[at] = v;
 }
 
-// Up to 16 rows of x. A block splits x (or `chunk` column tiles of it) into its
-// terms in LDS once; its 8 waves are WK along the columns, 8 / WK along the row
-// tiles of W, and each streams 1 KB of codes a step into one instruction (ROW1:
-// up to 3 rows, whose terms are rows of one operand) or five.
-constexpr int kGemvWaves = 8;
-struct GemvLds {  // byte offsets of a block's LDS
-    int p8, sc, red, bytes;
-    __host__ __device__ GemvLds(int M, int chunk) {
-        const int slots = chunk * 4 * kMxTerms * M;
-        p8 = slots * 16;
-        sc = p8 + slots * 8;
-        red = sc + chunk * 4 * M * 8;
-        bytes = red + 2 * kGemvWaves * 1024;
-    }
-};
-template <bool ROW1, int WK>
-__global__ __launch_bounds__(64 * kGemvWaves) void k_mx_gemv(MxLinearArgs a) {
-    constexpr int WN = kGemvWaves / WK, U = 4;
-    extern __shared__ __align__(16) char lds[];
-    const GemvLds at(a.M, a.chunk);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
-    const int M = a.M, R = kMxTerms * M;
-    const int groups = (a.nt + WN - 1) / WN, wk = wave % WK, wn = wave / WK;
-    const int chunks = (a.nk + a.chunk - 1) / a.chunk;
-    struct Step {
-        u32x4 codes[U];
-        uint32_t scale[U];
-    };
-    const auto load = [&](Step& s, int t, int j, int jb) {
-        const int tt = min(t, a.nt - 1);
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int jj = min(min(j + u, jb - 1), a.nk - 1);
-            s.codes[u] = __builtin_nontemporal_load(a.wp + ((size_t)tt * a.nk + jj) * 64 + lane);
-            s.scale[u] = a.wsc[((size_t)tt * a.nq + (jj >> 2)) * 64 + lane] >> (8 * (jj & 3));
-        }
-    };
-    int turn = 0;
-    for (int group = blockIdx.x; group < groups; group += gridDim.x) {
-        const int t = group * WN + wn;
-        floatx4 acc = {0.f, 0.f, 0.f, 0.f};
-        for (int ch = 0; ch < chunks; ch++) {
-            const int c0 = ch * a.chunk, c1 = min(c0 + a.chunk, a.nk), per = (c1 - c0 + WK - 1) / WK;
-            const int ja = c0 + wk * per, jb = min(ja + per, c1);
-            Step s;
-            load(s, t, ja, max(jb, 1));
-            if (chunks > 1 || group == (int)blockIdx.x) {
-                lds_sync();
-                for (int i = threadIdx.x; i < (c1 - c0) * 4 * M; i += 64 * kGemvWaves) {
-                    const int m = i / ((c1 - c0) * 4), kb = i - m * (c1 - c0) * 4, j = kb >> 2, gg = kb & 3;
-                    MxTerms r;
-                    mx_split(load_group(a.x, m, M, 128 * c0 + 32 * kb, a.K), r);
-#pragma unroll
-                    for (int q = 0; q < kMxTerms; q++) {
-                        const int slot = ROW1 ? (j * 4 + gg) * R + m * kMxTerms + q : ((j * kMxTerms + q) * 4 + gg) * M + m;
-                        *reinterpret_cast<u32x4*>(lds + slot * 16) = u32x4{r.t[q][0], r.t[q][1], r.t[q][2], r.t[q][3]};
-                        *reinterpret_cast<u32x2*>(lds + at.p8 + slot * 8) = u32x2{r.t[q][4], r.t[q][5]};
-                    }
-                    if constexpr (ROW1) {
-                        uint8_t* sc = reinterpret_cast<uint8_t*>(lds + at.sc) + (j * 4 + gg) * R + m * kMxTerms;
-#pragma unroll
-                        for (int q = 0; q < 4; q++) sc[q] = (uint8_t)(r.scale >> (8 * q));
-                        sc[4] = (uint8_t)r.last;
-                    } else {
-                        *reinterpret_cast<u32x2*>(lds + at.sc + ((j * 4 + gg) * M + m) * 8) = u32x2{r.scale, r.last};
-                    }
-                }
-                lds_sync();
-            }
-            for (int j = ja; j < jb; j += U) {
-                const Step now = s;
-                load(s, t, j + U, jb);
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    if (j + u >= jb) break;
-                    const int jl = j + u - c0;
-                    const i32x8 w = mx_op4(now.codes[u]);
-                    if constexpr (ROW1) {
-                        const int slot = (jl * 4 + g) * R + min(c, R - 1);
-                        const i32x8 six = mx_op6(*reinterpret_cast<const u32x4*>(lds + slot * 16),
-                                                 *reinterpret_cast<const u32x2*>(lds + at.p8 + slot * 8));
-                        acc = mx_mfma<0, 0>(six, *reinterpret_cast<const uint8_t*>(lds + at.sc + slot), w, now.scale[u], acc);
-                    } else {
-                        const int m = min(c, M - 1);
-                        const u32x2 sx = *reinterpret_cast<const u32x2*>(lds + at.sc + ((jl * 4 + g) * M + m) * 8);
-                        const auto six = [&](int q) {
-                            const int slot = ((jl * kMxTerms + q) * 4 + g) * M + m;
-                            return mx_op6(*reinterpret_cast<const u32x4*>(lds + slot * 16),
-                                          *reinterpret_cast<const u32x2*>(lds + at.p8 + slot * 8));
-                        };
-                        acc = mx_mfma<0, 0>(six(4), sx[1], w, now.scale[u], acc);
-                        acc = mx_mfma<3, 0>(six(3), sx[0], w, now.scale[u], acc);
-                        acc = mx_mfma<2, 0>(six(2), sx[0], w, now.scale[u], acc);
-                        acc = mx_mfma<1, 0>(six(1), sx[0], w, now.scale[u], acc);
-                        acc = mx_mfma<0, 0>(six(0), sx[0], w, now.scale[u], acc);
-                    }
-                }
-            }
-        }
-        // the waves' sums in wave order; row 4 g + i of a result is at i * 64 + lane
-        float* red = reinterpret_cast<float*>(lds + at.red) + turn * kGemvWaves * 256;
-        turn ^= 1;
-#pragma unroll
-        for (int i = 0; i < 4; i++) red[wave * 256 + i * 64 + lane] = acc[i];
-        lds_sync();
-        for (int i = threadIdx.x; i < WN * M * 16; i += 64 * kGemvWaves) {
-            const int n16 = i & 15, m = (i >> 4) % M, w = (i >> 4) / M;
-            const int n = (group * WN + w) * 16 + n16;
-            if (n >= a.N) continue;
-            float v = 0.f;
-#pragma unroll
-            for (int k = 0; k < WK; k++) {
-                const float* from = red + (w * WK + k) * 256 + n16;
-                if constexpr (ROW1) {
-#pragma unroll
-                    for (int q = kMxTerms - 1; q >= 0; q--) {
-                        const int row = m * kMxTerms + q;
-                        v += from[(row & 3) * 64 + (row >> 2) * 16];
-                    }
-                } else {
-                    v += from[(m & 3) * 64 + (m >> 2) * 16];
-                }
-            }
-            mx_store(a, m, n, v);
-        }
-    }
-}
-
-// More rows: x's operands first, 8 KB for each 16 rows and 128 columns (the
-// terms' first 16 bytes, then their last 8, then the scale words, each in lane
-// order), in row tile, column tile order.
+// x's operands made once for all blocks, 8 KB for each 16 rows and 128 columns:
+// the terms' first 16 bytes, then their last 8, then the scale words, each in
+// lane order; in row tile, column tile order.
 constexpr int kTermBytes = 8192, kTerm8 = kMxTerms * 1024, kTermScale = kTerm8 + kMxTerms * 512;
+// (Rows go through LDS: a lane's 128 bytes straight from memory would take 64
+// lines a load, eight times.)
 __global__ __launch_bounds__(256) void k_mx_terms(MxLinearArgs a) {
-    const int lane = threadIdx.x & 63, i = blockIdx.y, j = blockIdx.x * 4 + (threadIdx.x >> 6);
+    constexpr int ROW = 132;
+    __shared__ __align__(16) float xs[4][16 * ROW];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.y, j = blockIdx.x * 4 + wave;
     if (j >= a.nk) return;
+    {
+        const int col = 128 * j + 4 * (lane & 31), from = min(col, a.K - 4);
+        floatx4 f[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int m = 16 * i + 2 * k + (lane >> 5);
+            f[k] = *reinterpret_cast<const floatx4*>(a.x + (size_t)min(m, a.M - 1) * a.K + from);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int r = 2 * k + (lane >> 5);
+            if (16 * i + r >= a.M || col >= a.K) f[k] = floatx4{0.f, 0.f, 0.f, 0.f};
+            *reinterpret_cast<floatx4*>(xs[wave] + r * ROW + 4 * (lane & 31)) = f[k];
+        }
+    }
+    floatx32 v;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const floatx4 f = *reinterpret_cast<const floatx4*>(xs[wave] + (lane & 15) * ROW + 32 * (lane >> 4) + 4 * k);
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[4 * k + e] = f[e];
+    }
     MxTerms r;
-    mx_split(load_group(a.x, 16 * i + (lane & 15), a.M, 128 * j + 32 * (lane >> 4), a.K), r);
+    mx_split(v, r);
     char* to = a.terms + ((size_t)i * a.nk + j) * kTermBytes;
 #pragma unroll
     for (int q = 0; q < kMxTerms; q++) {
@@ -196,121 +102,605 @@ __global__ __launch_bounds__(256) void k_mx_terms(MxLinearArgs a) {
     }
     *reinterpret_cast<u32x2*>(to + kTermScale + lane * 8) = u32x2{r.scale, r.last};
 }
+// The same for up to 16 rows, where it is waited for: a wave a term.
+__global__ __launch_bounds__(64 * kMxTerms) void k_mx_terms16(MxLinearArgs a) {
+    const int lane = threadIdx.x & 63, q = threadIdx.x >> 6, j = blockIdx.x;
+    uint32_t s;
+    const u32x6 t = mx_term(load_group(a.x, lane & 15, a.M, 128 * j + 32 * (lane >> 4), a.K), q, s);
+    char* to = a.terms + (size_t)j * kTermBytes;
+    *reinterpret_cast<u32x4*>(to + q * 1024 + lane * 16) = u32x4{t[0], t[1], t[2], t[3]};
+    *reinterpret_cast<u32x2*>(to + kTerm8 + q * 512 + lane * 8) = u32x2{t[4], t[5]};
+    reinterpret_cast<uint8_t*>(to + kTermScale + lane * 8)[q] = (uint8_t)s;
+}
 
-// WM x WN waves of MT x NT tiles of 16 x 16: x's operands through a two-stage
-// ring in LDS, W's codes straight to the operand registers.
-template <int MT, int NT, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void k_mx_gemm(MxLinearArgs a) {
-    constexpr int BMT = MT * WM, NW = WM * WN;
+// Up to 16 rows of x. A block takes a slice of K and some row tiles of W: it
+// splits its columns of x into terms in LDS once, and its 8 waves, WK along the
+// columns and 8 / WK along the row tiles, stream 1 KB of codes a step into one
+// instruction (kRow1: up to 3 rows, whose terms are rows of one operand) or
+// five. For many columns of more rows another kernel has made the terms
+// (kMade), which are loaded. The last block of a slice's fellows to finish adds up the slices, in
+// their order.
+constexpr int kGemvWaves = 8;
+constexpr int kGemvSlices = 16;
+enum GemvKind { kRow1, kFive, kMade };
+struct GemvLds {  // byte offsets of a block's LDS
+    int p8, sc, red, bytes;
+    __host__ __device__ GemvLds(int M, int tiles, bool made) {
+        if (made) {
+            p8 = kTerm8;
+            sc = kTermScale;
+            red = tiles * kTermBytes;
+            bytes = red + kGemvWaves * 1024;
+            return;
+        }
+        const int slots = tiles * 4 * kMxTerms * M;
+        p8 = slots * 16;
+        sc = p8 + slots * 8;
+        red = sc + tiles * 4 * M * 8;
+        bytes = red + kGemvWaves * 1024;
+    }
+};
+// 16 bytes past the caches of an XCD (agent scope).
+__device__ __forceinline__ void store_far(__amdgpu_buffer_rsrc_t rs, int at, floatx4 v) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rs, at, 0, 16);
+}
+template <GemvKind KIND, int WK, int U, int NT>
+__global__ __launch_bounds__(64 * kGemvWaves, 2) void k_mx_gemv(MxLinearArgs a) {
+    constexpr int WN = kGemvWaves / WK, T = WK * U;
+    constexpr bool ROW1 = KIND == kRow1, MADE = KIND == kMade;
     extern __shared__ __align__(16) char lds[];
+    __shared__ int last;
+    // blocks of the same row tiles run on one XCD (every eighth block)
+    const int eight = blockIdx.x >> 3, slice = eight % a.slices, nb = eight / a.slices * 8 + (blockIdx.x & 7);
+    if (nb >= a.blocks) return;
+    const GemvLds at(a.M, min(T, a.nk), MADE);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
-    const int wm = wave % WM, wn = wave / WM;
-    const int i0 = blockIdx.y * BMT, t0 = (blockIdx.x * WN + wn) * NT;
-    const auto stage = [&](int j, int b) {
-        typedef __attribute__((address_space(1))) const uint32_t* global_ptr;
-        typedef __attribute__((address_space(3))) uint32_t* lds_ptr;
+    const int M = a.M, R = kMxTerms * M, wk = wave % WK, wn = wave / WK;
+    const int t0 = nb * a.per, t1 = min(t0 + a.per, a.nt);
+    float* red = reinterpret_cast<float*>(lds + at.red);
+    struct Step {
+        u32x4 codes[NT][U];
+        uint32_t scale[NT][(U + 3) / 4];
+    };
+    // U column tiles from j on of row tiles t .. (what lies past the last is not looked at)
+    const auto load = [&](Step& s, int t, int j) {
 #pragma unroll
-        for (int k = 0; k < BMT * 8 / NW; k++) {
-            const int kb = k * NW + wave;  // KB of the stage
-            const char* from = a.terms + ((size_t)(i0 + (kb >> 3)) * a.nk + j) * kTermBytes + (kb & 7) * 1024 + lane * 16;
-            __builtin_amdgcn_global_load_lds((global_ptr)from, (lds_ptr)(lds + (b * BMT * 8 + kb) * 1024), 16, 0, 0);
+        for (int i = 0; i < NT; i++) {
+            const size_t tt = min(t + i, a.nt - 1);
+#pragma unroll
+            for (int u = 0; u < U; u += 4) s.scale[i][u / 4] = a.wsc[(tt * a.nq + (min(j + u, a.nk - 1) >> 2)) * 64 + lane];
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                s.codes[i][u] = __builtin_nontemporal_load(a.wp + (tt * a.nk + min(j + u, a.nk - 1)) * 64 + lane);
         }
     };
-    u32x4 wc[NT];
-    uint32_t ws[NT];
-    const auto codes = [&](int j) {
+    floatx4 acc[NT];
+    const auto multiply = [&](const Step& s, int j, int jl) {
+        const auto one = [&](auto uc) {
+            constexpr int u = decltype(uc)::value, B = u & 3;
+            if constexpr (u < U) {
+                if (j + u >= a.nk) return;
+                uint32_t sw[NT];
+                i32x8 w[NT];
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int t = min(t0 + n, a.nt - 1);
-            wc[n] = a.wp[((size_t)t * a.nk + j) * 64 + lane];
-            ws[n] = a.wsc[((size_t)t * a.nq + (j >> 2)) * 64 + lane] >> (8 * (j & 3));
+                for (int i = 0; i < NT; i++) {
+                    sw[i] = s.scale[i][u / 4] >> (U < 4 ? 8 * (j & 3) : 0);
+                    w[i] = mx_op4(s.codes[i][u]);
+                }
+                if constexpr (ROW1) {
+                    const int slot = ((jl + u) * 4 + g) * R + min(c, R - 1);
+                    const i32x8 six = mx_op6(*reinterpret_cast<const u32x4*>(lds + slot * 16),
+                                             *reinterpret_cast<const u32x2*>(lds + at.p8 + slot * 8));
+                    const uint32_t sx = *reinterpret_cast<const uint8_t*>(lds + at.sc + slot);
+#pragma unroll
+                    for (int i = 0; i < NT; i++) acc[i] = mx_mfma<0, B>(six, sx, w[i], sw[i], acc[i]);
+                } else {
+                    const int m = min(c, M - 1);
+                    const char* made = lds + (jl + u) * kTermBytes;
+                    const u32x2 sx = *reinterpret_cast<const u32x2*>(
+                        MADE ? made + kTermScale + lane * 8 : lds + at.sc + (((jl + u) * 4 + g) * M + m) * 8);
+                    const auto six = [&](int q) {
+                        if constexpr (MADE)
+                            return mx_op6(*reinterpret_cast<const u32x4*>(made + q * 1024 + lane * 16),
+                                          *reinterpret_cast<const u32x2*>(made + kTerm8 + q * 512 + lane * 8));
+                        const int slot = (((jl + u) * kMxTerms + q) * 4 + g) * M + m;
+                        return mx_op6(*reinterpret_cast<const u32x4*>(lds + slot * 16),
+                                      *reinterpret_cast<const u32x2*>(lds + at.p8 + slot * 8));
+                    };
+                    const i32x8 x4 = six(4), x3 = six(3), x2 = six(2), x1 = six(1), x0 = six(0);
+#pragma unroll
+                    for (int i = 0; i < NT; i++) acc[i] = mx_mfma<0, B>(x4, sx[1], w[i], sw[i], acc[i]);
+#pragma unroll
+                    for (int i = 0; i < NT; i++) acc[i] = mx_mfma<3, B>(x3, sx[0], w[i], sw[i], acc[i]);
+#pragma unroll
+                    for (int i = 0; i < NT; i++) acc[i] = mx_mfma<2, B>(x2, sx[0], w[i], sw[i], acc[i]);
+#pragma unroll
+                    for (int i = 0; i < NT; i++) acc[i] = mx_mfma<1, B>(x1, sx[0], w[i], sw[i], acc[i]);
+#pragma unroll
+                    for (int i = 0; i < NT; i++) acc[i] = mx_mfma<0, B>(x0, sx[0], w[i], sw[i], acc[i]);
+                }
+            }
+        };
+        one(std::integral_constant<int, 0>{});
+        one(std::integral_constant<int, 1>{});
+        one(std::integral_constant<int, 2>{});
+        one(std::integral_constant<int, 3>{});
+        one(std::integral_constant<int, 4>{});
+        one(std::integral_constant<int, 5>{});
+        one(std::integral_constant<int, 6>{});
+        one(std::integral_constant<int, 7>{});
+    };
+    // x's columns of chunk ch as terms
+    const auto split = [&](int j0) {
+        const int groups = min(T, a.nk - j0) * 4, tasks = groups * M;
+        const auto slot_of = [&](int m, int kb, int q) {
+            const int j = kb >> 2, gg = kb & 3;
+            return ROW1 ? (j * 4 + gg) * R + m * kMxTerms + q : ((j * kMxTerms + q) * 4 + gg) * M + m;
+        };
+        const auto put = [&](int slot, const u32x6& t) {
+            *reinterpret_cast<u32x4*>(lds + slot * 16) = u32x4{t[0], t[1], t[2], t[3]};
+            *reinterpret_cast<u32x2*>(lds + at.p8 + slot * 8) = u32x2{t[4], t[5]};
+        };
+        const auto scales_of = [&](int m, int kb) {  // bytes of the terms' scales
+            return reinterpret_cast<uint8_t*>(lds + at.sc) + (ROW1 ? kb * R + m * kMxTerms : (kb * M + m) * 8);
+        };
+        if (tasks * kMxTerms <= 64 * kGemvWaves) {
+            // few groups: a thread a term
+            const int i = threadIdx.x / kMxTerms, q = threadIdx.x - i * kMxTerms;
+            const int m = i / groups, kb = i - m * groups;
+            const floatx32 x = load_group(a.x, i < tasks ? m : M, M, 128 * j0 + 32 * kb, a.K);
+            uint32_t s;
+            const u32x6 t = mx_term(x, q, s);
+            if (i < tasks) {
+                put(slot_of(m, kb, q), t);
+                scales_of(m, kb)[q] = (uint8_t)s;
+            }
+        } else {
+            for (int i = threadIdx.x; i < tasks; i += 64 * kGemvWaves) {
+                const int m = i / groups, kb = i - m * groups;
+                MxTerms r;
+                mx_split(load_group(a.x, m, M, 128 * j0 + 32 * kb, a.K), r);
+#pragma unroll
+                for (int q = 0; q < kMxTerms; q++) put(slot_of(m, kb, q), r.t[q]);
+                uint8_t* sc = scales_of(m, kb);
+                if constexpr (ROW1) {
+#pragma unroll
+                    for (int q = 0; q < 4; q++) sc[q] = (uint8_t)(r.scale >> (8 * q));
+                    sc[4] = (uint8_t)r.last;
+                } else {
+                    *reinterpret_cast<u32x2*>(sc) = u32x2{r.scale, r.last};
+                }
+            }
         }
+    };
+    // a wave's sums of row tile t (lane: rows 4 g .. 4 g + 3 of x or of terms, column c) to y
+    const auto finish = [&](int t, floatx4 d) {
+        const int n = 16 * t + c;
+        if constexpr (ROW1) {
+            float* mine = red + wave * 256;
+#pragma unroll
+            for (int i = 0; i < 4; i++) mine[i * 64 + lane] = d[i];
+            // (a wave reads back what it wrote)
+            float v = 0.f;
+#pragma unroll
+            for (int q = kMxTerms - 1; q >= 0; q--) {
+                const int row = min(g, M - 1) * kMxTerms + q;
+                v += mine[(row & 3) * 64 + (row >> 2) * 16 + c];
+            }
+            if (g < M && n < a.N) mx_store(a, g, n, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (4 * g + i < M && n < a.N) mx_store(a, 4 * g + i, n, d[i]);
+        }
+    };
+    // (partial sums of a block's row tiles: up to 2^31 bytes)
+    const __amdgpu_buffer_rsrc_t part =
+        make_rsrc(a.part + (size_t)t0 * a.slices * 256, (long long)(t1 - t0) * a.slices * 1024);
+    // one column range and one round of row tiles after another
+    const int j00 = slice * a.chunks * T, rounds = (t1 - t0 + WN * NT - 1) / (WN * NT);
+    Step s;
+    load(s, t0 + wn * NT, j00 + wk * U);
+#pragma unroll
+    for (int i = 0; i < NT; i++) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int r = 0, ch = 0; r < rounds;) {
+        const int j0 = j00 + ch * T, t = t0 + (r * WN + wn) * NT;
+        const bool more = ch + 1 < a.chunks && j0 + T < a.nk;
+        if (ch > 0 || r == 0 || a.chunks > 1) {
+            if (ch > 0 || r > 0) lds_sync();
+            if constexpr (MADE) {
+                typedef __attribute__((address_space(1))) const uint32_t* global_ptr;
+                typedef __attribute__((address_space(3))) uint32_t* lds_ptr;
+                const int kb = min(T, a.nk - j0) * (kTermBytes / 1024);
+                for (int k = wave; k < kb; k += kGemvWaves)
+                    __builtin_amdgcn_global_load_lds((global_ptr)(a.terms + (size_t)j0 * kTermBytes + k * 1024 + lane * 16),
+                                                     (lds_ptr)(lds + k * 1024), 16, 0, 0);
+                block_sync_dma();
+            } else {
+                split(j0);
+                lds_sync();
+            }
+        }
+        const int nr = more ? r : r + 1, nch = more ? ch + 1 : 0;
+        const Step now = s;
+        load(s, t0 + (nr * WN + wn) * NT, j00 + nch * T + wk * U);
+        multiply(now, j0 + wk * U, wk * U);
+        r = nr;
+        ch = nch;
+        if (more) continue;
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+            floatx4 d = acc[i];
+            acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+            // the waves' sums along the columns, in wave order
+            if constexpr (WK > 1) {
+                if (i > 0 || r > 1) lds_sync();
+                if (wk > 0) *reinterpret_cast<floatx4*>(red + (wave * 64 + lane) * 4) = d;
+                lds_sync();
+                if (wk > 0) continue;
+#pragma unroll
+                for (int k = 1; k < WK; k++) d += *reinterpret_cast<const floatx4*>(red + ((wave + k) * 64 + lane) * 4);
+            }
+            if (t + i >= t1) continue;
+            if (a.slices == 1) finish(t + i, d);
+            else store_far(part, ((t + i - t0) * a.slices + slice) * 1024 + lane * 16, d);
+        }
+    }
+    if (a.slices == 1) return;
+    // Partial sums were stored, and are loaded, past the XCD's caches, so that
+    // they are there once their stores are waited for; a fence that writes the
+    // L2 back costs 38 us here (16 x 1600 x 6400: 48.6 us with it).
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (threadIdx.x == 0) last = __hip_atomic_fetch_add(a.done + nb, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == (unsigned)a.slices;
+    __syncthreads();
+    if (!last) return;
+    if (threadIdx.x == 0) __hip_atomic_store(a.done + nb, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int t = t0 + wave; t < t1; t += kGemvWaves) {
+        floatx4 p[kGemvSlices];
+#pragma unroll
+        for (int k = 0; k < kGemvSlices; k++)  // (slices that there are not lie past the resource: zeros)
+            p[k] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(
+                part, k < a.slices ? ((t - t0) * a.slices + k) * 1024 + lane * 16 : kOutOfRange, 0, 16));
+#pragma unroll
+        for (int k = 1; k < kGemvSlices; k++) p[0] += p[k];
+        finish(t, p[0]);
+    }
+}
+
+// More rows: eight waves, WM along the rows of x (16 each) and WK along the
+// columns, over NT row tiles of W. A wave's operands of x go from memory to its
+// registers (no two waves need the same), W's codes and scale words to LDS,
+// where the WM waves share them: rows two column tiles ahead, codes three, and
+// the next tile's first codes from LDS before the block meets. A row tile's five
+// products follow each other, which leaves two of three operands where they are
+// (on all CUs the matrix cores run at what power allows, 6.2 PFLOP/s with the
+// terms outermost, 6.9 so).
+template <int MT, int NT, int WM>
+struct GemmLds {
+    static constexpr int WK = 8 / MT / WM, STAGE = NT * 1024, WORDS = (NT + 3) / 4 * 1024;
+    static constexpr int RING = WK * (4 * STAGE + 2 * WORDS), JOIN = (WK - 1) * WM * MT * NT * 1024;
+    static constexpr int BYTES = RING > JOIN ? RING : JOIN;
+};
+template <int MT, int NT, int WM>
+__global__ __launch_bounds__(512 / MT, 2 / MT) void k_mx_gemm(MxLinearArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)  // (the host's pass cannot instantiate the loads in its lambdas)
+    using L = GemmLds<MT, NT, WM>;
+    constexpr int WK = L::WK, NB = NT < 2 ? NT : 2, DMA = (NT + WM - 1) / WM, ROWS = 2 * kMxTerms + 1;
+    constexpr int KB = L::WORDS / 1024, LOADS = DMA + MT * ROWS + (KB + WM - 1) / WM;
+    extern __shared__ __align__(16) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
+    const int wm = wave % WM, wk = wave / WM;
+    // blocks that share x's rows run on one XCD (every eighth block)
+    const int cols = (a.nt + NT - 1) / NT, each = (gridDim.x + 7) / 8, at = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
+    const int mt = (a.M + 15) / 16, by = at / cols, i0 = (by * WM + wm) * MT, t0 = (at - by * cols) * NT;
+    if (by * WM * MT >= mt) return;
+    // this wave's columns: whole words of four tiles
+    const int per = (a.nq + WK - 1) / WK, q0 = wk * per, j1 = min(4 * (q0 + per), a.nk);
+    // Resources in place of pointers, whose 64-bit sums per lane the compiler
+    // would keep and spill: a wave's rows of x, and the row tiles of W that it
+    // loads, which end with its columns (past them are zeros, whose products
+    // change nothing: no branch stands around a step).
+    __amdgpu_buffer_rsrc_t from[MT], wrs[DMA];
+#pragma unroll
+    for (int m = 0; m < MT; m++) from[m] = make_rsrc(a.terms + (size_t)min(i0 + m, mt - 1) * a.nk * kTermBytes, (long long)a.nk * kTermBytes);
+#pragma unroll
+    for (int i = 0; i < DMA; i++)
+        wrs[i] = make_rsrc(a.wp + (size_t)min(t0 + min(i * WM + wm, NT - 1), a.nt - 1) * a.nk * 64, (long long)j1 * 1024);
+    char* ring = lds + wk * 4 * L::STAGE;
+    char* words = lds + WK * 4 * L::STAGE + wk * 2 * L::WORDS;
+    struct Six {
+        u32x4 lo[kMxTerms];
+        u32x2 hi[kMxTerms], s;
+    };
+    typedef __attribute__((address_space(1))) const uint32_t* global_ptr;
+    typedef __attribute__((address_space(3))) uint32_t* lds_ptr;
+    typedef __attribute__((address_space(3))) void* lds_void;
+    // Load i of column tile j's rows (to x), codes (to stage b) and scale words
+    // (`word`, where it `has` one; a KB holds four row tiles', some waves load the same).
+    const auto load = [&](auto ic, Six (&x)[MT], int j, int jc, int b, auto has, int word) {
+        constexpr int i = decltype(ic)::value;
+        if constexpr (i < DMA) {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(wrs[i], (lds_void)(ring + b * L::STAGE + min(i * WM + wm, NT - 1) * 1024), 16,
+                                                     lane * 16, min(jc, a.nk) * 1024, 0, 0);
+        } else if constexpr (i < DMA + MT * ROWS) {
+            constexpr int m = (i - DMA) / ROWS, k = (i - DMA) % ROWS, q = k / 2;
+            const int at = min(j, a.nk - 1) * kTermBytes;
+            if constexpr (k == 2 * kMxTerms) x[m].s = __builtin_amdgcn_raw_buffer_load_b64(from[m], lane * 8, at + kTermScale, 0);
+            else if constexpr (k % 2 == 0) x[m].lo[q] = __builtin_amdgcn_raw_buffer_load_b128(from[m], lane * 16, at + q * 1024, 0);
+            else x[m].hi[q] = __builtin_amdgcn_raw_buffer_load_b64(from[m], lane * 8, at + kTerm8 + q * 512, 0);
+        } else if constexpr (decltype(has)::value) {
+            const int k = ((i - DMA - MT * ROWS) * WM + wm) % KB, n = 4 * k + (lane >> 4);
+            const uint32_t* p = a.wsc + ((size_t)min(t0 + n, a.nt - 1) * a.nq + min(word, a.nq - 1)) * 64 + (lane & 15) * 4;
+            __builtin_amdgcn_global_load_lds((global_ptr)p, (lds_ptr)(words + (word & 1) * L::WORDS + k * 1024), 16, 0, 0);
+        }
+    };
+    const auto loads = [&](auto lo, auto n, Six (&x)[MT], int j, int jc, int b, auto has, int word) {
+        [&]<int... I>(std::integer_sequence<int, I...>) {
+            (load(std::integral_constant<int, decltype(lo)::value + I>{}, x, j, jc, b, has, word), ...);
+        }(std::make_integer_sequence<int, decltype(n)::value>{});
     };
     floatx4 acc[MT][NT];
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int n = 0; n < NT; n++) acc[m][n] = floatx4{0.f, 0.f, 0.f, 0.f};
-    stage(0, 0);
-    codes(0);
-    for (int j = 0; j < a.nk; j++) {
+    Six x[3][MT];
+    uint32_t ws[NT];
+    u32x4 w[2 * NB];
+    constexpr bool EARLY = NT >= 2 * NB;  // the next words' registers are free before this step's last row tiles
+    const auto word_of = [&](int n, int word) {
+        ws[n] = *reinterpret_cast<const uint32_t*>(words + (word & 1) * L::WORDS + n * 256 + lane * 4);
+    };
+    // row tile n's codes of stage b (and where it `has` a word their scale words)
+    const auto fetch = [&](u32x4& to, int n, int b, auto has, int word) {
+        to = *reinterpret_cast<const u32x4*>(ring + b * L::STAGE + n * 1024 + lane * 16);
+        if constexpr (decltype(has)::value) word_of(n, word);
+    };
+    {
+        using Zero = std::integral_constant<int, 0>;
+        loads(Zero{}, std::integral_constant<int, LOADS>{}, x[0], 4 * q0, 4 * q0, 0, std::true_type{}, q0);
+        loads(Zero{}, std::integral_constant<int, LOADS>{}, x[1], 4 * q0 + 1, 4 * q0 + 1, 1, std::false_type{}, 0);
+        loads(Zero{}, std::integral_constant<int, DMA>{}, x[0], 0, 4 * q0 + 2, 2, std::false_type{}, 0);
         block_sync_dma();
-        i32x8 w[NT];
-        uint32_t s[NT];
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            w[n] = mx_op4(wc[n]);
-            s[n] = ws[n];
-        }
-        if (j + 1 < a.nk) {
-            stage(j + 1, (j + 1) & 1);
-            codes(j + 1);
-        }
-        const char* base = lds + ((j & 1) * BMT + wm * MT) * kTermBytes;
-#pragma unroll
-        for (int m = 0; m < MT; m++) {
-            const char* from = base + m * kTermBytes;
-            const u32x2 sx = *reinterpret_cast<const u32x2*>(from + kTermScale + lane * 8);
-            const auto six = [&](int q) {
-                return mx_op6(*reinterpret_cast<const u32x4*>(from + q * 1024 + lane * 16),
-                              *reinterpret_cast<const u32x2*>(from + kTerm8 + q * 512 + lane * 8));
-            };
-            const i32x8 x4 = six(4), x3 = six(3), x2 = six(2), x1 = six(1), x0 = six(0);
-#pragma unroll
-            for (int n = 0; n < NT; n++) acc[m][n] = mx_mfma<0, 0>(x4, sx[1], w[n], s[n], acc[m][n]);
-#pragma unroll
-            for (int n = 0; n < NT; n++) acc[m][n] = mx_mfma<3, 0>(x3, sx[0], w[n], s[n], acc[m][n]);
-#pragma unroll
-            for (int n = 0; n < NT; n++) acc[m][n] = mx_mfma<2, 0>(x2, sx[0], w[n], s[n], acc[m][n]);
-#pragma unroll
-            for (int n = 0; n < NT; n++) acc[m][n] = mx_mfma<1, 0>(x1, sx[0], w[n], s[n], acc[m][n]);
-#pragma unroll
-            for (int n = 0; n < NT; n++) acc[m][n] = mx_mfma<0, 0>(x0, sx[0], w[n], s[n], acc[m][n]);
-        }
+        for (int n = 0; n < NB; n++) fetch(w[n], n, 0, std::true_type{}, q0);
     }
+    // A wave issues in order, and eight at once take 1,300 cycles to hand over a
+    // column tile's loads: they go out between the products.
+    const auto step = [&](auto uc, auto rc, int j) {
+        constexpr int u = decltype(uc)::value, r = decltype(rc)::value % 3;
+        // all loads have landed but those of the last step (and of its words)
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(wait_vm(DMA + MT * ROWS, true));
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const auto& now = x[r];
+        [&]<int... N>(std::integer_sequence<int, N...>) {
+            const auto one = [&](auto nc) {
+                constexpr int n = decltype(nc)::value, from = n * LOADS / NT, to = (n + 1) * LOADS / NT;
+                // (slots of w turn over NT row tiles a step)
+                constexpr int slot = (NT % (2 * NB) ? n + u * NT : n) % (2 * NB), ahead = (slot + NB) % (2 * NB);
+                loads(std::integral_constant<int, from>{}, std::integral_constant<int, to - from>{}, x[(r + 2) % 3], j + 2, j + 3, (u + 3) & 3,
+                      std::bool_constant<u == 0>{}, j / 4 + 1);
+                if constexpr (n + NB < NT) fetch(w[ahead], n + NB, u, std::bool_constant<u == 0>{}, j / 4);
+                else fetch(w[ahead], n + NB - NT, (u + 1) & 3, std::bool_constant<u == 3 && EARLY>{}, j / 4 + 1);
+                if constexpr (u == 0 && !EARLY) word_of(n, j / 4);
+                __builtin_amdgcn_sched_barrier(0);
+                const i32x8 v = mx_op4(w[slot]);
+                const auto product = [&](auto qc) {
+                    constexpr int q = decltype(qc)::value;
+#pragma unroll
+                    for (int m = 0; m < MT; m++)
+                        acc[m][n] = mx_mfma<q & 3, u>(mx_op6(now[m].lo[q], now[m].hi[q]), now[m].s[q / 4], v, ws[n], acc[m][n]);
+                };
+                product(std::integral_constant<int, 4>{});
+                product(std::integral_constant<int, 3>{});
+                product(std::integral_constant<int, 2>{});
+                product(std::integral_constant<int, 1>{});
+                product(std::integral_constant<int, 0>{});
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            (one(std::integral_constant<int, N>{}), ...);
+        }(std::make_integer_sequence<int, NT>{});
+    };
+    const auto quad = [&](auto rc, int q) {
+        constexpr int r = decltype(rc)::value;
+        [&]<int... U>(std::integer_sequence<int, U...>) {
+            (step(std::integral_constant<int, U>{}, std::integral_constant<int, r + U>{}, 4 * (q0 + q) + U), ...);
+        }(std::make_integer_sequence<int, 4>{});
+    };
+    for (int q = 0;; q++) {
+        quad(std::integral_constant<int, 0>{}, q);
+        if (++q >= per) break;
+        quad(std::integral_constant<int, 1>{}, q);
+        if (++q >= per) break;
+        quad(std::integral_constant<int, 2>{}, q);
+        if (q + 1 >= per) break;
+    }
+    block_sync_dma();
+    if constexpr (WK > 1) {
+        block_sync_dma();
+        floatx4* join = reinterpret_cast<floatx4*>(lds);
+        if (wk > 0)
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int n = 0; n < NT; n++) join[((((wk - 1) * WM + wm) * MT + m) * NT + n) * 64 + lane] = acc[m][n];
+        __syncthreads();
+        if (wk > 0) return;
+#pragma unroll
+        for (int k = 0; k < WK - 1; k++)
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int n = 0; n < NT; n++) acc[m][n] += join[(((k * WM + wm) * MT + m) * NT + n) * 64 + lane];
+    }
+    // (what is added is asked for by up to four row tiles at a time)
+    constexpr int EB = NT < 4 ? NT : 4;
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int n0 = 0; n0 < NT; n0 += EB) {
+            float bias[EB], r[EB][4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int row = 16 * (i0 + wm * MT + m) + 4 * g + i, col = 16 * (t0 + n) + c;
-                if (row < a.M && col < a.N) mx_store(a, row, col, acc[m][n][i]);
+            for (int n = 0; n < EB; n++) {
+                const int col = min(16 * (t0 + n0 + n) + c, a.N - 1);
+                bias[n] = a.bias ? a.bias[col] : 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    r[n][i] = a.residual ? a.residual[(size_t)min(16 * (i0 + m) + 4 * g + i, a.M - 1) * a.N + col] : 0.f;
             }
+#pragma unroll
+            for (int n = 0; n < EB; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int row = 16 * (i0 + m) + 4 * g + i, col = 16 * (t0 + n0 + n) + c;
+                    float v = acc[m][n0 + n][i] + bias[n];
+                    if (a.epi == GORCH_HIP_EPI_GELU) v = gelu_gemm(v);
+                    if (row < a.M && col < a.N) a.y[(size_t)row * a.N + col] = v + r[n][i];
+                }
+        }
+#endif
 }
 
-constexpr int kGemmRowTiles = 4;  // of the GEMM's blocks
-static size_t terms_bytes(int M, int K) {
-    const size_t tiles = ((size_t)M + 15) / 16, padded = (tiles + kGemmRowTiles - 1) / kGemmRowTiles * kGemmRowTiles;
-    return M <= 16 ? 0 : padded * ((K + 127) / 128) * kTermBytes;
+static size_t terms_bytes(int M, int K) { return (size_t)((M + 15) / 16) * ((K + 127) / 128) * kTermBytes; }
+
+// How the rows of a decode step are cut into blocks: slices of K (at most 16),
+// row tiles per block, waves along the columns.
+struct GemvPlan {
+    GemvKind kind;
+    int tiles, slices, chunks, per, blocks, wk, nt;
+    size_t terms, part, bytes;
+};
+static GemvPlan gemv_plan(int M, int N, int K) {
+    GemvPlan p{};
+    const int nt = (N + 15) / 16, nk = (K + 127) / 128;
+    // (a block splits 512 groups, M * nk = 128, in 1.7 us; another kernel takes
+    // 3 us for all of them)
+    p.kind = M <= 3 ? kRow1 : ((long long)M * nk >= (M > 8 ? 128 : 257) ? kMade : kFive);
+    // Column tiles whose terms a block holds: up to 64 KB of them, a round of
+    // splitting; made ones 128 KB.
+    const int most = p.kind == kMade ? 16 : (M <= 4 ? 32 : (M <= 8 ? 16 : 8));
+    p.tiles = 8;
+    while (p.tiles < nk && p.tiles < most) p.tiles *= 2;
+    const int ranges = (nk + p.tiles - 1) / p.tiles;
+    p.slices = std::min(ranges, kGemvSlices);
+    // (joining slices takes 2.3 us, as much as loading the terms of 48 tiles)
+    if (p.kind == kMade) p.slices = nk <= 48 ? 1 : std::min((nk + 31) / 32, kGemvSlices);
+    p.chunks = (ranges + p.slices - 1) / p.slices;
+    p.slices = (ranges + p.chunks - 1) / p.chunks;
+    // 256 blocks, one a CU, of which each has a row tile at least
+    const int blocks = std::max(1, 256 / p.slices);
+    p.per = (nt + blocks - 1) / blocks;
+    p.blocks = (nt + p.per - 1) / p.per;
+    p.wk = 8;
+    while (p.wk > p.tiles / 8 && kGemvWaves / p.wk < p.per) p.wk /= 2;
+    // (two row tiles a wave at a time share what it reads of x's terms)
+    p.nt = p.kind != kRow1 && p.tiles / p.wk <= 4 && p.per > kGemvWaves / p.wk ? 2 : 1;
+    p.terms = p.kind == kMade ? (size_t)nk * kTermBytes : 0;
+    p.part = p.slices == 1 ? 0 : (size_t)p.slices * nt * 1024;
+    p.bytes = p.terms + p.part + (p.slices == 1 ? 0 : (size_t)p.blocks * 4);
+    return p;
 }
 
-static void launch_mx_gemv(hipStream_t s, MxLinearArgs a) {
-    // columns whose terms fit 48 KB (with the waves' sums 64: two blocks a CU)
-    const int per = 4 * a.M * (kMxTerms * 24 + 8);
-    a.chunk = std::min(a.nk, std::max(1, (48 << 10) / per));
-    const int bytes = GemvLds(a.M, a.chunk).bytes;
-    int wk = 8;
-    while (wk > 1 && (a.nk < wk || (long long)a.nt * wk / 8 >= 512)) wk /= 2;
-    const int wn = kGemvWaves / wk, groups = (a.nt + wn - 1) / wn;
-    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(std::min(groups, 512)), dim3(64 * kGemvWaves), bytes, s, a); };
-    const auto form = [&](auto k) {
-        constexpr int WK = decltype(k)::value;
-        a.M <= 3 ? go(k_mx_gemv<true, WK>) : go(k_mx_gemv<false, WK>);
-    };
-    if (wk == 8) form(std::integral_constant<int, 8>{});
-    else if (wk == 4) form(std::integral_constant<int, 4>{});
-    else if (wk == 2) form(std::integral_constant<int, 2>{});
-    else form(std::integral_constant<int, 1>{});
+template <GemvKind KIND, int WK, int U, int NT>
+static int launch_mx_gemv_t(hipStream_t s, const MxLinearArgs& a) {
+    const int bytes = GemvLds(a.M, std::min(WK * U, a.nk), KIND == kMade).bytes;
+    if (bytes > 64 << 10)
+        GH_TRY(check(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_mx_gemv<KIND, WK, U, NT>),
+                                         hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "mx_gemv attribute"));
+    hipLaunchKernelGGL((k_mx_gemv<KIND, WK, U, NT>), dim3((a.blocks + 7) / 8 * 8 * a.slices), dim3(64 * kGemvWaves), bytes, s, a);
+    return GORCH_HIP_OK;
+}
+template <int WK, int U>
+static int launch_mx_gemv_f(hipStream_t s, const MxLinearArgs& a, const GemvPlan& p) {
+    if (p.kind == kRow1) return launch_mx_gemv_t<kRow1, WK, U, 1>(s, a);
+    if constexpr (U <= 4)
+        if (p.nt == 2) return p.kind == kFive ? launch_mx_gemv_t<kFive, WK, U, 2>(s, a) : launch_mx_gemv_t<kMade, WK, U, 2>(s, a);
+    if constexpr (WK * U <= 16)
+        if (p.kind == kMade) return launch_mx_gemv_t<kMade, WK, U, 1>(s, a);
+    return launch_mx_gemv_t<kFive, WK, U, 1>(s, a);
+}
+static int launch_mx_gemv(hipStream_t s, MxLinearArgs a, char* ws) {
+    const GemvPlan p = gemv_plan(a.M, a.N, a.K);
+    a.slices = p.slices;
+    a.chunks = p.chunks;
+    a.per = p.per;
+    a.blocks = p.blocks;
+    a.terms = ws;
+    a.part = reinterpret_cast<float*>(ws + p.terms);
+    a.done = reinterpret_cast<unsigned*>(ws + p.terms + p.part);
+    if (p.kind == kMade) hipLaunchKernelGGL(k_mx_terms16, dim3(a.nk), dim3(64 * kMxTerms), 0, s, a);
+    if (p.tiles == 8) {
+        if (p.wk == 8) return launch_mx_gemv_f<8, 1>(s, a, p);
+        if (p.wk == 4) return launch_mx_gemv_f<4, 2>(s, a, p);
+        if (p.wk == 2) return launch_mx_gemv_f<2, 4>(s, a, p);
+        return launch_mx_gemv_f<1, 8>(s, a, p);
+    }
+    if (p.tiles == 16) {
+        if (p.wk == 8) return launch_mx_gemv_f<8, 2>(s, a, p);
+        if (p.wk == 4) return launch_mx_gemv_f<4, 4>(s, a, p);
+        return launch_mx_gemv_f<2, 8>(s, a, p);
+    }
+    return p.wk == 8 ? launch_mx_gemv_f<8, 4>(s, a, p) : launch_mx_gemv_f<4, 8>(s, a, p);
 }
 
-static void launch_mx_gemm(hipStream_t s, const MxLinearArgs& a) {
-    const int row_tiles = (a.M + 15) / 16, blocks = (row_tiles + kGemmRowTiles - 1) / kGemmRowTiles;
-    hipLaunchKernelGGL(k_mx_terms, dim3((a.nk + 3) / 4, blocks * kGemmRowTiles), dim3(256), 0, s, a);
-    constexpr int MT = 2, NT = 4, WM = 2, WN = 2;
-    static_assert(MT * WM == kGemmRowTiles);
-    hipLaunchKernelGGL((k_mx_gemm<MT, NT, WM, WN>), dim3((a.nt + NT * WN - 1) / (NT * WN), blocks), dim3(64 * WM * WN),
-                       2 * kGemmRowTiles * kTermBytes, s, a);
+// The block (MT x WM row tiles of x, NT of W) of the least estimated time:
+// rounds of 256 blocks, times a wave's steps (a column tile each), times what a
+// step takes: measured with K = 4096 where few blocks ran; loading x's terms
+// bounds it, 64 KB a step, which the wider blocks use more often. (us, wide
+// first: 2000 x 4096 x 4096 91 101 113 143 178 286; 512 x 4096 x 4096 66 43 32
+// 41 51 77; 64 x 4096 x 4096 60 37 24 20 15 14.)
+struct GemmShape {
+    int mt, nt, wm;
+    double step;
+    const char* name;
+};
+static constexpr GemmShape kGemmShapes[] = {{2, 16, 4, 1.70, "gemm128x256"}, {2, 8, 4, 0.97, "gemm128x128"},
+                                            {1, 8, 4, 1.10, "gemm64x128"},   {1, 4, 4, 0.89, "gemm64x64"},
+                                            {1, 4, 2, 1.18, "gemm32x64"},    {1, 2, 2, 1.00, "gemm32x32"}};
+static int gemm_shape(int M, int N, int K) {
+    const long long mt = (M + 15) / 16, nt = (N + 15) / 16, nq = (K + 511) / 512;
+    int best = 0;
+    double least = 0;
+    for (int i = 0; i < (int)std::size(kGemmShapes); i++) {
+        const GemmShape& g = kGemmShapes[i];
+        const long long wk = 8 / g.mt / g.wm, blocks = ((mt + g.mt * g.wm - 1) / (g.mt * g.wm)) * ((nt + g.nt - 1) / g.nt);
+        const double t = (double)((blocks + 255) / 256) * ((nq + wk - 1) / wk) * g.step;
+        if (i == 0 || t < least) best = i, least = t;
+    }
+    return best;
+}
+template <int MT, int NT, int WM>
+static int launch_mx_gemm_t(hipStream_t s, const MxLinearArgs& a) {
+    constexpr int bytes = GemmLds<MT, NT, WM>::BYTES;
+    if constexpr (bytes > 64 << 10)
+        GH_TRY(check(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_mx_gemm<MT, NT, WM>),
+                                         hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "mx_gemm attribute"));
+    const long long blocks = (long long)((a.nt + NT - 1) / NT) * (((a.M + 15) / 16 + WM * MT - 1) / (WM * MT));
+    hipLaunchKernelGGL((k_mx_gemm<MT, NT, WM>), dim3((unsigned)((blocks + 7) / 8 * 8)), dim3(512 / MT), bytes, s, a);
+    return GORCH_HIP_OK;
+}
+static int launch_mx_gemm(hipStream_t s, const MxLinearArgs& a) {
+    hipLaunchKernelGGL(k_mx_terms, dim3((a.nk + 3) / 4, (a.M + 15) / 16), dim3(256), 0, s, a);
+    switch (gemm_shape(a.M, a.N, a.K)) {
+        case 0: return launch_mx_gemm_t<2, 16, 4>(s, a);
+        case 1: return launch_mx_gemm_t<2, 8, 4>(s, a);
+        case 2: return launch_mx_gemm_t<1, 8, 4>(s, a);
+        case 3: return launch_mx_gemm_t<1, 4, 4>(s, a);
+        case 4: return launch_mx_gemm_t<1, 4, 2>(s, a);
+        default: return launch_mx_gemm_t<1, 2, 2>(s, a);
+    }
+}
+
+const char* mx_linear_choice_name(int M, int N, int K) {
+    if (M > 16) return kGemmShapes[gemm_shape(M, N, K)].name;
+    const GemvPlan p = gemv_plan(M, N, K);
+    static const char* const names[3][2] = {{"gemv", "gemv split"}, {"gemv5", "gemv5 split"}, {"gemv5 made", "gemv5 made split"}};
+    return names[p.kind == kRow1 ? 0 : (p.kind == kFive ? 1 : 2)][p.slices > 1];
 }
 
 }  // namespace gh
@@ -318,7 +708,8 @@ static void launch_mx_gemm(hipStream_t s, const MxLinearArgs& a) {
 using namespace gh;
 
 extern "C" size_t gorch_hip_linear_mxfp4_workspace_size(int M, int N, int K) {
-    return M <= 0 || N <= 0 || K <= 0 ? 0 : terms_bytes(M, K);
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    return M <= 16 ? gemv_plan(M, N, K).bytes : terms_bytes(M, K);
 }
 
 extern "C" int gorch_hip_linear_mxfp4(void* stream, const float* x, const void* Wp, const float* bias, const float* residual,
@@ -333,7 +724,7 @@ extern "C" int gorch_hip_linear_mxfp4(void* stream, const float* x, const void* 
     GH_SUPPORTED((uintptr_t)x % 16 == 0 && (uintptr_t)Wp % 16 == 0 && (uintptr_t)workspace % 16 == 0,
                  "gorch_hip_linear_mxfp4: x, Wp and the workspace must be 16-byte aligned");
     GH_SUPPORTED(M <= 1 << 20 && N <= 16 * 65535 && K <= 1 << 24, "gorch_hip_linear_mxfp4: M, N or K out of range");
-    const size_t need = terms_bytes(M, K);
+    const size_t need = M <= 16 ? gemv_plan(M, N, K).bytes : terms_bytes(M, K);
     GH_REQUIRE(workspace_bytes >= need && (workspace || need == 0), "gorch_hip_linear_mxfp4: workspace too small");
     hipStream_t s = stream_of(stream);
     GH_TRY(bf16_gate(s));
@@ -352,8 +743,8 @@ extern "C" int gorch_hip_linear_mxfp4(void* stream, const float* x, const void* 
     a.wp = static_cast<const u32x4*>(Wp);
     a.wsc = reinterpret_cast<const uint32_t*>(static_cast<const char*>(Wp) + (size_t)a.nt * a.nk * 1024);
     a.terms = static_cast<char*>(workspace);
-    if (M <= 16) launch_mx_gemv(s, a);
-    else launch_mx_gemm(s, a);
+    if (M <= 16) GH_TRY(launch_mx_gemv(s, a, static_cast<char*>(workspace)));
+    else GH_TRY(launch_mx_gemm(s, a));
     count(M <= 16 ? CNT_GEMV : CNT_GEMM);
     return finish(stream, check_launch("linear_mxfp4"));
 }

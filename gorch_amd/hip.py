@@ -493,19 +493,19 @@ def pack_mxfp4(codes, scales):
 
 
 def linear_mxfp4_workspace(M, N, K):
-    """A device workspace for linear_mxfp4 of M rows, or None where none is
-    needed."""
+    """A zeroed device workspace for linear_mxfp4 of M rows, or None where
+    none is needed."""
     import torch
 
     n = lib().gorch_hip_linear_mxfp4_workspace_size(M, N, K)
-    return torch.empty(n, dtype=torch.uint8, device="cuda") if n else None
+    return torch.zeros(n, dtype=torch.uint8, device="cuda") if n else None
 
 
 def linear_mxfp4(x, Wp, N, bias, y, residual=None, epilogue=EPI_NONE, ws=None) -> None:
     """gorch_hip_linear_mxfp4: y = residual + epi(x @ W^T + bias) over a
     pack_mxfp4 weight of N rows; x [M, K] and y [M, N] f32. ws from
-    linear_mxfp4_workspace (a new one if None); calls that can overlap must not
-    share it."""
+    linear_mxfp4_workspace for these sizes, whose calls leave it as they need it
+    (a new one if None); calls that can overlap must not share it."""
     dev = _device()
     if x.dim() != 2:
         raise ValueError("gorch_amd.hip: x must be [M, K]")

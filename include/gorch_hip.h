@@ -143,6 +143,7 @@ void gorch_hip_reset_dispatch_counts(void);
  * that launch nothing. op and dims:
  *   "linear" {M, N, K, flags}: gorch_hip_linear_bf16_ex above 16 rows (any
  *     number of rows with GORCH_HIP_LINEAR_ACT_BF16);
+ *   "linear_mxfp4" {M, N, K}: gorch_hip_linear_mxfp4;
  *   "gate_up" {rows, inter, dim}: a Qwen block's gate/up product and SwiGLU
  *     above 16 rows ("pair...": in one kernel);
  *   "matmul" {M, N, K, batch, aBF16, bBF16}: the general product
@@ -266,8 +267,10 @@ int gorch_hip_pack_mxfp4(void* stream, const uint8_t* codes, const uint8_t* scal
  * may alias y, x must not. K % 8 == 0, M up to 2^20, K up to 2^24, x, Wp and
  * the workspace 16-byte aligned (else GORCH_HIP_EUNSUPPORTED). The workspace
  * (gorch_hip_linear_mxfp4_workspace_size bytes of device memory; NULL where
- * that is 0) is the caller's: calls that can overlap must not share one.
- * Nothing is allocated, so the call can be captured. */
+ * that is 0) is the caller's: zeroed before its first use with these M, N and
+ * K (with up to 16 rows it holds counters, zero again after every call), and
+ * not shared by calls that can overlap. Nothing is allocated, so the call can
+ * be captured. */
 size_t gorch_hip_linear_mxfp4_workspace_size(int M, int N, int K);
 int gorch_hip_linear_mxfp4(void* stream, const float* x, const void* Wp, const float* bias, const float* residual,
                            float* y, int M, int N, int K, int epilogue, void* workspace, size_t workspace_bytes);

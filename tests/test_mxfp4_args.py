@@ -72,7 +72,7 @@ def test_linear_of_nothing_and_workspaces():
     assert linear(M=0, x=None, Wp=None, y=None) == 0 and linear(N=0, x=None, Wp=None, y=None) == 0
     size = L().gorch_hip_linear_mxfp4_workspace_size
     assert size(0, 16, 64) == size(-1, 16, 64) == size(16, 0, 64) == size(17, 16, 0) == 0
-    assert size(17, 16, 128) > 0 and size(2000, 16, 4096) >= 125 * 32 * 7680
+    assert size(1, 4096, 1024) == 0 and size(1, 16, 8192) > 0 and size(17, 16, 128) > 0 and size(2000, 16, 4096) >= 125 * 32 * 7680
 
 
 MX = dict(dtype=2, k_scale=FAKE, v_scale=FAKE)

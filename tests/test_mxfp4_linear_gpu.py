@@ -89,6 +89,19 @@ def test_larger(gpu, M, N, K, act):
     check(call(gpu, x, codes, scales, b, None, act), *expected(x, codes, scales, b, None, act))
 
 
+@pytest.mark.parametrize("name,M,N,K", [
+    ("gemv", 1, 4100, 4096), ("gemv split", 2, 300, 9000), ("gemv5", 5, 3000, 2048), ("gemv5 split", 4, 300, 6000),
+    ("gemv5 made", 13, 5000, 2048), ("gemv5 made split", 16, 1000, 9000), ("gemm128x256", 1000, 4200, 1032),
+    ("gemm128x128", 600, 6000, 520), ("gemm64x128", 500, 4000, 1160), ("gemm64x64", 64, 16300, 600),
+    ("gemm32x64", 128, 4001, 2056), ("gemm32x32", 64, 4000, 1096)])
+def test_every_kernel(gpu, name, M, N, K):
+    assert gpu.kernel_choice("linear_mxfp4", M, N, K) == name
+    rng, x, codes, scales = inputs(K, M, N, K)
+    b = rng.standard_normal(N).astype(np.float32)
+    r = rng.standard_normal((M, N)).astype(np.float32)
+    check(call(gpu, x, codes, scales, b, r, M % 2 == 0), *expected(x, codes, scales, b, r, M % 2 == 0))
+
+
 @pytest.mark.parametrize("M", [1, 9, 40])
 def test_residual_may_be_the_output(gpu, M):
     rng, x, codes, scales = inputs(M, M, 100, 264)
@@ -135,14 +148,15 @@ def test_nonfinite_rows_and_columns_stay_apart(gpu, M, bad):
 
 
 @pytest.mark.parametrize("M", [1, 6, 16, 90])
-def test_same_bits_every_time_whatever_the_workspace_held(gpu, M):
-    rng, x, codes, scales = inputs(M, M, 200, 1160)
+def test_same_bits_every_time(gpu, M):
+    # one workspace for all: partial sums of the last call are no part of the next
+    rng, x, codes, scales = inputs(M, M, 200, 5160)
     first = call(gpu, x, codes, scales)
-    for fill in (0, 0xff):
-        ws = gpu.linear_mxfp4_workspace(M, 200, 1160)
-        if ws is not None:
-            ws.fill_(fill)
+    check(first, *expected(x, codes, scales))
+    ws = gpu.linear_mxfp4_workspace(M, 200, 5160)
+    for _ in range(3):
         np.testing.assert_array_equal(call(gpu, x, codes, scales, ws=ws), first)
+        call(gpu, -3 * x[::-1], codes, scales, ws=ws)
 
 
 def test_rows_do_not_depend_on_their_batch(gpu):
@@ -153,16 +167,16 @@ def test_rows_do_not_depend_on_their_batch(gpu):
 
 @pytest.mark.parametrize("M", [1, 4, 100])
 def test_captured_and_replayed(gpu, M):
-    rng, x, codes, scales = inputs(M, M, 300, 520)
+    rng, x, codes, scales = inputs(M, M, 300, 2520)
     Wp = gpu.pack_mxfp4(dev(codes), dev(scales))
     xd, b, y = dev(x), dev(rng.standard_normal(300).astype(np.float32)), torch.zeros((M, 300), device="cuda")
-    ws = gpu.linear_mxfp4_workspace(M, 300, 520)
+    ws = gpu.linear_mxfp4_workspace(M, 300, 2520)
     torch.cuda.synchronize()
     graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
     with torch.cuda.graph(graph, stream=side):
         gpu.linear_mxfp4(xd, Wp, 300, b, y, ws=ws)
     for turn in range(3):
-        x = rng.standard_normal((M, 520)).astype(np.float32)
+        x = rng.standard_normal((M, 2520)).astype(np.float32)
         xd.copy_(dev(x))
         y.fill_(7)
         graph.replay()
