@@ -27,11 +27,9 @@ struct MxRow {
     uint32_t s[MxTile<HD>::NU];
 };
 template <int HD, bool PART>
-__device__ __forceinline__ void mx_fetch(const void* pool, const float* scales, long long row, int hd, int g, MxRow<HD>& r) {
+__device__ __forceinline__ void mx_fetch(const void* pool, long long row, int hd, int g, MxRow<HD>& r) {
     const char* zero = reinterpret_cast<const char*>(kZeros);
-    const int gpr = PART ? (hd + 31) / 32 : HD / 32;
-    const char* p = row >= 0 ? static_cast<const char*>(pool) + row * (PART ? hd / 2 : HD / 2) : zero;
-    const uint8_t* s = row >= 0 ? reinterpret_cast<const uint8_t*>(scales) + row * gpr : reinterpret_cast<const uint8_t*>(kZeros);
+    const char* p = static_cast<const char*>(pool) + row * (PART ? hd / 2 : HD / 2);
 #pragma unroll
     for (int u = 0; u < MxTile<HD>::NU; u++) {
         const int at = 4 * u + g;
@@ -41,16 +39,71 @@ __device__ __forceinline__ void mx_fetch(const void* pool, const float* scales, 
             const u32x2 hi = *reinterpret_cast<const u32x2*>(32 * at + 16 < hd ? p + 16 * at + 8 : zero);
             r.c[u] = u32x4{lo[0], lo[1], hi[0], hi[1]};
         } else {
-            r.c[u] = *reinterpret_cast<const u32x4*>(at < gpr ? p + 16 * at : zero);
+            r.c[u] = *reinterpret_cast<const u32x4*>(HD >= 128 || g < HD / 32 ? p + 16 * at : zero);
         }
-        r.s[u] = *(at < gpr ? s + at : reinterpret_cast<const uint8_t*>(zero));
     }
 }
-// A value's pieces to a tile in LDS (16-key group j) as bf16; true where its
-// scale is NaN (zeros are written).
+// The scale bytes of a tile's K and V rows: as they are fetched, and dealt to
+// the lanes when they have come. row: that of this lane's key (of 32); lo, hi:
+// those of its key in each 16-key group. Heads of whole words of scales: lanes
+// 0 .. 31 fetch their key's K words, the others V's.
+template <int HD, bool PART>
+struct MxScales {
+    static constexpr int NU = MxTile<HD>::NU;
+    static constexpr bool WORDS = !PART;
+    uint32_t w[WORDS ? NU : 4 * NU];
+
+    template <typename Pair>
+    __device__ __forceinline__ void fetch(const PagedArgs& p, long long row, Pair lo, Pair hi, int g) {
+        if constexpr (WORDS) {
+            const uint8_t* from = reinterpret_cast<const uint8_t*>((threadIdx.x & 32) ? p.vs : p.ks) + row * (HD / 32);
+#pragma unroll
+            for (int u = 0; u < NU; u++) {
+                if constexpr (HD == 64) w[u] = *reinterpret_cast<const uint16_t*>(from);
+                else w[u] = *reinterpret_cast<const uint32_t*>(from + 4 * u);
+            }
+        } else {
+            const int gpr = (p.hd + 31) / 32;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const long long at = (long long)(((uint64_t)hi[j] << 32) | lo[j]) * gpr;
+#pragma unroll
+                for (int u = 0; u < NU; u++) {
+                    const uint8_t* zero = reinterpret_cast<const uint8_t*>(kZeros);
+                    const int i = 4 * u + g;
+                    w[4 * u + j] = *(i < gpr ? reinterpret_cast<const uint8_t*>(p.ks) + at + i : zero);
+                    w[4 * u + 2 + j] = *(i < gpr ? reinterpret_cast<const uint8_t*>(p.vs) + at + i : zero);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void deal(int g, MxRow<HD> (&k)[2], MxRow<HD> (&v)[2]) const {
+#pragma unroll
+        for (int u = 0; u < NU; u++) {
+            if constexpr (WORDS) {
+                const auto h = __builtin_amdgcn_permlane16_swap(w[u], w[u], false, false);
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const auto kv = __builtin_amdgcn_permlane32_swap(h[j], h[j], false, false);
+                    // (of 64 columns the lanes of groups 2 and 3 have none: byte 0)
+                    k[j].s[u] = kv[0] >> (8 * g) & 0xff;
+                    v[j].s[u] = kv[1] >> (8 * g) & 0xff;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    k[j].s[u] = w[4 * u + j];
+                    v[j].s[u] = w[4 * u + 2 + j];
+                }
+            }
+        }
+    }
+};
+// A value's pieces to its place (key `key`) of a tile in LDS as bf16; true
+// where its scale is NaN (zeros are written).
 template <int HD>
-__device__ __forceinline__ bool mx_put(const MxRow<HD>& r, char* vt, int j, int lane) {
-    const int g = lane >> 4, key = lane & 15;
+__device__ __forceinline__ bool mx_put(const MxRow<HD>& r, char* vt, int key, int lane) {
+    const int g = lane >> 4;
     bool odd = false;
 #pragma unroll
     for (int u = 0; u < MxTile<HD>::NU; u++) {
@@ -58,20 +111,21 @@ __device__ __forceinline__ bool mx_put(const MxRow<HD>& r, char* vt, int j, int 
         const bool nan = r.s[u] == kMxNaN, none = nan || r.s[u] == 0;
         odd |= nan;
         const float s = __uint_as_float(none ? 0x3f800000u : r.s[u] << 23);
-        char* to = vt + j * MxTile<HD>::GROUP + (4 * u + g) * 1024 + key * 16;
+        const uint32_t keep = none ? 0u : ~0u;  // (a mask: a choice per word becomes a branch)
+        char* to = vt + (key >> 4) * MxTile<HD>::GROUP + (4 * u + g) * 1024 + (key & 15) * 16;
 #pragma unroll
-        for (int i = 0; i < 4; i++) *reinterpret_cast<u32x4*>(to + i * 256) = mx_widen8(none ? 0u : r.c[u][i], s);
+        for (int i = 0; i < 4; i++) *reinterpret_cast<u32x4*>(to + i * 256) = mx_widen8(r.c[u][i] & keep, s);
     }
     return odd;
 }
 // NaN groups of a value (key `key`) noted for every row that sees it.
 template <int BM, int HD>
 __device__ __forceinline__ void mx_note(OddBits<BM, HD>& odd, const PagedAttnArgs& a, const SeqAt& s, int r0, int key,
-                                        const MxRow<HD>& v, int g) {
+                                        const uint32_t (&scale)[MxTile<HD>::NU], int g) {
     const int G = a.group.d, n = s.end - s.begin;
 #pragma unroll
     for (int u = 0; u < MxTile<HD>::NU; u++) {
-        if (v.s[u] != kMxNaN || 4 * u + g >= HD / 32) continue;
+        if (scale[u] != kMxNaN || 4 * u + g >= HD / 32) continue;
         odd.any = 1;
 #pragma unroll 1
         for (int r = 0; r < BM && r0 + r < n * G; r++) {
@@ -105,89 +159,211 @@ __device__ __forceinline__ void mx_terms(const floatx4 (&x)[8], float scale, MxT
     mx_split(f, t);
 }
 
-// FewRows over keys of four bits. CW = 4: a row in four columns, which hold its
-// first four terms for one instruction; the fifth is the first column's of
-// another.
-template <int HD, int CW>
-struct MxFewRows : FewRows<false, HD, CW> {
-    static constexpr int NU = MxTile<HD>::NU, NQ = CW == 4 ? 2 : kMxTerms;
-    u32x6 q6[NU][NQ];
+// FewRows over keys of four bits.
+template <int HD>
+struct MxFewRows : FewRows<false, HD, 16> {
+    static constexpr int NU = MxTile<HD>::NU;
+    u32x6 q6[NU][kMxTerms];
     uint32_t sq[NU][2];
 
-    template <bool PART>
-    __device__ __forceinline__ void fetch(const PagedAttnArgs& a, const SeqAt& s, int r0, int kvh, floatx4 (&x)[NU][8]) {
+    template <bool PART, typename Block>
+    __device__ __forceinline__ void begin(const PagedAttnArgs& a, const SeqAt& s, int r0, int kvh, Block&) {
         const int lane = threadIdx.x & 63, G = a.group.d, n = s.end - s.begin;
-        const int r = r0 + (lane & (CW - 1));
+        const int r = r0 + (lane & 15);
         const int tok = (int)a.group.div((uint32_t)r);
         this->pos = r < n * G ? (a.causal ? s.len - n + tok : s.len - 1) : -1;
         this->first = a.causal ? s.len - n + (int)a.group.div((uint32_t)r0) : s.len - 1;
+        floatx4 x[NU][8];
         mx_fetch_q<PART, NU>(a, s, r, kvh, lane >> 4, PART ? a.p.hd : HD, x);
-    }
-    __device__ __forceinline__ void begin(const PagedAttnArgs& a, const floatx4 (&x)[NU][8]) {
-        const int k = (int)(threadIdx.x & 15) / CW;
 #pragma unroll
         for (int u = 0; u < NU; u++) {
             MxTerms t;
             mx_terms(x[u], a.scale, t);
-            if constexpr (CW == 4) {
 #pragma unroll
-                for (int e = 0; e < 6; e++) {
-                    q6[u][0][e] = k == 0 ? t.t[0][e] : (k == 1 ? t.t[1][e] : (k == 2 ? t.t[2][e] : t.t[3][e]));
-                    q6[u][1][e] = k == 0 ? t.t[4][e] : 0;
-                }
-                sq[u][0] = t.scale >> (8 * k);
-            } else {
-#pragma unroll
-                for (int e = 0; e < kMxTerms; e++) q6[u][e] = t.t[e];
-                sq[u][0] = t.scale;
-            }
+            for (int e = 0; e < kMxTerms; e++) q6[u][e] = t.t[e];
+            sq[u][0] = t.scale;
             sq[u][1] = t.last;
         }
         this->clear();
     }
+    template <typename Block>
+    __device__ __forceinline__ void ready(Block&) {}
     // scores of a group's 16 keys: lane group g holds keys 4 g .. 4 g + 3
     __device__ __forceinline__ floatx4 score(const MxRow<HD>& key) {
         floatx4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < NU; u++) {
             const i32x8 k = mx_op4(key.c[u]);
-            s = mx_mfma_t<0, 0>(k, key.s[u], mx_op6(q6[u][NQ - 1]), sq[u][1], s);
-            if constexpr (CW == 16) {
-                s = mx_mfma_t<0, 3>(k, key.s[u], mx_op6(q6[u][3]), sq[u][0], s);
-                s = mx_mfma_t<0, 2>(k, key.s[u], mx_op6(q6[u][2]), sq[u][0], s);
-                s = mx_mfma_t<0, 1>(k, key.s[u], mx_op6(q6[u][1]), sq[u][0], s);
-            }
+            s = mx_mfma_t<0, 0>(k, key.s[u], mx_op6(q6[u][4]), sq[u][1], s);
+            s = mx_mfma_t<0, 3>(k, key.s[u], mx_op6(q6[u][3]), sq[u][0], s);
+            s = mx_mfma_t<0, 2>(k, key.s[u], mx_op6(q6[u][2]), sq[u][0], s);
+            s = mx_mfma_t<0, 1>(k, key.s[u], mx_op6(q6[u][1]), sq[u][0], s);
             s = mx_mfma_t<0, 0>(k, key.s[u], mx_op6(q6[u][0]), sq[u][0], s);
         }
-        if constexpr (CW == 4)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                s[e] += dpp_f<0x128>(s[e]);  // 16 lanes rotated by 8
-                s[e] += dpp_f<0x124>(s[e]);  // and by 4
-            }
         return s;
+    }
+    __device__ __forceinline__ void weigh(floatx4 (&sc)[2], int key0, uint32_t seen, const char* vt, char*) {
+        this->take(sc, key0, seen, nullptr, nullptr, vt);
+    }
+    // a row's maximum and sum of weights, in the lanes of group 0
+    __device__ __forceinline__ void totals(float& m, float& l, int& r) const {
+        m = this->m;
+        l = col_sum(this->l);
+        r = (threadIdx.x & 63) < 16 ? (int)(threadIdx.x & 15) : -1;
+    }
+};
+
+// Up to four rows: S = Q K^T, the first four terms of row g as rows 4 g .. 4 g
+// + 3 of one operand and its fifth as row 4 g of another, so that a lane (g, c)
+// adds up the score of row g and key c itself and a tile's 32 keys are two
+// scores a lane (as columns of the other form they would be eight, each four
+// times over: 57 -> 44 us for 64 conversations of up to 8,192 tokens). The
+// weights' three bf16 terms then go through LDS to their places in P^T: column
+// 4 t + g of the operand holds term t of row g; lanes c and c + 1 first trade
+// one of their two weights, so that each has two neighbours there. (A numbering
+// of the keys that made a lane's own two neighbours read every second row of a
+// cache line: 74 us.) A block's first waves split q for all.
+template <int HD>
+struct MxFour {
+    static constexpr int NU = MxTile<HD>::NU, TP = 4;
+    u32x6 q6[NU][2];
+    uint32_t sq[NU][2];
+    floatx4 o[HD / 16];
+    float m, l;
+    int pos, first;
+
+    template <bool PART, typename Block>
+    __device__ __forceinline__ void begin(const PagedAttnArgs& a, const SeqAt& s, int r0, int kvh, Block& sh) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+        const int G = a.group.d, n = s.end - s.begin, r = r0 + g;
+        pos = r < n * G ? (a.causal ? s.len - n + (int)a.group.div((uint32_t)r) : s.len - 1) : -1;
+        first = a.causal ? s.len - n + (int)a.group.div((uint32_t)r0) : s.len - 1;
+        if (wave < 2 * NU) {
+            // wave 2 u: terms 0 .. 3 of columns 128 u .., wave 2 u + 1: term 4
+            const int u = wave >> 1, fifth = wave & 1, t = fifth ? 4 : (c & 3);
+            floatx4 x[1][8];
+            mx_fetch_q<PART, 1>(a, s, r0 + (c >> 2), kvh, 4 * u + g, PART ? a.p.hd : HD, x);
+            floatx32 f;
+#pragma unroll
+            for (int i = 0; i < 32; i++) f[i] = x[0][i >> 2][i & 3] * a.scale;
+            uint32_t sc;
+            u32x6 six = mx_term(f, t, sc);
+            if (fifth && (c & 3) != 0) six = u32x6{0, 0, 0, 0, 0, 0}, sc = sc == kMxNaN ? sc : 0;
+            sh.q[wave].lo[lane] = u32x4{six[0], six[1], six[2], six[3]};
+            sh.q[wave].hi[lane] = u32x2{six[4], six[5]};
+            sh.q[wave].s[lane] = sc;
+        }
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++) o[d] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+    template <typename Block>
+    __device__ __forceinline__ void ready(Block& sh) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int u = 0; u < NU; u++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const u32x4 lo = sh.q[2 * u + k].lo[lane];
+                const u32x2 hi = sh.q[2 * u + k].hi[lane];
+                q6[u][k] = u32x6{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1]};
+                sq[u][k] = sh.q[2 * u + k].s[lane];
+            }
+    }
+    // the score of row g and the group's key c
+    __device__ __forceinline__ float score(const MxRow<HD>& key) {
+        floatx4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < NU; u++) {
+            const i32x8 k = mx_op4(key.c[u]);
+            s = mx_mfma<0, 0>(mx_op6(q6[u][1]), sq[u][1], k, key.s[u], s);
+            s = mx_mfma<0, 0>(mx_op6(q6[u][0]), sq[u][0], k, key.s[u], s);
+        }
+        return ((s[3] + s[2]) + s[1]) + s[0];
+    }
+    // pt: a KB of LDS of the wave's own
+    __device__ __forceinline__ void weigh(float (&sc)[2], int key0, uint32_t seen, const char* vt, char* pt) {
+        using T = Tile<false, HD>;
+        const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+        if (key0 + 31 > first || seen != 0xffffffffu) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int sees = (int)(seen >> (16 * j + c) & 1u) & (key0 + 16 * j + c <= pos ? 1 : 0);
+                sc[j] = sees ? sc[j] : -INFINITY;
+            }
+        }
+        float top = fmaxf(sc[0], sc[1]);
+        top = fmaxf(top, dpp_f<kDppQuadSwap1>(top));
+        top = fmaxf(top, dpp_f<kDppQuadSwap2>(top));
+        top = fmaxf(top, dpp_f<kDppRowHalfMirror>(top));
+        top = fmaxf(top, dpp_f<kDppRowMirror>(top));
+        const float mn = fmaxf(m, top), use = mn == -INFINITY ? 0.f : mn;
+        const bool grew = mn != m;
+        if (__any(grew)) {
+            const float al = __builtin_amdgcn_exp2f(m - use);
+            l *= al;
+            // a column's row is its number's last two bits
+            const float a0 = readlane_f(al, 0), a1 = readlane_f(al, 16), a2 = readlane_f(al, 32), a3 = readlane_f(al, 48);
+            const float f = c & 2 ? (c & 1 ? a3 : a2) : (c & 1 ? a1 : a0);
+#pragma unroll
+            for (int d = 0; d < HD / 16; d++) o[d] *= f;
+        }
+        m = mn;
+        // of keys c, c + 1 of group 0 (c even), or c - 1, c of group 1
+        const float x0 = __builtin_amdgcn_exp2f(sc[0] - use), x1 = __builtin_amdgcn_exp2f(sc[1] - use);
+        l += x0 + x1;
+        const bool odd = (c & 1) != 0;
+        const float other = dpp_f<kDppQuadSwap1>(odd ? x0 : x1);
+        const float x[2] = {odd ? other : x0, odd ? x1 : other};
+        uint32_t w[2][3];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const float r1 = x[j] - __uint_as_float(__float_as_uint(x[j]) & 0xffff0000u);
+            w[j][0] = __float_as_uint(x[j]);
+            w[j][1] = __float_as_uint(r1);
+            w[j][2] = __float_as_uint(r1 - __uint_as_float(__float_as_uint(r1) & 0xffff0000u));
+        }
+        char* to = pt + g * 64 + 16 * (c >> 2) + (odd ? 8 : 0) + 2 * (c & 2);
+#pragma unroll
+        for (int t = 0; t < 3; t++)
+            *reinterpret_cast<uint32_t*>(to + t * 256) = __builtin_amdgcn_perm(w[1][t], w[0][t], 0x07060302u);
+        const bf16x8 p = *reinterpret_cast<const bf16x8*>(pt + c * 64 + g * 16);
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++) o[d] = mfma16x16x32(T::vfrag(vt, d, lane), p, o[d]);
+    }
+    __device__ __forceinline__ void totals(float& mt, float& lt, int& r) const {
+        mt = m;
+        lt = seg_sum<16>(l);
+        r = (threadIdx.x & 15) == 0 ? (int)(threadIdx.x & 63) >> 4 : -1;
     }
 };
 
 // Few rows: as k_paged_attn_few, the values widened on their way to LDS.
 template <int HD, bool PART, int CW>
 struct MxFewBlock {
-    static constexpr int NW = 4, NB = 2, OROW = HD + 4;
-    static constexpr int STAGE = NW * Tile<false, HD>::BYTES, JOIN = NW * 16 * (OROW + 2) * 4;
+    static constexpr int NW = 4, NB = 2, OROW = HD + 4, PT = CW == 4 ? 1024 : 0;
+    static constexpr int STAGE = NW * (Tile<false, HD>::BYTES + PT), JOIN = NW * 16 * (OROW + 2) * 4;
     char lds[STAGE > JOIN ? STAGE : JOIN];
+    struct Operand {
+        u32x4 lo[64];
+        u32x2 hi[64];
+        uint32_t s[64];
+    };
+    Operand q[CW == 4 ? 2 * MxTile<HD>::NU : 1];
     OddBits<CW, HD> odd;
 };
 template <int HD, bool PART, int CW>
 __device__ __forceinline__ void mx_few_tile(const PagedAttnArgs& a, const SeqAt& s, int r0, int kvh, int split,
                                             const int (&page)[MxFewBlock<HD, PART, CW>::NB + 1],
                                             MxFewBlock<HD, PART, CW>& sh) {
-    using R = MxFewRows<HD, CW>;
+    using R = typename std::conditional<CW == 4, MxFour<HD>, MxFewRows<HD>>::type;
     using Sh = MxFewBlock<HD, PART, CW>;
     constexpr int NW = Sh::NW, STEP = 32 * NW, NB = Sh::NB, OROW = Sh::OROW;
     char* const lds = sh.lds;
     auto& odd = sh.odd;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
-    const int G = a.group.d, n = s.end - s.begin;
+    const int G = a.group.d, n = s.end - s.begin, mine = lane & 31;
     const int end_tok = (int)a.group.div((uint32_t)(min(r0 + CW, n * G) - 1));
     const int T1 = min((a.causal ? s.len - n + end_tok : s.len - 1) + 1, a.p.limit);
     const int k0 = split * a.chunk, k1 = a.splits == 1 ? T1 : min(T1, k0 + a.chunk);
@@ -195,52 +371,57 @@ __device__ __forceinline__ void mx_few_tile(const PagedAttnArgs& a, const SeqAt&
         if (split == 0) put_nothing<CW>(a, split, s, r0, kvh);
         return;
     }
-    char* vt = lds + wave * Tile<false, HD>::BYTES;
+    char* vt = lds + wave * (Tile<false, HD>::BYTES + Sh::PT);
+    char* pt = vt + Tile<false, HD>::BYTES;
     struct Buf {
         MxRow<HD> k[2], v[2];
+        MxScales<HD, PART> s;
         uint32_t seen;
     } buf[NB];
-    // row: the pool row of key lane % 32 of the tile
+    // row: the pool row of this lane's key of the tile (-1: none; what row 0
+    // holds is read then, and not looked at)
     auto fetch = [&](long long row, Buf& b) {
+        b.seen = (uint32_t)__ballot(row >= 0);
+        row = row < 0 ? 0 : row;
         const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)row, (uint32_t)row, false, false);
         const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(row >> 32), (uint32_t)(row >> 32), false, false);
-        b.seen = (uint32_t)__ballot(row >= 0);
 #pragma unroll
-        for (int j = 0; j < 2; j++) mx_fetch<HD, PART>(a.p.k, a.p.ks, (long long)(((uint64_t)hi[j] << 32) | lo[j]), a.p.hd, g, b.k[j]);
+        for (int j = 0; j < 2; j++) mx_fetch<HD, PART>(a.p.k, (long long)(((uint64_t)hi[j] << 32) | lo[j]), a.p.hd, g, b.k[j]);
+        b.s.fetch(a.p, row, lo, hi, g);
 #pragma unroll
-        for (int j = 0; j < 2; j++) mx_fetch<HD, PART>(a.p.v, a.p.vs, (long long)(((uint64_t)hi[j] << 32) | lo[j]), a.p.hd, g, b.v[j]);
+        for (int j = 0; j < 2; j++) mx_fetch<HD, PART>(a.p.v, (long long)(((uint64_t)hi[j] << 32) | lo[j]), a.p.hd, g, b.v[j]);
     };
     R rows;
     int key0 = k0 + 32 * wave;
     int next = page[NB];  // the page of the next tile to fetch
-    {
-        floatx4 x[R::NU][8];
-        rows.template fetch<PART>(a, s, r0, kvh, x);
 #pragma unroll
-        for (int i = 0; i < NB; i++) fetch(key_row(a.p, page[i], key0 + i * STEP + (lane & 31), k1, kvh), buf[i]);
-        for (int i = threadIdx.x; i < (int)(sizeof(odd) / 4); i += 64 * NW) reinterpret_cast<uint32_t*>(&odd)[i] = 0;
-        rows.begin(a, x);
-    }
+    for (int i = 0; i < NB; i++) fetch(key_row(a.p, page[i], key0 + i * STEP + mine, k1, kvh), buf[i]);
+    for (int i = threadIdx.x; i < (int)(sizeof(odd) / 4); i += 64 * NW) reinterpret_cast<uint32_t*>(&odd)[i] = 0;
+    rows.template begin<PART>(a, s, r0, kvh, sh);
     __syncthreads();
+    rows.ready(sh);
     auto step = [&](Buf& b, int key) {
         const bool on = key < k1;
         const uint32_t here = b.seen;
-        floatx4 scores[2];
+        decltype(rows.score(b.k[0])) scores[2];
         if (on) {
+            b.s.deal(g, b.k, b.v);
 #pragma unroll
             for (int j = 0; j < 2; j++) scores[j] = rows.score(b.k[j]);
             bool nan = false;
 #pragma unroll
-            for (int j = 0; j < 2; j++) nan |= mx_put<HD>(b.v[j], vt, j, lane);
-            if (__any(nan))
-#pragma unroll 1
-                for (int j = 0; j < 2; j++) mx_note<CW, HD>(odd, a, s, r0, key + 16 * j + (lane & 15), j ? b.v[1] : b.v[0], g);
+            for (int j = 0; j < 2; j++) nan |= mx_put<HD>(b.v[j], vt, 16 * j + (lane & 15), lane);
+            if (__any(nan)) {
+                // (a dynamic choice of the rows themselves would put them into scratch memory)
+                if (here >> (lane & 15) & 1u) mx_note<CW, HD>(odd, a, s, r0, key + (lane & 15), b.v[0].s, g);
+                if (here >> (16 + (lane & 15)) & 1u) mx_note<CW, HD>(odd, a, s, r0, key + 16 + (lane & 15), b.v[1].s, g);
+            }
         }
-        const int after = key_page(a.p, s.s, key + (NB + 1) * STEP + (lane & 31));
+        const int after = key_page(a.p, s.s, key + (NB + 1) * STEP + mine);
         __builtin_amdgcn_sched_barrier(0);
-        fetch(key_row(a.p, next, key + NB * STEP + (lane & 31), k1, kvh), b);
+        fetch(key_row(a.p, next, key + NB * STEP + mine, k1, kvh), b);
         next = after;
-        if (on) rows.take(scores, key, here, nullptr, nullptr, vt);
+        if (on) rows.weigh(scores, key, here, vt, pt);
     };
     for (; key0 < k1; key0 += NB * STEP)
 #pragma unroll
@@ -250,14 +431,18 @@ __device__ __forceinline__ void mx_few_tile(const PagedAttnArgs& a, const SeqAt&
     float* jo = reinterpret_cast<float*>(lds);
     float* jm = jo + NW * 16 * OROW;
     float* jl = jm + NW * 16;
-    const float l = col_sum(rows.l);
+    {
+        float m, l;
+        int r;
+        rows.totals(m, l, r);
+        if (r >= 0) {
+            jm[wave * 16 + r] = m;
+            jl[wave * 16 + r] = l;
+        }
+    }
 #pragma unroll
     for (int d = 0; d < HD / 16; d++)
         *reinterpret_cast<floatx4*>(jo + (wave * 16 + (lane & 15)) * OROW + 16 * d + 4 * g) = rows.o[d];
-    if (g == 0) {
-        jm[wave * 16 + lane] = rows.m;
-        jl[wave * 16 + lane] = l;
-    }
     __syncthreads();
     for (int i = threadIdx.x; i < CW * (HD / 4); i += 64 * NW) {
         const int r = i / (HD / 4), c = 4 * (i % (HD / 4));
@@ -295,7 +480,8 @@ __device__ __forceinline__ void mx_few_block(const PagedAttnArgs& a, int block, 
     int page[Sh::NB + 1];
 #pragma unroll
     for (int i = 0; i <= Sh::NB; i++)
-        page[i] = key_page(a.p, s.s, split * a.chunk + 32 * (int)(threadIdx.x >> 6) + i * 32 * Sh::NW + (int)(threadIdx.x & 31));
+        page[i] = key_page(a.p, s.s, split * a.chunk + 32 * (int)(threadIdx.x >> 6) + i * 32 * Sh::NW +
+                                         (int)(threadIdx.x & 31));
     const int b = seq_begin(a.p, s.s), e = seq_begin(a.p, s.s + 1), len = a.p.lens[s.s];
     s.begin = __builtin_amdgcn_readfirstlane(b);
     s.end = __builtin_amdgcn_readfirstlane(max(b, e));
@@ -436,9 +622,10 @@ __device__ __forceinline__ void mx_many_block(const PagedAttnArgs& a, int block,
         } else if (HD >= 128 || g < HD / 32) {
             const bool nan = raw.s[0] == kMxNaN, none = nan || raw.s[0] == 0;
             const float f = __uint_as_float(none ? 0x3f800000u : raw.s[0] << 23);
+            const uint32_t keep = none ? 0u : ~0u;
             char* to = sh.vt[b] + j * MxTile<HD>::GROUP + (4 * u + g) * 1024 + (lane & 15) * 16;
 #pragma unroll
-            for (int i = 0; i < 4; i++) *reinterpret_cast<u32x4*>(to + i * 256) = mx_widen8(none ? 0u : raw.c[0][i], f);
+            for (int i = 0; i < 4; i++) *reinterpret_cast<u32x4*>(to + i * 256) = mx_widen8(raw.c[0][i] & keep, f);
             if (nan) {
                 sh.odd.any = 1;
 #pragma unroll 1
