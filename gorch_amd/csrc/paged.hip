@@ -264,17 +264,27 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
 // TOK tokens a block: their places first, then every load of K and V (a thread
 // keeps its four columns), then the stores. Bound by memory: 57,512 tokens of
 // 8 x 128 in e4m3 116 us with four tokens a block (5.1 TB/s), 172 with one;
-// few tokens have one a block (1,000 in bf16 4.3 us against 5.0).
-template <int KV, int TOK>
+// few tokens have one a block (1,000 in bf16 4.3 us against 5.0). Heads that
+// need fewer than 256 threads a token share the block between tokens, LG lanes
+// a token: 15,518 tokens of 2 x 64 in MXFP4 12.6 -> 9.9 us with four tokens in
+// turn, 7.1 with one (its lookups then overlap between waves).
+template <int KV, int TOK, int LG>
 __global__ __launch_bounds__(256) void k_paged_read(PagedArgs p, float* ko, float* vo) {
-    const int t0 = blockIdx.x * TOK, hd4 = p.hd / 4, n4 = p.num_kv * hd4;
-    const int i0 = blockIdx.y * 256 + threadIdx.x, i = min(i0, n4 - 1), h = i / hd4, c = i - h * hd4;
+    constexpr int S = LG < 64 ? 64 / LG : 1;  // tokens side by side in a wave
+    const int hd4 = p.hd / 4, n4 = p.num_kv * hd4;
+    const int i0 = blockIdx.y * LG + threadIdx.x % LG, i = min(i0, n4 - 1), h = i / hd4, c = i - h * hd4;
+    const int t0 = (blockIdx.x * (256 / LG) + threadIdx.x / LG) * TOK;
     long long row[TOK];
 #pragma unroll
     for (int j = 0; j < TOK; j++) {
-        SeqAt sq;
         row[j] = -1;
-        if (t0 + j < p.tokens && token_seq(p, t0 + j, sq)) row[j] = pool_row(p, sq.s, sq.len - sq.end + t0 + j, h);
+#pragma unroll
+        for (int u = 0; u < S; u++) {
+            const int t = __builtin_amdgcn_readlane(t0, u * LG % 64) + j;
+            SeqAt sq;
+            if (t < p.tokens && token_seq(p, t, sq) && (S == 1 || t == t0 + j))
+                row[j] = pool_row(p, sq.s, sq.len - sq.end + t, h);
+        }
     }
     if (i0 >= n4) return;
     constexpr bool F8 = KV == GORCH_HIP_KV_E4M3, F4 = KV == GORCH_HIP_KV_MXFP4;
@@ -391,17 +401,25 @@ extern "C" int gorch_hip_paged_read(void* stream, const gorch_hip_paged_kv* kv, 
     GH_TRY(paged_args("gorch_hip_paged_read", kv, b, p));
     GH_SUPPORTED(aligned(k_out, 16) && aligned(v_out, 16), "gorch_hip_paged_read: outputs must be 16-byte aligned");
     if (b->tokens == 0 || b->seqs == 0 || (!k_out && !v_out)) return GORCH_HIP_OK;
-    const auto go = [&](auto kernel, int tok) {
-        hipLaunchKernelGGL(kernel, dim3((p.tokens + tok - 1) / tok, (p.num_kv * p.hd / 4 + 255) / 256), dim3(256), 0,
-                           stream_of(stream), p, k_out, v_out);
+    const int n4 = p.num_kv * p.hd / 4;
+    const auto go = [&](auto kernel, int tok, int lg) {
+        const int per = tok * 256 / lg;
+        hipLaunchKernelGGL(kernel, dim3((p.tokens + per - 1) / per, (n4 + lg - 1) / lg), dim3(256), 0, stream_of(stream), p,
+                           k_out, v_out);
     };
-    const auto of = [&](auto kind) {
-        constexpr int KV = decltype(kind)::value;
-        p.tokens < 4096 ? go(k_paged_read<KV, 1>, 1) : go(k_paged_read<KV, 4>, 4);
+    const auto of = [&](auto kind, auto lanes) {
+        constexpr int KV = decltype(kind)::value, LG = decltype(lanes)::value;
+        p.tokens * (LG / 32) < 32768 ? go(k_paged_read<KV, 1, LG>, 1, LG) : go(k_paged_read<KV, 4, LG>, 4, LG);
     };
-    if (kv->dtype == GORCH_HIP_KV_MXFP4) of(std::integral_constant<int, GORCH_HIP_KV_MXFP4>{});
-    else if (kv->dtype == GORCH_HIP_KV_E4M3) of(std::integral_constant<int, GORCH_HIP_KV_E4M3>{});
-    else of(std::integral_constant<int, GORCH_HIP_KV_BF16>{});
+    const auto by = [&](auto kind) {
+        if (n4 <= 32) of(kind, std::integral_constant<int, 32>{});
+        else if (n4 <= 64) of(kind, std::integral_constant<int, 64>{});
+        else if (n4 <= 128) of(kind, std::integral_constant<int, 128>{});
+        else of(kind, std::integral_constant<int, 256>{});
+    };
+    if (kv->dtype == GORCH_HIP_KV_MXFP4) by(std::integral_constant<int, GORCH_HIP_KV_MXFP4>{});
+    else if (kv->dtype == GORCH_HIP_KV_E4M3) by(std::integral_constant<int, GORCH_HIP_KV_E4M3>{});
+    else by(std::integral_constant<int, GORCH_HIP_KV_BF16>{});
     count(CNT_CODEC);
     return finish(stream, check_launch("paged_read"));
 }
