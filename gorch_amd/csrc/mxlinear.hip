@@ -566,7 +566,10 @@ __global__ __launch_bounds__(512 / MT, 2 / MT) void k_mx_gemm(MxLinearArgs a) {
 #endif
 }
 
-static size_t terms_bytes(int M, int K) { return (size_t)((M + 15) / 16) * ((K + 127) / 128) * kTermBytes; }
+// A workspace begins with the counters of every shape's blocks (at most 128 of
+// several slices), so that one may serve calls of all sizes in turn.
+constexpr size_t kCounterBytes = 512;
+static size_t terms_bytes(int M, int K) { return kCounterBytes + (size_t)((M + 15) / 16) * ((K + 127) / 128) * kTermBytes; }
 
 // How the rows of a decode step are cut into blocks: slices of K (at most 16),
 // row tiles per block, waves along the columns.
@@ -602,7 +605,8 @@ static GemvPlan gemv_plan(int M, int N, int K) {
     p.nt = p.kind != kRow1 && p.tiles / p.wk <= 4 && p.per > kGemvWaves / p.wk ? 2 : 1;
     p.terms = p.kind == kMade ? (size_t)nk * kTermBytes : 0;
     p.part = p.slices == 1 ? 0 : (size_t)p.slices * nt * 1024;
-    p.bytes = p.terms + p.part + (p.slices == 1 ? 0 : (size_t)p.blocks * 4);
+    p.bytes = p.terms + p.part;
+    if (p.bytes) p.bytes += kCounterBytes;
     return p;
 }
 
@@ -626,13 +630,14 @@ static int launch_mx_gemv_f(hipStream_t s, const MxLinearArgs& a, const GemvPlan
 }
 static int launch_mx_gemv(hipStream_t s, MxLinearArgs a, char* ws) {
     const GemvPlan p = gemv_plan(a.M, a.N, a.K);
+    static_assert(kCounterBytes >= 256 / 2 * sizeof(unsigned));
     a.slices = p.slices;
     a.chunks = p.chunks;
     a.per = p.per;
     a.blocks = p.blocks;
-    a.terms = ws;
-    a.part = reinterpret_cast<float*>(ws + p.terms);
-    a.done = reinterpret_cast<unsigned*>(ws + p.terms + p.part);
+    a.done = reinterpret_cast<unsigned*>(ws);
+    a.terms = ws + kCounterBytes;
+    a.part = reinterpret_cast<float*>(ws + kCounterBytes + p.terms);
     if (p.kind == kMade) hipLaunchKernelGGL(k_mx_terms16, dim3(a.nk), dim3(64 * kMxTerms), 0, s, a);
     if (p.tiles == 8) {
         if (p.wk == 8) return launch_mx_gemv_f<8, 1>(s, a, p);
@@ -684,7 +689,8 @@ static int launch_mx_gemm_t(hipStream_t s, const MxLinearArgs& a) {
     hipLaunchKernelGGL((k_mx_gemm<MT, NT, WM>), dim3((unsigned)((blocks + 7) / 8 * 8)), dim3(512 / MT), bytes, s, a);
     return GORCH_HIP_OK;
 }
-static int launch_mx_gemm(hipStream_t s, const MxLinearArgs& a) {
+static int launch_mx_gemm(hipStream_t s, MxLinearArgs a, char* ws) {
+    a.terms = ws + kCounterBytes;
     hipLaunchKernelGGL(k_mx_terms, dim3((a.nk + 3) / 4, (a.M + 15) / 16), dim3(256), 0, s, a);
     switch (gemm_shape(a.M, a.N, a.K)) {
         case 0: return launch_mx_gemm_t<2, 16, 4>(s, a);
@@ -723,7 +729,7 @@ extern "C" int gorch_hip_linear_mxfp4(void* stream, const float* x, const void* 
     GH_SUPPORTED(K % 8 == 0, "gorch_hip_linear_mxfp4: K must be a multiple of 8");
     GH_SUPPORTED((uintptr_t)x % 16 == 0 && (uintptr_t)Wp % 16 == 0 && (uintptr_t)workspace % 16 == 0,
                  "gorch_hip_linear_mxfp4: x, Wp and the workspace must be 16-byte aligned");
-    GH_SUPPORTED(M <= 1 << 20 && N <= 16 * 65535 && K <= 1 << 24, "gorch_hip_linear_mxfp4: M, N or K out of range");
+    GH_SUPPORTED(M <= 16 * 65535 && N <= 16 * 65535 && K <= 1 << 24, "gorch_hip_linear_mxfp4: M, N or K out of range");
     const size_t need = M <= 16 ? gemv_plan(M, N, K).bytes : terms_bytes(M, K);
     GH_REQUIRE(workspace_bytes >= need && (workspace || need == 0), "gorch_hip_linear_mxfp4: workspace too small");
     hipStream_t s = stream_of(stream);
@@ -742,9 +748,8 @@ extern "C" int gorch_hip_linear_mxfp4(void* stream, const float* x, const void* 
     a.nq = (a.nk + 3) / 4;
     a.wp = static_cast<const u32x4*>(Wp);
     a.wsc = reinterpret_cast<const uint32_t*>(static_cast<const char*>(Wp) + (size_t)a.nt * a.nk * 1024);
-    a.terms = static_cast<char*>(workspace);
     if (M <= 16) GH_TRY(launch_mx_gemv(s, a, static_cast<char*>(workspace)));
-    else GH_TRY(launch_mx_gemm(s, a));
+    else GH_TRY(launch_mx_gemm(s, a, static_cast<char*>(workspace)));
     count(M <= 16 ? CNT_GEMV : CNT_GEMM);
     return finish(stream, check_launch("linear_mxfp4"));
 }

@@ -487,7 +487,7 @@ const char* gorch_hip_kernel_choice(const char* op, const int* d, int n) {
     const auto is = [&](const char* name, int count) { return n == count && !strcmp(op, name); };
     if (is("linear", 4) && d[0] > 0 && d[1] > 0)
         return gemm_choice_name(d[0], d[1], d[2], (d[3] & GORCH_HIP_LINEAR_ACT_BF16) != 0);
-    if (is("linear_mxfp4", 3) && d[0] > 0 && d[0] <= 1 << 20 && d[1] > 0 && d[1] <= 16 * 65535 && d[2] > 0 && d[2] <= 1 << 24 &&
+    if (is("linear_mxfp4", 3) && d[0] > 0 && d[0] <= 16 * 65535 && d[1] > 0 && d[1] <= 16 * 65535 && d[2] > 0 && d[2] <= 1 << 24 &&
         d[2] % 8 == 0)
         return mx_linear_choice_name(d[0], d[1], d[2]);
     if (is("gate_up", 3) && d[0] > 16 && d[1] > 0 && d[1] < 1 << 30)

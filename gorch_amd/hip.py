@@ -504,19 +504,20 @@ def linear_mxfp4_workspace(M, N, K):
 def linear_mxfp4(x, Wp, N, bias, y, residual=None, epilogue=EPI_NONE, ws=None) -> None:
     """gorch_hip_linear_mxfp4: y = residual + epi(x @ W^T + bias) over a
     pack_mxfp4 weight of N rows; x [M, K] and y [M, N] f32. ws from
-    linear_mxfp4_workspace for these sizes, whose calls leave it as they need it
-    (a new one if None); calls that can overlap must not share it."""
+    linear_mxfp4_workspace for these sizes or larger needs (a new one if None),
+    for one call after another: calls that can overlap must not share it."""
+    import torch
+
     dev = _device()
     if x.dim() != 2:
         raise ValueError("gorch_amd.hip: x must be [M, K]")
     M, K = x.shape
     if ws is None:
         ws = linear_mxfp4_workspace(M, N, K)
-    elif ws.get_device() != dev:
-        raise ValueError("gorch_amd.hip: ws is not on the current device")
-    if Wp.get_device() != dev or Wp.numel() * Wp.element_size() != lib().gorch_hip_packed_mxfp4_bytes(N, K):
-        raise ValueError(f"gorch_amd.hip: Wp must be a packed weight [{N}, {K}] on the current device")
-    _ok(lib().gorch_hip_linear_mxfp4(_stream(), _typed(x, _f32_t, (M, K), "x", dev), _p(Wp),
+    elif ws.get_device() != dev or not ws.is_contiguous():
+        raise ValueError("gorch_amd.hip: ws must be contiguous, on the current device")
+    w = _typed(Wp, torch.uint8, (lib().gorch_hip_packed_mxfp4_bytes(N, K),), "Wp", dev)
+    _ok(lib().gorch_hip_linear_mxfp4(_stream(), _typed(x, _f32_t, (M, K), "x", dev), w,
                                      _typed(bias, _f32_t, (N,), "bias", dev),
                                      _typed(residual, _f32_t, (M, N), "residual", dev),
                                      _typed(y, _f32_t, (M, N), "y", dev), M, N, K, epilogue, _p(ws),

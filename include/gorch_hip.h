@@ -173,9 +173,10 @@ int gorch_hip_f32_to_bf16(void* stream, const float* in, uint16_t* out, int64_t 
  * of 8, rows * cols at most 2^40 (else GORCH_HIP_EUNSUPPORTED).
  * Encoding takes the smallest scale that the group's largest magnitude exceeds
  * at most 7 times and rounds to the nearest code, ties to even: half a step at
- * most, everywhere. A group below 2^-100 throughout becomes zeros (s = 0), one
+ * most. A group below 2^-100 throughout becomes zeros (s = 0), one
  * that holds an infinity or NaN becomes NaN (s = 255). Decoding is exact in f32
- * and in bf16. The values are f32, or with the flag bf16, in rows that begin at
+ * and in bf16; what lies past their range (of groups beyond 2.97e38, whose codes
+ * may stand for 2^128, and of scales 253 and 254) is infinite. The values are f32, or with the flag bf16, in rows that begin at
  * multiples of the stride (in elements); rows are 16-byte and codes 4-byte
  * aligned. */
 int gorch_hip_mxfp4_encode(void* stream, const void* in, int in_bf16, int64_t in_stride, uint8_t* codes,
@@ -261,15 +262,16 @@ int gorch_hip_pack_mxfp4(void* stream, const uint8_t* codes, const uint8_t* scal
 /* gorch_hip_linear_bf16 (nn/module.go:61-88) over a weight in MXFP4, for any
  * number of rows: y[m,n] = residual[m,n] + epi(sum_k x[m,k] W[n,k] + bias[n])
  * with the weight's values exact and x held to 2^-24 of the largest magnitude
- * among each 32 of a row's columns (k / 32), products and sums in f32: f32
+ * among each 32 of a row's columns (k / 32) or to 2^-130, products and sums in f32: f32
  * accuracy, in a fixed order of sums. An infinity or NaN in x makes its row of
  * y NaN, a NaN group of W its column. bias and residual may be NULL; residual
- * may alias y, x must not. K % 8 == 0, M up to 2^20, K up to 2^24, x, Wp and
+ * may alias y, x must not. K % 8 == 0, M up to 2^20 - 16, K up to 2^24, x, Wp and
  * the workspace 16-byte aligned (else GORCH_HIP_EUNSUPPORTED). The workspace
  * (gorch_hip_linear_mxfp4_workspace_size bytes of device memory; NULL where
- * that is 0) is the caller's: zeroed before its first use with these M, N and
- * K (with up to 16 rows it holds counters, zero again after every call), and
- * not shared by calls that can overlap. Nothing is allocated, so the call can
+ * that is 0) is the caller's: zeroed before its first use, after which it may
+ * serve calls of any sizes that it is large enough for, one after another (its
+ * first 512 bytes are counters, zero again after every call), but not calls
+ * that can overlap. Nothing is allocated, so the call can
  * be captured. */
 size_t gorch_hip_linear_mxfp4_workspace_size(int M, int N, int K);
 int gorch_hip_linear_mxfp4(void* stream, const float* x, const void* Wp, const float* bias, const float* residual,
@@ -489,7 +491,9 @@ int gorch_hip_qwen_generate_sampled(void* stream, gorch_hip_qwen* m, const int* 
  * unused with GORCH_HIP_KV_BF16). With GORCH_HIP_KV_MXFP4 k and v are
  * [num_pages][num_kv][page_size][head_dim / 2] bytes of codes as
  * gorch_hip_mxfp4_encode writes rows of head_dim, and k_scale and v_scale point
- * at bytes, [num_pages][num_kv][page_size][ceil(head_dim / 32)]. head_dim is a multiple of 16 up to 256,
+ * at bytes, 4-byte aligned, [num_pages][num_kv][page_size][ceil(head_dim /
+ * 32)]; attention takes V's codes of scale byte 0 (below 2^-124) as zeros.
+ * head_dim is a multiple of 16 up to 256,
  * num_kv below 2^16 (else GORCH_HIP_EUNSUPPORTED); page_size is any positive
  * number. */
 typedef struct {

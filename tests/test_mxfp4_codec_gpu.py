@@ -136,3 +136,34 @@ def test_pack_holds_every_code_once(gpu, N, K):
     s = s.reshape(nt, 16, nq, 4, 4)  # tile, row, word, column tile of it, group
     np.testing.assert_array_equal(got[:nt * nk * 1024], c.transpose(0, 2, 3, 1, 4).ravel())
     np.testing.assert_array_equal(got[nt * nk * 1024:], s.transpose(0, 2, 4, 1, 3).ravel())
+
+
+def test_on_another_stream_and_captured(gpu):
+    x = rows(np.random.default_rng(5), 40, 520, False)
+    xd, back = dev(x), torch.zeros((40, 520), device="cuda")
+    codes, scales = (torch.zeros((40, n), dtype=torch.uint8, device="cuda") for n in (260, 17))
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=side):
+        gpu.mxfp4_encode(xd, codes, scales)
+        gpu.mxfp4_decode(codes, scales, back)
+    for turn in range(3):
+        y = np.roll(x, turn, 0)
+        xd.copy_(dev(y))
+        back.zero_()
+        graph.replay()
+        np.testing.assert_array_equal(host(back).astype(np.float64), values(*encode(y)))
+
+
+def test_refusals(gpu):
+    x = torch.zeros((4, 64), device="cuda")
+    codes, scales = (torch.zeros((4, n), dtype=torch.uint8, device="cuda") for n in (32, 2))
+    for call in (lambda *a: gpu.mxfp4_encode(*a), lambda v, c, s: gpu.mxfp4_decode(c, s, v)):
+        call(x, codes, scales)
+        for bad in ((x.half(), codes, scales), (x.cpu(), codes, scales), (x[:, ::2], codes[:, :16], scales[:, :1]),
+                    (x[0], codes, scales), (x, codes[:, :31], scales), (x, codes, scales[:, :1]), (x, codes.int(), scales),
+                    (x, codes, scales.cpu()), (x[:1].expand(4, 64), codes, scales)):
+            with pytest.raises((ValueError, TypeError)):
+                call(*bad)
+        with pytest.raises(Exception, match="multiple of 8"):
+            call(x[:, :60], codes[:, :30].contiguous(), scales)

@@ -217,3 +217,69 @@ def test_reaches_past_32_bit_offsets(gpu):
         check(got[1], want[1], tol[1])
         check(got[0], want[0 if rows == M else 1], tol[0 if rows == M else 1])
         assert int(y[rows - 1].count_nonzero()) <= len(some)
+
+
+def test_one_workspace_for_all_sizes(gpu):
+    # counters, terms and partial sums of one size are no part of the next
+    sizes = [(2, 300, 9000), (40, 90, 5160), (16, 1000, 9000), (1, 64, 128), (4, 300, 6000), (70, 33, 9000), (13, 500, 2048),
+             (2, 300, 9000), (1, 20, 20000), (16, 1000, 9000)]
+    spaces = [gpu.linear_mxfp4_workspace(*s) for s in sizes]
+    ws = max((w for w in spaces if w is not None), key=lambda w: w.numel())
+    for seed, (M, N, K) in enumerate(sizes):
+        rng, x, codes, scales = inputs(seed, M, N, K)
+        check(call(gpu, x, codes, scales, ws=ws), *expected(x, codes, scales))
+        assert not ws[:512].any()
+
+
+@pytest.mark.parametrize("M", [1, 5, 16, 40])
+@pytest.mark.parametrize("lo,hi", [(0, 12), (240, 252)])
+def test_extreme_scales(gpu, M, lo, hi):
+    # weights at both ends of their range, against x of the other end
+    rng = np.random.default_rng(M)
+    N, K = 40, 264
+    codes = rng.integers(0, 256, (N, K // 2)).astype(np.uint8)
+    scales = rng.integers(lo, hi, (N, -(-K // GROUP))).astype(np.uint8)
+    x = (rng.standard_normal((M, K)) * 2.0 ** (100 if lo == 0 else -90)).astype(np.float32)
+    check(call(gpu, x, codes, scales), *expected(x, codes, scales))
+
+
+def test_two_graphs_at_once(gpu):
+    parts = []
+    for seed, (M, N, K) in enumerate([(2, 300, 9000), (16, 1000, 9000), (100, 300, 2520)]):
+        rng, x, codes, scales = inputs(seed, M, N, K)
+        Wp, y, ws = gpu.pack_mxfp4(dev(codes), dev(scales)), torch.zeros((M, N), device="cuda"), gpu.linear_mxfp4_workspace(M, N, K)
+        parts.append([dev(x), Wp, y, ws, expected(x, codes, scales), torch.cuda.CUDAGraph(), torch.cuda.Stream()])
+    torch.cuda.synchronize()
+    for x, Wp, y, ws, _, graph, side in parts:
+        with torch.cuda.graph(graph, stream=side):
+            gpu.linear_mxfp4(x, Wp, y.shape[1], None, y, ws=ws)
+    for _ in range(3):
+        for p in parts:
+            p[2].zero_()
+        torch.cuda.synchronize()
+        for *_, graph, side in parts:
+            with torch.cuda.stream(side):
+                graph.replay()
+        torch.cuda.synchronize()
+        for p in parts:
+            check(host(p[2]), *p[4])
+
+
+def test_refusals(gpu):
+    rng, x, codes, scales = inputs(0, 20, 48, 64)
+    Wp, xd, y = gpu.pack_mxfp4(dev(codes), dev(scales)), dev(x), torch.zeros((20, 48), device="cuda")
+    ws = gpu.linear_mxfp4_workspace(20, 48, 64)
+    good = dict(x=xd, Wp=Wp, N=48, bias=None, y=y, ws=ws)
+    gpu.linear_mxfp4(**good)
+    for over in (dict(x=xd.half()), dict(x=xd[0]), dict(x=xd.t()), dict(x=xd.cpu()), dict(Wp=Wp[:-1]), dict(Wp=Wp.cpu()),
+                 dict(Wp=Wp.view(torch.float32)), dict(N=64), dict(y=y[:, :40]), dict(y=y.double()), dict(bias=y[0, :40]),
+                 dict(residual=y.t()), dict(ws=ws.cpu()), dict(ws=torch.zeros(1, dtype=torch.uint8, device="cuda").expand(1 << 20))):
+        with pytest.raises((ValueError, TypeError)):
+            gpu.linear_mxfp4(**{**good, **over})
+    for over in (dict(ws=ws[:-16]), dict(epilogue=7)):
+        with pytest.raises(Exception, match="linear_mxfp4"):
+            gpu.linear_mxfp4(**{**good, **over})
+    with pytest.raises(ValueError):
+        gpu.pack_mxfp4(dev(codes), dev(scales)[:, :1])
+    for sizes in ((0, 16, 64), (1, 0, 64), (1, 16, 60), (1, 16, 0), (1 << 20, 16, 64), (1, 1 << 20, 64)):
+        assert gpu.kernel_choice("linear_mxfp4", *sizes) is None
