@@ -33,6 +33,8 @@ int paged_args(const char* who, const gorch_hip_paged_kv* kv, const gorch_hip_pa
             return fail(GORCH_HIP_EINVAL, "null pool or batch array");
         if (kv->dtype != GORCH_HIP_KV_BF16 && (!kv->k_scale || !kv->v_scale))
             return fail(GORCH_HIP_EINVAL, "e4m3 and MXFP4 pools need k_scale and v_scale");
+        if (kv->dtype == GORCH_HIP_KV_MXFP4 && (!aligned(kv->k_scale, 4) || !aligned(kv->v_scale, 4)))
+            return fail(GORCH_HIP_EUNSUPPORTED, "MXFP4 scales must be 4-byte aligned");
         if (!aligned(kv->k, 16) || !aligned(kv->v, 16)) return fail(GORCH_HIP_EUNSUPPORTED, "pools must be 16-byte aligned");
     }
     a.k = kv->k;

@@ -99,8 +99,27 @@ struct MxScales {
         }
     }
 };
+// The nibbles of codes that scale byte s takes past f32: 4 and 6 of 253, 2 to 6
+// of 254, all of 255.
+__device__ __forceinline__ uint32_t mx_past(uint32_t w, uint32_t s) {
+    const uint32_t m = s == 253 ? w >> 2 & w >> 1 : (s == 254 ? w >> 2 : (s == kMxNaN ? ~0u : 0u));
+    return (m & 0x11111111u) * 15u;
+}
+// A lane's codes as a tile of values holds them, and true where some are
+// infinite or NaN (zeros are left, since a weight of 0 would make them NaN).
+__device__ __forceinline__ bool mx_finite(u32x4& c, uint32_t s) {
+    if (!__any(s >= 253)) return false;
+    uint32_t past = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t p = mx_past(c[i], s);
+        past |= p;
+        c[i] &= ~p;
+    }
+    return past != 0;
+}
 // A value's pieces to its place (key `key`) of a tile in LDS as bf16; true
-// where its scale is NaN (zeros are written).
+// where some are not finite.
 template <int HD>
 __device__ __forceinline__ bool mx_put(const MxRow<HD>& r, char* vt, int key, int lane) {
     const int g = lane >> 4;
@@ -108,32 +127,43 @@ __device__ __forceinline__ bool mx_put(const MxRow<HD>& r, char* vt, int key, in
 #pragma unroll
     for (int u = 0; u < MxTile<HD>::NU; u++) {
         if (HD < 128 && g >= HD / 32) continue;
-        const bool nan = r.s[u] == kMxNaN, none = nan || r.s[u] == 0;
-        odd |= nan;
+        u32x4 codes = r.c[u];
+        odd |= mx_finite(codes, r.s[u]);
+        const bool none = r.s[u] == kMxNaN || r.s[u] == 0;
         const float s = __uint_as_float(none ? 0x3f800000u : r.s[u] << 23);
         const uint32_t keep = none ? 0u : ~0u;  // (a mask: a choice per word becomes a branch)
         char* to = vt + (key >> 4) * MxTile<HD>::GROUP + (4 * u + g) * 1024 + (key & 15) * 16;
 #pragma unroll
-        for (int i = 0; i < 4; i++) *reinterpret_cast<u32x4*>(to + i * 256) = mx_widen8(r.c[u][i] & keep, s);
+        for (int i = 0; i < 4; i++) *reinterpret_cast<u32x4*>(to + i * 256) = mx_widen8(codes[i] & keep, s);
     }
     return odd;
 }
-// NaN groups of a value (key `key`) noted for every row that sees it.
+// The values that are not finite of a group of 32 (the word-th; of key `key`,
+// codes c, scale byte s) noted for every row that sees them.
 template <int BM, int HD>
 __device__ __forceinline__ void mx_note(OddBits<BM, HD>& odd, const PagedAttnArgs& a, const SeqAt& s, int r0, int key,
-                                        const uint32_t (&scale)[MxTile<HD>::NU], int g) {
+                                        u32x4 c, uint32_t scale, int word) {
+    if (scale < 253 || word >= HD / 32) return;
     const int G = a.group.d, n = s.end - s.begin;
+    uint32_t up = 0, down = 0;
 #pragma unroll
-    for (int u = 0; u < MxTile<HD>::NU; u++) {
-        if (scale[u] != kMxNaN || 4 * u + g >= HD / 32) continue;
-        odd.any = 1;
+    for (int i = 0; i < 4; i++) {
+        const uint32_t past = mx_past(c[i], scale);
 #pragma unroll 1
-        for (int r = 0; r < BM && r0 + r < n * G; r++) {
-            const int pos = a.causal ? s.len - n + (int)a.group.div((uint32_t)(r0 + r)) : s.len - 1;
-            if (key > pos) continue;
-            atomicOr(&odd.bits[0][r][4 * u + g], ~0u);
-            atomicOr(&odd.bits[1][r][4 * u + g], ~0u);
+        for (int e = 0; e < 8; e++) {
+            const uint32_t bit = (past >> 4 * e & 1u) << (8 * i + e);
+            const bool neg = (c[i] >> (4 * e + 3) & 1u) != 0;
+            up |= neg && scale != kMxNaN ? 0u : bit;
+            down |= neg || scale == kMxNaN ? bit : 0u;
         }
+    }
+    odd.any = 1;
+#pragma unroll 1
+    for (int r = 0; r < BM && r0 + r < n * G; r++) {
+        const int pos = a.causal ? s.len - n + (int)a.group.div((uint32_t)(r0 + r)) : s.len - 1;
+        if (key > pos) continue;
+        atomicOr(&odd.bits[0][r][word], up);
+        atomicOr(&odd.bits[1][r][word], down);
     }
 }
 
@@ -413,8 +443,12 @@ __device__ __forceinline__ void mx_few_tile(const PagedAttnArgs& a, const SeqAt&
             for (int j = 0; j < 2; j++) nan |= mx_put<HD>(b.v[j], vt, 16 * j + (lane & 15), lane);
             if (__any(nan)) {
                 // (a dynamic choice of the rows themselves would put them into scratch memory)
-                if (here >> (lane & 15) & 1u) mx_note<CW, HD>(odd, a, s, r0, key + (lane & 15), b.v[0].s, g);
-                if (here >> (16 + (lane & 15)) & 1u) mx_note<CW, HD>(odd, a, s, r0, key + 16 + (lane & 15), b.v[1].s, g);
+#pragma unroll
+                for (int u = 0; u < MxTile<HD>::NU; u++) {
+                    const int w = 4 * u + g, c = lane & 15;
+                    if (here >> c & 1u) mx_note<CW, HD>(odd, a, s, r0, key + c, b.v[0].c[u], b.v[0].s[u], w);
+                    if (here >> (16 + c) & 1u) mx_note<CW, HD>(odd, a, s, r0, key + 16 + c, b.v[1].c[u], b.v[1].s[u], w);
+                }
             }
         }
         const int after = key_page(a.p, s.s, key + (NB + 1) * STEP + mine);
@@ -620,22 +654,14 @@ __device__ __forceinline__ void mx_many_block(const PagedAttnArgs& a, int block,
             sh.ks[b][(j * NU + u) * 64 + lane] = (uint8_t)raw.s[0];
             if (lane == 0 && u == 0) sh.seen_of[b][j] = here;
         } else if (HD >= 128 || g < HD / 32) {
-            const bool nan = raw.s[0] == kMxNaN, none = nan || raw.s[0] == 0;
+            u32x4 codes = raw.c[0];
+            const bool far = mx_finite(codes, raw.s[0]), none = raw.s[0] == kMxNaN || raw.s[0] == 0;
             const float f = __uint_as_float(none ? 0x3f800000u : raw.s[0] << 23);
             const uint32_t keep = none ? 0u : ~0u;
             char* to = sh.vt[b] + j * MxTile<HD>::GROUP + (4 * u + g) * 1024 + (lane & 15) * 16;
 #pragma unroll
-            for (int i = 0; i < 4; i++) *reinterpret_cast<u32x4*>(to + i * 256) = mx_widen8(raw.c[0][i] & keep, f);
-            if (nan) {
-                sh.odd.any = 1;
-#pragma unroll 1
-                for (int r = 0; r < BM && r0 + r < n * G; r++) {
-                    const int pos = a.causal ? s.len - n + (int)a.group.div((uint32_t)(r0 + r)) : s.len - 1;
-                    if (key0 + 16 * j + (lane & 15) > pos) continue;
-                    atomicOr(&sh.odd.bits[0][r][4 * u + g], ~0u);
-                    atomicOr(&sh.odd.bits[1][r][4 * u + g], ~0u);
-                }
-            }
+            for (int i = 0; i < 4; i++) *reinterpret_cast<u32x4*>(to + i * 256) = mx_widen8(codes[i] & keep, f);
+            if (far) mx_note<BM, HD>(sh.odd, a, s, r0, key0 + 16 * j + (lane & 15), raw.c[0], raw.s[0], 4 * u + g);
         }
     };
     MxRowsOf<HD, NR> rows;

@@ -79,7 +79,8 @@ MX = dict(dtype=2, k_scale=FAKE, v_scale=FAKE)
 
 
 @pytest.mark.parametrize("over,rc", [(dict(k_scale=None), 2), (dict(v_scale=None), 2), (dict(head_dim=72), 1),
-                                     (dict(head_dim=272), 1), (dict(k=ODD), 1), (dict(dtype=3), 2), (dict(dtype=-1), 2)])
+                                     (dict(head_dim=272), 1), (dict(k=ODD), 1), (dict(k_scale=FAKE + 2), 1),
+                                     (dict(v_scale=FAKE + 1), 1), (dict(dtype=3), 2), (dict(dtype=-1), 2)])
 def test_cache_refusals(over, rc):
     kv, b = cache(**{**MX, **over}), batch()
     w = heads(head_dim=kv.head_dim, num_kv=kv.num_kv)

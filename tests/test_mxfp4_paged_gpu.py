@@ -89,7 +89,7 @@ def test_append_of_extremes(gpu):
         np.testing.assert_array_equal(host(got), values(*encode(y)).astype(np.float32))
 
 
-@pytest.mark.parametrize("hkv,hd", [(8, 128), (2, 64), (1, 256), (2, 96), (1, 80), (3, 16), (2, 48)])
+@pytest.mark.parametrize("hkv,hd", [(8, 128), (2, 64), (1, 256), (2, 96), (1, 80), (3, 16), (2, 48), (4, 128), (6, 64)])
 @pytest.mark.parametrize("seqs", [[(40, 7), (0, 0), (130, 130)], [(3000, 2990), (2500, 2500)]])
 def test_read_is_exact(gpu, hkv, hd, seqs):
     c = MxCase(hkv, hd, 24, seqs, seed=hd)
@@ -167,6 +167,41 @@ def test_nan_keys_and_values_stay_with_who_sees_them(gpu, hq, hkv, hd, length, n
     assert np.isnan(got[k_from:n]).all()
 
 
+@pytest.mark.parametrize("hq,hkv,hd,length,n", [(4, 2, 64, 90, 20), (4, 2, 128, 300, 200), (2, 1, 256, 40, 40),
+                                                (2, 1, 80, 70, 5), (32, 4, 64, 100, 3)])
+def test_infinite_values_stay_in_their_columns(gpu, hq, hkv, hd, length, n):
+    # 4 * 2^126 and 2 * 2^127 are past f32; their groups' other codes, and the rows before them, are not
+    c = MxCase(hkv, hd, 16, [(length, n), (50, 1)], seed=14)
+    q = queries(c, hq) / 8  # (weights that do not vanish)
+    g = c.vs.shape[-1] - 1
+    at = [length - n + n // 2, length - n // 3 - 1]
+    for p, scale, code in ((at[0], 253, 0x6f), (at[1], 254, 0x34)):
+        c.v[c.slot(0, p)][:, 16 * g:] = 0  # the group is zeros but for two columns
+        c.v[c.slot(0, p)][:, 16 * g + 2] = code
+        c.vs[c.slot(0, p)][:, g] = scale
+    got = attend(gpu, c, q, hq)
+    # without what is infinite (0x34: 2 * 2^127 is, 1.5 * 2^127 is not; 0x6f: -6 and 4, times 2^126)
+    for p, scale, code in ((at[0], 253, 0), (at[1], 254, 0x30)):
+        c.v[c.slot(0, p)][:, 16 * g:] = 0
+        c.v[c.slot(0, p)][:, 16 * g + 2] = code
+        c.vs[c.slot(0, p)][:, g] = scale
+    want, tol = c.attention(q, hq)
+    first, second = (p - (length - n) for p in at)
+    if first == second:
+        first = n  # (3 rows: the later write is the only one)
+    a, b = 32 * g + 4, 32 * g + 5
+    for r in range(n):
+        row = np.ones(hd, bool)
+        row[a], row[b] = r < min(first, second), r < first
+        check(got[r][:, row], want[r][:, row], tol[r][:, row])
+        if r >= min(first, second):
+            is_a = np.isposinf if r < first else (np.isneginf if r < second else np.isnan)
+            assert is_a(got[r, :, a]).all()
+        if r >= first:
+            assert np.isposinf(got[r, :, b]).all()
+    check(got[n:], want[n:], tol[n:])
+
+
 def test_large_magnitudes(gpu):
     # scales at the ends of f32's range where their products stay inside it, and scale 0, whose values count as zeros
     c = MxCase(1, 64, 16, [(100, 1), (90, 60)], seed=9)
@@ -233,3 +268,40 @@ def test_append_then_attend_then_read(gpu):
     want, tol = c.attention(host(q_out).reshape(T, hq, hd), hq)
     check(host(out).reshape(T, hq, hd), want, tol)
     check(host(stream), *expected(host(out), *wo, residual=x))
+
+
+def test_on_another_stream(gpu):
+    c = MxCase(2, 64, 16, [(600, 1), (90, 40)], seed=12)
+    q = queries(c, 4)
+    kv, b = c.cache(gpu), c.batch(gpu)
+    qd, out = dev(q.reshape(c.tokens, -1)), torch.zeros((c.tokens, 256), device="cuda")
+    ko, vo = (torch.zeros((c.tokens, 128), device="cuda") for _ in "kv")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        kv.attention(b, qd, out)
+        kv.read(b, ko, vo)
+    side.synchronize()
+    want, tol = c.attention(q, 4)
+    check(host(out).reshape(want.shape), want, tol)
+    for got, which in ((ko, "k"), (vo, "v")):
+        rows = np.concatenate([c.rows(which, s)[0][n - m:] for s, (n, m) in enumerate(c.seqs)])
+        np.testing.assert_array_equal(host(got).reshape(rows.shape), rows.astype(np.float32))
+
+
+def test_refusals(gpu):
+    k = torch.zeros((4, 2, 16, 32), dtype=torch.uint8, device="cuda")
+    s = torch.zeros((4, 2, 16, 2), dtype=torch.uint8, device="cuda")
+    gpu.PagedKV(k, k, s, s)
+    for bad in (s[..., :1], s.int(), s.cpu(), torch.zeros((4, 2, 16), dtype=torch.uint8, device="cuda")):
+        with pytest.raises((ValueError, TypeError)):
+            gpu.PagedKV(k, k, s, bad)
+    with pytest.raises(ValueError):
+        gpu.PagedKV(k, k, s)
+    with pytest.raises(ValueError):
+        gpu.PagedKV.new(4, 16, 2, 64, "fp4")
+    c = MxCase(2, 64, 16, [(5, 1)])
+    kv, b = c.cache(gpu), c.batch(gpu)
+    apart = torch.zeros(kv.k_scale.numel() + 2, dtype=torch.uint8, device="cuda")[2:].view(kv.k_scale.shape)
+    with pytest.raises(Exception, match="4-byte"):
+        gpu.PagedKV(kv.k, kv.v, apart, kv.v_scale).read(b, torch.zeros((1, 128), device="cuda"), None)
