@@ -64,7 +64,9 @@ __device__ __forceinline__ void mx_store(const MxLinearArgs& a, int m, int n, fl
 // lane order; in row tile, column tile order.
 constexpr int kTermBytes = 8192, kTerm8 = kMxTerms * 1024, kTermScale = kTerm8 + kMxTerms * 512;
 // (Rows go through LDS: a lane's 128 bytes straight from memory would take 64
-// lines a load, eight times.)
+// lines a load, eight times.) Bound by memory: 2,000 x 4,096 12.2 us, 64 MB at
+// the rate of a large copy (blocks that multiply would each split the same rows
+// again).
 __global__ __launch_bounds__(256) void k_mx_terms(MxLinearArgs a) {
     constexpr int ROW = 132;
     __shared__ __align__(16) float xs[4][16 * ROW];
@@ -102,7 +104,8 @@ __global__ __launch_bounds__(256) void k_mx_terms(MxLinearArgs a) {
     }
     *reinterpret_cast<u32x2*>(to + kTermScale + lane * 8) = u32x2{r.scale, r.last};
 }
-// The same for up to 16 rows, where it is waited for: a wave a term.
+// The same for up to 16 rows, where it is waited for: a wave a term. 16 x 1,600
+// 3.6 us, of which a launch's latency is the most.
 __global__ __launch_bounds__(64 * kMxTerms) void k_mx_terms16(MxLinearArgs a) {
     const int lane = threadIdx.x & 63, q = threadIdx.x >> 6, j = blockIdx.x;
     uint32_t s;
@@ -118,8 +121,11 @@ __global__ __launch_bounds__(64 * kMxTerms) void k_mx_terms16(MxLinearArgs a) {
 // columns and 8 / WK along the row tiles, stream 1 KB of codes a step into one
 // instruction (kRow1: up to 3 rows, whose terms are rows of one operand) or
 // five. For many columns of more rows another kernel has made the terms
-// (kMade), which are loaded. The last block of a slice's fellows to finish adds up the slices, in
-// their order.
+// (kMade), which are loaded. The last of a row tile's blocks to finish adds up
+// the slices, in their order. The floor is the weight's bytes: 1 x 1,024 x
+// 151,936 16.2 us (5.1 TB/s of 83 MB); of small weights it is a chain of loads
+// and a split: 1 x 1,024 x 4,096 4.5 us; 16 x 1,600 x 6,400 5.8 us after 3.6 for
+// the terms (34 us when each block split all of x).
 constexpr int kGemvWaves = 8;
 constexpr int kGemvSlices = 16;
 enum GemvKind { kRow1, kFive, kMade };
@@ -377,7 +383,11 @@ __global__ __launch_bounds__(64 * kGemvWaves, 2) void k_mx_gemv(MxLinearArgs a) 
 // the next tile's first codes from LDS before the block meets. A row tile's five
 // products follow each other, which leaves two of three operands where they are
 // (on all CUs the matrix cores run at what power allows, 6.2 PFLOP/s with the
-// terms outermost, 6.9 so).
+// terms outermost, 6.9 so). 2,000 x 4,096 x 4,096 82 to 89 us (174 with x split by
+// every block and one buffer): five products of 67 GFLOP, 49 us at 6.9 PFLOP/s;
+// the rest is waits for x's terms, 64 KB a step and CU, each used 16 times. A
+// larger tile would use them more often, but sums and three sets of operands
+// take 320 of a lane's 512 registers already.
 template <int MT, int NT, int WM>
 struct GemmLds {
     static constexpr int WK = 8 / MT / WM, STAGE = NT * 1024, WORDS = (NT + 3) / 4 * 1024;

@@ -165,8 +165,10 @@ struct AppendArgs {
 // Bound by memory: the rows go out before anything else, and the chain
 // sequence -> page -> store runs beside them. Large calls (P > 1) read them
 // past the caches: 15,518 tokens of 14 + 2 + 2 heads of 64 into e4m3 38.7 ->
-// 35.5 us (3.8 TB/s; two or four tokens a block: 39.4, 46). One token 3.6 us
-// on the GPU.
+// 35.5 us (3.8 TB/s; two or four tokens a block: 39.4, 46), into MXFP4 31. One
+// token 3.6 us on the GPU, 64 of 16 + 8 + 8 heads of 128 into MXFP4 4.1. (In
+// MXFP4 codes leave as two bytes a lane and scales as a byte of every eighth:
+// 136 of the 3,720 bytes that a token of the 14 + 2 + 2 heads writes.)
 template <int KV, int NL, bool FULL, int P>
 __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
 #pragma clang fp contract(off)
@@ -269,7 +271,8 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
 // few tokens have one a block (1,000 in bf16 4.3 us against 5.0). Heads that
 // need fewer than 256 threads a token share the block between tokens, LG lanes
 // a token: 15,518 tokens of 2 x 64 in MXFP4 12.6 -> 9.9 us with four tokens in
-// turn, 7.1 with one (its lookups then overlap between waves).
+// turn, 7.1 with one (its lookups then overlap between waves). Two tokens a wave
+// look up twice: few tokens have a wave each (976 of 2 x 64 3.1 us, else 3.4).
 template <int KV, int TOK, int LG>
 __global__ __launch_bounds__(256) void k_paged_read(PagedArgs p, float* ko, float* vo) {
     constexpr int S = LG < 64 ? 64 / LG : 1;  // tokens side by side in a wave
@@ -414,7 +417,7 @@ extern "C" int gorch_hip_paged_read(void* stream, const gorch_hip_paged_kv* kv, 
         p.tokens * (LG / 32) < 32768 ? go(k_paged_read<KV, 1, LG>, 1, LG) : go(k_paged_read<KV, 4, LG>, 4, LG);
     };
     const auto by = [&](auto kind) {
-        if (n4 <= 32) of(kind, std::integral_constant<int, 32>{});
+        if (n4 <= 32 && p.tokens > 4096) of(kind, std::integral_constant<int, 32>{});
         else if (n4 <= 64) of(kind, std::integral_constant<int, 64>{});
         else if (n4 <= 128) of(kind, std::integral_constant<int, 128>{});
         else of(kind, std::integral_constant<int, 256>{});

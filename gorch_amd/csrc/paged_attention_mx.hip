@@ -247,7 +247,7 @@ struct MxFewRows : FewRows<false, HD, 16> {
 // + 3 of one operand and its fifth as row 4 g of another, so that a lane (g, c)
 // adds up the score of row g and key c itself and a tile's 32 keys are two
 // scores a lane (as columns of the other form they would be eight, each four
-// times over: 57 -> 44 us for 64 conversations of up to 8,192 tokens). The
+// times over: 57 -> 42 us for 64 conversations of up to 8,192 tokens). The
 // weights' three bf16 terms then go through LDS to their places in P^T: column
 // 4 t + g of the operand holds term t of row g; lanes c and c + 1 first trade
 // one of their two weights, so that each has two neighbours there. (A numbering
@@ -369,7 +369,11 @@ struct MxFour {
     }
 };
 
-// Few rows: as k_paged_attn_few, the values widened on their way to LDS.
+// Few rows: as k_paged_attn_few, the values widened on their way to LDS. The
+// floor is the codes: 64 tokens over 187,323 keys of 8 x 128 42 to 44 us (4.6 TB/s
+// of 197 MB), where e4m3's 386 MB take 100. Two tiles are on their way; three
+// and four were no faster (48.6, 48.1 us with the join against 46.3). One token
+// over 777 keys 6.0 us, a chain of loads (page, keys, join).
 template <int HD, bool PART, int CW>
 struct MxFewBlock {
     static constexpr int NW = 4, NB = 2, OROW = HD + 4, PT = CW == 4 ? 1024 : 0;
@@ -599,7 +603,13 @@ struct MxRowsOf : Rows<false, HD, NR> {
 // Many rows: 128 rows of a sequence a block, 16 NR a wave, tiles of 32 keys
 // that all waves read from LDS. Waves 0 and 1 (of each step of 128 columns)
 // fetch the keys' two groups, 2 and 3 the values', into registers a tile ahead
-// and from there to the other of two stages, the values widened.
+// and from there to the other of two stages, the values widened. Bound by issue: for
+// 2,048 tokens over 16,384 keys of 8 x 128 (16 query heads), 560 us or 0.46 PFLOP/s
+// of the product, vector instructions (exponentials, the weights' three terms,
+// LDS addresses) fill 59% of the cycles and matrix instructions 42%, one after
+// the other in a wave and hardly side by side between a SIMD's two. A third
+// stage with the next tile's scores computed ahead of this one's weights did
+// not change that (543 us against 540 with the join).
 template <int HD>
 struct MxManyBlock {
     alignas(16) char kt[2][2 * MxTile<HD>::NU * 1024], vt[2][Tile<false, HD>::BYTES];
