@@ -14,6 +14,11 @@
 
 namespace gh {
 
+// What weights are relative to may stay behind the largest score by this much
+// (they are then up to 2^8, to the same relative accuracy), so that few tiles
+// rescale the sums.
+constexpr float kSlack = 8.0f;
+
 // A lane's pieces of one key's row: 16 bytes of codes and a scale byte for each
 // step of 128 columns; zeros where there is no row or no column.
 template <int HD>
@@ -324,14 +329,13 @@ struct MxFour {
             }
         }
         float top = fmaxf(sc[0], sc[1]);
-        top = fmaxf(top, dpp_f<kDppQuadSwap1>(top));
-        top = fmaxf(top, dpp_f<kDppQuadSwap2>(top));
-        top = fmaxf(top, dpp_f<kDppRowHalfMirror>(top));
-        top = fmaxf(top, dpp_f<kDppRowMirror>(top));
-        const float mn = fmaxf(m, top), use = mn == -INFINITY ? 0.f : mn;
-        const bool grew = mn != m;
-        if (__any(grew)) {
-            const float al = __builtin_amdgcn_exp2f(m - use);
+        if (__any(top > m + kSlack)) {
+            top = fmaxf(top, dpp_f<kDppQuadSwap1>(top));
+            top = fmaxf(top, dpp_f<kDppQuadSwap2>(top));
+            top = fmaxf(top, dpp_f<kDppRowHalfMirror>(top));
+            top = fmaxf(top, dpp_f<kDppRowMirror>(top));
+            const float mn = fmaxf(m, top), al = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+            m = mn;
             l *= al;
             // a column's row is its number's last two bits
             const float a0 = readlane_f(al, 0), a1 = readlane_f(al, 16), a2 = readlane_f(al, 32), a3 = readlane_f(al, 48);
@@ -339,7 +343,7 @@ struct MxFour {
 #pragma unroll
             for (int d = 0; d < HD / 16; d++) o[d] *= f;
         }
-        m = mn;
+        const float use = m == -INFINITY ? 0.f : m;
         // of keys c, c + 1 of group 0 (c even), or c - 1, c of group 1
         const float x0 = __builtin_amdgcn_exp2f(sc[0] - use), x1 = __builtin_amdgcn_exp2f(sc[1] - use);
         l += x0 + x1;
@@ -539,6 +543,8 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void k_paged_attn_mx_few(Pag
 template <int HD, int NR>
 struct MxRowsOf : Rows<false, HD, NR> {
     static constexpr int NU = MxTile<HD>::NU;
+    floatx4 less[NR];
+    float limit[NR];  // less: -m; limit: what a score less m must pass to move it (of m -infinity: 0, -infinity)
     u32x6 q6[NR][NU][kMxTerms];
     uint32_t sq[NR][NU][2];
 
@@ -568,34 +574,104 @@ struct MxRowsOf : Rows<false, HD, NR> {
                 sq[i][u][0] = t.scale;
                 sq[i][u][1] = t.last;
             }
-            this->m[i] = -INFINITY;
+            this->m[i] = limit[i] = -INFINITY;
             this->l[i] = 0.f;
+            less[i] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int d = 0; d < HD / 16; d++) this->o[i][d] = floatx4{0.f, 0.f, 0.f, 0.f};
         }
     }
-    // kt: a tile's codes, [group][step] KB in lane order; ks: their scale bytes
+    // kt: a tile's codes, [group][step] KB in lane order; ks: their scale bytes.
+    // Scores less what weights are relative to: the first products take it as the
+    // sum to add to, and what the smaller terms are added to is then small.
     __device__ __forceinline__ void score(const char* kt, const uint8_t* ks, floatx4 (&sc)[2][NR]) {
         const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-#pragma unroll
-            for (int i = 0; i < NR; i++) sc[j][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+            i32x8 k[NU];
+            uint32_t s[NU];
 #pragma unroll
             for (int u = 0; u < NU; u++) {
-                const i32x8 k = mx_op4(*reinterpret_cast<const u32x4*>(kt + ((j * NU + u) * 64 + lane) * 16));
-                const uint32_t s = ks[(j * NU + u) * 64 + lane];
-#pragma unroll
-                for (int i = 0; i < NR; i++) sc[j][i] = mx_mfma_t<0, 0>(k, s, mx_op6(q6[i][u][4]), sq[i][u][1], sc[j][i]);
-#pragma unroll
-                for (int i = 0; i < NR; i++) sc[j][i] = mx_mfma_t<0, 3>(k, s, mx_op6(q6[i][u][3]), sq[i][u][0], sc[j][i]);
-#pragma unroll
-                for (int i = 0; i < NR; i++) sc[j][i] = mx_mfma_t<0, 2>(k, s, mx_op6(q6[i][u][2]), sq[i][u][0], sc[j][i]);
-#pragma unroll
-                for (int i = 0; i < NR; i++) sc[j][i] = mx_mfma_t<0, 1>(k, s, mx_op6(q6[i][u][1]), sq[i][u][0], sc[j][i]);
-#pragma unroll
-                for (int i = 0; i < NR; i++) sc[j][i] = mx_mfma_t<0, 0>(k, s, mx_op6(q6[i][u][0]), sq[i][u][0], sc[j][i]);
+                k[u] = mx_op4(*reinterpret_cast<const u32x4*>(kt + ((j * NU + u) * 64 + lane) * 16));
+                s[u] = ks[(j * NU + u) * 64 + lane];
             }
+#pragma unroll
+            for (int i = 0; i < NR; i++) sc[j][i] = less[i];
+            const auto term = [&](auto tc) {
+                constexpr int t = decltype(tc)::value;
+#pragma unroll
+                for (int u = 0; u < NU; u++)
+#pragma unroll
+                    for (int i = 0; i < NR; i++)
+                        sc[j][i] = mx_mfma_t<0, t & 3>(k[u], s[u], mx_op6(q6[i][u][t]), sq[i][u][t / 4], sc[j][i]);
+            };
+            term(std::integral_constant<int, 0>{});
+            term(std::integral_constant<int, 1>{});
+            term(std::integral_constant<int, 2>{});
+            term(std::integral_constant<int, 3>{});
+            term(std::integral_constant<int, 4>{});
+        }
+    }
+    // A tile's 32 keys from key0 on, as Rows::take.
+    __device__ __forceinline__ void take(floatx4 (&sc)[2][NR], int key0, uint32_t seen, const char* vt) {
+        using T = Tile<false, HD>;
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+        if (key0 + 31 > this->first || seen != 0xffffffffu) {
+#pragma unroll
+            for (int i = 0; i < NR; i++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int k = 16 * (e >> 2) + 4 * g + (e & 3);
+                    const int sees = (int)(seen >> k & 1u) & (key0 + k <= this->pos[i] ? 1 : 0);
+                    sc[e >> 2][i][e & 3] = sees ? sc[e >> 2][i][e & 3] : -INFINITY;
+                }
+        }
+        float top[NR];
+        bool grew = false;
+#pragma unroll
+        for (int i = 0; i < NR; i++) {
+            top[i] = sc[0][i][0];
+#pragma unroll
+            for (int e = 1; e < 8; e++) top[i] = fmaxf(top[i], sc[e >> 2][i][e & 3]);
+            grew |= top[i] > limit[i];
+        }
+        if (__any(grew)) {
+#pragma unroll
+            for (int i = 0; i < NR; i++) {
+                const float mn = fmaxf(this->m[i], col_max(top[i]) - less[i][0]), use = mn == -INFINITY ? 0.f : mn;
+                const float al = __builtin_amdgcn_exp2f(this->m[i] - use), by = use + less[i][0];
+                this->m[i] = mn;
+                less[i] = floatx4{-use, -use, -use, -use};
+                limit[i] = mn == -INFINITY ? mn : kSlack;
+                this->l[i] *= al;
+#pragma unroll
+                for (int e = 0; e < 8; e++) sc[e >> 2][i][e & 3] -= by;
+#pragma unroll
+                for (int d = 0; d < HD / 16; d++) this->o[i][d] *= al;
+            }
+        }
+        bf16x8 p[NR][3];
+#pragma unroll
+        for (int i = 0; i < NR; i++) {
+            float w[8], sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                w[e] = __builtin_amdgcn_exp2f(sc[e >> 2][i][e & 3]);
+                sum += w[e];
+            }
+            this->l[i] += sum;
+            split3(w, p[i]);
+        }
+        bf16x8 v = T::vfrag(vt, 0, lane);
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++) {
+            const bf16x8 ahead = d + 1 < HD / 16 ? T::vfrag(vt, d + 1, lane) : v;
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int t = 2; t >= 0; t--)
+#pragma unroll
+                for (int i = 0; i < NR; i++) this->o[i][d] = mfma16x16x32(v, p[i][t], this->o[i][d]);
+            v = ahead;
         }
     }
 };
@@ -604,12 +680,14 @@ struct MxRowsOf : Rows<false, HD, NR> {
 // that all waves read from LDS. Waves 0 and 1 (of each step of 128 columns)
 // fetch the keys' two groups, 2 and 3 the values', into registers a tile ahead
 // and from there to the other of two stages, the values widened. Bound by issue: for
-// 2,048 tokens over 16,384 keys of 8 x 128 (16 query heads), 560 us or 0.46 PFLOP/s
-// of the product, vector instructions (exponentials, the weights' three terms,
-// LDS addresses) fill 59% of the cycles and matrix instructions 42%, one after
-// the other in a wave and hardly side by side between a SIMD's two. A third
-// stage with the next tile's scores computed ahead of this one's weights did
-// not change that (543 us against 540 with the join).
+// 2,048 tokens over 16,384 keys of 8 x 128 (16 query heads) 484 us with the join,
+// 0.53 PFLOP/s of the product; vector instructions (exponentials, the weights'
+// three terms) and matrix instructions take about half of the cycles each and
+// overlap little. A reference that may stay behind the maximum took off 3%, and
+// scores that come out less that reference 4% (of 525). No faster: the next
+// tile's scores ahead in a third stage (543 against 540), a row tile's weights
+// between the other's products (500 against 484; values are then read twice),
+// K and V staged by all waves alike (490).
 template <int HD>
 struct MxManyBlock {
     alignas(16) char kt[2][2 * MxTile<HD>::NU * 1024], vt[2][Tile<false, HD>::BYTES];
@@ -696,7 +774,7 @@ __device__ __forceinline__ void mx_many_block(const PagedAttnArgs& a, int block,
         if (key0 <= rows.last) {
             floatx4 scores[2][NR];
             rows.score(sh.kt[b], sh.ks[b], scores);
-            rows.take(scores, key0, sh.seen_of[b][0] | (sh.seen_of[b][1] << 16), nullptr, nullptr, sh.vt[b]);
+            rows.take(scores, key0, sh.seen_of[b][0] | (sh.seen_of[b][1] << 16), sh.vt[b]);
         }
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(0xc07f);  // LDS alone: the next tile's loads stay in flight
