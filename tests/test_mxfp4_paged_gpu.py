@@ -305,3 +305,43 @@ def test_refusals(gpu):
     apart = torch.zeros(kv.k_scale.numel() + 2, dtype=torch.uint8, device="cuda")[2:].view(kv.k_scale.shape)
     with pytest.raises(Exception, match="4-byte"):
         gpu.PagedKV(kv.k, kv.v, apart, kv.v_scale).read(b, torch.zeros((1, 128), device="cuda"), None)
+
+
+def test_pools_past_32_bits(gpu):
+    # the same pages behind 2^32 bytes of codes: the same bits
+    off = (1 << 26) // (8 * 16) + 3
+    results = []
+    for base in (0, off):
+        c = MxCase(8, 128, 16, [(100, 1), (60, 40), (700, 2)], seed=13)
+        q, k, v = (dev(c.rng.standard_normal((c.tokens, n * 128)).astype(np.float32)) for n in (16, 8, 8))
+        pools = []
+        for pool in (c.k, c.v, c.ks, c.vs):
+            big = torch.zeros((base + c.pages,) + pool.shape[1:], dtype=torch.uint8, device="cuda")
+            big[base:] = dev(pool)
+            pools.append(big)
+        c.table += base
+        kv, b = gpu.PagedKV(*pools), c.batch(gpu)
+        heads = gpu.GQA(dict(dim=2048, num_q=16, num_kv=8, head_dim=128))
+        out, q_out = torch.zeros_like(q), torch.zeros_like(q)
+        ko, vo = torch.zeros_like(k), torch.zeros_like(v)
+        kv.append(b, heads, q, k, v, q_out)
+        kv.attention(b, q_out, out)
+        kv.read(b, ko, vo)
+        results.append([host(t) for t in (out, ko, vo)] + [host(p[base:]) for p in pools])
+        assert base == 0 or not any(p[:64].any() or p[base - 64:base].any() for p in pools)
+        del kv, pools
+    assert np.isfinite(results[0][0]).all() and results[0][0].any()
+    for small, large in zip(*results):
+        np.testing.assert_array_equal(small, large)
+
+
+@pytest.mark.parametrize("hq,n,down", [(2, 1, False), (2, 1, True), (14, 1, False), (2, 200, False), (2, 200, True)])
+def test_scores_that_rise_or_fall(gpu, hq, n, down):
+    # from 2^-6 to some 60, or back: the running maximum moves by a little, then by a lot, or never again
+    c = MxCase(2 if hq == 2 else 1, 64, 16, [(800, n), (30, 1)], seed=15)
+    for p in range(800):
+        k = c.slot(0, 799 - p if down else p)
+        c.k[k] = (c.k[k] & 0x33) | 0x22  # 1 or 1.5
+        c.ks[k] = 115 + p // 64
+    q = np.abs(queries(c, hq)) + np.float32(0.5)
+    check(attend(gpu, c, q, hq), *c.attention(q, hq))
