@@ -112,8 +112,17 @@ struct MxTerms {
     u32x6 t[kMxTerms];
     uint32_t scale, last;
 };
+// A group near f32's end is cut at 2^-64 of itself: its first term may be 2 *
+// 2^127, from 1.9375 * 2^127 on, and mx_term's constants are past its largest
+// value. The exponent to cut it with.
+__device__ __forceinline__ uint32_t mx_inside(floatx32& x, uint32_t e) {
+    if (!__any(e > 200)) return e;
+    const bool far = e > 200;
+    x *= far ? 0x1p-64f : 1.0f;
+    return far ? e - 64 : e;
+}
 __device__ __forceinline__ void mx_split(floatx32 x, MxTerms& r) {
-    const uint32_t top = mx_top(x), e = mx_exponent(top);
+    const uint32_t top = mx_top(x), whole = mx_exponent(top), e = mx_inside(x, whole);
     const bool odd = top >= 0x7f800000u;
 #pragma unroll
     for (int t = 0; t < kMxTerms; t++) {
@@ -121,22 +130,16 @@ __device__ __forceinline__ void mx_split(floatx32 x, MxTerms& r) {
         r.t[t] = mx_to6(x, s);
         if (t + 1 < kMxTerms) x -= mx_from6(r.t[t], s);
     }
-    r.scale = odd ? ~0u : e * 0x01010101u - 0x0f0a0500u;
-    r.last = odd ? kMxNaN : e - 20;
+    r.scale = odd ? ~0u : whole * 0x01010101u - 0x0f0a0500u;
+    r.last = odd ? kMxNaN : whole - 20;
 }
 // Term t alone, the same bits: the terms before it add up to x rounded to
 // multiples of 2^(e + 2 - 5 t), which adding and taking off 1.5 * 2^23 of those
 // leaves (of 2^(e + 40) for t = 0: nothing).
 __device__ __forceinline__ u32x6 mx_term(floatx32 x, int t, uint32_t& scale) {
-    const uint32_t top = mx_top(x);
-    uint32_t e = mx_exponent(top);
+    const uint32_t top = mx_top(x), whole = mx_exponent(top), e = mx_inside(x, whole);
     const bool odd = top >= 0x7f800000u;
-    scale = odd ? kMxNaN : e - 5 * t;
-    if (__any(e > 200)) {  // (that constant would leave f32)
-        const bool far = e > 200;
-        x *= far ? 0x1p-64f : 1.0f;
-        e -= far ? 64 : 0;
-    }
+    scale = odd ? kMxNaN : whole - 5 * t;
     const float c = __uint_as_float(t == 0 ? (e + 40) << 23 : ((e + 25 - 5 * t) << 23) | 0x400000u);
 #pragma unroll
     for (int i = 0; i < 32; i++) x[i] -= (x[i] + c) - c;

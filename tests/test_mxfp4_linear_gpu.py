@@ -283,3 +283,16 @@ def test_refusals(gpu):
         gpu.pack_mxfp4(dev(codes), dev(scales)[:, :1])
     for sizes in ((0, 16, 64), (1, 0, 64), (1, 16, 60), (1, 16, 0), (1 << 20, 16, 64), (1, 1 << 20, 64)):
         assert gpu.kernel_choice("linear_mxfp4", *sizes) is None
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 40, 264), (1, 40, 4096), (3, 40, 264), (3, 300, 9000), (5, 40, 136), (5, 300, 2048),
+                                   (13, 50, 2048), (20, 40, 264), (130, 40, 264)])
+def test_x_near_the_end_of_f32(gpu, M, N, K):
+    # whole groups from 3.3e38 on, whose first term of eighths is 2 * 2^127, and one of the largest finite value
+    rng = np.random.default_rng(K)
+    codes = rng.integers(0, 256, (N, K // 2)).astype(np.uint8)
+    scales = rng.integers(2, 12, (N, -(-K // GROUP))).astype(np.uint8)
+    x = (rng.uniform(3.3e38, 3.4e38, (M, K)) * rng.choice([-1, 1], (M, K))).astype(np.float32)
+    x[:, 32:64] *= rng.uniform(0, 1, (M, 32)).astype(np.float32)
+    x[:, 40] = np.finfo(np.float32).max
+    check(call(gpu, x, codes, scales), *expected(x, codes, scales))
