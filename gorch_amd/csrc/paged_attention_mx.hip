@@ -14,9 +14,10 @@
 
 namespace gh {
 
-// What weights are relative to may stay behind the largest score by this much
-// (they are then up to 2^8, to the same relative accuracy), so that few tiles
-// rescale the sums.
+// What weights are relative to (m below) is set this much past the largest score,
+// so that few tiles rescale the sums and no weight is above 1: sums leave f32's
+// range where those of the other caches do. Weights stay normal numbers down to
+// 2^-118 of the largest at least, in place of 2^-126.
 constexpr float kSlack = 8.0f;
 
 // A lane's pieces of one key's row: 16 bytes of codes and a scale byte for each
@@ -329,12 +330,12 @@ struct MxFour {
             }
         }
         float top = fmaxf(sc[0], sc[1]);
-        if (__any(top > m + kSlack)) {
+        if (__any(top > m)) {
             top = fmaxf(top, dpp_f<kDppQuadSwap1>(top));
             top = fmaxf(top, dpp_f<kDppQuadSwap2>(top));
             top = fmaxf(top, dpp_f<kDppRowHalfMirror>(top));
             top = fmaxf(top, dpp_f<kDppRowMirror>(top));
-            const float mn = fmaxf(m, top), al = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+            const float mn = fmaxf(m, top + kSlack), al = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
             m = mn;
             l *= al;
             // a column's row is its number's last two bits
@@ -544,7 +545,7 @@ template <int HD, int NR>
 struct MxRowsOf : Rows<false, HD, NR> {
     static constexpr int NU = MxTile<HD>::NU;
     floatx4 less[NR];
-    float limit[NR];  // less: -m; limit: what a score less m must pass to move it (of m -infinity: 0, -infinity)
+    float limit[NR];  // less: -m; limit: what a score less m must pass to move it, 0 (of m -infinity: 0, -infinity)
     u32x6 q6[NR][NU][kMxTerms];
     uint32_t sq[NR][NU][2];
 
@@ -638,11 +639,11 @@ struct MxRowsOf : Rows<false, HD, NR> {
         if (__any(grew)) {
 #pragma unroll
             for (int i = 0; i < NR; i++) {
-                const float mn = fmaxf(this->m[i], col_max(top[i]) - less[i][0]), use = mn == -INFINITY ? 0.f : mn;
+                const float mn = fmaxf(this->m[i], col_max(top[i]) - less[i][0] + kSlack), use = mn == -INFINITY ? 0.f : mn;
                 const float al = __builtin_amdgcn_exp2f(this->m[i] - use), by = use + less[i][0];
                 this->m[i] = mn;
                 less[i] = floatx4{-use, -use, -use, -use};
-                limit[i] = mn == -INFINITY ? mn : kSlack;
+                limit[i] = mn == -INFINITY ? mn : 0.f;
                 this->l[i] *= al;
 #pragma unroll
                 for (int e = 0; e < 8; e++) sc[e >> 2][i][e & 3] -= by;
@@ -683,7 +684,7 @@ struct MxRowsOf : Rows<false, HD, NR> {
 // 2,048 tokens over 16,384 keys of 8 x 128 (16 query heads) 484 us with the join,
 // 0.53 PFLOP/s of the product; vector instructions (exponentials, the weights'
 // three terms) and matrix instructions take about half of the cycles each and
-// overlap little. A reference that may stay behind the maximum took off 3%, and
+// overlap little. A reference that is moved by 8 at once took off 3%, and
 // scores that come out less that reference 4% (of 525). No faster: the next
 // tile's scores ahead in a third stage (543 against 540), a row tile's weights
 // between the other's products (500 against 484; values are then read twice),

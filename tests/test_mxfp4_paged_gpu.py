@@ -345,3 +345,20 @@ def test_scores_that_rise_or_fall(gpu, hq, n, down):
         c.ks[k] = 115 + p // 64
     q = np.abs(queries(c, hq)) + np.float32(0.5)
     check(attend(gpu, c, q, hq), *c.attention(q, hq))
+
+
+@pytest.mark.parametrize("hq,hkv,hd,n", [(2, 1, 64, 1), (16, 8, 128, 1), (4, 1, 80, 1), (14, 2, 64, 1), (2, 1, 64, 200),
+                                         (2, 1, 256, 90), (2, 1, 96, 200)])
+def test_values_whose_weighted_sum_stays_in_f32(gpu, hq, hkv, hd, n):
+    # the last keys outweigh the first ones by less than 2^8, and all 400 values add up to less than 2^127: weights above
+    # 1 would carry the sums of a wave's keys past f32 (a page of many slots, so that one range of keys has them all)
+    c = MxCase(hkv, hd, 32768, [(400, n), (30, 1)], seed=16)
+    c.vs[:] = np.where(c.vs == 255, 255, 242)
+    c.v &= 0x77  # positive, up to 6 * 2^115
+    for p in range(400):
+        k = c.slot(0, p)
+        c.k[k], c.ks[k] = 0, 127
+        c.k[k][:, 0] = 2 if p >= 128 else 0  # column 0: 1, or nothing
+    q = np.zeros((c.tokens, hq, hd), np.float32)
+    q[..., 0] = 5 * np.sqrt(hd)
+    check(attend(gpu, c, q, hq, causal=False, max_new=n), *c.attention(q, hq, causal=False))
