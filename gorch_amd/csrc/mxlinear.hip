@@ -3,6 +3,8 @@
 // codes go to the matrix cores as they are; x goes there as the five 6-bit
 // terms of mx.h, which keep f32's accuracy.
 #include <algorithm>
+#include <atomic>
+#include <chrono>
 #include <iterator>
 
 #include "mx.h"
@@ -22,10 +24,12 @@ struct MxLinearArgs {
     char* terms;     // of more than 16 rows: x's operands (k_mx_terms)
     // of up to 16 rows: K in `slices` ranges of `chunks` * T column tiles, W's
     // row tiles `per` to a block; of several slices, partial sums [row
-    // tile][slice][lane][4] and a counter for each block of row tiles
+    // tile][slice][lane][4] and a counter for each block of row tiles, which
+    // counts from `mark` on
     int slices, chunks, per, blocks;
     float* part;
-    unsigned* done;
+    uint64_t* done;
+    uint64_t mark;
 };
 
 // Barrier for LDS alone: loads into registers stay in flight.
@@ -128,6 +132,7 @@ __global__ __launch_bounds__(64 * kMxTerms) void k_mx_terms16(MxLinearArgs a) {
 // the terms (34 us when each block split all of x).
 constexpr int kGemvWaves = 8;
 constexpr int kGemvSlices = 16;
+constexpr uint64_t kMarkStep = 32;  // a mark is a multiple of it, more than a counter counts
 enum GemvKind { kRow1, kFive, kMade };
 struct GemvLds {  // byte offsets of a block's LDS
     int p8, sc, red, bytes;
@@ -163,6 +168,8 @@ __global__ __launch_bounds__(64 * kGemvWaves, 2) void k_mx_gemv(MxLinearArgs a) 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
     const int M = a.M, R = kMxTerms * M, wk = wave % WK, wn = wave / WK;
     const int t0 = nb * a.per, t1 = min(t0 + a.per, a.nt);
+    uint64_t was = 0;
+    if (a.slices > 1 && threadIdx.x == 0) was = __hip_atomic_load(a.done + nb, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     float* red = reinterpret_cast<float*>(lds + at.red);
     struct Step {
         u32x4 codes[NT][U];
@@ -303,6 +310,14 @@ __global__ __launch_bounds__(64 * kGemvWaves, 2) void k_mx_gemv(MxLinearArgs a) 
     // (partial sums of a block's row tiles: up to 2^31 bytes)
     const __amdgpu_buffer_rsrc_t part =
         make_rsrc(a.part + (size_t)t0 * a.slices * 256, (long long)(t1 - t0) * a.slices * 1024);
+    // What the counter held before the call does not matter: the first block
+    // that finds another call's mark, or anything else, puts this call's there
+    // (one such exchange succeeds, since all start from what was there before),
+    // and no block counts before it has seen the mark or tried that.
+    const auto set_mark = [&] {
+        if (a.slices > 1 && threadIdx.x == 0 && (was ^ a.mark) >= kMarkStep)
+            __hip_atomic_compare_exchange_strong(a.done + nb, &was, a.mark, __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
     // one column range and one round of row tiles after another
     const int j00 = slice * a.chunks * T, rounds = (t1 - t0 + WN * NT - 1) / (WN * NT);
     Step s;
@@ -314,6 +329,7 @@ __global__ __launch_bounds__(64 * kGemvWaves, 2) void k_mx_gemv(MxLinearArgs a) 
         const bool more = ch + 1 < a.chunks && j0 + T < a.nk;
         if (ch > 0 || r == 0 || a.chunks > 1) {
             if (ch > 0 || r > 0) lds_sync();
+            if (MADE && r == 0 && ch == 0) set_mark();
             if constexpr (MADE) {
                 typedef __attribute__((address_space(1))) const uint32_t* global_ptr;
                 typedef __attribute__((address_space(3))) uint32_t* lds_ptr;
@@ -324,6 +340,7 @@ __global__ __launch_bounds__(64 * kGemvWaves, 2) void k_mx_gemv(MxLinearArgs a) 
                 block_sync_dma();
             } else {
                 split(j0);
+                if (r == 0 && ch == 0) set_mark();
                 lds_sync();
             }
         }
@@ -360,10 +377,10 @@ __global__ __launch_bounds__(64 * kGemvWaves, 2) void k_mx_gemv(MxLinearArgs a) 
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (threadIdx.x == 0) last = __hip_atomic_fetch_add(a.done + nb, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == (unsigned)a.slices;
+    if (threadIdx.x == 0) last = __hip_atomic_fetch_add(a.done + nb, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == a.mark + a.slices;
     __syncthreads();
     if (!last) return;
-    if (threadIdx.x == 0) __hip_atomic_store(a.done + nb, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (threadIdx.x == 0) __hip_atomic_store(a.done + nb, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     for (int t = t0 + wave; t < t1; t += kGemvWaves) {
         floatx4 p[kGemvSlices];
 #pragma unroll
@@ -577,8 +594,20 @@ __global__ __launch_bounds__(512 / MT, 2 / MT) void k_mx_gemm(MxLinearArgs a) {
 }
 
 // A workspace begins with the counters of every shape's blocks (at most 128 of
-// several slices), so that one may serve calls of all sizes in turn.
-constexpr size_t kCounterBytes = 512;
+// several slices), so that one may serve calls of all sizes in turn; a call finds
+// in them what it will.
+constexpr size_t kCounterBytes = 1024;
+// A counter's value that no workspace holds by chance (2^-58): the bits of a
+// count mixed with the process's start, never 0, which a call leaves behind. A
+// captured call keeps its own; its replays follow each other.
+static uint64_t next_mark() {
+    static std::atomic<uint64_t> calls{0};
+    static const uint64_t seed = (uint64_t)std::chrono::system_clock::now().time_since_epoch().count() ^ ((uint64_t)(uintptr_t)&calls << 20);
+    uint64_t z = seed + 0x9e3779b97f4a7c15ull * (calls.fetch_add(1, std::memory_order_relaxed) + 1);
+    z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
+    z = (z ^ (z >> 27)) * 0x94d049bb133111ebull;
+    return ((z ^ (z >> 31)) | 1ull << 63) / kMarkStep * kMarkStep;
+}
 static size_t terms_bytes(int M, int K) { return kCounterBytes + (size_t)((M + 15) / 16) * ((K + 127) / 128) * kTermBytes; }
 
 // How the rows of a decode step are cut into blocks: slices of K (at most 16),
@@ -640,12 +669,13 @@ static int launch_mx_gemv_f(hipStream_t s, const MxLinearArgs& a, const GemvPlan
 }
 static int launch_mx_gemv(hipStream_t s, MxLinearArgs a, char* ws) {
     const GemvPlan p = gemv_plan(a.M, a.N, a.K);
-    static_assert(kCounterBytes >= 256 / 2 * sizeof(unsigned));
+    static_assert(kCounterBytes >= 256 / 2 * sizeof(uint64_t) && kMarkStep > kGemvSlices);
     a.slices = p.slices;
     a.chunks = p.chunks;
     a.per = p.per;
     a.blocks = p.blocks;
-    a.done = reinterpret_cast<unsigned*>(ws);
+    a.done = reinterpret_cast<uint64_t*>(ws);
+    a.mark = p.slices > 1 ? next_mark() : 0;
     a.terms = ws + kCounterBytes;
     a.part = reinterpret_cast<float*>(ws + kCounterBytes + p.terms);
     if (p.kind == kMade) hipLaunchKernelGGL(k_mx_terms16, dim3(a.nk), dim3(64 * kMxTerms), 0, s, a);

@@ -505,7 +505,8 @@ def linear_mxfp4(x, Wp, N, bias, y, residual=None, epilogue=EPI_NONE, ws=None) -
     """gorch_hip_linear_mxfp4: y = residual + epi(x @ W^T + bias) over a
     pack_mxfp4 weight of N rows; x [M, K] and y [M, N] f32. ws from
     linear_mxfp4_workspace for these sizes or larger needs (a new one if None),
-    for one call after another: calls that can overlap must not share it."""
+    whatever it holds, for one call after another: calls that can overlap must
+    not share it."""
     import torch
 
     dev = _device()

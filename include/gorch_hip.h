@@ -268,11 +268,9 @@ int gorch_hip_pack_mxfp4(void* stream, const uint8_t* codes, const uint8_t* scal
  * may alias y, x must not. K % 8 == 0, M up to 2^20 - 16, K up to 2^24, x, Wp and
  * the workspace 16-byte aligned (else GORCH_HIP_EUNSUPPORTED). The workspace
  * (gorch_hip_linear_mxfp4_workspace_size bytes of device memory; NULL where
- * that is 0) is the caller's: zeroed before its first use, after which it may
- * serve calls of any sizes that it is large enough for, one after another (its
- * first 512 bytes are counters, zero again after every call), but not calls
- * that can overlap. Nothing is allocated, so the call can
- * be captured. */
+ * that is 0) is the caller's, whatever it holds: it may serve calls of any sizes
+ * that it is large enough for and other operators, one after another, but not
+ * calls that can overlap. Nothing is allocated, so the call can be captured. */
 size_t gorch_hip_linear_mxfp4_workspace_size(int M, int N, int K);
 int gorch_hip_linear_mxfp4(void* stream, const float* x, const void* Wp, const float* bias, const float* residual,
                            float* y, int M, int N, int K, int epilogue, void* workspace, size_t workspace_bytes);

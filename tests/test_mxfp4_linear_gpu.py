@@ -296,3 +296,29 @@ def test_x_near_the_end_of_f32(gpu, M, N, K):
     x[:, 32:64] *= rng.uniform(0, 1, (M, 32)).astype(np.float32)
     x[:, 40] = np.finfo(np.float32).max
     check(call(gpu, x, codes, scales), *expected(x, codes, scales))
+
+
+@pytest.mark.parametrize("M,N,K", [(2, 300, 9000), (4, 300, 6000), (16, 1000, 9000), (1, 20, 20000), (13, 500, 2048), (40, 90, 5160)])
+def test_what_a_workspace_held_is_no_part_of_a_call(gpu, M, N, K):
+    rng, x, codes, scales = inputs(M, M, N, K)
+    want, tol = expected(x, codes, scales)
+    ws = gpu.linear_mxfp4_workspace(M, N, K)
+    first = call(gpu, x, codes, scales, ws=ws)
+    check(first, want, tol)
+    xd, Wp, y = dev(x), gpu.pack_mxfp4(dev(codes), dev(scales)), torch.zeros((M, N), device="cuda")
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        gpu.linear_mxfp4(xd, Wp, N, None, y, ws=ws)
+    n = ws.numel()
+    for held in (np.full(n, 255), np.full(n, 1), rng.integers(0, 256, n), np.arange(n) % 4 == 0, np.arange(n) % 8 == 0,
+                 np.full(n // 4, 1.0, np.float32).view(np.uint8)):
+        ws.copy_(dev(np.asarray(held).astype(np.uint8)))
+        np.testing.assert_array_equal(call(gpu, x, codes, scales, ws=ws), first)
+        ws.copy_(dev(np.asarray(held).astype(np.uint8)))
+        y.fill_(7)
+        graph.replay()
+        np.testing.assert_array_equal(host(y), first)
+        y.fill_(7)
+        graph.replay()
+        np.testing.assert_array_equal(host(y), first)
