@@ -1037,6 +1037,8 @@ class PagedKV:
         if dtype == "bf16":
             return cls(*(torch.zeros(shape, dtype=torch.bfloat16, device="cuda") for _ in "kv"))
         if dtype == "mxfp4":
+            if head_dim % 2:
+                raise ValueError(f"gorch_amd.hip: MXFP4 pools hold two columns a byte, head_dim must be even, got {head_dim}")
             widths = (head_dim // 2, -(-head_dim // 32)) * 2
             k, ks, v, vs = (torch.zeros(shape[:3] + (w,), dtype=torch.uint8, device="cuda") for w in widths)
             return cls(k, v, ks, vs)

@@ -101,3 +101,10 @@ def test_attention_workspace_is_checked():
     assert need > 0
     assert attend(kv, b, ws=FAKE, n=need - 1) == 2 and attend(kv, b, ws=None, n=need) == 2
     assert attend(kv, b, ws=FAKE + 8, n=need) == 1
+
+
+@pytest.mark.parametrize("head_dim", [17, 33, 49, 127])
+def test_new_pools_of_an_odd_head_are_refused(head_dim):
+    # (half of it rounded down would be the pools of another head)
+    with pytest.raises(ValueError, match="even"):
+        hip.PagedKV.new(4, 16, 2, head_dim, "mxfp4")
