@@ -155,7 +155,7 @@ struct GemvLds {  // byte offsets of a block's LDS
 __device__ __forceinline__ void store_far(__amdgpu_buffer_rsrc_t rs, int at, floatx4 v) {
     __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rs, at, 0, 16);
 }
-template <GemvKind KIND, int WK, int U, int NT>
+template <GemvKind KIND, int WK, int U>
 __global__ __launch_bounds__(64 * kGemvWaves, 2) void k_mx_gemv(MxLinearArgs a) {
     constexpr int WN = kGemvWaves / WK, T = WK * U;
     constexpr bool ROW1 = KIND == kRow1, MADE = KIND == kMade;
@@ -172,41 +172,31 @@ __global__ __launch_bounds__(64 * kGemvWaves, 2) void k_mx_gemv(MxLinearArgs a) 
     if (a.slices > 1 && threadIdx.x == 0) was = __hip_atomic_load(a.done + nb, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     float* red = reinterpret_cast<float*>(lds + at.red);
     struct Step {
-        u32x4 codes[NT][U];
-        uint32_t scale[NT][(U + 3) / 4];
+        u32x4 codes[U];
+        uint32_t scale[(U + 3) / 4];
     };
-    // U column tiles from j on of row tiles t .. (what lies past the last is not looked at)
+    // U column tiles from j on of row tile t (what lies past the last is not looked at)
     const auto load = [&](Step& s, int t, int j) {
+        const size_t tt = min(t, a.nt - 1);
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
-            const size_t tt = min(t + i, a.nt - 1);
+        for (int u = 0; u < U; u += 4) s.scale[u / 4] = a.wsc[(tt * a.nq + (min(j + u, a.nk - 1) >> 2)) * 64 + lane];
 #pragma unroll
-            for (int u = 0; u < U; u += 4) s.scale[i][u / 4] = a.wsc[(tt * a.nq + (min(j + u, a.nk - 1) >> 2)) * 64 + lane];
-#pragma unroll
-            for (int u = 0; u < U; u++)
-                s.codes[i][u] = __builtin_nontemporal_load(a.wp + (tt * a.nk + min(j + u, a.nk - 1)) * 64 + lane);
-        }
+        for (int u = 0; u < U; u++) s.codes[u] = __builtin_nontemporal_load(a.wp + (tt * a.nk + min(j + u, a.nk - 1)) * 64 + lane);
     };
-    floatx4 acc[NT];
+    floatx4 acc = {0.f, 0.f, 0.f, 0.f};
     const auto multiply = [&](const Step& s, int j, int jl) {
         const auto one = [&](auto uc) {
             constexpr int u = decltype(uc)::value, B = u & 3;
             if constexpr (u < U) {
                 if (j + u >= a.nk) return;
-                uint32_t sw[NT];
-                i32x8 w[NT];
-#pragma unroll
-                for (int i = 0; i < NT; i++) {
-                    sw[i] = s.scale[i][u / 4] >> (U < 4 ? 8 * (j & 3) : 0);
-                    w[i] = mx_op4(s.codes[i][u]);
-                }
+                const uint32_t sw = s.scale[u / 4] >> (U < 4 ? 8 * (j & 3) : 0);
+                const i32x8 w = mx_op4(s.codes[u]);
                 if constexpr (ROW1) {
                     const int slot = ((jl + u) * 4 + g) * R + min(c, R - 1);
                     const i32x8 six = mx_op6(*reinterpret_cast<const u32x4*>(lds + slot * 16),
                                              *reinterpret_cast<const u32x2*>(lds + at.p8 + slot * 8));
                     const uint32_t sx = *reinterpret_cast<const uint8_t*>(lds + at.sc + slot);
-#pragma unroll
-                    for (int i = 0; i < NT; i++) acc[i] = mx_mfma<0, B>(six, sx, w[i], sw[i], acc[i]);
+                    acc = mx_mfma<0, B>(six, sx, w, sw, acc);
                 } else {
                     const int m = min(c, M - 1);
                     const char* made = lds + (jl + u) * kTermBytes;
@@ -221,16 +211,11 @@ __global__ __launch_bounds__(64 * kGemvWaves, 2) void k_mx_gemv(MxLinearArgs a) 
                                       *reinterpret_cast<const u32x2*>(lds + at.p8 + slot * 8));
                     };
                     const i32x8 x4 = six(4), x3 = six(3), x2 = six(2), x1 = six(1), x0 = six(0);
-#pragma unroll
-                    for (int i = 0; i < NT; i++) acc[i] = mx_mfma<0, B>(x4, sx[1], w[i], sw[i], acc[i]);
-#pragma unroll
-                    for (int i = 0; i < NT; i++) acc[i] = mx_mfma<3, B>(x3, sx[0], w[i], sw[i], acc[i]);
-#pragma unroll
-                    for (int i = 0; i < NT; i++) acc[i] = mx_mfma<2, B>(x2, sx[0], w[i], sw[i], acc[i]);
-#pragma unroll
-                    for (int i = 0; i < NT; i++) acc[i] = mx_mfma<1, B>(x1, sx[0], w[i], sw[i], acc[i]);
-#pragma unroll
-                    for (int i = 0; i < NT; i++) acc[i] = mx_mfma<0, B>(x0, sx[0], w[i], sw[i], acc[i]);
+                    acc = mx_mfma<0, B>(x4, sx[1], w, sw, acc);
+                    acc = mx_mfma<3, B>(x3, sx[0], w, sw, acc);
+                    acc = mx_mfma<2, B>(x2, sx[0], w, sw, acc);
+                    acc = mx_mfma<1, B>(x1, sx[0], w, sw, acc);
+                    acc = mx_mfma<0, B>(x0, sx[0], w, sw, acc);
                 }
             }
         };
@@ -319,13 +304,11 @@ __global__ __launch_bounds__(64 * kGemvWaves, 2) void k_mx_gemv(MxLinearArgs a) 
             __hip_atomic_compare_exchange_strong(a.done + nb, &was, a.mark, __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     };
     // one column range and one round of row tiles after another
-    const int j00 = slice * a.chunks * T, rounds = (t1 - t0 + WN * NT - 1) / (WN * NT);
+    const int j00 = slice * a.chunks * T, rounds = (t1 - t0 + WN - 1) / WN;
     Step s;
-    load(s, t0 + wn * NT, j00 + wk * U);
-#pragma unroll
-    for (int i = 0; i < NT; i++) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    load(s, t0 + wn, j00 + wk * U);
     for (int r = 0, ch = 0; r < rounds;) {
-        const int j0 = j00 + ch * T, t = t0 + (r * WN + wn) * NT;
+        const int j0 = j00 + ch * T, t = t0 + r * WN + wn;
         const bool more = ch + 1 < a.chunks && j0 + T < a.nk;
         if (ch > 0 || r == 0 || a.chunks > 1) {
             if (ch > 0 || r > 0) lds_sync();
@@ -346,28 +329,25 @@ __global__ __launch_bounds__(64 * kGemvWaves, 2) void k_mx_gemv(MxLinearArgs a) 
         }
         const int nr = more ? r : r + 1, nch = more ? ch + 1 : 0;
         const Step now = s;
-        load(s, t0 + (nr * WN + wn) * NT, j00 + nch * T + wk * U);
+        load(s, t0 + nr * WN + wn, j00 + nch * T + wk * U);
         multiply(now, j0 + wk * U, wk * U);
         r = nr;
         ch = nch;
         if (more) continue;
+        floatx4 d = acc;
+        acc = floatx4{0.f, 0.f, 0.f, 0.f};
+        // the waves' sums along the columns, in wave order
+        if constexpr (WK > 1) {
+            if (r > 1) lds_sync();
+            if (wk > 0) *reinterpret_cast<floatx4*>(red + (wave * 64 + lane) * 4) = d;
+            lds_sync();
+            if (wk > 0) continue;
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
-            floatx4 d = acc[i];
-            acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
-            // the waves' sums along the columns, in wave order
-            if constexpr (WK > 1) {
-                if (i > 0 || r > 1) lds_sync();
-                if (wk > 0) *reinterpret_cast<floatx4*>(red + (wave * 64 + lane) * 4) = d;
-                lds_sync();
-                if (wk > 0) continue;
-#pragma unroll
-                for (int k = 1; k < WK; k++) d += *reinterpret_cast<const floatx4*>(red + ((wave + k) * 64 + lane) * 4);
-            }
-            if (t + i >= t1) continue;
-            if (a.slices == 1) finish(t + i, d);
-            else store_far(part, ((t + i - t0) * a.slices + slice) * 1024 + lane * 16, d);
+            for (int k = 1; k < WK; k++) d += *reinterpret_cast<const floatx4*>(red + ((wave + k) * 64 + lane) * 4);
         }
+        if (t >= t1) continue;
+        if (a.slices == 1) finish(t, d);
+        else store_far(part, ((t - t0) * a.slices + slice) * 1024 + lane * 16, d);
     }
     if (a.slices == 1) return;
     // Partial sums were stored, and are loaded, past the XCD's caches, so that
@@ -614,7 +594,7 @@ static size_t terms_bytes(int M, int K) { return kCounterBytes + (size_t)((M + 1
 // row tiles per block, waves along the columns.
 struct GemvPlan {
     GemvKind kind;
-    int tiles, slices, chunks, per, blocks, wk, nt;
+    int tiles, slices, chunks, per, blocks, wk;
     size_t terms, part, bytes;
 };
 static GemvPlan gemv_plan(int M, int N, int K) {
@@ -640,8 +620,6 @@ static GemvPlan gemv_plan(int M, int N, int K) {
     p.blocks = (nt + p.per - 1) / p.per;
     p.wk = 8;
     while (p.wk > p.tiles / 8 && kGemvWaves / p.wk < p.per) p.wk /= 2;
-    // (two row tiles a wave at a time share what it reads of x's terms)
-    p.nt = p.kind != kRow1 && p.tiles / p.wk <= 4 && p.per > kGemvWaves / p.wk ? 2 : 1;
     p.terms = p.kind == kMade ? (size_t)nk * kTermBytes : 0;
     p.part = p.slices == 1 ? 0 : (size_t)p.slices * nt * 1024;
     p.bytes = p.terms + p.part;
@@ -649,23 +627,22 @@ static GemvPlan gemv_plan(int M, int N, int K) {
     return p;
 }
 
-template <GemvKind KIND, int WK, int U, int NT>
+template <GemvKind KIND, int WK, int U>
 static int launch_mx_gemv_t(hipStream_t s, const MxLinearArgs& a) {
+    static_assert(KIND != kMade || WK * U * kTermBytes + kGemvWaves * 1024 <= 160 << 10);
     const int bytes = GemvLds(a.M, std::min(WK * U, a.nk), KIND == kMade).bytes;
     if (bytes > 64 << 10)
-        GH_TRY(check(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_mx_gemv<KIND, WK, U, NT>),
+        GH_TRY(check(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_mx_gemv<KIND, WK, U>),
                                          hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "mx_gemv attribute"));
-    hipLaunchKernelGGL((k_mx_gemv<KIND, WK, U, NT>), dim3((a.blocks + 7) / 8 * 8 * a.slices), dim3(64 * kGemvWaves), bytes, s, a);
+    hipLaunchKernelGGL((k_mx_gemv<KIND, WK, U>), dim3((a.blocks + 7) / 8 * 8 * a.slices), dim3(64 * kGemvWaves), bytes, s, a);
     return GORCH_HIP_OK;
 }
 template <int WK, int U>
 static int launch_mx_gemv_f(hipStream_t s, const MxLinearArgs& a, const GemvPlan& p) {
-    if (p.kind == kRow1) return launch_mx_gemv_t<kRow1, WK, U, 1>(s, a);
-    if constexpr (U <= 4)
-        if (p.nt == 2) return p.kind == kFive ? launch_mx_gemv_t<kFive, WK, U, 2>(s, a) : launch_mx_gemv_t<kMade, WK, U, 2>(s, a);
+    if (p.kind == kRow1) return launch_mx_gemv_t<kRow1, WK, U>(s, a);
     if constexpr (WK * U <= 16)
-        if (p.kind == kMade) return launch_mx_gemv_t<kMade, WK, U, 1>(s, a);
-    return launch_mx_gemv_t<kFive, WK, U, 1>(s, a);
+        if (p.kind == kMade) return launch_mx_gemv_t<kMade, WK, U>(s, a);
+    return launch_mx_gemv_t<kFive, WK, U>(s, a);
 }
 static int launch_mx_gemv(hipStream_t s, MxLinearArgs a, char* ws) {
     const GemvPlan p = gemv_plan(a.M, a.N, a.K);
