@@ -322,3 +322,36 @@ def test_what_a_workspace_held_is_no_part_of_a_call(gpu, M, N, K):
         y.fill_(7)
         graph.replay()
         np.testing.assert_array_equal(host(y), first)
+
+
+@pytest.mark.parametrize("M", [1, 3, 5, 16, 20, 200])
+@pytest.mark.parametrize("kind", ["random", "cancels", "faint"])
+def test_one_instruction(gpu, M, kind):
+    # x in eighths of its groups' powers of two: the first of five terms is x and the others nothing, so that an output is
+    # one matrix instruction's sum of 128 products; with "cancels" the largest of them, 2^12 to 2^24 times the rest, add up
+    # to nothing, with "faint" those of a group are 32 and each of the others' 96 products 1.875 * 2^-s of that. The
+    # instruction adds a group of 32 products to the sum of those before it, where the larger of that sum and the products
+    # has the power of two P: of each product what lies below 2^-27 P is cut off, 32 of them 4 U, or of the sum so far what
+    # lies below 2^-23 P, 2 U, and the result is rounded, U. 5 U of the magnitudes, four times.
+    rng = np.random.default_rng(M)
+    N, K = 3000, 128
+    codes, scales = weight(rng, N, K)
+    x = rng.integers(-15, 16, (M, K)) / 8
+    x[:, ::32] = rng.choice([-1, 1], (M, 4)) * rng.integers(8, 16, (M, 4)) / 8
+    if kind == "faint":
+        s = rng.integers(15, 31, N)
+        codes[:], scales[:] = 0x22, (127 - s)[:, None]
+        scales[np.arange(N), rng.integers(0, 4, N)] = 127
+        x[:] = 1.875
+        x[:, rng.permutation(128)[:M % 128]] = 1
+    elif kind == "cancels":
+        codes[:, 8:16] = codes[:, :8]
+        x[:, 16:32] = -x[:, :16]
+        x[:, :32] *= np.exp2(rng.integers(12, 25, (M, 1)))
+    else:
+        x *= np.exp2(rng.integers(-12, 13, (M, 4))).repeat(32, 1)
+    x = x.astype(np.float32)
+    W = values(codes, scales)
+    size = np.abs(x).astype(np.float64) @ np.abs(W).T
+    off = np.abs(call(gpu, x, codes, scales) - x.astype(np.float64) @ W.T) / size
+    assert (off <= 20 * U).all(), f"off by {off.max() / U} U of the sum of magnitudes"
