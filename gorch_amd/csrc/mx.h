@@ -12,8 +12,13 @@
 // e the exponent of the group's largest magnitude: |x| / 2^e < 2, what rounding
 // to eighths leaves is at most 1/16 = 2 / 32, and so on. An e2m3 (6-bit) code
 // holds every such d exactly, and five of them leave at most 2^-24 of the
-// largest, which itself is kept whole: f32's own rounding of the group's
-// largest value. The five products run at four times the bf16 rate each, with
+// largest, which itself is kept whole: a fixed point within the group, where a
+// value 2^j smaller than the largest keeps 24 - j bits. Where a group's values
+// are of one size that is f32's accuracy. Where one is much larger, sums that
+// rest on the others lose it: 4 and 64 x 4,096 x 4,096 with one column of x
+// 1,000 times the others, the outputs whose weight there is 0 2e-6 of their
+// norm (f32 5e-7), 10,000 times 3e-5; with such a column in every group and
+// weights as much smaller there, all outputs 2.6e-5 and 2.5e-4. The five products run at four times the bf16 rate each, with
 // no code widened, where three bf16 terms would need it; four terms (2^-19)
 // would leave errors ten times those of f32 sums.
 //

@@ -1,7 +1,7 @@
 // mxlinear.hip — Linear over MXFP4 weights (nn/module.go:61-88 with the
 // weight's values rounded to four bits): y = residual + epi(x W^T + bias). The
 // codes go to the matrix cores as they are; x goes there as the five 6-bit
-// terms of mx.h, which keep f32's accuracy.
+// terms of mx.h, which hold it to 2^-24 of the largest of each 32 columns.
 #include <algorithm>
 #include <atomic>
 #include <chrono>

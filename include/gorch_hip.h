@@ -262,8 +262,13 @@ int gorch_hip_pack_mxfp4(void* stream, const uint8_t* codes, const uint8_t* scal
 /* gorch_hip_linear_bf16 (nn/module.go:61-88) over a weight in MXFP4, for any
  * number of rows: y[m,n] = residual[m,n] + epi(sum_k x[m,k] W[n,k] + bias[n])
  * with the weight's values exact and x held to 2^-24 of the largest magnitude
- * among each 32 of a row's columns (k / 32) or to 2^-130, products and sums in f32: f32
- * accuracy, in a fixed order of sums. An infinity or NaN in x makes its row of
+ * among each 32 of a row's columns (k / 32) or to 2^-130, products and sums in f32, in
+ * a fixed order. That is f32 accuracy where such columns are of one size; a
+ * value 2^j smaller than the largest beside it is held to 24 - j bits, which
+ * shows in outputs that rest on it (one column 1,000 times the others: 2e-6 of
+ * the norm of outputs with a weight of 0 there, 10,000 times: 3e-5; a column in
+ * each 32, with weights as much smaller: 2.6e-5 and 2.5e-4 of the norm of all).
+ * An infinity or NaN in x makes its row of
  * y NaN, a NaN group of W its column. bias and residual may be NULL; residual
  * may alias y, x must not. K % 8 == 0, M up to 2^20 - 16, K up to 2^24, x, Wp and
  * the workspace 16-byte aligned (else GORCH_HIP_EUNSUPPORTED). The workspace
@@ -558,7 +563,10 @@ int gorch_hip_paged_read(void* stream, const gorch_hip_paged_kv* kv, const gorch
  * 16-byte aligned; query head h reads KV head h / (num_q / num_kv); scores
  * scaled by 1 / sqrt(head_dim). causal: a token sees the positions up to its
  * own, else all kv_lens[s]. Products and sums keep f32 accuracy (q and the
- * softmax weights as three bf16 terms against the cache's exact values), every
+ * softmax weights as three bf16 terms against the cache's exact values; over
+ * GORCH_HIP_KV_MXFP4 pools q is held to 2^-24 of the largest magnitude among
+ * each 32 columns, as gorch_hip_linear_mxfp4 holds x: with one column 1,000
+ * times the others outputs are off by some 2.5e-5 of their norm), every
  * sum has a fixed order. A key that a token does not see has no effect on it,
  * whatever its page holds; a token that sees none gets zeros; one that sees
  * an infinite value gets it, however small its weight; one that sees an

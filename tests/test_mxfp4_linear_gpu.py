@@ -355,3 +355,21 @@ def test_one_instruction(gpu, M, kind):
     size = np.abs(x).astype(np.float64) @ np.abs(W).T
     off = np.abs(call(gpu, x, codes, scales) - x.astype(np.float64) @ W.T) / size
     assert (off <= 20 * U).all(), f"off by {off.max() / U} U of the sum of magnitudes"
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 300, 4096), (3, 50, 264), (5, 300, 2048), (16, 300, 2048), (40, 300, 1096)])
+@pytest.mark.parametrize("times", [1e3, 3e4])
+def test_columns_much_larger_than_the_others(gpu, M, N, K, times):
+    # what x's values are held to beside the largest of their 32 columns: that much times the weights, in outputs to which
+    # the largest add nothing (their weights are 0), and 20 U of the other products' magnitudes for each instruction
+    rng, x, codes, scales = inputs(M, M, N, K)
+    x = (x / np.abs(x).max()).astype(np.float32)
+    x[:, 5::32] = times
+    codes[:, 2::16] &= 0x0f  # columns 5, 37, ..
+    W = values(codes, scales)
+    off = np.abs(call(gpu, x, codes, scales) - x.astype(np.float64) @ W.T)
+    rest = np.where(W == 0, 0, np.abs(W))
+    assert not rest[:, 5::32].any()
+    held = U * times * rest.sum(1)
+    assert (off <= held + 100 * -(-K // 128) * U * (np.abs(x).astype(np.float64) @ rest.T)).all()
+    assert (np.median(off, 0) <= held / 4).all()
