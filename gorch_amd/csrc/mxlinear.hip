@@ -672,8 +672,9 @@ static int launch_mx_gemv(hipStream_t s, MxLinearArgs a, char* ws) {
 
 // The block (MT x WM row tiles of x, NT of W) of the least estimated time:
 // rounds of 256 blocks, times a wave's steps (a column tile each), times what a
-// step takes: measured with K = 4096 where few blocks ran; loading x's terms
-// bounds it, 64 KB a step, which the wider blocks use more often. (us, wide
+// step takes: measured with N = K = 4096 where few blocks ran (other N and K rest
+// on that); loading x's terms bounds it, 64 KB a step, which the wider blocks use
+// more often. (us, wide
 // first: 2000 x 4096 x 4096 91 101 113 143 178 286; 512 x 4096 x 4096 66 43 32
 // 41 51 77; 64 x 4096 x 4096 60 37 24 20 15 14.)
 struct GemmShape {

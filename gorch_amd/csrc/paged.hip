@@ -165,7 +165,9 @@ struct AppendArgs {
 // Bound by memory: the rows go out before anything else, and the chain
 // sequence -> page -> store runs beside them. Large calls (P > 1) read them
 // past the caches: 15,518 tokens of 14 + 2 + 2 heads of 64 into e4m3 38.7 ->
-// 35.5 us (3.8 TB/s; two or four tokens a block: 39.4, 46), into MXFP4 31. One
+// 35.5 us (3.8 TB/s; two or four tokens a block: 39.4, 46). The types differ
+// little, since q and the rows read are most of the bytes: 12,594 tokens of those
+// heads into bf16, e4m3 and MXFP4 30.7, 31.2 and 30.5 us (3.7 to 3.5 TB/s). One
 // token 3.6 us on the GPU, 64 of 16 + 8 + 8 heads of 128 into MXFP4 4.1. (In
 // MXFP4 codes leave as two bytes a lane and scales as a byte of every eighth:
 // 136 of the 3,720 bytes that a token of the 14 + 2 + 2 heads writes.)
@@ -270,7 +272,7 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
 // 8 x 128 in e4m3 116 us with four tokens a block (5.1 TB/s), 172 with one;
 // few tokens have one a block (1,000 in bf16 4.3 us against 5.0). Heads that
 // need fewer than 256 threads a token share the block between tokens, LG lanes
-// a token: 15,518 tokens of 2 x 64 in MXFP4 12.6 -> 9.9 us with four tokens in
+// a token: 12,594 tokens of 2 x 64 in MXFP4 12.6 -> 9.9 us with four tokens in
 // turn, 7.1 with one (its lookups then overlap between waves). Two tokens a wave
 // look up twice: few tokens have a wave each (976 of 2 x 64 3.1 us, else 3.4).
 template <int KV, int TOK, int LG>
