@@ -239,6 +239,9 @@ __global__ __launch_bounds__(64 * kGemvWaves, 2) void k_mx_gemv(MxLinearArgs a) 
             *reinterpret_cast<u32x4*>(lds + slot * 16) = u32x4{t[0], t[1], t[2], t[3]};
             *reinterpret_cast<u32x2*>(lds + at.p8 + slot * 8) = u32x2{t[4], t[5]};
         };
+        // (One row's first terms may add up to 2^128 where its other rows take some
+        // off again: terms that are rows of an operand are held at half their size.)
+        const auto byte_of = [](uint32_t s) { return (uint8_t)(ROW1 && s != kMxNaN ? s - 1 : s); };
         const auto scales_of = [&](int m, int kb) {  // bytes of the terms' scales
             return reinterpret_cast<uint8_t*>(lds + at.sc) + (ROW1 ? kb * R + m * kMxTerms : (kb * M + m) * 8);
         };
@@ -251,7 +254,7 @@ __global__ __launch_bounds__(64 * kGemvWaves, 2) void k_mx_gemv(MxLinearArgs a) 
             const u32x6 t = mx_term(x, q, s);
             if (i < tasks) {
                 put(slot_of(m, kb, q), t);
-                scales_of(m, kb)[q] = (uint8_t)s;
+                scales_of(m, kb)[q] = byte_of(s);
             }
         } else {
             for (int i = threadIdx.x; i < tasks; i += 64 * kGemvWaves) {
@@ -263,8 +266,8 @@ __global__ __launch_bounds__(64 * kGemvWaves, 2) void k_mx_gemv(MxLinearArgs a) 
                 uint8_t* sc = scales_of(m, kb);
                 if constexpr (ROW1) {
 #pragma unroll
-                    for (int q = 0; q < 4; q++) sc[q] = (uint8_t)(r.scale >> (8 * q));
-                    sc[4] = (uint8_t)r.last;
+                    for (int q = 0; q < 4; q++) sc[q] = byte_of(r.scale >> (8 * q) & 0xff);
+                    sc[4] = byte_of(r.last);
                 } else {
                     *reinterpret_cast<u32x2*>(sc) = u32x2{r.scale, r.last};
                 }
@@ -285,7 +288,7 @@ __global__ __launch_bounds__(64 * kGemvWaves, 2) void k_mx_gemv(MxLinearArgs a) 
                 const int row = min(g, M - 1) * kMxTerms + q;
                 v += mine[(row & 3) * 64 + (row >> 2) * 16 + c];
             }
-            if (g < M && n < a.N) mx_store(a, g, n, v);
+            if (g < M && n < a.N) mx_store(a, g, n, 2 * v);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++)

@@ -373,3 +373,19 @@ def test_columns_much_larger_than_the_others(gpu, M, N, K, times):
     held = U * times * rest.sum(1)
     assert (off <= held + 100 * -(-K // 128) * U * (np.abs(x).astype(np.float64) @ rest.T)).all()
     assert (np.median(off, 0) <= held / 4).all()
+
+
+@pytest.mark.parametrize("M,K", [(1, 128), (3, 128), (3, 4096), (2, 9000), (5, 128), (16, 128), (16, 2048), (20, 128), (200, 128)])
+def test_outputs_near_the_end_of_f32(gpu, M, K):
+    # from 1.9 * 2^127 on, where a first term of eighths alone gives 2^128, and a second value that leaves the sum there
+    v = np.array([1.9, 1.9374, 1.95, 1.97, 1.99, 1.9999, -1.96, -1.9999], np.float32)
+    codes, scales = np.zeros((16, K // 2), np.uint8), np.zeros((16, -(-K // GROUP)), np.uint8)
+    codes[:, 1], scales[:, 0] = 0x20, 254        # column 3: 2^127
+    codes[8:, K // 2 - 1], scales[8:, -1] = 0x20, 127  # the last column: 1
+    for at in range(0, len(v), M):
+        x = np.zeros((M, K), np.float32)
+        part = v[at:at + M]
+        x[:len(part), 3], x[:len(part), -1] = part, -part * np.float32(2.0 ** 122)
+        want = x.astype(np.float64) @ values(codes, scales).T
+        got = call(gpu, x, codes, scales)
+        assert (np.abs(got - want) <= 20 * U * np.abs(want)).all()
