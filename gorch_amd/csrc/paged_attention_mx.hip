@@ -7,8 +7,7 @@
 // 128 columns, where widened codes and three bf16 terms would take twelve.
 // Values: their scales differ from key to key, along the sum, so codes are
 // widened (exactly) to bf16 on their way to LDS, a lane's 32 columns under one
-// scale, and multiplied as a bf16 cache's are. A value with scale byte 0 (below
-// 2^-124) counts as zero.
+// scale, and multiplied as a bf16 cache's are.
 #include "mx.h"
 #include "paged_attention.h"
 
@@ -135,8 +134,8 @@ __device__ __forceinline__ bool mx_put(const MxRow<HD>& r, char* vt, int key, in
         if (HD < 128 && g >= HD / 32) continue;
         u32x4 codes = r.c[u];
         odd |= mx_finite(codes, r.s[u]);
-        const bool none = r.s[u] == kMxNaN || r.s[u] == 0;
-        const float s = __uint_as_float(none ? 0x3f800000u : r.s[u] << 23);
+        const bool none = r.s[u] == kMxNaN;
+        const float s = mx_power(none ? 127 : r.s[u]);
         const uint32_t keep = none ? 0u : ~0u;  // (a mask: a choice per word becomes a branch)
         char* to = vt + (key >> 4) * MxTile<HD>::GROUP + (4 * u + g) * 1024 + (key & 15) * 16;
 #pragma unroll
@@ -744,8 +743,8 @@ __device__ __forceinline__ void mx_many_block(const PagedAttnArgs& a, int block,
             if (lane == 0 && u == 0) sh.seen_of[b][j] = here;
         } else if (HD >= 128 || g < HD / 32) {
             u32x4 codes = raw.c[0];
-            const bool far = mx_finite(codes, raw.s[0]), none = raw.s[0] == kMxNaN || raw.s[0] == 0;
-            const float f = __uint_as_float(none ? 0x3f800000u : raw.s[0] << 23);
+            const bool far = mx_finite(codes, raw.s[0]), none = raw.s[0] == kMxNaN;
+            const float f = mx_power(none ? 127 : raw.s[0]);
             const uint32_t keep = none ? 0u : ~0u;
             char* to = sh.vt[b] + j * MxTile<HD>::GROUP + (4 * u + g) * 1024 + (lane & 15) * 16;
 #pragma unroll

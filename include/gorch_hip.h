@@ -495,8 +495,7 @@ int gorch_hip_qwen_generate_sampled(void* stream, gorch_hip_qwen* m, const int* 
  * [num_pages][num_kv][page_size][head_dim / 2] bytes of codes as
  * gorch_hip_mxfp4_encode writes rows of head_dim, and k_scale and v_scale point
  * at bytes, 4-byte aligned, [num_pages][num_kv][page_size][ceil(head_dim /
- * 32)]; attention takes V's codes of scale byte 0 (below 2^-124) as zeros.
- * head_dim is a multiple of 16 up to 256,
+ * 32)]. head_dim is a multiple of 16 up to 256,
  * num_kv below 2^16 (else GORCH_HIP_EUNSUPPORTED); page_size is any positive
  * number. */
 typedef struct {

@@ -362,3 +362,18 @@ def test_values_whose_weighted_sum_stays_in_f32(gpu, hq, hkv, hd, n):
     q = np.zeros((c.tokens, hq, hd), np.float32)
     q[..., 0] = 5 * np.sqrt(hd)
     check(attend(gpu, c, q, hq, causal=False, max_new=n), *c.attention(q, hq, causal=False))
+
+
+@pytest.mark.parametrize("hq,hkv,hd,n", [(2, 1, 64, 1), (16, 8, 128, 1), (2, 1, 80, 1), (14, 2, 64, 1), (2, 1, 256, 1), (2, 1, 64, 40),
+                                         (8, 1, 256, 10), (6, 2, 96, 20)])
+def test_values_of_the_smallest_scales(gpu, hq, hkv, hd, n):
+    # byte 0 is 2^-127 here too; an output is a mean of 40 such values, whose weighted sum (weights of 2^-8) is held to
+    # 2^-149 a product or addition: 2^-141 in the output, three times 40
+    c = MxCase(hkv, hd, 16, [(40, n), (1, 1)], seed=17)
+    c.vs[:] = np.where(c.vs == 255, 255, c.rng.integers(0, 3, c.vs.shape))
+    c.k[:], c.ks[:] = 0, np.where(c.ks == 255, 255, 127)
+    q = queries(c, hq)
+    want, _ = c.attention(q, hq, causal=False)
+    got = attend(gpu, c, q, hq, causal=False, max_new=n)
+    assert (np.abs(want) > 2.0 ** -132).mean() > 0.8
+    assert (np.abs(got - want) <= 120 * 2.0 ** -141).all()
