@@ -680,8 +680,8 @@ struct MxRowsOf : Rows<false, HD, NR> {
 // that all waves read from LDS. Waves 0 and 1 (of each step of 128 columns)
 // fetch the keys' two groups, 2 and 3 the values', into registers a tile ahead
 // and from there to the other of two stages, the values widened. Bound by issue: for
-// 2,048 tokens over 16,384 keys of 8 x 128 (16 query heads) 484 us with the join,
-// 0.53 PFLOP/s of the product; vector instructions (exponentials, the weights'
+// 2,048 tokens over 16,384 keys of 8 x 128 (16 query heads) 480 us with the join,
+// 0.54 PFLOP/s of the product; vector instructions (exponentials, the weights'
 // three terms) and matrix instructions take about half of the cycles each and
 // overlap little. A reference that is moved by 8 at once took off 3%, and
 // scores that come out less that reference 4% (of 525). No faster: the next
