@@ -375,9 +375,9 @@ struct MxFour {
 
 // Few rows: as k_paged_attn_few, the values widened on their way to LDS. The
 // floor is the codes: 64 tokens over 179,769 keys of 8 x 128 42 to 43 us (4.6 TB/s
-// of 196 MB), with the join 46.6, where e4m3's 371 MB take 87. Two tiles are on their way; three
-// and four were no faster (48.6, 48.1 us with the join against 46.3). One token
-// over 777 keys 6.0 us, a chain of loads (page, keys, join).
+// of 196 MB), with the join 46.6, where e4m3's 371 MB take 87. Two tiles are on
+// their way; three and four were no faster (48.6, 48.1 us with the join against
+// 46.3). One token over 777 keys 6.0 us, a chain of loads (page, keys, join).
 template <int HD, bool PART, int CW>
 struct MxFewBlock {
     static constexpr int NW = 4, NB = 2, OROW = HD + 4, PT = CW == 4 ? 1024 : 0;
